@@ -32,6 +32,9 @@ __all__ = [
     "dequantize_mxfp8",
     "scaled_mm_nvfp4",
     "scaled_mm_mxfp8",
+    "quantize_int4",
+    "dequantize_int4",
+    "linear_int4",
     "apply_rope",
     "apply_rope1",
     "swap_nibbles",
@@ -192,6 +195,38 @@ def scaled_mm_fp8(a: torch.Tensor, b: torch.Tensor, scale_a: torch.Tensor, scale
     if direct(a, b, scale_a, scale_b, bias) and untouched("scaled_mm_fp8"):
         return _dispatch("scaled_mm_fp8", a=a, b=b, scale_a=scale_a, scale_b=scale_b, bias=bias, out_dtype=out_dtype)
     return torch.ops.comfy_kitchen.scaled_mm_fp8(a, b, scale_a, scale_b, bias, code)
+
+
+def quantize_int4(w: torch.Tensor, group_size: int = 128) -> tuple[torch.Tensor, torch.Tensor]:
+    """4-bit codes [N, K/2] (uint8, the even k in the low nibble) and scales [N, ceil(K/group_size)]
+    in w's dtype of a weight [N, K]: w ~= (code - 8) * scale, scale = amax(|group|) / 7.
+
+    K and group_size are multiples of 32; the last group of a row may be shorter."""
+    if type(group_size) is int and direct(w) and untouched("quantize_int4"):
+        return _dispatch("quantize_int4", w=w, group_size=group_size)
+    return torch.ops.comfy_kitchen.quantize_int4(w, group_size)
+
+
+def dequantize_int4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None,
+                    group_size: int = 128, output_type: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """(code - zero) * scale as [N, K] of output_type; zeros: uint8 of scales' shape (None: 8)."""
+    code = DTYPE_TO_CODE[output_type]
+    if type(group_size) is int and direct(codes, scales, zeros) and untouched("dequantize_int4"):
+        return _dispatch("dequantize_int4", codes=codes, scales=scales, zeros=zeros, group_size=group_size,
+                         output_type=output_type)
+    return torch.ops.comfy_kitchen.dequantize_int4(codes, scales, zeros, group_size, code)
+
+
+def linear_int4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None,
+                bias: torch.Tensor | None = None, group_size: int = 128) -> torch.Tensor:
+    """y = x @ W.T + bias for a weight W [N, K] of 4-bit codes with a scale (and zero point) for
+    each row and group of group_size inputs; x [..., K] in f16 / bf16, y [..., N] in x's dtype.
+
+    Made for the one to some dozens of rows of text generation, where reading the codes bounds
+    the call; any number of rows is served.  A row of x that holds an infinity or NaN gives NaNs."""
+    if type(group_size) is int and direct(x, codes, scales, zeros, bias) and untouched("linear_int4"):
+        return _dispatch("linear_int4", x=x, codes=codes, scales=scales, zeros=zeros, bias=bias, group_size=group_size)
+    return torch.ops.comfy_kitchen.linear_int4(x, codes, scales, zeros, bias, group_size)
 
 
 def apply_rope(xq: torch.Tensor, xk: torch.Tensor,

@@ -28,10 +28,13 @@ __all__ = [
     "amax_scale",
     "apply_rope",
     "apply_rope1",
+    "dequantize_int4",
     "dequantize_mxfp8",
     "dequantize_nvfp4",
     "dequantize_per_tensor_fp8",
+    "linear_int4",
     "quantize_fp8_dynamic",
+    "quantize_int4",
     "quantize_mxfp8",
     "quantize_nvfp4",
     "quantize_nvfp4_dynamic",
@@ -67,6 +70,9 @@ SIGNATURES: dict[str, tuple] = {
     "ckh_amax_scale_noalloc": (_i32, [_p, _i64, _i32, _f32, _p, _u64]),
     "ckh_quantize_fp8_dynamic": (_i32, [_p, _f32, _p, _p, _i64, _i32, _i32, _p, _u64]),
     "ckh_quantize_nvfp4_dynamic": (_i32, [_p, _f32, _p, _p, _p, _i64, _i64, _i64, _i64, _f32, _i32, _i32, _p, _u64]),
+    "ckh_quantize_int4": (_i32, [_p] * 3 + [_i64] * 3 + [_i32, _u64]),
+    "ckh_dequantize_int4": (_i32, [_p] * 4 + [_i64] * 3 + [_i32, _i32, _u64]),
+    "ckh_linear_int4": (_i32, [_p] * 6 + [_i64] * 5 + [_i32] * 3 + [_u64]),
 }
 ABI_VERSION = 8
 # CKH_AMAX_WORKSPACE_BYTES of include/ckh.h: the workspace ckh_amax_scale takes
@@ -387,6 +393,82 @@ def scaled_mm_nvfp4(a: torch.Tensor, b: torch.Tensor, tensor_scale_a: torch.Tens
     return out
 
 
+# -------------------------------------------------------------- weight-only 4-bit linears
+def quantize_int4(w: torch.Tensor, group_size: int) -> tuple[torch.Tensor, torch.Tensor]:
+    n, k = w.shape
+    if k % 32 or k == 0 or group_size < 32 or group_size % 32:
+        raise ValueError(f"quantize_int4: K ({k}) and group_size ({group_size}) must be positive multiples of 32")
+    w = w.contiguous()
+    codes = torch.empty((n, k // 2), dtype=torch.uint8, device=w.device)
+    scales = torch.empty((n, -(-k // group_size)), dtype=w.dtype, device=w.device)
+    _launch("ckh_quantize_int4", w, w.data_ptr(), codes.data_ptr(), scales.data_ptr(), n, k, group_size,
+            DTYPE_TO_CODE[w.dtype])
+    return codes, scales
+
+
+def _int4_weight(name: str, codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None,
+                 group_size: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None, int, int]:
+    """The weight's tensors, contiguous and of the shapes that the codes ask for, with N and K."""
+    n, half = codes.shape
+    k = 2 * half
+    if group_size < 32 or group_size % 32:
+        raise ValueError(f"{name}: group_size must be a positive multiple of 32, got {group_size}")
+    shape = (n, -(-k // group_size))
+    if scales.shape != shape:
+        raise ValueError(f"{name}: scales must be {list(shape)} for codes {list(codes.shape)} and group_size "
+                         f"{group_size}, got {list(scales.shape)}")
+    if zeros is not None:
+        if zeros.shape != shape:
+            raise ValueError(f"{name}: zeros must be {list(shape)}, got {list(zeros.shape)}")
+        zeros = zeros.contiguous()
+    return _aligned(codes), scales.contiguous(), zeros, n, k
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """t, contiguous and on a 16-byte boundary (copied where it is not)."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def _same_device(name: str, first: torch.Tensor, *others: torch.Tensor | None) -> None:
+    device = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"{name}: tensors on different devices ({first.device} and {t.device})")
+
+
+def dequantize_int4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None, group_size: int,
+                    output_type: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    _same_device("dequantize_int4", codes, scales, zeros)
+    codes, scales, zeros, n, k = _int4_weight("dequantize_int4", codes, scales, zeros, group_size)
+    out = torch.empty((n, k), dtype=output_type, device=codes.device)
+    _launch("ckh_dequantize_int4", codes, codes.data_ptr(), scales.data_ptr(), _ptr(zeros), out.data_ptr(), n, k,
+            group_size, DTYPE_TO_CODE[scales.dtype], DTYPE_TO_CODE[output_type])
+    return out
+
+
+def linear_int4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None,
+                bias: torch.Tensor | None = None, group_size: int = 128) -> torch.Tensor:
+    _same_device("linear_int4", x, codes, scales, zeros, bias)
+    codes, scales, zeros, n, k = _int4_weight("linear_int4", codes, scales, zeros, group_size)
+    if x.shape[-1] != k:
+        raise ValueError(f"linear_int4: x has {x.shape[-1]} inputs, the weight {k}")
+    rows = x if x.dim() == 2 else x.reshape(-1, k)
+    m = rows.shape[0]
+    stride = rows.stride(0)
+    if rows.stride(1) != 1 or rows.data_ptr() % 16 or (m > 1 and (stride % 8 or stride < k)):
+        rows = rows.contiguous()
+        if rows.data_ptr() % 16:
+            rows = rows.clone()
+        stride = k
+    bias, bias_code = _bias_args(bias, n, x.device)
+    out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
+    _launch("ckh_linear_int4", rows, rows.data_ptr(), codes.data_ptr(), scales.data_ptr(), _ptr(zeros), _ptr(bias),
+            out.data_ptr(), m, n, k, stride if m > 1 else k, group_size, DTYPE_TO_CODE[x.dtype],
+            DTYPE_TO_CODE[scales.dtype], bias_code)
+    return out
+
+
 # ----------------------------------------------------------------------------- RoPE
 def _rope_call(xq: torch.Tensor, xk: torch.Tensor | None, freqs_cis: torch.Tensor):
     if xq.dim() != 4 or freqs_cis.dim() != 6:
@@ -424,13 +506,14 @@ def apply_rope(xq: torch.Tensor, xk: torch.Tensor, freqs_cis: torch.Tensor) -> t
 
 # ---------------------------------------------------------------------- registration
 def _build_constraints() -> dict:
-    from ...constraints import DivisibleBy, ExactDims, FunctionConstraints, ParamConstraint
+    from ...constraints import DivisibleBy, ExactDims, FunctionConstraints, MinDims, ParamConstraint
 
     dev = frozenset({"cuda"})
     floats = frozenset({torch.float32, torch.float16, torch.bfloat16})
     half = frozenset({torch.float16, torch.bfloat16})
     fp8 = frozenset({torch.float8_e4m3fn, torch.float8_e5m2})
     f32 = frozenset({torch.float32})
+    u8 = frozenset({torch.uint8})
 
     def fc(**params):
         return FunctionConstraints(params=params, default_devices=dev, required_arch=REQUIRED_ARCH)
@@ -482,6 +565,16 @@ def _build_constraints() -> dict:
                               block_scale_b=ParamConstraint(dtypes=frozenset({torch.float8_e4m3fn})),
                               bias=ParamConstraint(dtypes=floats),
                               out_dtype=ParamConstraint(dtypes=floats)),
+        "quantize_int4": fc(w=ParamConstraint(dtypes=floats, shape_rules=two_d)),
+        "dequantize_int4": fc(codes=ParamConstraint(dtypes=u8, shape_rules=two_d + (DivisibleBy(1, 16),)),
+                              scales=ParamConstraint(dtypes=floats, shape_rules=two_d),
+                              zeros=ParamConstraint(dtypes=u8, shape_rules=two_d),
+                              output_type=ParamConstraint(dtypes=floats)),
+        "linear_int4": fc(x=ParamConstraint(dtypes=half, shape_rules=(MinDims(1),)),
+                          codes=ParamConstraint(dtypes=u8, shape_rules=two_d + (DivisibleBy(1, 16),)),
+                          scales=ParamConstraint(dtypes=floats, shape_rules=two_d),
+                          zeros=ParamConstraint(dtypes=u8, shape_rules=two_d),
+                          bias=ParamConstraint(dtypes=floats)),
         "apply_rope1": fc(x=ParamConstraint(dtypes=floats, shape_rules=(ExactDims(4),)),
                           freqs_cis=ParamConstraint(dtypes=floats, shape_rules=(ExactDims(6),))),
         "apply_rope": fc(xq=ParamConstraint(dtypes=floats, shape_rules=(ExactDims(4),)),

@@ -269,6 +269,43 @@ def _(a, b, scale_a, scale_b, bias, output_dtype_code):
     return torch.empty((a.shape[0], b.shape[0]), dtype=DTYPE_CODE_TO_DTYPE[output_dtype_code], device=a.device)
 
 
+# ------------------------------------------------------- weight-only 4-bit linears
+@torch.library.custom_op("comfy_kitchen::quantize_int4", mutates_args=())
+def quantize_int4(w: torch.Tensor, group_size: int) -> tuple[torch.Tensor, torch.Tensor]:
+    return _dispatch("quantize_int4", w=w, group_size=group_size)
+
+
+@quantize_int4.register_fake
+def _(w, group_size):
+    rows, cols = w.shape
+    return (torch.empty((rows, cols // 2), dtype=torch.uint8, device=w.device),
+            torch.empty((rows, -(-cols // group_size)), dtype=w.dtype, device=w.device))
+
+
+@torch.library.custom_op("comfy_kitchen::dequantize_int4", mutates_args=())
+def dequantize_int4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None, group_size: int,
+                    output_dtype_code: int) -> torch.Tensor:
+    return _dispatch("dequantize_int4", codes=codes, scales=scales, zeros=zeros, group_size=group_size,
+                     output_type=DTYPE_CODE_TO_DTYPE[output_dtype_code])
+
+
+@dequantize_int4.register_fake
+def _(codes, scales, zeros, group_size, output_dtype_code):
+    rows, half = codes.shape
+    return torch.empty((rows, half * 2), dtype=DTYPE_CODE_TO_DTYPE[output_dtype_code], device=codes.device)
+
+
+@torch.library.custom_op("comfy_kitchen::linear_int4", mutates_args=())
+def linear_int4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None,
+                bias: torch.Tensor | None, group_size: int) -> torch.Tensor:
+    return _dispatch("linear_int4", x=x, codes=codes, scales=scales, zeros=zeros, bias=bias, group_size=group_size)
+
+
+@linear_int4.register_fake
+def _(x, codes, scales, zeros, bias, group_size):
+    return x.new_empty((*x.shape[:-1], codes.shape[0]))
+
+
 # ------------------------------------------------------------------------- RoPE
 @torch.library.custom_op("comfy_kitchen::apply_rope", mutates_args=())
 def apply_rope(xq: torch.Tensor, xk: torch.Tensor, freqs_cis: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:

@@ -1,0 +1,393 @@
+// Weight-only 4-bit linears for gfx950: y = x W^T + bias with W[n, k] = s[n, g] (q[n, k] - z[n, g]),
+// g = k / group, codes q in 0..15 (two a byte, the even k in the low nibble), and the quantizer
+// and dequantizer of that format.
+//
+// linear_int4.  For one to some dozens of rows the call is bound by reading the codes once.
+//   - The codes become MFMA operands without arithmetic: a code under the exponent bits of 128
+//     (bf16) or 1024 (f16) is the number 128 + q (1024 + q), exactly, so two codes cost one
+//     shift and one and-or.  The offset and the zero point leave by the group's sum:
+//       sum_k x (q - z) = sum_k x (B + q) - (B + z) sum_k x,  B = 128 or 1024,
+//     where sum_k x comes from one more MFMA against ones, whose result every lane holds at
+//     the place of the product it corrects.  All sums are fp32; the cancellation costs some
+//     2^-24 B / 8 of sum |x| |q|, far below the rounding of a 16-bit result.
+//   - v_mfma_f32_16x16x32: 16 activation rows by 16 weight rows; a lane (row r = lane % 16,
+//     quarter c = lane / 16) loads 16 bytes = 32 codes of weight row r, so a wave's load takes
+//     64 bytes of 16 rows.  Word j of the four lanes of a row then has to hold codes of one
+//     32-code block, so that a scale belongs to one MFMA: a 4x4 transpose of words over the
+//     lane quarters, in four lane-swap instructions.
+//   - D[token][weight row]: the scale a lane needs is the one of the weight row it loads.
+//   - A workgroup owns 16 R weight rows; its waves split K and add their sums in LDS in wave
+//     order, so results do not depend on timing.
+#include "ckh_common.h"
+
+namespace ckh {
+namespace i4 {
+
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
+typedef unsigned v2u __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+struct LinearArgs {
+    const void* x;
+    const uint8_t* codes;
+    const void* scales;
+    const uint8_t* zeros;  // null: every zero point is 8
+    const void* bias;      // null: none
+    void* y;
+    int64_t x_stride;  // elements between activation rows
+    int m, n, k, groups, group;
+    int scale_code, bias_code;
+};
+
+template <int XC>
+__device__ __forceinline__ v4f mfma(v4u a, v4u b, v4f c) {
+    if constexpr (XC == CKH_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+
+// The 8 codes of a word as B + q, in the order (k0 k4)(k1 k5)(k2 k6)(k3 k7).
+template <int XC>
+__device__ __forceinline__ v4u widen(uint32_t w) {
+    constexpr uint32_t magic = XC == CKH_BF16 ? 0x43004300u : 0x64006400u;
+    return v4u{(w & 0x000f000fu) | magic, ((w >> 4) & 0x000f000fu) | magic, ((w >> 8) & 0x000f000fu) | magic,
+               ((w >> 12) & 0x000f000fu) | magic};
+}
+
+// 8 consecutive 16-bit activations in widen()'s order.
+__device__ __forceinline__ v4u pair_order(v4u x) {
+    return v4u{__builtin_amdgcn_perm(x[2], x[0], 0x05040100u), __builtin_amdgcn_perm(x[2], x[0], 0x07060302u),
+               __builtin_amdgcn_perm(x[3], x[1], 0x05040100u), __builtin_amdgcn_perm(x[3], x[1], 0x07060302u)};
+}
+
+// Word j of lane quarter c becomes word c of lane quarter j.
+__device__ __forceinline__ v4u transpose_quarters(v4u w) {
+    const v2u a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+    const v2u b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+    const v2u c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+    const v2u d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+    return v4u{c[0], c[1], d[0], d[1]};
+}
+
+__device__ __forceinline__ float widen_scale(uint32_t raw, int code) {
+    return code == CKH_F32 ? as_f(raw) : code == CKH_BF16 ? bf16_to_f(raw) : f16_to_f(raw);
+}
+
+// XC: activation type; T: 16-row activation tiles; R: 16-row weight tiles per workgroup;
+// W: waves per workgroup; U: steps of 128 codes whose loads a wave issues together; GB: the
+// scale changes after GB blocks of 32 codes (4: at most once a step).
+template <int XC, int T, int R, int W, int U, int GB>
+__global__ __launch_bounds__(W * 64) void linear_kernel(LinearArgs a) {
+    __shared__ float red[W > 1 ? W : 1][R * T * 4][64];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r16 = lane & 15, quarter = lane >> 4;
+    const int n0 = blockIdx.x * 16 * R;
+    const int m0 = blockIdx.y * 16 * T;
+    const int rows = min(16 * R, a.n - n0), toks = min(16 * T, a.m - m0);
+    const int pitch = a.k >> 1;  // code bytes per weight row
+
+    // loads outside the operands read zeros: a zero activation makes its products vanish
+    const __amdgpu_buffer_rsrc_t rw = buffer_rsrc(a.codes + static_cast<int64_t>(n0) * pitch, rows * pitch);
+    const __amdgpu_buffer_rsrc_t rx =
+        buffer_rsrc(static_cast<const uint16_t*>(a.x) + m0 * a.x_stride,
+                    static_cast<uint32_t>(((toks - 1) * a.x_stride + a.k) * 2));
+    const int ss = a.scale_code == CKH_F32 ? 4 : 2;
+    const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(
+        static_cast<const uint8_t*>(a.scales) + static_cast<int64_t>(n0) * a.groups * ss, rows * a.groups * ss);
+    const __amdgpu_buffer_rsrc_t rz =
+        buffer_rsrc(a.zeros ? a.zeros + static_cast<int64_t>(n0) * a.groups : a.codes, a.zeros ? rows * a.groups : 0);
+    constexpr uint32_t kOut = 0x80000000u;
+
+    const v4u ones = XC == CKH_BF16 ? v4u{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}
+                                    : v4u{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+    constexpr float kBase = XC == CKH_BF16 ? 128.0f : 1024.0f;
+    constexpr int NS = 4 / GB;  // scales per step
+
+    const int steps = (a.k + 127) >> 7;
+    const int per = (steps + W - 1) / W;
+    const int first = wave * per, last = min(steps, first + per);
+
+    v4f total[R][T];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int t = 0; t < T; ++t) total[r][t] = v4f{0, 0, 0, 0};
+
+    for (int s0 = first; s0 < last; s0 += U) {
+        v4u w[U][R], x[U][T][4];
+        uint32_t sc[U][R][NS], zp[U][R][NS];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int kq = (s0 + u) * 128;
+            const bool live = s0 + u < last;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int row = r * 16 + r16;
+                const bool in = live && row < rows && kq + quarter * 32 < a.k;
+                w[u][r] = __builtin_bit_cast(
+                    v4u, __builtin_amdgcn_raw_buffer_load_b128(rw, in ? row * pitch + (kq >> 1) + quarter * 16 : kOut, 0, 0));
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int row = r * 16 + r16;
+#pragma unroll
+                for (int g = 0; g < NS; ++g) {
+                    const int kg = kq + g * GB * 32;
+                    const bool in = live && row < rows && kg < a.k;
+                    const uint32_t at = row * a.groups + kg / a.group;
+                    sc[u][r][g] = ss == 4 ? __builtin_amdgcn_raw_buffer_load_b32(rs, in ? at * 4 : kOut, 0, 0)
+                                          : __builtin_amdgcn_raw_buffer_load_b16(rs, in ? at * 2 : kOut, 0, 0);
+                    zp[u][r][g] = 8;
+                    if (a.zeros) zp[u][r][g] = __builtin_amdgcn_raw_buffer_load_b8(rz, in ? at : kOut, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < T; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int tok = t * 16 + r16, k = kq + j * 32 + quarter * 8;
+                    const bool in = live && tok < toks && k < a.k;
+                    x[u][t][j] = __builtin_bit_cast(
+                        v4u, __builtin_amdgcn_raw_buffer_load_b128(
+                                 rx, in ? static_cast<uint32_t>((tok * a.x_stride + k) * 2) : kOut, 0, 0));
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            v4f acc[R][T], sum[T];
+#pragma unroll
+            for (int r = 0; r < R; ++r) w[u][r] = transpose_quarters(w[u][r]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool fresh = j % GB == 0;
+#pragma unroll
+                for (int t = 0; t < T; ++t) {
+                    x[u][t][j] = pair_order(x[u][t][j]);
+                    sum[t] = mfma<XC>(x[u][t][j], ones, fresh ? v4f{0, 0, 0, 0} : sum[t]);
+                }
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const v4u b = widen<XC>(w[u][r][j]);
+#pragma unroll
+                    for (int t = 0; t < T; ++t) acc[r][t] = mfma<XC>(x[u][t][j], b, fresh ? v4f{0, 0, 0, 0} : acc[r][t]);
+                }
+                if (j % GB == GB - 1) {
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        const float s = widen_scale(sc[u][r][j / GB], a.scale_code);
+                        const float off = -(kBase + static_cast<float>(zp[u][r][j / GB]));
+#pragma unroll
+                        for (int t = 0; t < T; ++t)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                total[r][t][i] = __fmaf_rn(s, __fmaf_rn(off, sum[t][i], acc[r][t][i]), total[r][t][i]);
+                    }
+                }
+            }
+        }
+    }
+
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) red[wave][(r * T + t) * 4 + i][lane] = total[r][t][i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < R * T * 4 * 64; e += W * 64) {
+        const int l = e & 63, slot = e >> 6;
+        float v = red[0][slot][l];
+#pragma unroll
+        for (int w = 1; w < W; ++w) v += red[w][slot][l];
+        const int row = slot / (4 * T) * 16 + (l & 15);
+        const int tok = slot / 4 % T * 16 + (l >> 4) * 4 + (slot & 3);
+        if (row >= rows || tok >= toks) continue;
+        if (a.bias) {
+            const int64_t at = n0 + row;
+            v += a.bias_code == CKH_F32    ? load1<CKH_F32>(a.bias, at)
+                 : a.bias_code == CKH_BF16 ? load1<CKH_BF16>(a.bias, at)
+                                           : load1<CKH_F16>(a.bias, at);
+        }
+        static_cast<uint16_t*>(a.y)[static_cast<int64_t>(m0 + tok) * a.n + n0 + row] =
+            static_cast<uint16_t>(XC == CKH_BF16 ? f_to_bf16_rne(v) : f_to_f16(v));
+    }
+}
+
+template <int XC, int T, int R, int W, int U>
+void launch_linear(const LinearArgs& a, hipStream_t st) {
+    const dim3 grid(static_cast<unsigned>(cdiv(a.n, 16 * R)), static_cast<unsigned>(cdiv(a.m, 16 * T)));
+    if (a.group % 128 == 0)
+        linear_kernel<XC, T, R, W, U, 4><<<grid, W * 64, 0, st>>>(a);
+    else if (a.group % 64 == 0)
+        linear_kernel<XC, T, R, W, U, 2><<<grid, W * 64, 0, st>>>(a);
+    else
+        linear_kernel<XC, T, R, W, U, 1><<<grid, W * 64, 0, st>>>(a);
+}
+
+template <int XC>
+void linear(const LinearArgs& a, hipStream_t st) {
+    if (a.m <= 16) launch_linear<XC, 1, 1, 8, 2>(a, st);
+    else launch_linear<XC, 2, 1, 8, 1>(a, st);
+}
+
+// ------------------------------------------------------------ quantize / dequantize
+// Symmetric quantize: s = amax / 7 over the group, rounded to x's type (so that the codes fit
+// the scale that is stored), q = clamp(rint(x / s), -8, 7) + 8.  16 lanes take a group.
+template <int C>
+__global__ __launch_bounds__(256) void quantize_kernel(const void* x, uint8_t* codes, void* scales, int64_t total,
+                                                       int groups, int group, int k) {
+    const int64_t id = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 4;
+    if (id >= total) return;  // whole groups of 16 lanes leave
+    const int sub = threadIdx.x & 15;
+    const int64_t row = id / groups;
+    const int g = static_cast<int>(id - row * groups);
+    const int begin = g * group, end = min(k, begin + group);
+    float top = 0.0f;
+    bool bad = false;
+    for (int c = begin + sub * 8; c < end; c += 128) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            v[i] = load1<C>(x, row * k + c + i);
+            top = fmaxf(top, fabsf(v[i]));
+            bad |= is_nan(v[i]);
+        }
+    }
+#pragma unroll
+    for (int s = 8; s >= 1; s >>= 1) {
+        top = fmaxf(top, __shfl_xor(top, s, 16));
+        bad |= __shfl_xor(static_cast<int>(bad), s, 16) != 0;
+    }
+    const float scale = round_to<C>(bad ? __builtin_nanf("") : __fdiv_rn(top, 7.0f));
+    for (int c = begin + sub * 8; c < end; c += 128) {
+        uint32_t word = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float q = scale > 0.0f ? rintf(__fdiv_rn(load1<C>(x, row * k + c + i), scale)) : 0.0f;
+            word |= static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(q, -8.0f), 7.0f)) + 8) << (4 * i);
+        }
+        *reinterpret_cast<uint32_t*>(codes + (row * k + c) / 2) = word;
+    }
+    if (sub == 0) {
+        if constexpr (C == CKH_F32) static_cast<float*>(scales)[id] = scale;
+        else static_cast<uint16_t*>(scales)[id] = static_cast<uint16_t>(C == CKH_BF16 ? f_to_bf16(scale) : f_to_f16(scale));
+    }
+}
+
+// out = (q - z) s with one rounding; a thread takes 8 codes.
+template <int OC>
+__global__ __launch_bounds__(256) void dequantize_kernel(const uint8_t* codes, const void* scales, const uint8_t* zeros,
+                                                         void* out, int64_t words, int k, int groups, int group,
+                                                         int scale_code) {
+    const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (id >= words) return;
+    const int64_t row = id / (k >> 3);
+    const int c = static_cast<int>(id - row * (k >> 3)) * 8;
+    const uint32_t w = reinterpret_cast<const uint32_t*>(codes)[id];
+    const int64_t at = row * groups + c / group;
+    const float s = scale_code == CKH_F32    ? load1<CKH_F32>(scales, at)
+                    : scale_code == CKH_BF16 ? load1<CKH_BF16>(scales, at)
+                                             : load1<CKH_F16>(scales, at);
+    const float z = zeros ? static_cast<float>(zeros[at]) : 8.0f;
+    uint32_t o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float v = (static_cast<float>((w >> (4 * i)) & 15u) - z) * s;
+        o[i] = OC == CKH_F32 ? as_u(v) : OC == CKH_BF16 ? f_to_bf16(v) : f_to_f16(v);
+    }
+    if constexpr (OC == CKH_F32) {
+        uint4* p = reinterpret_cast<uint4*>(static_cast<float*>(out) + id * 8);
+        p[0] = make_uint4(o[0], o[1], o[2], o[3]);
+        p[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    } else {
+        reinterpret_cast<uint4*>(out)[id] =
+            make_uint4(o[0] | (o[1] << 16), o[2] | (o[3] << 16), o[4] | (o[5] << 16), o[6] | (o[7] << 16));
+    }
+}
+
+bool is_float(int code) { return code == CKH_F32 || code == CKH_F16 || code == CKH_BF16; }
+
+}  // namespace i4
+}  // namespace ckh
+
+using namespace ckh;
+
+// Sizes and pointers that every entry point of this file checks alike.
+#define CKH_REQUIRE_INT4(fn, n, k, group)                                                                       \
+    CKH_REQUIRE((n) >= 0 && (k) >= 32 && (k) % 32 == 0 && (k) <= (1 << 23), fn ": K must be a multiple of 32 in 32..2^23, got %lld", \
+                static_cast<long long>(k));                                                                     \
+    CKH_REQUIRE((group) >= 32 && (group) % 32 == 0 && (group) <= (1 << 23), fn ": group size must be a multiple of 32, got %lld", \
+                static_cast<long long>(group));                                                                 \
+    CKH_REQUIRE((n) <= INT32_MAX - 64, fn ": too many rows")
+
+extern "C" int ckh_quantize_int4(const void* x, void* codes, void* scales, int64_t n, int64_t k, int64_t group,
+                                 int in_code, uintptr_t stream) {
+    CKH_REQUIRE_INT4("quantize_int4", n, k, group);
+    CKH_REQUIRE(i4::is_float(in_code), "quantize_int4: unsupported input dtype %d", in_code);
+    if (n == 0) return CKH_OK;
+    CKH_REQUIRE(x && codes && scales, "quantize_int4: null pointer");
+    CKH_REQUIRE(aligned(codes, 4) && aligned(x, in_code == CKH_F32 ? 4 : 2) && aligned(scales, in_code == CKH_F32 ? 4 : 2),
+                "quantize_int4: misaligned pointer");
+    const int groups = static_cast<int>(cdiv(k, group));
+    const int64_t total = n * groups;
+    CKH_REQUIRE(cdiv(total, 16) <= INT32_MAX, "quantize_int4: tensor too large");
+    const unsigned grid = static_cast<unsigned>(cdiv(total, 16));
+    const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    uint8_t* q = static_cast<uint8_t*>(codes);
+    const int gs = static_cast<int>(group), kk = static_cast<int>(k);
+    if (in_code == CKH_F32) i4::quantize_kernel<CKH_F32><<<grid, 256, 0, st>>>(x, q, scales, total, groups, gs, kk);
+    else if (in_code == CKH_BF16) i4::quantize_kernel<CKH_BF16><<<grid, 256, 0, st>>>(x, q, scales, total, groups, gs, kk);
+    else i4::quantize_kernel<CKH_F16><<<grid, 256, 0, st>>>(x, q, scales, total, groups, gs, kk);
+    return check_launch("quantize_int4");
+}
+
+extern "C" int ckh_dequantize_int4(const void* codes, const void* scales, const void* zeros, void* out, int64_t n,
+                                   int64_t k, int64_t group, int scale_code, int out_code, uintptr_t stream) {
+    CKH_REQUIRE_INT4("dequantize_int4", n, k, group);
+    CKH_REQUIRE(i4::is_float(out_code), "dequantize_int4: unsupported output dtype %d", out_code);
+    CKH_REQUIRE(i4::is_float(scale_code), "dequantize_int4: unsupported scale dtype %d", scale_code);
+    if (n == 0) return CKH_OK;
+    CKH_REQUIRE(codes && scales && out, "dequantize_int4: null pointer");
+    CKH_REQUIRE(aligned(codes, 4) && aligned(out, 16) && aligned(scales, scale_code == CKH_F32 ? 4 : 2),
+                "dequantize_int4: misaligned pointer");
+    const int64_t words = n * (k / 8);
+    CKH_REQUIRE(cdiv(words, 256) <= INT32_MAX, "dequantize_int4: tensor too large");
+    const unsigned grid = static_cast<unsigned>(cdiv(words, 256));
+    const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    const uint8_t* q = static_cast<const uint8_t*>(codes);
+    const uint8_t* z = static_cast<const uint8_t*>(zeros);
+    const int groups = static_cast<int>(cdiv(k, group)), gs = static_cast<int>(group), kk = static_cast<int>(k);
+    if (out_code == CKH_F32) i4::dequantize_kernel<CKH_F32><<<grid, 256, 0, st>>>(q, scales, z, out, words, kk, groups, gs, scale_code);
+    else if (out_code == CKH_BF16) i4::dequantize_kernel<CKH_BF16><<<grid, 256, 0, st>>>(q, scales, z, out, words, kk, groups, gs, scale_code);
+    else i4::dequantize_kernel<CKH_F16><<<grid, 256, 0, st>>>(q, scales, z, out, words, kk, groups, gs, scale_code);
+    return check_launch("dequantize_int4");
+}
+
+extern "C" int ckh_linear_int4(const void* x, const void* codes, const void* scales, const void* zeros, const void* bias,
+                               void* y, int64_t m, int64_t n, int64_t k, int64_t x_stride, int64_t group, int x_code,
+                               int scale_code, int bias_code, uintptr_t stream) {
+    CKH_REQUIRE_INT4("linear_int4", n, k, group);
+    CKH_REQUIRE(x_code == CKH_F16 || x_code == CKH_BF16, "linear_int4: unsupported activation dtype %d", x_code);
+    CKH_REQUIRE(i4::is_float(scale_code), "linear_int4: unsupported scale dtype %d", scale_code);
+    CKH_REQUIRE(!bias || i4::is_float(bias_code), "linear_int4: unsupported bias dtype %d", bias_code);
+    CKH_REQUIRE(m >= 0 && m <= 65535 * 16, "linear_int4: at most %d activation rows, got %lld", 65535 * 16,
+                static_cast<long long>(m));
+    if (m == 0 || n == 0) return CKH_OK;
+    CKH_REQUIRE(x && codes && scales && y, "linear_int4: null pointer");
+    CKH_REQUIRE(x_stride >= k || m == 1, "linear_int4: activation rows overlap (stride %lld < K)", static_cast<long long>(x_stride));
+    CKH_REQUIRE(aligned(x, 16) && x_stride % 8 == 0 && aligned(codes, 16) && aligned(y, 2) &&
+                    aligned(scales, scale_code == CKH_F32 ? 4 : 2) && (!bias || aligned(bias, bias_code == CKH_F32 ? 4 : 2)),
+                "linear_int4: misaligned pointer or row stride");
+    CKH_REQUIRE(x_stride <= (int64_t(1) << 23), "linear_int4: activation row stride too large");
+    const i4::LinearArgs a{x, static_cast<const uint8_t*>(codes), scales, static_cast<const uint8_t*>(zeros), bias, y,
+                           m == 1 ? k : x_stride, static_cast<int>(m), static_cast<int>(n), static_cast<int>(k),
+                           static_cast<int>(cdiv(k, group)), static_cast<int>(group), scale_code, bias_code};
+    const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    if (x_code == CKH_BF16) i4::linear<CKH_BF16>(a, st);
+    else i4::linear<CKH_F16>(a, st);
+    return check_launch("linear_int4");
+}

@@ -289,6 +289,29 @@ int ckh_quantize_nvfp4_dynamic(const void* x, float divisor, void* scale_out, vo
                                float epsilon, int in_code, int hi_first, void* workspace,
                                uintptr_t stream);
 
+/*
+ * Weight-only 4-bit linears.  A weight W [n, k] is codes [n, k/2] u8 (two codes 0..15 a byte,
+ * the even k in the low nibble), scales [n, ceil(k/group)] of scale_code (f32/f16/bf16) and
+ * optional zero points [n, ceil(k/group)] u8 (NULL: 8 everywhere):
+ *   W[n, k] = (code - zero) * scale.
+ * k % 32 == 0, group % 32 == 0; the last group of a row may be shorter than `group`.
+ *
+ * quantize: scale = amax(|x|) / 7 over the group, rounded to in_code, code =
+ * clamp(rint(x / scale), -8, 7) + 8 (8 where the scale is 0).  A NaN in a group makes its
+ * scale NaN.
+ * dequantize: one rounding to out_code.
+ * linear: y [m, n] = x W^T + bias, x [m, k] of x_code (f16/bf16) with x_stride elements between
+ * rows (x 16-byte aligned, x_stride % 8 == 0), y of x_code, bias [n] of bias_code or NULL; sums
+ * in fp32, one rounding.  An activation that is not finite makes its row of y NaN.
+ */
+int ckh_quantize_int4(const void* x, void* codes, void* scales, int64_t n, int64_t k, int64_t group, int in_code,
+                      uintptr_t stream);
+int ckh_dequantize_int4(const void* codes, const void* scales, const void* zeros, void* out, int64_t n, int64_t k,
+                        int64_t group, int scale_code, int out_code, uintptr_t stream);
+int ckh_linear_int4(const void* x, const void* codes, const void* scales, const void* zeros, const void* bias,
+                    void* y, int64_t m, int64_t n, int64_t k, int64_t x_stride, int64_t group, int x_code,
+                    int scale_code, int bias_code, uintptr_t stream);
+
 #ifdef __cplusplus
 }
 #endif
