@@ -18,6 +18,8 @@
 //   - D[token][weight row]: the scale a lane needs is the one of the weight row it loads.
 //   - A workgroup owns 16 R weight rows; its waves split K and add their sums in LDS in wave
 //     order, so results do not depend on timing.
+#include <algorithm>
+
 #include "ckh_common.h"
 
 namespace ckh {
@@ -25,9 +27,13 @@ namespace i4 {
 
 typedef unsigned v4u __attribute__((ext_vector_type(4)));
 typedef unsigned v2u __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+constexpr int kScaleGroups = 128;  // groups whose scales are in LDS at a time
+constexpr int kVecCodes = 8192;    // matvec_kernel: codes whose activations are in LDS at a time, half as many for 4 rows
 
 struct LinearArgs {
     const void* x;
@@ -38,7 +44,13 @@ struct LinearArgs {
     void* y;
     int64_t x_stride;  // elements between activation rows
     int m, n, k, groups, group;
+    uint32_t per_group;  // ceil(2^32 / (group / 32)): block b of 32 codes is in group (b * per_group) >> 32
+    int chunk;  // steps of 128 codes whose groups fit kScaleGroups
     int scale_code, bias_code;
+
+    __device__ __forceinline__ int group_of(uint32_t block) const {
+        return per_group ? static_cast<int>((static_cast<uint64_t>(block) * per_group) >> 32) : static_cast<int>(block);
+    }
 };
 
 template <int XC>
@@ -72,125 +84,195 @@ __device__ __forceinline__ v4u transpose_quarters(v4u w) {
     return v4u{c[0], c[1], d[0], d[1]};
 }
 
-__device__ __forceinline__ float widen_scale(uint32_t raw, int code) {
-    return code == CKH_F32 ? as_f(raw) : code == CKH_BF16 ? bf16_to_f(raw) : f16_to_f(raw);
+// y[m][n] = v + bias[n], rounded.
+template <int XC>
+__device__ __forceinline__ void store_result(const LinearArgs& a, int m, int n, float v) {
+    if (a.bias)
+        v += a.bias_code == CKH_F32    ? load1<CKH_F32>(a.bias, n)
+             : a.bias_code == CKH_BF16 ? load1<CKH_BF16>(a.bias, n)
+                                       : load1<CKH_F16>(a.bias, n);
+    static_cast<uint16_t*>(a.y)[static_cast<int64_t>(m) * a.n + n] =
+        static_cast<uint16_t>(XC == CKH_BF16 ? f_to_bf16_rne(v) : f_to_f16(v));
 }
+
+// The scales and zero points of a chunk's at most kScaleGroups groups for a workgroup's 16 R rows,
+// on their way to LDS as (s, -s (B + z)): a wave takes every W-th row, its lanes 64 groups at a
+// time.  All loads go out at once, before the codes', so that they are waited for alone.
+template <int XC, int R, int W>
+struct ScaleLoads {
+    static constexpr int kPer = 16 * R / W > 0 ? 16 * R / W : 1;  // rows per wave
+    uint32_t s[kPer][2], z[kPer][2];
+
+    __device__ __forceinline__ void load(const LinearArgs& a, int n0, int rows, int wave, int lane, int g0, int gn) {
+        const bool wide = a.scale_code == CKH_F32;
+        const int ss = wide ? 4 : 2;
+        const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(
+            static_cast<const uint8_t*>(a.scales) + static_cast<int64_t>(n0) * a.groups * ss, rows * a.groups * ss);
+        const __amdgpu_buffer_rsrc_t rz = buffer_rsrc(a.zeros ? a.zeros + static_cast<int64_t>(n0) * a.groups : a.codes,
+                                                      a.zeros ? rows * a.groups : 0);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int row = wave + i * W, g = h * 64 + lane;
+                const uint32_t at = g < gn && row < rows ? row * a.groups + g0 + g : 0x20000000u;
+                s[i][h] = z[i][h] = 0;
+                if (h == 0 || gn > 64) {
+                    s[i][h] = wide ? __builtin_amdgcn_raw_buffer_load_b32(rs, at * 4, 0, 0)
+                                   : __builtin_amdgcn_raw_buffer_load_b16(rs, at * 2, 0, 0);
+                    z[i][h] = a.zeros ? __builtin_amdgcn_raw_buffer_load_b8(rz, at, 0, 0) : 8;
+                }
+            }
+    }
+
+    __device__ __forceinline__ void store(const LinearArgs& a, v2f (*sp)[16 * R + 1], int wave, int lane, int gn) const {
+        constexpr float kBase = XC == CKH_BF16 ? 128.0f : 1024.0f;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int row = wave + i * W, g = h * 64 + lane;
+                const float v = a.scale_code == CKH_F32    ? as_f(s[i][h])
+                                : a.scale_code == CKH_BF16 ? bf16_to_f(s[i][h])
+                                                           : f16_to_f(s[i][h]);
+                if (g < gn && row < 16 * R) sp[g][row] = v2f{v, -v * (kBase + static_cast<float>(z[i][h]))};
+            }
+    }
+};
 
 // XC: activation type; T: 16-row activation tiles; R: 16-row weight tiles per workgroup;
 // W: waves per workgroup; U: steps of 128 codes whose loads a wave issues together; GB: the
 // scale changes after GB blocks of 32 codes (4: at most once a step).
 template <int XC, int T, int R, int W, int U, int GB>
 __global__ __launch_bounds__(W * 64) void linear_kernel(LinearArgs a) {
-    __shared__ float red[W > 1 ? W : 1][R * T * 4][64];
+    constexpr int kRows = 16 * R;
+    constexpr int kSums = W * R * T * 4 * 64 * 4;  // bytes of the waves' sums
+    constexpr int kScales = kScaleGroups * (kRows + 1) * 8;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kSums > kScales ? kSums : kScales];
+    v2f(*sp)[kRows + 1] = reinterpret_cast<v2f(*)[kRows + 1]>(lds);  // [group][row]: s, -s (B + z)
+    float(*red)[R * T * 4][64] = reinterpret_cast<float(*)[R * T * 4][64]>(lds);
+
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, quarter = lane >> 4;
-    const int n0 = blockIdx.x * 16 * R;
+    const int n0 = blockIdx.x * kRows;
     const int m0 = blockIdx.y * 16 * T;
-    const int rows = min(16 * R, a.n - n0), toks = min(16 * T, a.m - m0);
+    const int rows = min(kRows, a.n - n0), toks = min(16 * T, a.m - m0);
     const int pitch = a.k >> 1;  // code bytes per weight row
 
-    // loads outside the operands read zeros: a zero activation makes its products vanish
     const __amdgpu_buffer_rsrc_t rw = buffer_rsrc(a.codes + static_cast<int64_t>(n0) * pitch, rows * pitch);
     const __amdgpu_buffer_rsrc_t rx =
         buffer_rsrc(static_cast<const uint16_t*>(a.x) + m0 * a.x_stride,
                     static_cast<uint32_t>(((toks - 1) * a.x_stride + a.k) * 2));
-    const int ss = a.scale_code == CKH_F32 ? 4 : 2;
-    const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(
-        static_cast<const uint8_t*>(a.scales) + static_cast<int64_t>(n0) * a.groups * ss, rows * a.groups * ss);
-    const __amdgpu_buffer_rsrc_t rz =
-        buffer_rsrc(a.zeros ? a.zeros + static_cast<int64_t>(n0) * a.groups : a.codes, a.zeros ? rows * a.groups : 0);
-    constexpr uint32_t kOut = 0x80000000u;
+
+    // Weight rows past N and activation rows past M repeat the last one: what they give is not stored.
+    uint32_t ow[R], ox[T];
+#pragma unroll
+    for (int r = 0; r < R; ++r) ow[r] = min(r * 16 + r16, rows - 1) * pitch + quarter * 16;
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+        ox[t] = static_cast<uint32_t>((min(t * 16 + r16, toks - 1) * a.x_stride + quarter * 8) * 2);
 
     const v4u ones = XC == CKH_BF16 ? v4u{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}
                                     : v4u{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
-    constexpr float kBase = XC == CKH_BF16 ? 128.0f : 1024.0f;
-    constexpr int NS = 4 / GB;  // scales per step
 
-    const int steps = (a.k + 127) >> 7;
-    const int per = (steps + W - 1) / W;
-    const int first = wave * per, last = min(steps, first + per);
-
+    struct Step {
+        v4u w[R], x[T][4];
+    };
+    // Step s's loads.  Where K ends inside the step, words of later codes (of the next row, or
+    // zeros past the operand) arrive, which use() leaves alone.
+    const auto load = [&](Step& d, int s) {
+        const int kq = s * 128;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            d.w[r] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rw, ow[r], kq >> 1, 0));
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                d.x[t][j] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rx, ox[t] + j * 64, kq * 2, 0));
+    };
     v4f total[R][T];
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int t = 0; t < T; ++t) total[r][t] = v4f{0, 0, 0, 0};
-
-    for (int s0 = first; s0 < last; s0 += U) {
-        v4u w[U][R], x[U][T][4];
-        uint32_t sc[U][R][NS], zp[U][R][NS];
+    int g0 = 0;  // the staged groups' first
+    // Adds the products of step s's first `blocks` blocks of 32 codes.
+    const auto use = [&](Step& d, int s, int blocks) {
+        v4f acc[R][T], sum[T];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int kq = (s0 + u) * 128;
-            const bool live = s0 + u < last;
+        for (int r = 0; r < R; ++r) d.w[r] = transpose_quarters(d.w[r]);
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int row = r * 16 + r16;
-                const bool in = live && row < rows && kq + quarter * 32 < a.k;
-                w[u][r] = __builtin_bit_cast(
-                    v4u, __builtin_amdgcn_raw_buffer_load_b128(rw, in ? row * pitch + (kq >> 1) + quarter * 16 : kOut, 0, 0));
-            }
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int row = r * 16 + r16;
-#pragma unroll
-                for (int g = 0; g < NS; ++g) {
-                    const int kg = kq + g * GB * 32;
-                    const bool in = live && row < rows && kg < a.k;
-                    const uint32_t at = row * a.groups + kg / a.group;
-                    sc[u][r][g] = ss == 4 ? __builtin_amdgcn_raw_buffer_load_b32(rs, in ? at * 4 : kOut, 0, 0)
-                                          : __builtin_amdgcn_raw_buffer_load_b16(rs, in ? at * 2 : kOut, 0, 0);
-                    zp[u][r][g] = 8;
-                    if (a.zeros) zp[u][r][g] = __builtin_amdgcn_raw_buffer_load_b8(rz, in ? at : kOut, 0, 0);
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < T; ++t)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int tok = t * 16 + r16, k = kq + j * 32 + quarter * 8;
-                    const bool in = live && tok < toks && k < a.k;
-                    x[u][t][j] = __builtin_bit_cast(
-                        v4u, __builtin_amdgcn_raw_buffer_load_b128(
-                                 rx, in ? static_cast<uint32_t>((tok * a.x_stride + k) * 2) : kOut, 0, 0));
-                }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            v4f acc[R][T], sum[T];
-#pragma unroll
-            for (int r = 0; r < R; ++r) w[u][r] = transpose_quarters(w[u][r]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 4; ++j) {
+            if (j < blocks) {
                 const bool fresh = j % GB == 0;
 #pragma unroll
                 for (int t = 0; t < T; ++t) {
-                    x[u][t][j] = pair_order(x[u][t][j]);
-                    sum[t] = mfma<XC>(x[u][t][j], ones, fresh ? v4f{0, 0, 0, 0} : sum[t]);
+                    d.x[t][j] = pair_order(d.x[t][j]);
+                    sum[t] = mfma<XC>(d.x[t][j], ones, fresh ? v4f{0, 0, 0, 0} : sum[t]);
                 }
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    const v4u b = widen<XC>(w[u][r][j]);
+                    const v4u b = widen<XC>(d.w[r][j]);
 #pragma unroll
-                    for (int t = 0; t < T; ++t) acc[r][t] = mfma<XC>(x[u][t][j], b, fresh ? v4f{0, 0, 0, 0} : acc[r][t]);
-                }
-                if (j % GB == GB - 1) {
-#pragma unroll
-                    for (int r = 0; r < R; ++r) {
-                        const float s = widen_scale(sc[u][r][j / GB], a.scale_code);
-                        const float off = -(kBase + static_cast<float>(zp[u][r][j / GB]));
-#pragma unroll
-                        for (int t = 0; t < T; ++t)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                total[r][t][i] = __fmaf_rn(s, __fmaf_rn(off, sum[t][i], acc[r][t][i]), total[r][t][i]);
-                    }
+                    for (int t = 0; t < T; ++t) acc[r][t] = mfma<XC>(d.x[t][j], b, fresh ? v4f{0, 0, 0, 0} : acc[r][t]);
                 }
             }
+            if (j % GB == GB - 1 && j - (GB - 1) < blocks) {
+                const int g = a.group_of(s * 4 + j - (GB - 1)) - g0;
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const v2f p = sp[g][r * 16 + r16];
+#pragma unroll
+                    for (int t = 0; t < T; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            total[r][t][i] = __fmaf_rn(p[0], acc[r][t][i], __fmaf_rn(p[1], sum[t][i], total[r][t][i]));
+                }
+            }
+            if constexpr (GB < 4) __builtin_amdgcn_sched_barrier(0);  // else every block's scales are read ahead, into scratch
+        }
+    };
+
+    const int steps = (a.k + 127) >> 7;
+    for (int c0 = 0; c0 < steps; c0 += a.chunk) {  // one round unless K has very many groups
+        const int c1 = min(steps, c0 + a.chunk);
+        const int per = (c1 - c0 + W - 1) / W;
+        const int first = c0 + wave * per, last = min(c1, first + per);
+        const int full = min(last, a.k >> 7);
+        int s0 = first;
+        g0 = a.group_of(c0 * 4);
+        const int gn = min(a.groups, a.group_of(c1 * 4 - 1) + 1) - g0;
+        ScaleLoads<XC, R, W> sl;
+        sl.load(a, n0, rows, wave, lane, g0, gn);
+        Step d[U];
+        const bool ahead = s0 + U <= full;
+        if (ahead) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) load(d[u], s0 + u);
+        }
+        if (c0 > 0) __syncthreads();
+        sl.store(a, sp, wave, lane, gn);
+        __syncthreads();
+        if (ahead) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) use(d[u], s0 + u, 4);
+            s0 += U;
+        }
+        for (; s0 + U <= full; s0 += U) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) load(d[u], s0 + u);
+#pragma unroll
+            for (int u = 0; u < U; ++u) use(d[u], s0 + u, 4);
+        }
+        for (; s0 < last; ++s0) {
+            load(d[0], s0);
+            use(d[0], s0, min(4, (a.k >> 5) - s0 * 4));
         }
     }
 
+    __syncthreads();
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -205,16 +287,143 @@ __global__ __launch_bounds__(W * 64) void linear_kernel(LinearArgs a) {
         for (int w = 1; w < W; ++w) v += red[w][slot][l];
         const int row = slot / (4 * T) * 16 + (l & 15);
         const int tok = slot / 4 % T * 16 + (l >> 4) * 4 + (slot & 3);
-        if (row >= rows || tok >= toks) continue;
-        if (a.bias) {
-            const int64_t at = n0 + row;
-            v += a.bias_code == CKH_F32    ? load1<CKH_F32>(a.bias, at)
-                 : a.bias_code == CKH_BF16 ? load1<CKH_BF16>(a.bias, at)
-                                           : load1<CKH_F16>(a.bias, at);
-        }
-        static_cast<uint16_t*>(a.y)[static_cast<int64_t>(m0 + tok) * a.n + n0 + row] =
-            static_cast<uint16_t>(XC == CKH_BF16 ? f_to_bf16_rne(v) : f_to_f16(v));
+        if (row < rows && tok < toks) store_result<XC>(a, m0 + tok, n0 + row, v);
     }
+}
+
+// The same for at most MT = 1, 2 or 4 activation rows, staged in LDS once for the workgroup in the
+// operand's order (lanes of the 16-row operand repeat the MT rows), so that the step reads nothing
+// but codes from memory; a wave keeps D steps of codes in flight.
+template <int XC, int MT, int R, int W, int D, int GB>
+__global__ __launch_bounds__(W * 64, 4) void matvec_kernel(LinearArgs a) {
+    constexpr int kRows = 16 * R;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    v4u* xs = reinterpret_cast<v4u*>(lds);  // [8 codes][row]
+    const int x_bytes = min(a.k, a.chunk * 128) / 8 * MT * 16;
+    v2f(*sp)[kRows + 1] = reinterpret_cast<v2f(*)[kRows + 1]>(lds + x_bytes);  // [group][row]: s, -s (B + z)
+    float(*red)[R * 4][64] = reinterpret_cast<float(*)[R * 4][64]>(lds);
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r16 = lane & 15, quarter = lane >> 4;
+    const int n0 = blockIdx.x * kRows;
+    const int rows = min(kRows, a.n - n0);
+    const int pitch = a.k >> 1;  // code bytes per weight row
+
+    const uint8_t* wbase = a.codes + static_cast<int64_t>(n0) * pitch;
+    const __amdgpu_buffer_rsrc_t rw = buffer_rsrc(wbase, rows * pitch);
+    const __amdgpu_buffer_rsrc_t none = buffer_rsrc(wbase, 0);
+    const __amdgpu_buffer_rsrc_t rx = buffer_rsrc(a.x, static_cast<uint32_t>(((a.m - 1) * a.x_stride + a.k) * 2));
+    constexpr int kAhead = 3;  // activation loads a thread issues before the codes'
+    uint32_t ow[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) ow[r] = min(r * 16 + r16, rows - 1) * pitch + quarter * 16;
+
+    const v4u ones = XC == CKH_BF16 ? v4u{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}
+                                    : v4u{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+
+    v4f total[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) total[r] = v4f{0, 0, 0, 0};
+    int g0 = 0, c0 = 0;  // the staged groups' first, the chunk's first step
+    const auto use = [&](const v4u (&codes)[R], int s, int blocks) {
+        v4f acc[R], sum;
+        v4u w[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) w[r] = transpose_quarters(codes[r]);
+        const v4u* xp = xs + ((s - c0) * 16 + quarter) * MT + (r16 & (MT - 1));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j < blocks) {
+                const bool fresh = j % GB == 0;
+                const v4u x = xp[j * 4 * MT];
+                sum = mfma<XC>(x, ones, fresh ? v4f{0, 0, 0, 0} : sum);
+#pragma unroll
+                for (int r = 0; r < R; ++r) acc[r] = mfma<XC>(x, widen<XC>(w[r][j]), fresh ? v4f{0, 0, 0, 0} : acc[r]);
+            }
+            if (j % GB == GB - 1 && j - (GB - 1) < blocks) {
+                const int g = a.group_of(s * 4 + j - (GB - 1)) - g0;
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const v2f p = sp[g][r * 16 + r16];
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+                        total[r][i] = __fmaf_rn(p[0], acc[r][i], __fmaf_rn(p[1], sum[i], total[r][i]));
+                }
+            }
+            if constexpr (GB < 4) __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+
+    const int steps = (a.k + 127) >> 7;
+    for (; c0 < steps; c0 += a.chunk) {  // one round unless K is very long or has very many groups
+        const int c1 = min(steps, c0 + a.chunk);
+        const int per = (c1 - c0 + W - 1) / W;
+        const int first = c0 + wave * per, last = min(c1, first + per);
+        const int full = min(last, a.k >> 7);
+        v4u w[D][R];
+        const auto load = [&](v4u (&d)[R], int s) {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                d[r] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(s < last ? rw : none, ow[r], s * 64, 0));
+        };
+        // activations and scales first, codes behind them
+        g0 = a.group_of(c0 * 4);
+        const int gn = min(a.groups, a.group_of(c1 * 4 - 1) + 1) - g0;
+        const int units = (min(a.k, c1 * 128) - c0 * 128) >> 3;  // 8 activations each
+        const auto x_at = [&](int e) {
+            const int unit = e / MT, tok = e % MT;
+            return e < units * MT ? static_cast<uint32_t>((min(tok, a.m - 1) * a.x_stride + c0 * 128 + unit * 8) * 2) : 0x80000000u;
+        };
+        v4u xr[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            xr[i] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rx, x_at(threadIdx.x + i * W * 64), 0, 0));
+        ScaleLoads<XC, R, W> sl;
+        sl.load(a, n0, rows, wave, lane, g0, gn);
+#pragma unroll
+        for (int u = 0; u < D; ++u) load(w[u], first + u);
+        if (c0 > 0) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int e = threadIdx.x + i * W * 64;
+            if (e < units * MT) xs[e] = pair_order(xr[i]);
+        }
+        sl.store(a, sp, wave, lane, gn);
+        for (int e = threadIdx.x + kAhead * W * 64; e < units * MT; e += W * 64)
+            xs[e] = pair_order(__builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rx, x_at(e), 0, 0)));
+        __syncthreads();
+        int s0 = first;
+        for (; s0 + D <= full; s0 += D) {
+#pragma unroll
+            for (int u = 0; u < D; ++u) {
+                use(w[u], s0 + u, 4);
+                load(w[u], s0 + u + D);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < D; ++u)
+            if (s0 + u < last) use(w[u], s0 + u, min(4, (a.k >> 5) - (s0 + u) * 4));
+    }
+
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) red[wave][r * 4 + i][lane] = total[r][i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < R * MT * 16; e += W * 64) {
+        const int l = e & 15, i = (e >> 4) % MT, r = (e >> 4) / MT;
+        float v = red[0][r * 4 + i][l];
+#pragma unroll
+        for (int w = 1; w < W; ++w) v += red[w][r * 4 + i][l];
+        if (r * 16 + l < rows && i < a.m) store_result<XC>(a, i, n0 + r * 16 + l, v);
+    }
+}
+
+// Steps of 128 codes that touch at most kScaleGroups groups, wherever the first begins.
+int chunk_steps(int64_t group) {
+    return static_cast<int>((128 % group == 0 ? kScaleGroups : kScaleGroups - 1) * group / 128);
 }
 
 template <int XC, int T, int R, int W, int U>
@@ -228,10 +437,49 @@ void launch_linear(const LinearArgs& a, hipStream_t st) {
         linear_kernel<XC, T, R, W, U, 1><<<grid, W * 64, 0, st>>>(a);
 }
 
+template <int XC, int MT, int R, int W, int D, int GB>
+void launch_matvec(LinearArgs a, hipStream_t st) {
+    a.chunk = std::min(a.chunk, kVecCodes / 128 / (MT > 1 ? 2 : 1));
+    const int codes = std::min(a.k, a.chunk * 128);
+    const int groups = std::min(a.groups, std::min(kScaleGroups, codes / a.group + 2));
+    const size_t lds = std::max<size_t>(codes / 8 * MT * 16 + groups * (16 * R + 1) * 8, W * R * 4 * 64 * 4);
+    matvec_kernel<XC, MT, R, W, D, GB><<<static_cast<unsigned>(cdiv(a.n, 16 * R)), W * 64, lds, st>>>(a);
+}
+
+template <int XC, int MT, int R, int W, int D>
+void launch_matvec(const LinearArgs& a, hipStream_t st) {
+    if (a.group % 128 == 0) launch_matvec<XC, MT, R, W, D, 4>(a, st);
+    else if (a.group % 64 == 0) launch_matvec<XC, MT, R, W, D, 2>(a, st);
+    else launch_matvec<XC, MT, R, W, D, 1>(a, st);
+}
+
+// Tiles and waves by the rows of x and by whether the tiles fill the 256 CUs (us at K = 5120 and
+// N = 13824, groups of 128, unless said; the operands not in cache):
+//   1 row      16 weight rows a workgroup; 4 waves from two workgroups a CU on (11.3; 8 waves 12.5),
+//              else 8 (N = 5120: 6.8; 4 waves 7.3)
+//   2-4 rows   32 weight rows from one workgroup a CU on (14.2; 16 rows 16.3), else, and with groups
+//              under 128 (their scales would not fit the registers), 16
+//   5-16 rows  32 weight rows, 8 waves (16.7; 16 rows 19.9), 16 waves where there are fewer
+//              workgroups than CUs (N = K = 5120, 16 rows: 12.0 against 13.6)
+//   more       64 weight rows, 8 waves (32 rows of x: 23.6; 32 weight rows 29.0), and 32 weight rows,
+//              where 64 leave CUs idle (24 rows, N = 5120, K = 13824: 30.6 against 37)
 template <int XC>
 void linear(const LinearArgs& a, hipStream_t st) {
-    if (a.m <= 16) launch_linear<XC, 1, 1, 8, 2>(a, st);
-    else launch_linear<XC, 2, 1, 8, 1>(a, st);
+    const int cus = device_cus();
+    if (a.m == 1) {
+        if (a.n > 32 * cus) launch_matvec<XC, 1, 1, 4, 2>(a, st);
+        else launch_matvec<XC, 1, 1, 8, 2>(a, st);
+    } else if (a.m <= 4) {
+        if (a.n > 32 * cus && a.group % 128 == 0) launch_matvec<XC, 4, 2, 8, 2, 4>(a, st);
+        else launch_matvec<XC, 4, 1, 8, 2>(a, st);
+    } else if (a.m <= 16) {
+        if (a.n > 32 * cus) launch_linear<XC, 1, 2, 8, 1>(a, st);
+        else launch_linear<XC, 1, 2, 16, 1>(a, st);
+    } else if (static_cast<int64_t>(a.n) * cdiv(a.m, 32) > 48 * cus) {
+        launch_linear<XC, 2, 4, 8, 1>(a, st);
+    } else {
+        launch_linear<XC, 2, 2, 8, 1>(a, st);
+    }
 }
 
 // ------------------------------------------------------------ quantize / dequantize
@@ -385,7 +633,9 @@ extern "C" int ckh_linear_int4(const void* x, const void* codes, const void* sca
     CKH_REQUIRE(x_stride <= (int64_t(1) << 23), "linear_int4: activation row stride too large");
     const i4::LinearArgs a{x, static_cast<const uint8_t*>(codes), scales, static_cast<const uint8_t*>(zeros), bias, y,
                            m == 1 ? k : x_stride, static_cast<int>(m), static_cast<int>(n), static_cast<int>(k),
-                           static_cast<int>(cdiv(k, group)), static_cast<int>(group), scale_code, bias_code};
+                           static_cast<int>(cdiv(k, group)), static_cast<int>(group),
+                           group == 32 ? 0u : static_cast<uint32_t>(cdiv(int64_t(1) << 32, group / 32)),
+                           i4::chunk_steps(group), scale_code, bias_code};
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (x_code == CKH_BF16) i4::linear<CKH_BF16>(a, st);
     else i4::linear<CKH_F16>(a, st);

@@ -53,7 +53,10 @@ def check(y, x, w, scales, group, bias=None):
 # 128, more steps than waves, groups of every alignment, a last group that is shorter
 SHAPES = [(1, 1, 32, 32), (1, 16, 128, 128), (1, 1000, 5120, 128), (2, 33, 160, 64), (3, 77, 416, 96), (15, 50, 4096, 32),
           (16, 129, 1088, 128), (17, 64, 2080, 64), (31, 100, 96, 256), (32, 17, 992, 32), (33, 48, 1312, 160),
-          (48, 250, 640, 128), (64, 31, 2016, 64), (65, 100, 512, 512), (130, 40, 288, 64), (1, 5000, 2048, 64)]
+          (48, 250, 640, 128), (64, 31, 2016, 64), (65, 100, 512, 512), (130, 40, 288, 64), (1, 5000, 2048, 64),
+          # more groups, or more activations, than are staged at a time; wide enough for the other tiles
+          (1, 40, 16416, 32), (3, 40, 16416, 32), (4, 9000, 4256, 128), (2, 9000, 1056, 32), (20, 40, 16416, 32),
+          (1, 20, 36864, 128), (2, 20, 36896, 256), (9, 9000, 544, 64), (40, 9000, 1056, 96)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
