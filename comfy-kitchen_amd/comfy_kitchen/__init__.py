@@ -17,6 +17,7 @@ from .exceptions import (
 )
 from .float_utils import from_blocked, swap_nibbles, to_blocked
 from .ops import DTYPE_TO_CODE, _dispatch, _quantize_fp8_dynamic, direct, untouched
+from .paged import OutOfPages, PagedKVCache
 from .registry import registry
 
 __version__ = "0.1.0"
@@ -35,6 +36,11 @@ __all__ = [
     "quantize_int4",
     "dequantize_int4",
     "linear_int4",
+    "paged_attention",
+    "paged_write",
+    "paged_copy",
+    "PagedKVCache",
+    "OutOfPages",
     "apply_rope",
     "apply_rope1",
     "swap_nibbles",
@@ -227,6 +233,53 @@ def linear_int4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zero
     if type(group_size) is int and direct(x, codes, scales, zeros, bias) and untouched("linear_int4"):
         return _dispatch("linear_int4", x=x, codes=codes, scales=scales, zeros=zeros, bias=bias, group_size=group_size)
     return torch.ops.comfy_kitchen.linear_int4(x, codes, scales, zeros, bias, group_size)
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                    lengths: torch.Tensor, scale: float | None = None, window: int = 0, sinks: int = 0,
+                    k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one new token per sequence, q [B, heads, head_dim] in f16 / bf16, over a cache
+    held in pages; the result has q's shape and dtype.
+
+    k_cache, v_cache: [pages, page_size, kv_heads, head_dim], in q's dtype or as E4M3 codes of
+    value / k_scale, value / v_scale (one-element fp32 tensors; None: 1); any strides that are
+    multiples of 16 bytes with head_dim contiguous, so [pages, kv_heads, page_size, head_dim] is a
+    permuted view away.  heads is a multiple of kv_heads; head_dim 64, 96, 128 or 256.
+    page_table: int32 [B, n]; token t of sequence b is row t % page_size of page
+    page_table[b, t // page_size].  lengths: int32 [B], the tokens of each sequence, the new one
+    (written before the call) among them; a sequence of none gives zeros.
+    window > 0: only the last `window` tokens and the first `sinks` are visible; pages without a
+    visible token are not read and may have been given away.
+    scale: of the scores, head_dim ** -0.5 by default."""
+    if direct(q, k_cache, v_cache, page_table, lengths, k_scale, v_scale) and untouched("paged_attention"):
+        return _dispatch("paged_attention", q=q, k_cache=k_cache, v_cache=v_cache, page_table=page_table,
+                         lengths=lengths, scale=scale, window=window, sinks=sinks, k_scale=k_scale, v_scale=v_scale)
+    return torch.ops.comfy_kitchen.paged_attention(q, k_cache, v_cache, page_table, lengths, scale, window, sinks,
+                                                   k_scale, v_scale)
+
+
+def paged_write(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                slots: torch.Tensor, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> None:
+    """Store the keys and values of new tokens [T, kv_heads, head_dim] (f16 / bf16) in their slots of
+    a cache held in pages, in place: slot page * page_size + row for each token (int32 or int64,
+    on the device; a slot outside the cache, such as -1, skips its token; slots are distinct).
+
+    The caches are [pages, page_size, kv_heads, head_dim] of key's dtype, or E4M3, which take
+    the codes of clamp(x / scale, +-448).  head_dim is a multiple of 16."""
+    if direct(key, value, k_cache, v_cache, slots, k_scale, v_scale) and untouched("paged_write"):
+        return _dispatch("paged_write", key=key, value=value, k_cache=k_cache, v_cache=v_cache, slots=slots,
+                         k_scale=k_scale, v_scale=v_scale)
+    torch.ops.comfy_kitchen.paged_write(key, value, k_cache, v_cache, slots, k_scale, v_scale)
+
+
+def paged_copy(k_cache: torch.Tensor, v_cache: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Copy token rows of a cache held in pages from slots src to slots dst (int32 or int64, on the
+    device), in place, in K and V: [pages, page_size, kv_heads, head_dim], or of all layers at
+    once with a leading dimension.  No slot of dst may be in src; pairs with a slot outside the
+    cache are skipped."""
+    if direct(k_cache, v_cache, src, dst) and untouched("paged_copy"):
+        return _dispatch("paged_copy", k_cache=k_cache, v_cache=v_cache, src=src, dst=dst)
+    torch.ops.comfy_kitchen.paged_copy(k_cache, v_cache, src, dst)
 
 
 def apply_rope(xq: torch.Tensor, xk: torch.Tensor,

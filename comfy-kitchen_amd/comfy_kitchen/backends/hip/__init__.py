@@ -33,6 +33,9 @@ __all__ = [
     "dequantize_nvfp4",
     "dequantize_per_tensor_fp8",
     "linear_int4",
+    "paged_attention",
+    "paged_copy",
+    "paged_write",
     "quantize_fp8_dynamic",
     "quantize_int4",
     "quantize_mxfp8",
@@ -73,6 +76,10 @@ SIGNATURES: dict[str, tuple] = {
     "ckh_quantize_int4": (_i32, [_p] * 3 + [_i64] * 3 + [_i32, _u64]),
     "ckh_dequantize_int4": (_i32, [_p] * 4 + [_i64] * 3 + [_i32, _i32, _u64]),
     "ckh_linear_int4": (_i32, [_p] * 6 + [_i64] * 5 + [_i32] * 3 + [_u64]),
+    "ckh_paged_attention_workspace_bytes": (_i64, [_i64] * 6),
+    "ckh_paged_attention": (_i32, [_p] * 8 + [_i64] * 8 + [_p] + [_i64] * 2 + [_f32, _i32, _i32, _p, _i64, _u64]),
+    "ckh_paged_write": (_i32, [_p] * 7 + [_i64] * 5 + [_p] + [_i32] * 3 + [_u64]),
+    "ckh_paged_copy": (_i32, [_p] * 4 + [_i64] * 6 + [_p] + [_i32] * 2 + [_u64]),
 }
 ABI_VERSION = 8
 # CKH_AMAX_WORKSPACE_BYTES of include/ckh.h: the workspace ckh_amax_scale takes
@@ -469,6 +476,121 @@ def linear_int4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zero
     return out
 
 
+# -------------------------------------------------------- key-value cache held in pages
+def _strides(*values: int):
+    return (_i64 * len(values))(*values)
+
+
+def _cache_pair(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
+    """What every call asks of the two caches: one shape and dtype, rows that 16-byte pieces fit.
+    They are used in place, so nothing is copied to fit."""
+    if k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
+        raise ValueError(f"{name}: k_cache {list(k_cache.shape)} {k_cache.dtype} and v_cache {list(v_cache.shape)} "
+                         f"{v_cache.dtype} differ")
+    size = k_cache.element_size()
+    for t in (k_cache, v_cache):
+        if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s * size % 16 for s in t.stride()[:-1]):
+            raise ValueError(f"{name}: a cache of strides {t.stride()} is not 16-byte aligned with head_dim contiguous")
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """t, its last dimension contiguous and its rows on 16-byte boundaries (copied where they are not)."""
+    stride, size = t.stride(), t.element_size()
+    if stride[-1] == 1 and not t.data_ptr() % 16 and not any(s * size % 16 for s in stride[:-1]):
+        return t
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+@functools.lru_cache(maxsize=256)
+def _paged_workspace_bytes(*sizes: int) -> int:
+    return int(_lib.ckh_paged_attention_workspace_bytes(*sizes))
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                    lengths: torch.Tensor, scale: float | None = None, window: int = 0, sinks: int = 0,
+                    k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> torch.Tensor:
+    _same_device("paged_attention", q, k_cache, v_cache, page_table, lengths)
+    _cache_pair("paged_attention", k_cache, v_cache)
+    batch, heads, dim = q.shape
+    pages, page_size, kv_heads, cache_dim = k_cache.shape
+    if dim != cache_dim or kv_heads == 0 or heads % kv_heads:
+        raise ValueError(f"paged_attention: q {list(q.shape)} does not fit a cache of {kv_heads} heads of {cache_dim}")
+    if dim not in (64, 96, 128, 256):
+        raise ValueError(f"paged_attention: head_dim {dim} is not 64, 96, 128 or 256")
+    if k_cache.dtype not in (q.dtype, torch.float8_e4m3fn):
+        raise ValueError(f"paged_attention: a cache of {k_cache.dtype} with queries of {q.dtype}")
+    if page_table.shape[0] != batch or lengths.shape[0] != batch:
+        raise ValueError(f"paged_attention: page_table {list(page_table.shape)} and lengths {list(lengths.shape)} "
+                         f"for {batch} sequences")
+    if window < 0 or sinks < 0:
+        raise ValueError(f"paged_attention: window ({window}) and sinks ({sinks}) must not be negative")
+    q = _rows16(q)
+    if page_table.stride(1) != 1 and page_table.shape[1] > 1:
+        page_table = page_table.contiguous()
+    lengths = lengths.contiguous()
+    if k_scale is not None:
+        k_scale = _scalar_on(k_scale, q.device, "k_scale")
+    if v_scale is not None:
+        v_scale = _scalar_on(v_scale, q.device, "v_scale")
+    out = torch.empty((batch, heads, dim), dtype=q.dtype, device=q.device)
+    max_pages = page_table.shape[1]
+    nbytes = _paged_workspace_bytes(batch, heads, kv_heads, dim, page_size, max_pages)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _launch("ckh_paged_attention", q, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(),
+            lengths.data_ptr(), _ptr(k_scale), _ptr(v_scale), out.data_ptr(), batch, heads, kv_heads, dim, pages,
+            page_size, max_pages, page_table.stride(0),
+            _strides(q.stride(0), q.stride(1), *k_cache.stride()[:3], *v_cache.stride()[:3]), window, sinks,
+            dim ** -0.5 if scale is None else scale, DTYPE_TO_CODE[q.dtype], DTYPE_TO_CODE[k_cache.dtype], _ptr(ws), nbytes)
+    return out
+
+
+def paged_write(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                slots: torch.Tensor, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> None:
+    _same_device("paged_write", key, value, k_cache, v_cache, slots)
+    _cache_pair("paged_write", k_cache, v_cache)
+    tokens, kv_heads, dim = key.shape
+    pages, page_size = k_cache.shape[:2]
+    if value.shape != key.shape or value.dtype != key.dtype or k_cache.shape[2:] != key.shape[1:]:
+        raise ValueError(f"paged_write: key {list(key.shape)} {key.dtype}, value {list(value.shape)} {value.dtype} and "
+                         f"a cache {list(k_cache.shape)} do not fit")
+    if k_cache.dtype not in (key.dtype, torch.float8_e4m3fn):
+        raise ValueError(f"paged_write: {key.dtype} into a cache of {k_cache.dtype}")
+    if dim % 16:
+        raise ValueError(f"paged_write: head_dim {dim} is not a multiple of 16")
+    if slots.shape[0] != tokens:
+        raise ValueError(f"paged_write: {slots.shape[0]} slots for {tokens} tokens")
+    key, value, slots = _rows16(key), _rows16(value), slots.contiguous()
+    if k_scale is not None:
+        k_scale = _scalar_on(k_scale, key.device, "k_scale")
+    if v_scale is not None:
+        v_scale = _scalar_on(v_scale, key.device, "v_scale")
+    _launch("ckh_paged_write", key, key.data_ptr(), value.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            slots.data_ptr(), _ptr(k_scale), _ptr(v_scale), tokens, kv_heads, dim, pages, page_size,
+            _strides(*key.stride()[:2], *value.stride()[:2], *k_cache.stride()[:3], *v_cache.stride()[:3]),
+            DTYPE_TO_CODE[key.dtype], DTYPE_TO_CODE[k_cache.dtype], int(slots.dtype == torch.int64))
+
+
+def paged_copy(k_cache: torch.Tensor, v_cache: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
+    _same_device("paged_copy", k_cache, v_cache, src, dst)
+    _cache_pair("paged_copy", k_cache, v_cache)
+    if k_cache.dim() not in (4, 5):
+        raise ValueError(f"paged_copy: a cache has 4 dimensions, or 5 with the layers first, got {k_cache.dim()}")
+    if src.shape != dst.shape or src.dtype != dst.dtype:
+        raise ValueError(f"paged_copy: src {list(src.shape)} {src.dtype} and dst {list(dst.shape)} {dst.dtype} differ")
+    layers = k_cache.shape[0] if k_cache.dim() == 5 else 1
+    pages, page_size, kv_heads, dim = k_cache.shape[-4:]
+    if dim * k_cache.element_size() % 16:
+        raise ValueError(f"paged_copy: a head of {dim} elements is not a multiple of 16 bytes")
+    src, dst = src.contiguous(), dst.contiguous()
+    ks, vs = k_cache.stride(), v_cache.stride()
+    if layers == 1:
+        ks, vs = (0, *ks[-4:]), (0, *vs[-4:])
+    _launch("ckh_paged_copy", k_cache, k_cache.data_ptr(), v_cache.data_ptr(), src.data_ptr(), dst.data_ptr(), layers,
+            src.shape[0], kv_heads, dim, pages, page_size, _strides(*ks[:4], *vs[:4]), k_cache.element_size(),
+            int(src.dtype == torch.int64))
+
+
 # ----------------------------------------------------------------------------- RoPE
 def _rope_call(xq: torch.Tensor, xk: torch.Tensor | None, freqs_cis: torch.Tensor):
     if xq.dim() != 4 or freqs_cis.dim() != 6:
@@ -514,6 +636,8 @@ def _build_constraints() -> dict:
     fp8 = frozenset({torch.float8_e4m3fn, torch.float8_e5m2})
     f32 = frozenset({torch.float32})
     u8 = frozenset({torch.uint8})
+    i32, ints = frozenset({torch.int32}), frozenset({torch.int32, torch.int64})
+    e4m3 = frozenset({torch.float8_e4m3fn})
 
     def fc(**params):
         return FunctionConstraints(params=params, default_devices=dev, required_arch=REQUIRED_ARCH)
@@ -575,6 +699,24 @@ def _build_constraints() -> dict:
                           scales=ParamConstraint(dtypes=floats, shape_rules=two_d),
                           zeros=ParamConstraint(dtypes=u8, shape_rules=two_d),
                           bias=ParamConstraint(dtypes=floats)),
+        "paged_attention": fc(q=ParamConstraint(dtypes=half, shape_rules=(ExactDims(3),)),
+                              k_cache=ParamConstraint(dtypes=half | e4m3, shape_rules=(ExactDims(4),)),
+                              v_cache=ParamConstraint(dtypes=half | e4m3, shape_rules=(ExactDims(4),)),
+                              page_table=ParamConstraint(dtypes=i32, shape_rules=two_d),
+                              lengths=ParamConstraint(dtypes=i32, shape_rules=(ExactDims(1),)),
+                              k_scale=ParamConstraint(dtypes=f32, devices=frozenset({"cuda", "cpu"})),
+                              v_scale=ParamConstraint(dtypes=f32, devices=frozenset({"cuda", "cpu"}))),
+        "paged_write": fc(key=ParamConstraint(dtypes=half, shape_rules=(ExactDims(3),)),
+                          value=ParamConstraint(dtypes=half, shape_rules=(ExactDims(3),)),
+                          k_cache=ParamConstraint(dtypes=half | e4m3, shape_rules=(ExactDims(4),)),
+                          v_cache=ParamConstraint(dtypes=half | e4m3, shape_rules=(ExactDims(4),)),
+                          slots=ParamConstraint(dtypes=ints, shape_rules=(ExactDims(1),)),
+                          k_scale=ParamConstraint(dtypes=f32, devices=frozenset({"cuda", "cpu"})),
+                          v_scale=ParamConstraint(dtypes=f32, devices=frozenset({"cuda", "cpu"}))),
+        "paged_copy": fc(k_cache=ParamConstraint(dtypes=half | e4m3, shape_rules=(MinDims(4),)),
+                         v_cache=ParamConstraint(dtypes=half | e4m3, shape_rules=(MinDims(4),)),
+                         src=ParamConstraint(dtypes=ints, shape_rules=(ExactDims(1),)),
+                         dst=ParamConstraint(dtypes=ints, shape_rules=(ExactDims(1),))),
         "apply_rope1": fc(x=ParamConstraint(dtypes=floats, shape_rules=(ExactDims(4),)),
                           freqs_cis=ParamConstraint(dtypes=floats, shape_rules=(ExactDims(6),))),
         "apply_rope": fc(xq=ParamConstraint(dtypes=floats, shape_rules=(ExactDims(4),)),

@@ -306,6 +306,42 @@ def _(x, codes, scales, zeros, bias, group_size):
     return x.new_empty((*x.shape[:-1], codes.shape[0]))
 
 
+# ------------------------------------------------- key-value cache held in pages
+@torch.library.custom_op("comfy_kitchen::paged_attention", mutates_args=())
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                    lengths: torch.Tensor, scale: float | None, window: int, sinks: int,
+                    k_scale: torch.Tensor | None, v_scale: torch.Tensor | None) -> torch.Tensor:
+    return _dispatch("paged_attention", q=q, k_cache=k_cache, v_cache=v_cache, page_table=page_table, lengths=lengths,
+                     scale=scale, window=window, sinks=sinks, k_scale=k_scale, v_scale=v_scale)
+
+
+@paged_attention.register_fake
+def _(q, k_cache, v_cache, page_table, lengths, scale, window, sinks, k_scale, v_scale):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("comfy_kitchen::paged_write", mutates_args=("k_cache", "v_cache"))
+def paged_write(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                slots: torch.Tensor, k_scale: torch.Tensor | None, v_scale: torch.Tensor | None) -> None:
+    _dispatch("paged_write", key=key, value=value, k_cache=k_cache, v_cache=v_cache, slots=slots, k_scale=k_scale,
+              v_scale=v_scale)
+
+
+@paged_write.register_fake
+def _(key, value, k_cache, v_cache, slots, k_scale, v_scale):
+    return None
+
+
+@torch.library.custom_op("comfy_kitchen::paged_copy", mutates_args=("k_cache", "v_cache"))
+def paged_copy(k_cache: torch.Tensor, v_cache: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
+    _dispatch("paged_copy", k_cache=k_cache, v_cache=v_cache, src=src, dst=dst)
+
+
+@paged_copy.register_fake
+def _(k_cache, v_cache, src, dst):
+    return None
+
+
 # ------------------------------------------------------------------------- RoPE
 @torch.library.custom_op("comfy_kitchen::apply_rope", mutates_args=())
 def apply_rope(xq: torch.Tensor, xk: torch.Tensor, freqs_cis: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:

@@ -312,6 +312,47 @@ int ckh_linear_int4(const void* x, const void* codes, const void* scales, const 
                     void* y, int64_t m, int64_t n, int64_t k, int64_t x_stride, int64_t group, int x_code,
                     int scale_code, int bias_code, uintptr_t stream);
 
+/*
+ * A key-value cache held in pages: K and V are [pages, page_size, kv_heads, dim] of cache_code with
+ * any strides (elements; 16-byte multiples, the last dimension contiguous), 16-byte aligned.  Token
+ * t of a sequence is row t % page_size of page table[t / page_size]; a slot is page * page_size + row
+ * (int32, or int64 where wide_slots != 0), and slots outside the cache are skipped.
+ *
+ * ckh_paged_attention: one query token per sequence.  out[b, h] = softmax(scale q[b, h] K^T) V over
+ * sequence b's visible tokens: its lengths[b] tokens (int32, taken into 0 .. max_pages * page_size),
+ * or with window > 0 its last `window` and its first `sinks`.  q [batch, heads, dim] and out
+ * (contiguous) of q_code (f16/bf16); cache_code the same, or e4m3 with values code * *k_scale,
+ * code * *v_scale (device f32, NULL: 1).  heads % kv_heads == 0; dim 64, 96, 128 or 256.  Query head h
+ * reads key-value head h / (heads / kv_heads).  A sequence without visible tokens gives zeros.
+ * page_table: int32 [batch, max_pages], table_stride elements a row; entries that no visible token
+ * needs are not read, others outside 0 .. pages-1 are read as the last page.
+ * strides: q batch, head; k page, token, head; v page, token, head.
+ * The workspace of ckh_paged_attention_workspace_bytes lets long sequences be split (0: never
+ * split); with NULL or a short one every sequence is read by one workgroup per key-value head.
+ *
+ * ckh_paged_write: key, value [tokens, kv_heads, dim] of x_code (f16/bf16) to slots[tokens] of K and
+ * V, as they are (cache_code == x_code) or as e4m3 codes of clamp(x / *scale, +-448).  dim % 16 == 0.
+ * strides: key token, head; value token, head; k page, token, head; v page, token, head.
+ *
+ * ckh_paged_copy: rows src[i] to dst[i], i < rows, of K and V in each of `layers` caches; no slot of
+ * dst may be in src.  strides: k layer, page, token, head; v layer, page, token, head.
+ */
+int64_t ckh_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim,
+                                            int64_t page_size, int64_t max_pages);
+int ckh_paged_attention(const void* q, const void* k_cache, const void* v_cache, const void* page_table,
+                        const void* lengths, const void* k_scale, const void* v_scale, void* out, int64_t batch,
+                        int64_t heads, int64_t kv_heads, int64_t dim, int64_t pages, int64_t page_size,
+                        int64_t max_pages, int64_t table_stride, const int64_t* strides, int64_t window,
+                        int64_t sinks, float scale, int q_code, int cache_code, void* workspace,
+                        int64_t workspace_bytes, uintptr_t stream);
+int ckh_paged_write(const void* key, const void* value, void* k_cache, void* v_cache, const void* slots,
+                    const void* k_scale, const void* v_scale, int64_t tokens, int64_t kv_heads, int64_t dim,
+                    int64_t pages, int64_t page_size, const int64_t* strides, int x_code, int cache_code,
+                    int wide_slots, uintptr_t stream);
+int ckh_paged_copy(void* k_cache, void* v_cache, const void* src, const void* dst, int64_t layers, int64_t rows,
+                   int64_t kv_heads, int64_t dim, int64_t pages, int64_t page_size, const int64_t* strides,
+                   int element_bytes, int wide_slots, uintptr_t stream);
+
 #ifdef __cplusplus
 }
 #endif
