@@ -39,6 +39,7 @@ __all__ = [
     "paged_attention",
     "paged_write",
     "paged_copy",
+    "window_attention",
     "PagedKVCache",
     "OutOfPages",
     "apply_rope",
@@ -280,6 +281,24 @@ def paged_copy(k_cache: torch.Tensor, v_cache: torch.Tensor, src: torch.Tensor, 
     if direct(k_cache, v_cache, src, dst) and untouched("paged_copy"):
         return _dispatch("paged_copy", k_cache=k_cache, v_cache=v_cache, src=src, dst=dst)
     torch.ops.comfy_kitchen.paged_copy(k_cache, v_cache, src, dst)
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int = 0, sinks: int = 0,
+                     lengths: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
+    """Causal attention of prompts: q [B, queries, heads, head_dim], k and v [B, keys, kv_heads,
+    head_dim] in one of f16 / bf16; the result has q's shape and dtype.
+
+    Query i stands at position i + keys - queries (the last query at the last key, so k and v may
+    begin with tokens of earlier calls) and sees the keys up to its position: with window > 0 the
+    last `window` of them, and in any case the first `sinks` keys of the sequence.  lengths:
+    int32 [B], keys of each sequence where the batch is padded behind (keys past them are not
+    seen).  A query that sees nothing gives zeros.
+    heads is a multiple of kv_heads; head_dim 64, 96, 128 or 256.  Any strides with head_dim
+    contiguous are taken ([B, heads, tokens, head_dim] is a transposed view away); tensors whose
+    rows are not on 16-byte boundaries are copied.  scale: of the scores, head_dim ** -0.5 by default."""
+    if direct(q, k, v, lengths) and untouched("window_attention"):
+        return _dispatch("window_attention", q=q, k=k, v=v, window=window, sinks=sinks, lengths=lengths, scale=scale)
+    return torch.ops.comfy_kitchen.window_attention(q, k, v, window, sinks, lengths, scale)
 
 
 def apply_rope(xq: torch.Tensor, xk: torch.Tensor,

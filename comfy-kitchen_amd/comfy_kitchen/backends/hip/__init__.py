@@ -45,6 +45,7 @@ __all__ = [
     "scaled_mm_fp8",
     "scaled_mm_mxfp8",
     "scaled_mm_nvfp4",
+    "window_attention",
 ]
 
 LIB_PATH = Path(os.environ.get("CKH_LIBRARY", Path(__file__).with_name("libckh.so")))
@@ -80,6 +81,7 @@ SIGNATURES: dict[str, tuple] = {
     "ckh_paged_attention": (_i32, [_p] * 8 + [_i64] * 8 + [_p] + [_i64] * 2 + [_f32, _i32, _i32, _p, _i64, _u64]),
     "ckh_paged_write": (_i32, [_p] * 7 + [_i64] * 5 + [_p] + [_i32] * 3 + [_u64]),
     "ckh_paged_copy": (_i32, [_p] * 4 + [_i64] * 6 + [_p] + [_i32] * 2 + [_u64]),
+    "ckh_window_attention": (_i32, [_p] * 5 + [_i64] * 6 + [_p] + [_i64] * 2 + [_f32, _i32, _u64]),
 }
 ABI_VERSION = 8
 # CKH_AMAX_WORKSPACE_BYTES of include/ckh.h: the workspace ckh_amax_scale takes
@@ -591,6 +593,34 @@ def paged_copy(k_cache: torch.Tensor, v_cache: torch.Tensor, src: torch.Tensor, 
             int(src.dtype == torch.int64))
 
 
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int = 0, sinks: int = 0,
+                     lengths: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
+    _same_device("window_attention", q, k, v, lengths)
+    batch, queries, heads, dim = q.shape
+    keys, kv_heads = k.shape[1:3]
+    if k.shape != v.shape or k.shape[0] != batch or k.shape[3] != dim or kv_heads == 0 or heads % kv_heads:
+        raise ValueError(f"window_attention: q {list(q.shape)}, k {list(k.shape)} and v {list(v.shape)} do not fit")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"window_attention: q, k and v of different dtypes ({q.dtype}, {k.dtype}, {v.dtype})")
+    if dim not in (64, 96, 128, 256):
+        raise ValueError(f"window_attention: head_dim {dim} is not 64, 96, 128 or 256")
+    if window < 0 or sinks < 0:
+        raise ValueError(f"window_attention: window ({window}) and sinks ({sinks}) must not be negative")
+    if lengths is not None:
+        if lengths.shape[0] != batch:
+            raise ValueError(f"window_attention: {lengths.shape[0]} lengths for a batch of {batch}")
+        lengths = lengths.contiguous()
+    q, k, v = _rows16(q), _rows16(k), _rows16(v)
+    if keys > 1:  # broadcast keys have no rows of their own
+        k = k.contiguous() if k.stride(1) < dim else k
+        v = v.contiguous() if v.stride(1) < dim else v
+    out = torch.empty((batch, queries, heads, dim), dtype=q.dtype, device=q.device)
+    _launch("ckh_window_attention", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(lengths), out.data_ptr(), batch,
+            queries, keys, heads, kv_heads, dim, _strides(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]), window, sinks,
+            dim ** -0.5 if scale is None else scale, DTYPE_TO_CODE[q.dtype])
+    return out
+
+
 # ----------------------------------------------------------------------------- RoPE
 def _rope_call(xq: torch.Tensor, xk: torch.Tensor | None, freqs_cis: torch.Tensor):
     if xq.dim() != 4 or freqs_cis.dim() != 6:
@@ -717,6 +747,10 @@ def _build_constraints() -> dict:
                          v_cache=ParamConstraint(dtypes=half | e4m3, shape_rules=(MinDims(4),)),
                          src=ParamConstraint(dtypes=ints, shape_rules=(ExactDims(1),)),
                          dst=ParamConstraint(dtypes=ints, shape_rules=(ExactDims(1),))),
+        "window_attention": fc(q=ParamConstraint(dtypes=half, shape_rules=(ExactDims(4),)),
+                               k=ParamConstraint(dtypes=half, shape_rules=(ExactDims(4),)),
+                               v=ParamConstraint(dtypes=half, shape_rules=(ExactDims(4),)),
+                               lengths=ParamConstraint(dtypes=i32, shape_rules=(ExactDims(1),))),
         "apply_rope1": fc(x=ParamConstraint(dtypes=floats, shape_rules=(ExactDims(4),)),
                           freqs_cis=ParamConstraint(dtypes=floats, shape_rules=(ExactDims(6),))),
         "apply_rope": fc(xq=ParamConstraint(dtypes=floats, shape_rules=(ExactDims(4),)),

@@ -342,6 +342,17 @@ def _(k_cache, v_cache, src, dst):
     return None
 
 
+@torch.library.custom_op("comfy_kitchen::window_attention", mutates_args=())
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int,
+                     lengths: torch.Tensor | None, scale: float | None) -> torch.Tensor:
+    return _dispatch("window_attention", q=q, k=k, v=v, window=window, sinks=sinks, lengths=lengths, scale=scale)
+
+
+@window_attention.register_fake
+def _(q, k, v, window, sinks, lengths, scale):
+    return q.new_empty(q.shape)
+
+
 # ------------------------------------------------------------------------- RoPE
 @torch.library.custom_op("comfy_kitchen::apply_rope", mutates_args=())
 def apply_rope(xq: torch.Tensor, xk: torch.Tensor, freqs_cis: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:

@@ -353,6 +353,20 @@ int ckh_paged_copy(void* k_cache, void* v_cache, const void* src, const void* ds
                    int64_t kv_heads, int64_t dim, int64_t pages, int64_t page_size, const int64_t* strides,
                    int element_bytes, int wide_slots, uintptr_t stream);
 
+/*
+ * Causal attention of prompts with a sliding window and sinks.  q [batch, queries, heads, dim],
+ * k, v [batch, keys, kv_heads, dim] of one code (f16/bf16) with any strides (elements; 16-byte
+ * multiples, the last dimension contiguous); out contiguous, of q's shape.  Query i stands at
+ * position p = i + keys - queries and sees key j if j <= p, j < lengths[batch] (int32; NULL: all
+ * keys), and p - j < window or j < sinks; window 0: no window.  A query that sees nothing gives
+ * zeros.  What a pair that is not visible holds has no influence, infinities and NaN included.
+ * heads % kv_heads == 0; dim 64, 96, 128 or 256.  strides: q, k, v: batch, token, head each.
+ */
+int ckh_window_attention(const void* q, const void* k, const void* v, const void* lengths, void* out, int64_t batch,
+                         int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim,
+                         const int64_t* strides, int64_t window, int64_t sinks, float scale, int code,
+                         uintptr_t stream);
+
 #ifdef __cplusplus
 }
 #endif
