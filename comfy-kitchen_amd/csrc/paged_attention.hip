@@ -40,7 +40,8 @@ struct PagedArgs {
     const int* lengths;
     const float *k_scale, *v_scale;  // null: 1
     void* out;
-    float* part;  // [slot][16][D + 2]: unnormalised output, maximum, sum
+    float* part;  // [chunk][16][D + 2]: unnormalised output, maximum, sum
+    int2* plan;   // [unit]: its first chunk, its chunks (null: one each)
     int64_t q_b, q_h, k_page, k_tok, k_head, v_page, v_tok, v_head;  // strides in elements
     int64_t table_stride;
     int batch, heads, kv_heads, group, head_tiles;  // group: query heads of a key-value head
@@ -72,57 +73,50 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
 }
 
 // Chunks.  A unit is a sequence, a key-value head and 16 of its query heads; a unit's tiles go in
-// chunks of `size`; chunks are numbered sequence by sequence, unit by unit.
-struct Schedule {
-    int size;   // tiles per chunk
-    int units;  // units per sequence
-    __device__ __forceinline__ Schedule(const PagedArgs& a, int lane) {
-        units = a.kv_heads * a.head_tiles;
-        int64_t total = 0;
-        for (int i = 0; i < a.batch; i += 64) {
-            const int n = i + lane < a.batch ? Visible(a, a.lengths[i + lane]).tiles : 0;
-            total += __shfl(wave_scan(n, lane), 63, 64);
-        }
-        const int64_t want = (total * units + a.target - 1) / a.target;
-        size = static_cast<int>(min(max(want, static_cast<int64_t>(kMinTiles)), static_cast<int64_t>(1) << 30));
-    }
-    __device__ __forceinline__ int chunks(int tiles) const { return max(1, (tiles + size - 1) / size); }
-    // The sequence, unit and chunk of number `at`, and the number of the unit's first chunk;
-    // b = -1 past the end.
-    struct Place {
-        int b, unit, chunk, count;
-    };
-    __device__ __forceinline__ Place find(const PagedArgs& a, int at, int lane) const {
-        int before = 0;
-        for (int i = 0; i < a.batch; i += 64) {
-            const int per = i + lane < a.batch ? chunks(Visible(a, a.lengths[i + lane]).tiles) : 0;
-            const int end = before + wave_scan(per * units, lane);
-            const uint64_t past = __ballot(end > at);
-            if (past) {
-                const int l = __builtin_ctzll(past);
-                const int count = __builtin_amdgcn_readlane(per, l);
-                const int in = at - (__builtin_amdgcn_readlane(end, l) - count * units);
-                return {i + l, in / count, in % count, count};
-            }
-            before = __builtin_amdgcn_readlane(end, 63);
-        }
-        return {-1, 0, 0, 0};
-    }
-    // The number of sequence b's first chunk and its chunks per unit.
-    __device__ __forceinline__ void of(const PagedArgs& a, int b, int lane, int& first, int& count) const {
-        first = count = 0;
-        for (int i = 0; i <= b; i += 64) {
-            const int per = i + lane < a.batch ? chunks(Visible(a, a.lengths[i + lane]).tiles) : 0;
-            const int end = wave_scan(per * units, lane);
-            if (b < i + 64) {
-                count = __builtin_amdgcn_readlane(per, b - i);
-                first += __builtin_amdgcn_readlane(end, b - i) - count * units;
-            } else {
-                first += __builtin_amdgcn_readlane(end, 63);
-            }
-        }
-    }
+// chunks of one size, chosen so that there are about `target` chunks.  Chunks are numbered sequence by
+// sequence, then chunk by chunk, then unit by unit: workgroups that run together then read the
+// heads of the same tokens, which lie next to each other in memory.
+struct Place {
+    int b, unit, chunk, count;  // count: chunks of each of the sequence's units; b -1: no such chunk
+    int length, size;           // of the sequence; tiles of a chunk
 };
+__device__ __forceinline__ Place find_chunk(const PagedArgs& a, int at, int units, int lane) {
+    Place p{-1, 0, 0, 1, 0, 1 << 30};
+    if (a.target == 1) {  // every unit is one chunk
+        p.b = at / units;
+        p.unit = at - p.b * units;
+        p.length = a.lengths[p.b];
+        return p;
+    }
+    // the lane's sequences: the first 64 stay in registers
+    const int length = lane < a.batch ? a.lengths[lane] : 0;
+    const int tiles = lane < a.batch ? Visible(a, length).tiles : 0;
+    int64_t total = __shfl(wave_scan(tiles, lane), 63, 64);
+    for (int i = 64; i < a.batch; i += 64)
+        total += __shfl(wave_scan(i + lane < a.batch ? Visible(a, a.lengths[i + lane]).tiles : 0, lane), 63, 64);
+    const int64_t want = (total * units + a.target - 1) / a.target;
+    p.size = static_cast<int>(min(max(want, static_cast<int64_t>(kMinTiles)), static_cast<int64_t>(1) << 30));
+    int before = 0;
+    for (int i = 0; i < a.batch; i += 64) {
+        const int n = i == 0 ? length : i + lane < a.batch ? a.lengths[i + lane] : 0;
+        const int t = i == 0 ? tiles : Visible(a, n).tiles;
+        const int per = i + lane < a.batch ? max(1, (t + p.size - 1) / p.size) : 0;
+        const int end = before + wave_scan(per * units, lane);
+        const uint64_t past = __ballot(end > at);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            p.b = i + l;
+            p.count = __builtin_amdgcn_readlane(per, l);
+            p.length = __builtin_amdgcn_readlane(n, l);
+            const int in = at - (__builtin_amdgcn_readlane(end, l) - p.count * units);
+            p.chunk = in / units;
+            p.unit = in - p.chunk * units;
+            return p;
+        }
+        before = __builtin_amdgcn_readlane(end, 63);
+    }
+    return p;
+}
 
 // How a lane holds D dims of K and V.
 template <int D, bool F8>
@@ -180,14 +174,15 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void paged_kernel(Pa
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, c = lane >> 4;
 
-    const Schedule plan(a, lane);
-    const Schedule::Place place = plan.find(a, blockIdx.x, lane);
+    const int units = a.kv_heads * a.head_tiles;
+    const Place place = find_chunk(a, blockIdx.x, units, lane);
     if (place.b < 0) return;  // the whole workgroup
     const int b = __builtin_amdgcn_readfirstlane(place.b), unit = __builtin_amdgcn_readfirstlane(place.unit);
     const int kvh = unit / a.head_tiles, h0 = (unit - kvh * a.head_tiles) * 16;
     const int nh = min(16, a.group - h0);  // query heads of this unit
-    const Visible vis(a, a.lengths[b]);
-    const int t0 = place.chunk * plan.size, t1 = min(vis.tiles, t0 + plan.size);
+    const Visible vis(a, __builtin_amdgcn_readfirstlane(place.length));
+    const int size = __builtin_amdgcn_readfirstlane(place.size);
+    const int t0 = __builtin_amdgcn_readfirstlane(place.chunk) * size, t1 = min(vis.tiles, t0 + size);
     const int* table = a.table + b * a.table_stride;
 
     v4u q[D / 32];
@@ -403,6 +398,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void paged_kernel(Pa
                 for (int i = 0; i < 4; ++i) lo[wave][L::base(st) + (4 * c + i) * L::width(st) + e][r16] = acc[n][i];
     }
     __syncthreads();
+    if (a.plan && place.chunk == 0 && threadIdx.x == 0) a.plan[b * units + unit] = make_int2(blockIdx.x, place.count);
     const float vs = a.v_scale ? *a.v_scale : 1.0f;
     for (int e = threadIdx.x; e < nh * D; e += kWaves * 64) {
         const int h = e / D, d = e % D;
@@ -431,45 +427,55 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void paged_kernel(Pa
     }
 }
 
-// Joins the chunks of the sequences that have several: a workgroup per sequence and query head,
-// in chunk order.
+// Joins the chunks of the sequences that have several: a workgroup per sequence and query head.
+// The chunks' factors go to LDS first, so that their outputs are read without waiting for them.
 template <int QC, int D>
 __global__ __launch_bounds__(256) void join_kernel(PagedArgs a) {
-    constexpr int N = 256 / D;  // chunks taken at a time
-    __shared__ float so[N][D], ss[N];
-    const int lane = threadIdx.x & 63;
+    constexpr int N = 256 / D;    // chunks taken at a time
+    constexpr int kAtOnce = 1024;  // chunks whose factors LDS holds
+    __shared__ float so[N][D], factor[kAtOnce], red[8];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int b = blockIdx.y, h = blockIdx.x;
-    const Schedule plan(a, lane);
-    int first, count;
-    plan.of(a, b, lane, first, count);
-    if (count == 1) return;
+    const int units = a.kv_heads * a.head_tiles;
     const int kvh = h / a.group, in = h - kvh * a.group;
-    first += (kvh * a.head_tiles + (in >> 4)) * count;
-    const float* part = a.part + (static_cast<int64_t>(first) * 16 + (in & 15)) * (D + 2);
-    const int64_t step = 16 * (D + 2);
+    const int2 plan = a.plan[b * units + kvh * a.head_tiles + (in >> 4)];
+    const int count = plan.y;
+    if (count == 1) return;
+    const float* part = a.part + (static_cast<int64_t>(plan.x) * 16 + (in & 15)) * (D + 2);
+    const int64_t step = static_cast<int64_t>(units) * 16 * (D + 2);
     float top = -1e30f;
-    for (int i = lane; i < count; i += 64) top = fmaxf(top, part[i * step + D]);
+    for (int i = threadIdx.x; i < count; i += 256) top = fmaxf(top, part[i * step + D]);
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
+    if (lane == 0) red[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     const int d = threadIdx.x % D, g = threadIdx.x / D;
-    if (g < N) {
-        float o = 0.0f, sum = 0.0f;
-        for (int i = g; i < count; i += N) {
+    float o = 0.0f, sum = 0.0f;
+    for (int first = 0; first < count; first += kAtOnce) {
+        const int last = min(count, first + kAtOnce);
+        if (first > 0) __syncthreads();
+        for (int i = first + threadIdx.x; i < last; i += 256) {
             const float f = exp2_hw(part[i * step + D] - top);
-            o += f * part[i * step + d];
+            factor[i - first] = f;
             sum += f * part[i * step + D + 1];
         }
-        so[g][d] = o;
-        if (d == 0) ss[g] = sum;
+        __syncthreads();
+        if (g < N) {
+#pragma unroll 8
+            for (int i = first + g; i < last; i += N) o += factor[i - first] * part[i * step + d];
+        }
     }
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) sum += __shfl_xor(sum, s, 64);
+    if (lane == 0) red[4 + wave] = sum;
+    if (g < N) so[g][d] = o;
     __syncthreads();
     if (threadIdx.x < D) {
-        float o = so[0][d], sum = ss[0];
+        o = so[0][d];
 #pragma unroll
-        for (int i = 1; i < N; ++i) {
-            o += so[i][d];
-            sum += ss[i];
-        }
+        for (int i = 1; i < N; ++i) o += so[i][d];
+        sum = red[4] + red[5] + red[6] + red[7];
         const float y = sum == 0.0f ? 0.0f : o / sum * (a.v_scale ? *a.v_scale : 1.0f);
         static_cast<uint16_t*>(a.out)[(static_cast<int64_t>(b) * a.heads + h) * D + d] =
             static_cast<uint16_t>(QC == CKH_BF16 ? f_to_bf16_rne(y) : f_to_f16(y));
@@ -515,7 +521,7 @@ extern "C" int64_t ckh_paged_attention_workspace_bytes(int64_t batch, int64_t he
     if (batch <= 0 || heads <= 0 || kv_heads <= 0 || dim <= 0 || page_size <= 0 || max_pages < 0) return 0;
     const int64_t units = paged_units(batch, heads, kv_heads), capacity = page_size * max_pages;
     if (cdiv(cdiv(capacity, 32) + 2, attn::kMinTiles) <= 1) return 0;  // always one chunk
-    return attn::paged_slots(units, capacity, attn::paged_target()) * 16 * (dim + 2) * 4;
+    return attn::paged_slots(units, capacity, attn::paged_target()) * 16 * (dim + 2) * 4 + units * 8;
 }
 
 extern "C" int ckh_paged_attention(const void* q, const void* k_cache, const void* v_cache, const void* page_table,
@@ -553,7 +559,7 @@ extern "C" int ckh_paged_attention(const void* q, const void* k_cache, const voi
     CKH_REQUIRE(units <= (1 << 28), "paged_attention: too many heads and sequences");
     const int64_t need = ckh_paged_attention_workspace_bytes(batch, heads, kv_heads, dim, page_size, max_pages);
     // without a workspace every sequence is one chunk
-    const bool split = need > 0 && workspace && workspace_bytes >= need && aligned(workspace, 4);
+    const bool split = need > 0 && workspace && workspace_bytes >= need && aligned(workspace, 8);
     attn::PagedArgs a{};
     a.q = static_cast<const uint8_t*>(q);
     a.k = static_cast<const uint8_t*>(k_cache);
@@ -572,10 +578,11 @@ extern "C" int ckh_paged_attention(const void* q, const void* k_cache, const voi
     a.group = static_cast<int>(heads / kv_heads), a.head_tiles = static_cast<int>(cdiv(a.group, 16));
     a.pages = static_cast<int>(pages), a.page_size = static_cast<int>(page_size), a.max_pages = static_cast<int>(max_pages);
     a.window = static_cast<int>(window), a.sinks = static_cast<int>(sinks);
-    a.target = split ? attn::paged_target() : 1;
+    a.target = split ? std::max(2, attn::paged_target()) : 1;
     a.scale = scale;
     a.by_page = attn::fast_div(static_cast<uint32_t>(page_size));
     const int64_t slots = split ? attn::paged_slots(units, capacity, a.target) : units;
+    if (split) a.plan = reinterpret_cast<int2*>(static_cast<uint8_t*>(workspace) + slots * 16 * (dim + 2) * 4);
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const int d = static_cast<int>(dim);
     if (q_code == CKH_BF16) {
