@@ -76,7 +76,8 @@ SIGNATURES: dict[str, tuple] = {
     "ckh_quantize_nvfp4_dynamic": (_i32, [_p, _f32, _p, _p, _p, _i64, _i64, _i64, _i64, _f32, _i32, _i32, _p, _u64]),
     "ckh_quantize_int4": (_i32, [_p] * 3 + [_i64] * 3 + [_i32, _u64]),
     "ckh_dequantize_int4": (_i32, [_p] * 4 + [_i64] * 3 + [_i32, _i32, _u64]),
-    "ckh_linear_int4": (_i32, [_p] * 6 + [_i64] * 5 + [_i32] * 3 + [_u64]),
+    "ckh_linear_int4_workspace_bytes": (_i64, [_i64] * 4),
+    "ckh_linear_int4": (_i32, [_p] * 6 + [_i64] * 5 + [_i32] * 3 + [_p, _i64, _u64]),
     "ckh_paged_attention_workspace_bytes": (_i64, [_i64] * 6),
     "ckh_paged_attention": (_i32, [_p] * 8 + [_i64] * 8 + [_p] + [_i64] * 2 + [_f32, _i32, _i32, _p, _i64, _u64]),
     "ckh_paged_write": (_i32, [_p] * 7 + [_i64] * 5 + [_p] + [_i32] * 3 + [_u64]),
@@ -456,6 +457,11 @@ def dequantize_int4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tens
     return out
 
 
+@functools.lru_cache(maxsize=256)
+def _int4_workspace_bytes(m: int, n: int, k: int, group: int) -> int:
+    return int(_lib.ckh_linear_int4_workspace_bytes(m, n, k, group))
+
+
 def linear_int4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None,
                 bias: torch.Tensor | None = None, group_size: int = 128) -> torch.Tensor:
     _same_device("linear_int4", x, codes, scales, zeros, bias)
@@ -472,9 +478,11 @@ def linear_int4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zero
         stride = k
     bias, bias_code = _bias_args(bias, n, x.device)
     out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
+    nbytes = _int4_workspace_bytes(m, n, k, group_size) if m > 16 else 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
     _launch("ckh_linear_int4", rows, rows.data_ptr(), codes.data_ptr(), scales.data_ptr(), _ptr(zeros), _ptr(bias),
             out.data_ptr(), m, n, k, stride if m > 1 else k, group_size, DTYPE_TO_CODE[x.dtype],
-            DTYPE_TO_CODE[scales.dtype], bias_code)
+            DTYPE_TO_CODE[scales.dtype], bias_code, _ptr(ws), nbytes)
     return out
 
 

@@ -33,6 +33,8 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr int kScaleGroups = 128;  // groups whose scales are in LDS at a time
+constexpr int kTileRows = 32;       // activation rows of a workgroup of tile_kernel
+constexpr int kMaxSplits = 16;
 constexpr int kVecCodes = 8192;    // matvec_kernel: codes whose activations are in LDS at a time, half as many for 4 rows
 
 struct LinearArgs {
@@ -47,6 +49,8 @@ struct LinearArgs {
     uint32_t per_group;  // ceil(2^32 / (group / 32)): block b of 32 codes is in group (b * per_group) >> 32
     int chunk;  // steps of 128 codes whose groups fit kScaleGroups
     int scale_code, bias_code;
+    int splits;   // tile_kernel: ranges of K
+    float* part;  // their sums, [splits][m][n]
 
     __device__ __forceinline__ int group_of(uint32_t block) const {
         return per_group ? static_cast<int>((static_cast<uint64_t>(block) * per_group) >> 32) : static_cast<int>(block);
@@ -421,6 +425,161 @@ __global__ __launch_bounds__(W * 64, 4) void matvec_kernel(LinearArgs a) {
     }
 }
 
+// More rows: a workgroup takes 32 activation rows, 64 weight rows (four waves of 16) and one of
+// `splits` ranges of K, and its waves share the activations, which go through LDS in the operand's
+// order (two buffers, a barrier a step): read by every wave itself they would cost more than the
+// codes.  Where K is split, the sums go to memory in fp32 and reduce_kernel adds them in order.
+// 24 rows, N = 5120, K = 13824: 24.7 us with 12 ranges, 26.9 with 6; linear_kernel 31.  No one unit
+// bounds it: codes, LDS, MFMAs (half of them the sums of x) and VALU take 4-6 us each, and the
+// second launch as much.  32 weight rows a wave, or a third step in flight, measured no better.
+template <int XC, int GB>
+__global__ __launch_bounds__(256, 4) void tile_kernel(LinearArgs a) {
+    constexpr int T = kTileRows / 16, R = 1;  // 16-row tiles of activations, and of a wave's weight rows
+    constexpr int W = 4, D = 2;               // waves; steps in flight
+    constexpr int kRows = 16 * R * W;
+    constexpr int kUnits = T * 256;       // 16-byte pieces of a step's activations
+    constexpr int kPer = kUnits / 256;    // a thread's
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    v4u* xs = reinterpret_cast<v4u*>(lds);  // [2][block][tile][quarter][row]
+    v2f(*sp)[16 * R * W + 1] = reinterpret_cast<v2f(*)[16 * R * W + 1]>(lds + 2 * kUnits * 16);
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r16 = lane & 15, quarter = lane >> 4;
+    const int n0 = blockIdx.x * kRows, m0 = blockIdx.z * 16 * T;
+    const int rows = min(kRows, a.n - n0), toks = min(16 * T, a.m - m0);
+    const int pitch = a.k >> 1;  // code bytes per weight row
+    const int steps = (a.k + 127) >> 7;
+    const int first = static_cast<int>(static_cast<int64_t>(steps) * blockIdx.y / a.splits);
+    const int last = static_cast<int>(static_cast<int64_t>(steps) * (blockIdx.y + 1) / a.splits);
+
+    const uint8_t* wbase = a.codes + static_cast<int64_t>(n0) * pitch;
+    const __amdgpu_buffer_rsrc_t rw = buffer_rsrc(wbase, rows * pitch);
+    const __amdgpu_buffer_rsrc_t none = buffer_rsrc(wbase, 0);
+    const __amdgpu_buffer_rsrc_t rx =
+        buffer_rsrc(static_cast<const uint16_t*>(a.x) + m0 * a.x_stride,
+                    static_cast<uint32_t>(((toks - 1) * a.x_stride + a.k) * 2));
+    uint32_t ow[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) ow[r] = min((wave * R + r) * 16 + r16, rows - 1) * pitch + quarter * 16;
+    // piece e of a step: block e / (64 T), tile, then quarter and row as the operand's lanes
+    uint32_t ox[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int e = threadIdx.x + i * 256, l = e & 63, t = (e >> 6) % T, j = (e >> 6) / T;
+        ox[i] = static_cast<uint32_t>((min(t * 16 + (l & 15), toks - 1) * a.x_stride + j * 32 + (l >> 4) * 8) * 2);
+    }
+    v4u w[D][R], x[D][kPer];
+    const auto load_codes = [&](v4u (&d)[R], int s) __attribute__((always_inline)) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            d[r] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(s < last ? rw : none, ow[r], s * 64, 0));
+    };
+    const auto load_x = [&](v4u (&d)[kPer], int s) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            d[i] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rx, ox[i], s * 256, 0));
+    };
+    const auto store_x = [&](const v4u (&d)[kPer], int s) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) xs[(s & 1) * kUnits + threadIdx.x + i * 256] = pair_order(d[i]);
+    };
+
+    const v4u ones = XC == CKH_BF16 ? v4u{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}
+                                    : v4u{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+    v4f total[R][T];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int t = 0; t < T; ++t) total[r][t] = v4f{0, 0, 0, 0};
+    const int g0 = a.group_of(first * 4);
+    const auto use = [&](const v4u (&codes)[R], int s, int blocks) __attribute__((always_inline)) {
+        v4f acc[R][T], sum[T];
+        v4u c[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) c[r] = transpose_quarters(codes[r]);
+        const v4u* xp = xs + (s & 1) * kUnits + lane;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j < blocks) {
+                const bool fresh = j % GB == 0;
+                v4u b[R];
+#pragma unroll
+                for (int r = 0; r < R; ++r) b[r] = widen<XC>(c[r][j]);
+#pragma unroll
+                for (int t = 0; t < T; ++t) {
+                    const v4u f = xp[(j * T + t) * 64];
+                    sum[t] = mfma<XC>(f, ones, fresh ? v4f{0, 0, 0, 0} : sum[t]);
+#pragma unroll
+                    for (int r = 0; r < R; ++r) acc[r][t] = mfma<XC>(f, b[r], fresh ? v4f{0, 0, 0, 0} : acc[r][t]);
+                }
+            }
+            if (j % GB == GB - 1 && j - (GB - 1) < blocks) {
+                const int g = a.group_of(s * 4 + j - (GB - 1)) - g0;
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const v2f p = sp[g][(wave * R + r) * 16 + r16];
+#pragma unroll
+                    for (int t = 0; t < T; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            total[r][t][i] = __fmaf_rn(p[0], acc[r][t][i], __fmaf_rn(p[1], sum[t][i], total[r][t][i]));
+                }
+            }
+        }
+    };
+
+    const int gn = min(a.groups, a.group_of(last * 4 - 1) + 1) - g0;
+    ScaleLoads<XC, R * W, W> sl;
+    load_x(x[0], first);
+    sl.load(a, n0, rows, wave, lane, g0, gn);
+#pragma unroll
+    for (int u = 0; u < D; ++u) load_codes(w[u], first + u);
+#pragma unroll
+    for (int u = 1; u < D; ++u) load_x(x[u], first + u);
+    store_x(x[0], first);
+    sl.store(a, sp, wave, lane, gn);
+    __syncthreads();
+    for (int s0 = first; s0 < last; s0 += D) {
+#pragma unroll
+        for (int u = 0; u < D; ++u) {
+            const int s = s0 + u;
+            if (s >= last) break;
+            load_x(x[u], s + D);  // past the range: unused, within the operand or zeros
+            use(w[u], s, min(4, (a.k >> 5) - s * 4));
+            load_codes(w[u], s + D);
+            store_x(x[(u + 1) % D], s + 1);
+            __syncthreads();
+        }
+    }
+
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int row = (wave * R + r) * 16 + r16;
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int tok = t * 16 + quarter * 4 + i;
+                if (row < rows && tok < toks) {
+                    if (a.splits == 1) store_result<XC>(a, m0 + tok, n0 + row, total[r][t][i]);
+                    else a.part[(static_cast<int64_t>(blockIdx.y) * a.m + m0 + tok) * a.n + n0 + row] = total[r][t][i];
+                }
+            }
+    }
+}
+
+template <int XC>
+__global__ __launch_bounds__(256) void reduce_kernel(LinearArgs a) {
+    const int64_t size = static_cast<int64_t>(a.m) * a.n, at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (at >= size) return;
+    float v = a.part[at];
+#pragma unroll 8
+    for (int s = 1; s < a.splits; ++s) v += a.part[s * size + at];
+    const int m = static_cast<int>(at / a.n);
+    store_result<XC>(a, m, static_cast<int>(at - static_cast<int64_t>(m) * a.n), v);
+}
+
 // Steps of 128 codes that touch at most kScaleGroups groups, wherever the first begins.
 int chunk_steps(int64_t group) {
     return static_cast<int>((128 % group == 0 ? kScaleGroups : kScaleGroups - 1) * group / 128);
@@ -453,6 +612,30 @@ void launch_matvec(const LinearArgs& a, hipStream_t st) {
     else launch_matvec<XC, MT, R, W, D, 1>(a, st);
 }
 
+// Ranges of K for a call (1: not split), 0 where tile_kernel does not serve it: few rows, rows that
+// linear_kernel's 64-row workgroups serve better (32 rows, N = 13824: 25.9 against 27.7), or more
+// groups in a range than LDS holds.  Three workgroups a CU are wanted, of four steps at least.
+int tile_splits(int64_t m, int64_t n, int64_t k, int64_t group, bool may_split) {
+    const int cus = device_cus();
+    if (m <= 16 || (m <= 32 && n > 48 * cus)) return 0;
+    const int64_t blocks = cdiv(n, 64) * cdiv(m, kTileRows), steps = cdiv(k, 128);
+    int64_t s = std::min<int64_t>({kMaxSplits, cdiv(3 * cus, blocks), std::max<int64_t>(1, steps / 4)});
+    s = may_split ? std::max(s, cdiv(steps, chunk_steps(group))) : 1;
+    return s <= kMaxSplits && cdiv(steps, s) <= chunk_steps(group) ? static_cast<int>(s) : 0;
+}
+
+template <int XC>
+void launch_tile(const LinearArgs& a, hipStream_t st) {
+    const dim3 grid(static_cast<unsigned>(cdiv(a.n, 64)), static_cast<unsigned>(a.splits), static_cast<unsigned>(cdiv(a.m, kTileRows)));
+    const int64_t codes = cdiv(cdiv(a.k, 128), a.splits) * 128;
+    const int64_t groups = std::min<int64_t>({a.groups, kScaleGroups, codes / a.group + 2});
+    const size_t lds = 2 * kTileRows * 256 + groups * 65 * 8;  // two steps' activations, the scales
+    if (a.group % 128 == 0) tile_kernel<XC, 4><<<grid, 256, lds, st>>>(a);
+    else if (a.group % 64 == 0) tile_kernel<XC, 2><<<grid, 256, lds, st>>>(a);
+    else tile_kernel<XC, 1><<<grid, 256, lds, st>>>(a);
+    if (a.splits > 1) reduce_kernel<XC><<<static_cast<unsigned>(cdiv(static_cast<int64_t>(a.m) * a.n, 256)), 256, 0, st>>>(a);
+}
+
 // Tiles and waves by the rows of x and by whether the tiles fill the 256 CUs (us at K = 5120 and
 // N = 13824, groups of 128, unless said; the operands not in cache):
 //   1 row      16 weight rows a workgroup; 4 waves from two workgroups a CU on (11.3; 8 waves 12.5),
@@ -461,12 +644,14 @@ void launch_matvec(const LinearArgs& a, hipStream_t st) {
 //              under 128 (their scales would not fit the registers), 16
 //   5-16 rows  32 weight rows, 8 waves (16.7; 16 rows 19.9), 16 waves where there are fewer
 //              workgroups than CUs (N = K = 5120, 16 rows: 12.0 against 13.6)
-//   more       64 weight rows, 8 waves (32 rows of x: 23.6; 32 weight rows 29.0), and 32 weight rows,
-//              where 64 leave CUs idle (24 rows, N = 5120, K = 13824: 30.6 against 37)
+//   more       tile_kernel (64 rows: 39; 45 with 64 weight rows and 8 waves of linear_kernel), but
+//              linear_kernel for up to 32 rows of wide layers, and where tile_splits says so
 template <int XC>
 void linear(const LinearArgs& a, hipStream_t st) {
     const int cus = device_cus();
-    if (a.m == 1) {
+    if (a.splits > 0) {
+        launch_tile<XC>(a, st);
+    } else if (a.m == 1) {
         if (a.n > 32 * cus) launch_matvec<XC, 1, 1, 4, 2>(a, st);
         else launch_matvec<XC, 1, 1, 8, 2>(a, st);
     } else if (a.m <= 4) {
@@ -475,10 +660,8 @@ void linear(const LinearArgs& a, hipStream_t st) {
     } else if (a.m <= 16) {
         if (a.n > 32 * cus) launch_linear<XC, 1, 2, 8, 1>(a, st);
         else launch_linear<XC, 1, 2, 16, 1>(a, st);
-    } else if (static_cast<int64_t>(a.n) * cdiv(a.m, 32) > 48 * cus) {
-        launch_linear<XC, 2, 4, 8, 1>(a, st);
     } else {
-        launch_linear<XC, 2, 2, 8, 1>(a, st);
+        launch_linear<XC, 2, 4, 8, 1>(a, st);
     }
 }
 
@@ -615,14 +798,21 @@ extern "C" int ckh_dequantize_int4(const void* codes, const void* scales, const 
     return check_launch("dequantize_int4");
 }
 
+extern "C" int64_t ckh_linear_int4_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t group) {
+    if (m <= 0 || n <= 0 || k <= 0 || group < 32) return 0;
+    const int64_t s = i4::tile_splits(m, n, k, group, true);
+    return s > 1 ? s * m * n * 4 : 0;
+}
+
 extern "C" int ckh_linear_int4(const void* x, const void* codes, const void* scales, const void* zeros, const void* bias,
                                void* y, int64_t m, int64_t n, int64_t k, int64_t x_stride, int64_t group, int x_code,
-                               int scale_code, int bias_code, uintptr_t stream) {
+                               int scale_code, int bias_code, void* workspace, int64_t workspace_bytes,
+                               uintptr_t stream) {
     CKH_REQUIRE_INT4("linear_int4", n, k, group);
     CKH_REQUIRE(x_code == CKH_F16 || x_code == CKH_BF16, "linear_int4: unsupported activation dtype %d", x_code);
     CKH_REQUIRE(i4::is_float(scale_code), "linear_int4: unsupported scale dtype %d", scale_code);
     CKH_REQUIRE(!bias || i4::is_float(bias_code), "linear_int4: unsupported bias dtype %d", bias_code);
-    CKH_REQUIRE(m >= 0 && m <= 65535 * 16, "linear_int4: at most %d activation rows, got %lld", 65535 * 16,
+    CKH_REQUIRE(m >= 0 && m <= 65535 * 16 && m * n < (int64_t(1) << 38), "linear_int4: at most %d activation rows, got %lld", 65535 * 16,
                 static_cast<long long>(m));
     if (m == 0 || n == 0) return CKH_OK;
     CKH_REQUIRE(x && codes && scales && y, "linear_int4: null pointer");
@@ -631,11 +821,18 @@ extern "C" int ckh_linear_int4(const void* x, const void* codes, const void* sca
                     aligned(scales, scale_code == CKH_F32 ? 4 : 2) && (!bias || aligned(bias, bias_code == CKH_F32 ? 4 : 2)),
                 "linear_int4: misaligned pointer or row stride");
     CKH_REQUIRE(x_stride <= (int64_t(1) << 23), "linear_int4: activation row stride too large");
-    const i4::LinearArgs a{x, static_cast<const uint8_t*>(codes), scales, static_cast<const uint8_t*>(zeros), bias, y,
-                           m == 1 ? k : x_stride, static_cast<int>(m), static_cast<int>(n), static_cast<int>(k),
-                           static_cast<int>(cdiv(k, group)), static_cast<int>(group),
-                           group == 32 ? 0u : static_cast<uint32_t>(cdiv(int64_t(1) << 32, group / 32)),
-                           i4::chunk_steps(group), scale_code, bias_code};
+    const int64_t need = ckh_linear_int4_workspace_bytes(m, n, k, group);
+    const bool split = need > 0 && workspace && workspace_bytes >= need && aligned(workspace, 4);
+    i4::LinearArgs a{};
+    a.x = x, a.codes = static_cast<const uint8_t*>(codes), a.scales = scales, a.zeros = static_cast<const uint8_t*>(zeros);
+    a.bias = bias, a.y = y, a.x_stride = m == 1 ? k : x_stride;
+    a.m = static_cast<int>(m), a.n = static_cast<int>(n), a.k = static_cast<int>(k);
+    a.groups = static_cast<int>(cdiv(k, group)), a.group = static_cast<int>(group);
+    a.per_group = group == 32 ? 0u : static_cast<uint32_t>(cdiv(int64_t(1) << 32, group / 32));
+    a.chunk = i4::chunk_steps(group);
+    a.scale_code = scale_code, a.bias_code = bias_code;
+    a.splits = i4::tile_splits(m, n, k, group, split);
+    a.part = static_cast<float*>(workspace);
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (x_code == CKH_BF16) i4::linear<CKH_BF16>(a, st);
     else i4::linear<CKH_F16>(a, st);

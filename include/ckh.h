@@ -302,15 +302,18 @@ int ckh_quantize_nvfp4_dynamic(const void* x, float divisor, void* scale_out, vo
  * dequantize: one rounding to out_code.
  * linear: y [m, n] = x W^T + bias, x [m, k] of x_code (f16/bf16) with x_stride elements between
  * rows (x 16-byte aligned, x_stride % 8 == 0), y of x_code, bias [n] of bias_code or NULL; sums
- * in fp32, one rounding.  An activation that is not finite makes its row of y NaN.
+ * in fp32, one rounding.  An activation that is not finite makes its row of y NaN.  The workspace of
+ * ckh_linear_int4_workspace_bytes lets K be split (0: it is not); with NULL or a short one the call
+ * runs without (same result up to the order of fp32 sums).
  */
+int64_t ckh_linear_int4_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t group);
 int ckh_quantize_int4(const void* x, void* codes, void* scales, int64_t n, int64_t k, int64_t group, int in_code,
                       uintptr_t stream);
 int ckh_dequantize_int4(const void* codes, const void* scales, const void* zeros, void* out, int64_t n, int64_t k,
                         int64_t group, int scale_code, int out_code, uintptr_t stream);
 int ckh_linear_int4(const void* x, const void* codes, const void* scales, const void* zeros, const void* bias,
                     void* y, int64_t m, int64_t n, int64_t k, int64_t x_stride, int64_t group, int x_code,
-                    int scale_code, int bias_code, uintptr_t stream);
+                    int scale_code, int bias_code, void* workspace, int64_t workspace_bytes, uintptr_t stream);
 
 /*
  * A key-value cache held in pages: K and V are [pages, page_size, kv_heads, dim] of cache_code with

@@ -56,7 +56,10 @@ SHAPES = [(1, 1, 32, 32), (1, 16, 128, 128), (1, 1000, 5120, 128), (2, 33, 160, 
           (48, 250, 640, 128), (64, 31, 2016, 64), (65, 100, 512, 512), (130, 40, 288, 64), (1, 5000, 2048, 64),
           # more groups, or more activations, than are staged at a time; wide enough for the other tiles
           (1, 40, 16416, 32), (3, 40, 16416, 32), (4, 9000, 4256, 128), (2, 9000, 1056, 32), (20, 40, 16416, 32),
-          (1, 20, 36864, 128), (2, 20, 36896, 256), (9, 9000, 544, 64), (40, 9000, 1056, 96)]
+          (1, 20, 36864, 128), (2, 20, 36896, 256), (9, 9000, 544, 64), (40, 9000, 1056, 96),
+          # more rows, with K in ranges: odd ones, one that ends inside a step, more groups than one range may hold
+          (17, 200, 1696, 64), (24, 512, 5120, 128), (33, 100, 8224, 32), (64, 300, 14336, 128), (100, 70, 70016, 32),
+          (45, 20000, 544, 128), (200, 65, 1120, 96)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
@@ -158,6 +161,21 @@ def test_streams_and_graph(hip):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, ck.linear_int4(x * (i + 1), *args))
+
+
+def test_without_a_workspace(hip):
+    """The C entry point without the workspace that splits K: the same result up to fp32 sums, for a
+    K whose groups fit one range and one whose do not."""
+    import comfy_kitchen.backends.hip as hb
+
+    for k in (1024, 6144):
+        codes, scales, _ = weight(96, k, 32, False, torch.bfloat16, 4)
+        x = torch.randn(40, k, generator=torch.Generator().manual_seed(1)).bfloat16()
+        d = [t.cuda() for t in (x, codes, scales)]
+        y = torch.empty(40, 96, dtype=torch.bfloat16, device="cuda")
+        assert hb._lib.ckh_linear_int4_workspace_bytes(40, 96, k, 32) > 0
+        hb._launch("ckh_linear_int4", y, *(t.data_ptr() for t in d), None, None, y.data_ptr(), 40, 96, k, k, 32, 2, 2, 0, None, 0)
+        check(y, x, wide(codes, scales, None, 32), scales, 32)
 
 
 def test_refusals(hip):
