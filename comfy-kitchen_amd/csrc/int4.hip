@@ -100,47 +100,71 @@ __device__ __forceinline__ void store_result(const LinearArgs& a, int m, int n, 
 }
 
 // The scales and zero points of a chunk's at most kScaleGroups groups for a workgroup's 16 R rows,
-// on their way to LDS as (s, -s (B + z)): a wave takes every W-th row, its lanes 64 groups at a
-// time.  All loads go out at once, before the codes', so that they are waited for alone.
+// on their way to LDS as (s, -s (B + z)): 16 lanes take a row, a lane 4 groups next to each other
+// (of any alignment), then the 4 that are 64 groups on.  All loads go out at once, before the codes',
+// so that they are waited for alone.
 template <int XC, int R, int W>
 struct ScaleLoads {
-    static constexpr int kPer = 16 * R / W > 0 ? 16 * R / W : 1;  // rows per wave
-    uint32_t s[kPer][2], z[kPer][2];
+    static constexpr int kPer = (16 * R + 4 * W - 1) / (4 * W);  // times that a wave takes 4 rows
+    uint32_t s[kPer][2][4], z[kPer][2];
+
+    static __device__ __forceinline__ int row_of(int i, int wave, int lane) { return (i * W + wave) * 4 + (lane >> 4); }
 
     __device__ __forceinline__ void load(const LinearArgs& a, int n0, int rows, int wave, int lane, int g0, int gn) {
         const bool wide = a.scale_code == CKH_F32;
-        const int ss = wide ? 4 : 2;
-        const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(
-            static_cast<const uint8_t*>(a.scales) + static_cast<int64_t>(n0) * a.groups * ss, rows * a.groups * ss);
-        const __amdgpu_buffer_rsrc_t rz = buffer_rsrc(a.zeros ? a.zeros + static_cast<int64_t>(n0) * a.groups : a.codes,
-                                                      a.zeros ? rows * a.groups : 0);
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int row = wave + i * W, g = h * 64 + lane;
-                const uint32_t at = g < gn && row < rows ? row * a.groups + g0 + g : 0x20000000u;
-                s[i][h] = z[i][h] = 0;
-                if (h == 0 || gn > 64) {
-                    s[i][h] = wide ? __builtin_amdgcn_raw_buffer_load_b32(rs, at * 4, 0, 0)
-                                   : __builtin_amdgcn_raw_buffer_load_b16(rs, at * 2, 0, 0);
-                    z[i][h] = a.zeros ? __builtin_amdgcn_raw_buffer_load_b8(rz, at, 0, 0) : 8;
+                const int row = row_of(i, wave, lane), g = h * 64 + (lane & 15) * 4;
+                const int back = max(0, g + 4 - gn);  // the row's last 4 where its end cuts the lane's
+                const int64_t at = static_cast<int64_t>(n0 + row) * a.groups + g0 + g - back;
+                const uint8_t* sp = static_cast<const uint8_t*>(a.scales) + at * (wide ? 4 : 2);
+                z[i][h] = 0x08080808u;
+                if (row >= rows || g >= gn) continue;
+                if (gn < 4) {
+#pragma unroll
+                    for (int e = 0; e < 3; ++e) {
+                        if (e >= gn) break;
+                        const uint8_t* one = sp + (e + back) * (wide ? 4 : 2);
+                        s[i][h][e] = wide ? *reinterpret_cast<const uint32_t*>(one) : *reinterpret_cast<const uint16_t*>(one);
+                        if (a.zeros) z[i][h] = (z[i][h] & ~(255u << (8 * e))) | (static_cast<uint32_t>(a.zeros[at + back + e]) << (8 * e));
+                    }
+                    continue;
+                }
+                if (wide) {
+                    uint32_t v[4];
+                    __builtin_memcpy(v, sp, 16);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[i][h][e] = back == 0 ? v[e] : back == 1 ? v[min(e + 1, 3)] : back == 2 ? v[min(e + 2, 3)] : v[3];
+                } else {
+                    uint64_t v;
+                    __builtin_memcpy(&v, sp, 8);
+                    v >>= 16 * back;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[i][h][e] = static_cast<uint32_t>(v >> (16 * e)) & 0xffffu;
+                }
+                if (a.zeros) {
+                    __builtin_memcpy(&z[i][h], a.zeros + at, 4);
+                    z[i][h] >>= 8 * back;
                 }
             }
     }
 
-    __device__ __forceinline__ void store(const LinearArgs& a, v2f (*sp)[16 * R + 1], int wave, int lane, int gn) const {
+    __device__ __forceinline__ void store(const LinearArgs& a, v2f (*sp)[16 * R + 1], int rows, int wave, int lane, int gn) const {
         constexpr float kBase = XC == CKH_BF16 ? 128.0f : 1024.0f;
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int row = wave + i * W, g = h * 64 + lane;
-                const float v = a.scale_code == CKH_F32    ? as_f(s[i][h])
-                                : a.scale_code == CKH_BF16 ? bf16_to_f(s[i][h])
-                                                           : f16_to_f(s[i][h]);
-                if (g < gn && row < 16 * R) sp[g][row] = v2f{v, -v * (kBase + static_cast<float>(z[i][h]))};
-            }
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int row = row_of(i, wave, lane), g = h * 64 + (lane & 15) * 4 + e;
+                    const float v = a.scale_code == CKH_F32    ? as_f(s[i][h][e])
+                                    : a.scale_code == CKH_BF16 ? bf16_to_f(s[i][h][e])
+                                                               : f16_to_f(s[i][h][e]);
+                    if (g < gn && row < rows) sp[g][row] = v2f{v, -v * (kBase + static_cast<float>((z[i][h] >> (8 * e)) & 255u))};
+                }
     }
 };
 
@@ -257,7 +281,7 @@ __global__ __launch_bounds__(W * 64) void linear_kernel(LinearArgs a) {
             for (int u = 0; u < U; ++u) load(d[u], s0 + u);
         }
         if (c0 > 0) __syncthreads();
-        sl.store(a, sp, wave, lane, gn);
+        sl.store(a, sp, rows, wave, lane, gn);
         __syncthreads();
         if (ahead) {
 #pragma unroll
@@ -299,7 +323,7 @@ __global__ __launch_bounds__(W * 64) void linear_kernel(LinearArgs a) {
 // operand's order (lanes of the 16-row operand repeat the MT rows), so that the step reads nothing
 // but codes from memory; a wave keeps D steps of codes in flight.
 template <int XC, int MT, int R, int W, int D, int GB>
-__global__ __launch_bounds__(W * 64, 4) void matvec_kernel(LinearArgs a) {
+__global__ __launch_bounds__(W * 64, MT > 1 && GB == 1 ? 3 : 4) void matvec_kernel(LinearArgs a) {
     constexpr int kRows = 16 * R;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     v4u* xs = reinterpret_cast<v4u*>(lds);  // [8 codes][row]
@@ -393,7 +417,7 @@ __global__ __launch_bounds__(W * 64, 4) void matvec_kernel(LinearArgs a) {
             const int e = threadIdx.x + i * W * 64;
             if (e < units * MT) xs[e] = pair_order(xr[i]);
         }
-        sl.store(a, sp, wave, lane, gn);
+        sl.store(a, sp, rows, wave, lane, gn);
         for (int e = threadIdx.x + kAhead * W * 64; e < units * MT; e += W * 64)
             xs[e] = pair_order(__builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rx, x_at(e), 0, 0)));
         __syncthreads();
@@ -538,7 +562,7 @@ __global__ __launch_bounds__(256, 4) void tile_kernel(LinearArgs a) {
 #pragma unroll
     for (int u = 1; u < D; ++u) load_x(x[u], first + u);
     store_x(x[0], first);
-    sl.store(a, sp, wave, lane, gn);
+    sl.store(a, sp, rows, wave, lane, gn);
     __syncthreads();
     for (int s0 = first; s0 < last; s0 += D) {
 #pragma unroll
