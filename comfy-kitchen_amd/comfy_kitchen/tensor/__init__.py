@@ -11,11 +11,13 @@ from .base import (
     register_layout_op,
 )
 from .fp8 import TensorCoreFP8Layout
+from .int4 import GroupInt4Layout
 from .mxfp8 import TensorCoreMXFP8Layout
 from .nvfp4 import TensorCoreNVFP4Layout
 
 __all__ = [
     "BaseLayoutParams",
+    "GroupInt4Layout",
     "QuantizedLayout",
     "QuantizedTensor",
     "TensorCoreFP8Layout",
@@ -32,3 +34,4 @@ __all__ = [
 register_layout_class("TensorCoreFP8Layout", TensorCoreFP8Layout)
 register_layout_class("TensorCoreMXFP8Layout", TensorCoreMXFP8Layout)
 register_layout_class("TensorCoreNVFP4Layout", TensorCoreNVFP4Layout)
+register_layout_class("GroupInt4Layout", GroupInt4Layout)
