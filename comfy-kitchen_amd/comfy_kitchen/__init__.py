@@ -16,7 +16,7 @@ from .exceptions import (
     NoCapableBackendError,
 )
 from .float_utils import from_blocked, swap_nibbles, to_blocked
-from .ops import DTYPE_TO_CODE, _dispatch, _quantize_fp8_dynamic, direct, untouched
+from .ops import DTYPE_TO_CODE, _dispatch, _quantize_fp8_dynamic, changed, direct, untouched
 from .paged import OutOfPages, PagedKVCache
 from .registry import registry
 
@@ -268,8 +268,9 @@ def paged_write(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v
     The caches are [pages, page_size, kv_heads, head_dim] of key's dtype, or E4M3, which take
     the codes of clamp(x / scale, +-448).  head_dim is a multiple of 16."""
     if direct(key, value, k_cache, v_cache, slots, k_scale, v_scale) and untouched("paged_write"):
-        return _dispatch("paged_write", key=key, value=value, k_cache=k_cache, v_cache=v_cache, slots=slots,
-                         k_scale=k_scale, v_scale=v_scale)
+        _dispatch("paged_write", key=key, value=value, k_cache=k_cache, v_cache=v_cache, slots=slots,
+                  k_scale=k_scale, v_scale=v_scale)
+        return changed(k_cache, v_cache)
     torch.ops.comfy_kitchen.paged_write(key, value, k_cache, v_cache, slots, k_scale, v_scale)
 
 
@@ -279,7 +280,8 @@ def paged_copy(k_cache: torch.Tensor, v_cache: torch.Tensor, src: torch.Tensor, 
     once with a leading dimension.  No slot of dst may be in src; pairs with a slot outside the
     cache are skipped."""
     if direct(k_cache, v_cache, src, dst) and untouched("paged_copy"):
-        return _dispatch("paged_copy", k_cache=k_cache, v_cache=v_cache, src=src, dst=dst)
+        _dispatch("paged_copy", k_cache=k_cache, v_cache=v_cache, src=src, dst=dst)
+        return changed(k_cache, v_cache)
     torch.ops.comfy_kitchen.paged_copy(k_cache, v_cache, src, dst)
 
 

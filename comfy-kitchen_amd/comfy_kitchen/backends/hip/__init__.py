@@ -487,145 +487,199 @@ def linear_int4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zero
 
 
 # -------------------------------------------------------- key-value cache held in pages
+# A call's checks depend on its tensors' shapes, strides and dtypes alone, and cost more than the
+# call itself (14 us of paged_write's 22 on one token of each of 48 sequences), so each is a
+# function of those whose answers are kept: the call's sizes and strides as the C side takes them,
+# or None where a tensor that may be copied does not lie on 16-byte rows.
 def _strides(*values: int):
     return (_i64 * len(values))(*values)
 
 
-def _cache_pair(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
+def _on_rows16(stride: tuple, size: int) -> bool:
+    """Whether the last dimension is contiguous and the others step by multiples of 16 bytes."""
+    return stride[-1] == 1 and not any(s * size % 16 for s in stride[:-1])
+
+
+def _cache_pair(name: str, k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype) -> None:
     """What every call asks of the two caches: one shape and dtype, rows that 16-byte pieces fit.
     They are used in place, so nothing is copied to fit."""
-    if k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
-        raise ValueError(f"{name}: k_cache {list(k_cache.shape)} {k_cache.dtype} and v_cache {list(v_cache.shape)} "
-                         f"{v_cache.dtype} differ")
-    size = k_cache.element_size()
-    for t in (k_cache, v_cache):
-        if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s * size % 16 for s in t.stride()[:-1]):
-            raise ValueError(f"{name}: a cache of strides {t.stride()} is not 16-byte aligned with head_dim contiguous")
+    if k_shape != v_shape or k_dtype != v_dtype:
+        raise ValueError(f"{name}: k_cache {list(k_shape)} {k_dtype} and v_cache {list(v_shape)} {v_dtype} differ")
+    for stride in (k_stride, v_stride):
+        if not _on_rows16(stride, k_dtype.itemsize):
+            raise ValueError(f"{name}: a cache of strides {stride} is not 16-byte aligned with head_dim contiguous")
+
+
+def _cache_pointers(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int]:
+    k, v = k_cache.data_ptr(), v_cache.data_ptr()
+    if (k | v) & 15:
+        raise ValueError(f"{name}: a cache is not 16-byte aligned with head_dim contiguous")
+    return k, v
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """t, its last dimension contiguous and its rows on 16-byte boundaries (copied where they are not)."""
-    stride, size = t.stride(), t.element_size()
-    if stride[-1] == 1 and not t.data_ptr() % 16 and not any(s * size % 16 for s in stride[:-1]):
+    if not t.data_ptr() % 16 and _on_rows16(t.stride(), t.element_size()):
         return t
     t = t.contiguous()
     return t.clone() if t.data_ptr() % 16 else t
 
 
-@functools.lru_cache(maxsize=256)
-def _paged_workspace_bytes(*sizes: int) -> int:
-    return int(_lib.ckh_paged_attention_workspace_bytes(*sizes))
+@functools.lru_cache(maxsize=512)
+def _attention_plan(q_shape, q_stride, q_dtype, k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype, table_shape,
+                    table_stride, sequences, window, sinks, scale):
+    _cache_pair("paged_attention", k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype)
+    batch, heads, dim = q_shape
+    pages, page_size, kv_heads, cache_dim = k_shape
+    if dim != cache_dim or kv_heads == 0 or heads % kv_heads:
+        raise ValueError(f"paged_attention: q {list(q_shape)} does not fit a cache of {kv_heads} heads of {cache_dim}")
+    if dim not in (64, 96, 128, 256):
+        raise ValueError(f"paged_attention: head_dim {dim} is not 64, 96, 128 or 256")
+    if k_dtype not in (q_dtype, torch.float8_e4m3fn):
+        raise ValueError(f"paged_attention: a cache of {k_dtype} with queries of {q_dtype}")
+    if table_shape[0] != batch or sequences != batch:
+        raise ValueError(f"paged_attention: page_table {list(table_shape)} and {sequences} lengths for {batch} sequences")
+    if window < 0 or sinks < 0:
+        raise ValueError(f"paged_attention: window ({window}) and sinks ({sinks}) must not be negative")
+    if not _on_rows16(q_stride, 2):
+        return None
+    max_pages = table_shape[1]
+    nbytes = int(_lib.ckh_paged_attention_workspace_bytes(batch, heads, kv_heads, dim, page_size, max_pages))
+    return ((batch, heads, kv_heads, dim, pages, page_size, max_pages, table_stride[0],
+             _strides(*q_stride[:2], *k_stride[:3], *v_stride[:3]), window, sinks, dim ** -0.5 if scale is None else scale,
+             DTYPE_TO_CODE[q_dtype], DTYPE_TO_CODE[k_dtype]), nbytes)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
                     lengths: torch.Tensor, scale: float | None = None, window: int = 0, sinks: int = 0,
                     k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> torch.Tensor:
     _same_device("paged_attention", q, k_cache, v_cache, page_table, lengths)
-    _cache_pair("paged_attention", k_cache, v_cache)
-    batch, heads, dim = q.shape
-    pages, page_size, kv_heads, cache_dim = k_cache.shape
-    if dim != cache_dim or kv_heads == 0 or heads % kv_heads:
-        raise ValueError(f"paged_attention: q {list(q.shape)} does not fit a cache of {kv_heads} heads of {cache_dim}")
-    if dim not in (64, 96, 128, 256):
-        raise ValueError(f"paged_attention: head_dim {dim} is not 64, 96, 128 or 256")
-    if k_cache.dtype not in (q.dtype, torch.float8_e4m3fn):
-        raise ValueError(f"paged_attention: a cache of {k_cache.dtype} with queries of {q.dtype}")
-    if page_table.shape[0] != batch or lengths.shape[0] != batch:
-        raise ValueError(f"paged_attention: page_table {list(page_table.shape)} and lengths {list(lengths.shape)} "
-                         f"for {batch} sequences")
-    if window < 0 or sinks < 0:
-        raise ValueError(f"paged_attention: window ({window}) and sinks ({sinks}) must not be negative")
-    q = _rows16(q)
+    lengths = lengths.contiguous()
     if page_table.stride(1) != 1 and page_table.shape[1] > 1:
         page_table = page_table.contiguous()
-    lengths = lengths.contiguous()
+    rest = (k_cache.shape, k_cache.stride(), k_cache.dtype, v_cache.shape, v_cache.stride(), v_cache.dtype, page_table.shape,
+            page_table.stride(), lengths.shape[0], window, sinks, scale)
+    plan = _attention_plan(q.shape, q.stride(), q.dtype, *rest)
+    if plan is None or q.data_ptr() % 16:
+        q = _rows16(q)
+        plan = _attention_plan(q.shape, q.stride(), q.dtype, *rest)
+    sizes, nbytes = plan
+    k, v = _cache_pointers("paged_attention", k_cache, v_cache)
     if k_scale is not None:
         k_scale = _scalar_on(k_scale, q.device, "k_scale")
     if v_scale is not None:
         v_scale = _scalar_on(v_scale, q.device, "v_scale")
-    out = torch.empty((batch, heads, dim), dtype=q.dtype, device=q.device)
-    max_pages = page_table.shape[1]
-    nbytes = _paged_workspace_bytes(batch, heads, kv_heads, dim, page_size, max_pages)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _launch("ckh_paged_attention", q, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(),
-            lengths.data_ptr(), _ptr(k_scale), _ptr(v_scale), out.data_ptr(), batch, heads, kv_heads, dim, pages,
-            page_size, max_pages, page_table.stride(0),
-            _strides(q.stride(0), q.stride(1), *k_cache.stride()[:3], *v_cache.stride()[:3]), window, sinks,
-            dim ** -0.5 if scale is None else scale, DTYPE_TO_CODE[q.dtype], DTYPE_TO_CODE[k_cache.dtype], _ptr(ws), nbytes)
+    _launch("ckh_paged_attention", q, q.data_ptr(), k, v, page_table.data_ptr(), lengths.data_ptr(), _ptr(k_scale),
+            _ptr(v_scale), out.data_ptr(), *sizes, _ptr(ws), nbytes)
     return out
+
+
+@functools.lru_cache(maxsize=512)
+def _write_plan(key_shape, key_stride, key_dtype, value_shape, value_stride, value_dtype, k_shape, k_stride, k_dtype, v_shape,
+                v_stride, v_dtype, slots, slots_dtype):
+    _cache_pair("paged_write", k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype)
+    tokens, kv_heads, dim = key_shape
+    pages, page_size = k_shape[:2]
+    if value_shape != key_shape or value_dtype != key_dtype or k_shape[2:] != key_shape[1:]:
+        raise ValueError(f"paged_write: key {list(key_shape)} {key_dtype}, value {list(value_shape)} {value_dtype} and "
+                         f"a cache {list(k_shape)} do not fit")
+    if k_dtype not in (key_dtype, torch.float8_e4m3fn):
+        raise ValueError(f"paged_write: {key_dtype} into a cache of {k_dtype}")
+    if dim % 16:
+        raise ValueError(f"paged_write: head_dim {dim} is not a multiple of 16")
+    if slots != tokens:
+        raise ValueError(f"paged_write: {slots} slots for {tokens} tokens")
+    if not (_on_rows16(key_stride, 2) and _on_rows16(value_stride, 2)):
+        return None
+    return (tokens, kv_heads, dim, pages, page_size, _strides(*key_stride[:2], *value_stride[:2], *k_stride[:3], *v_stride[:3]),
+            DTYPE_TO_CODE[key_dtype], DTYPE_TO_CODE[k_dtype], int(slots_dtype == torch.int64))
 
 
 def paged_write(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                 slots: torch.Tensor, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> None:
     _same_device("paged_write", key, value, k_cache, v_cache, slots)
-    _cache_pair("paged_write", k_cache, v_cache)
-    tokens, kv_heads, dim = key.shape
-    pages, page_size = k_cache.shape[:2]
-    if value.shape != key.shape or value.dtype != key.dtype or k_cache.shape[2:] != key.shape[1:]:
-        raise ValueError(f"paged_write: key {list(key.shape)} {key.dtype}, value {list(value.shape)} {value.dtype} and "
-                         f"a cache {list(k_cache.shape)} do not fit")
-    if k_cache.dtype not in (key.dtype, torch.float8_e4m3fn):
-        raise ValueError(f"paged_write: {key.dtype} into a cache of {k_cache.dtype}")
-    if dim % 16:
-        raise ValueError(f"paged_write: head_dim {dim} is not a multiple of 16")
-    if slots.shape[0] != tokens:
-        raise ValueError(f"paged_write: {slots.shape[0]} slots for {tokens} tokens")
-    key, value, slots = _rows16(key), _rows16(value), slots.contiguous()
+    rest = (k_cache.shape, k_cache.stride(), k_cache.dtype, v_cache.shape, v_cache.stride(), v_cache.dtype, slots.shape[0],
+            slots.dtype)
+    plan = _write_plan(key.shape, key.stride(), key.dtype, value.shape, value.stride(), value.dtype, *rest)
+    if plan is None or (key.data_ptr() | value.data_ptr()) & 15:
+        key, value = _rows16(key), _rows16(value)
+        plan = _write_plan(key.shape, key.stride(), key.dtype, value.shape, value.stride(), value.dtype, *rest)
+    k, v = _cache_pointers("paged_write", k_cache, v_cache)
     if k_scale is not None:
         k_scale = _scalar_on(k_scale, key.device, "k_scale")
     if v_scale is not None:
         v_scale = _scalar_on(v_scale, key.device, "v_scale")
-    _launch("ckh_paged_write", key, key.data_ptr(), value.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-            slots.data_ptr(), _ptr(k_scale), _ptr(v_scale), tokens, kv_heads, dim, pages, page_size,
-            _strides(*key.stride()[:2], *value.stride()[:2], *k_cache.stride()[:3], *v_cache.stride()[:3]),
-            DTYPE_TO_CODE[key.dtype], DTYPE_TO_CODE[k_cache.dtype], int(slots.dtype == torch.int64))
+    slots = slots.contiguous()
+    _launch("ckh_paged_write", key, key.data_ptr(), value.data_ptr(), k, v, slots.data_ptr(), _ptr(k_scale), _ptr(v_scale), *plan)
+
+
+@functools.lru_cache(maxsize=512)
+def _copy_plan(k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype, src_shape, src_dtype, dst_shape, dst_dtype):
+    _cache_pair("paged_copy", k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype)
+    if len(k_shape) not in (4, 5):
+        raise ValueError(f"paged_copy: a cache has 4 dimensions, or 5 with the layers first, got {len(k_shape)}")
+    if src_shape != dst_shape or src_dtype != dst_dtype:
+        raise ValueError(f"paged_copy: src {list(src_shape)} {src_dtype} and dst {list(dst_shape)} {dst_dtype} differ")
+    layers = k_shape[0] if len(k_shape) == 5 else 1
+    pages, page_size, kv_heads, dim = k_shape[-4:]
+    if dim * k_dtype.itemsize % 16:
+        raise ValueError(f"paged_copy: a head of {dim} elements is not a multiple of 16 bytes")
+    if layers == 1:
+        k_stride, v_stride = (0, *k_stride[-4:]), (0, *v_stride[-4:])
+    return (layers, src_shape[0], kv_heads, dim, pages, page_size, _strides(*k_stride[:4], *v_stride[:4]), k_dtype.itemsize,
+            int(src_dtype == torch.int64))
 
 
 def paged_copy(k_cache: torch.Tensor, v_cache: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
     _same_device("paged_copy", k_cache, v_cache, src, dst)
-    _cache_pair("paged_copy", k_cache, v_cache)
-    if k_cache.dim() not in (4, 5):
-        raise ValueError(f"paged_copy: a cache has 4 dimensions, or 5 with the layers first, got {k_cache.dim()}")
-    if src.shape != dst.shape or src.dtype != dst.dtype:
-        raise ValueError(f"paged_copy: src {list(src.shape)} {src.dtype} and dst {list(dst.shape)} {dst.dtype} differ")
-    layers = k_cache.shape[0] if k_cache.dim() == 5 else 1
-    pages, page_size, kv_heads, dim = k_cache.shape[-4:]
-    if dim * k_cache.element_size() % 16:
-        raise ValueError(f"paged_copy: a head of {dim} elements is not a multiple of 16 bytes")
+    k, v = _cache_pointers("paged_copy", k_cache, v_cache)
+    plan = _copy_plan(k_cache.shape, k_cache.stride(), k_cache.dtype, v_cache.shape, v_cache.stride(), v_cache.dtype,
+                      src.shape, src.dtype, dst.shape, dst.dtype)
     src, dst = src.contiguous(), dst.contiguous()
-    ks, vs = k_cache.stride(), v_cache.stride()
-    if layers == 1:
-        ks, vs = (0, *ks[-4:]), (0, *vs[-4:])
-    _launch("ckh_paged_copy", k_cache, k_cache.data_ptr(), v_cache.data_ptr(), src.data_ptr(), dst.data_ptr(), layers,
-            src.shape[0], kv_heads, dim, pages, page_size, _strides(*ks[:4], *vs[:4]), k_cache.element_size(),
-            int(src.dtype == torch.int64))
+    _launch("ckh_paged_copy", k_cache, k, v, src.data_ptr(), dst.data_ptr(), *plan)
+
+
+@functools.lru_cache(maxsize=512)
+def _window_plan(q_shape, q_stride, q_dtype, k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype, sequences, window, sinks,
+                 scale):
+    batch, queries, heads, dim = q_shape
+    keys, kv_heads = k_shape[1:3]
+    if k_shape != v_shape or k_shape[0] != batch or k_shape[3] != dim or kv_heads == 0 or heads % kv_heads:
+        raise ValueError(f"window_attention: q {list(q_shape)}, k {list(k_shape)} and v {list(v_shape)} do not fit")
+    if k_dtype != q_dtype or v_dtype != q_dtype:
+        raise ValueError(f"window_attention: q, k and v of different dtypes ({q_dtype}, {k_dtype}, {v_dtype})")
+    if dim not in (64, 96, 128, 256):
+        raise ValueError(f"window_attention: head_dim {dim} is not 64, 96, 128 or 256")
+    if window < 0 or sinks < 0:
+        raise ValueError(f"window_attention: window ({window}) and sinks ({sinks}) must not be negative")
+    if sequences is not None and sequences != batch:
+        raise ValueError(f"window_attention: {sequences} lengths for a batch of {batch}")
+    overlap = keys > 1 and min(k_stride[1], v_stride[1]) < dim  # broadcast keys have no rows of their own
+    if overlap or not (_on_rows16(q_stride, 2) and _on_rows16(k_stride, 2) and _on_rows16(v_stride, 2)):
+        return None
+    return (batch, queries, keys, heads, kv_heads, dim, _strides(*q_stride[:3], *k_stride[:3], *v_stride[:3]), window, sinks,
+            dim ** -0.5 if scale is None else scale, DTYPE_TO_CODE[q_dtype])
+
+
+def _own_rows16(t: torch.Tensor) -> torch.Tensor:
+    """_rows16 of keys or values, copied too where tokens share memory."""
+    return _rows16(t.contiguous() if t.shape[1] > 1 and t.stride(1) < t.shape[3] else t)
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int = 0, sinks: int = 0,
                      lengths: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
     _same_device("window_attention", q, k, v, lengths)
-    batch, queries, heads, dim = q.shape
-    keys, kv_heads = k.shape[1:3]
-    if k.shape != v.shape or k.shape[0] != batch or k.shape[3] != dim or kv_heads == 0 or heads % kv_heads:
-        raise ValueError(f"window_attention: q {list(q.shape)}, k {list(k.shape)} and v {list(v.shape)} do not fit")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise ValueError(f"window_attention: q, k and v of different dtypes ({q.dtype}, {k.dtype}, {v.dtype})")
-    if dim not in (64, 96, 128, 256):
-        raise ValueError(f"window_attention: head_dim {dim} is not 64, 96, 128 or 256")
-    if window < 0 or sinks < 0:
-        raise ValueError(f"window_attention: window ({window}) and sinks ({sinks}) must not be negative")
+    rest = (None if lengths is None else lengths.shape[0], window, sinks, scale)
+    plan = _window_plan(q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, *rest)
+    if plan is None or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+        q, k, v = _rows16(q), _own_rows16(k), _own_rows16(v)
+        plan = _window_plan(q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, *rest)
     if lengths is not None:
-        if lengths.shape[0] != batch:
-            raise ValueError(f"window_attention: {lengths.shape[0]} lengths for a batch of {batch}")
         lengths = lengths.contiguous()
-    q, k, v = _rows16(q), _rows16(k), _rows16(v)
-    if keys > 1:  # broadcast keys have no rows of their own
-        k = k.contiguous() if k.stride(1) < dim else k
-        v = v.contiguous() if v.stride(1) < dim else v
-    out = torch.empty((batch, queries, heads, dim), dtype=q.dtype, device=q.device)
-    _launch("ckh_window_attention", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(lengths), out.data_ptr(), batch,
-            queries, keys, heads, kv_heads, dim, _strides(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]), window, sinks,
-            dim ** -0.5 if scale is None else scale, DTYPE_TO_CODE[q.dtype])
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _launch("ckh_window_attention", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(lengths), out.data_ptr(), *plan)
     return out
 
 

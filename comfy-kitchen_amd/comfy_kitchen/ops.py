@@ -39,6 +39,7 @@ try:
     _forward_ad._current_level
     _registered = torch.library._impls  # "namespace/op/key" of every kernel registered from Python
     _registered.isdisjoint
+    _increment_version = _C._increment_version
     _OBSERVABLE = True
 except AttributeError:
     # A torch that lacks one of these (several are not public) gives no way to tell whether
@@ -54,11 +55,19 @@ class _Kernels(dict):
     """op name -> the entries that a program's own kernels for it make in torch's list."""
 
     def __missing__(self, op: str) -> frozenset:
-        entries = self[op] = frozenset(f"comfy_kitchen/{op}/{key}" for key in _KERNEL_KEYS)
+        entries = self[op] = frozenset(f"comfy_kitchen/{op}/{key}" for key in _KERNEL_KEYS) - _defined
         return entries
 
 
 _kernels = _Kernels()
+# What this module's own definitions put in torch's list (set behind them): an op that changes its
+# arguments has a kernel that counts the change.
+_defined: frozenset = frozenset()
+
+
+def changed(*tensors: torch.Tensor) -> None:
+    """Count a change of the tensors' memory, as that kernel does, where the custom op was skipped."""
+    _increment_version(tensors)
 
 
 def untouched(op: str) -> bool:
@@ -372,3 +381,7 @@ def apply_rope1(x: torch.Tensor, freqs_cis: torch.Tensor) -> torch.Tensor:
 @apply_rope1.register_fake
 def _(x, freqs_cis):
     return torch.empty_like(x)
+
+
+if _OBSERVABLE:
+    _defined = frozenset(entry for entry in _registered if entry.startswith("comfy_kitchen/"))

@@ -160,3 +160,17 @@ def test_random_walk_keeps_the_books(moved):
                 if t is not None:
                     assert store[pages[i // 4] * 4 + i % 4] == t
         assert c.free_pages == 24 - len(owned)
+
+
+def test_plain_calls_of_ops_that_change_their_arguments():
+    """They go past the custom op like the others, and count the change as it does."""
+    from comfy_kitchen.ops import changed, untouched
+
+    assert all(untouched(op) for op in ("paged_write", "paged_copy", "paged_attention"))
+    x = torch.zeros(3)
+    changed(x, x.view(3))
+    assert x._version == 2
+    with torch.inference_mode():
+        y = torch.zeros(2)
+        changed(y)
+    changed(y)
