@@ -82,7 +82,8 @@ SIGNATURES: dict[str, tuple] = {
     "ckh_paged_attention": (_i32, [_p] * 8 + [_i64] * 8 + [_p] + [_i64] * 2 + [_f32, _i32, _i32, _p, _i64, _u64]),
     "ckh_paged_write": (_i32, [_p] * 7 + [_i64] * 5 + [_p] + [_i32] * 3 + [_u64]),
     "ckh_paged_copy": (_i32, [_p] * 4 + [_i64] * 6 + [_p] + [_i32] * 2 + [_u64]),
-    "ckh_window_attention": (_i32, [_p] * 5 + [_i64] * 6 + [_p] + [_i64] * 2 + [_f32, _i32, _u64]),
+    "ckh_window_attention_workspace_bytes": (_i64, [_i64] * 8),
+    "ckh_window_attention": (_i32, [_p] * 5 + [_i64] * 6 + [_p] + [_i64] * 2 + [_f32, _i32, _p, _i64, _u64]),
 }
 ABI_VERSION = 8
 # CKH_AMAX_WORKSPACE_BYTES of include/ckh.h: the workspace ckh_amax_scale takes
@@ -659,8 +660,9 @@ def _window_plan(q_shape, q_stride, q_dtype, k_shape, k_stride, k_dtype, v_shape
     overlap = keys > 1 and min(k_stride[1], v_stride[1]) < dim  # broadcast keys have no rows of their own
     if overlap or not (_on_rows16(q_stride, 2) and _on_rows16(k_stride, 2) and _on_rows16(v_stride, 2)):
         return None
-    return (batch, queries, keys, heads, kv_heads, dim, _strides(*q_stride[:3], *k_stride[:3], *v_stride[:3]), window, sinks,
-            dim ** -0.5 if scale is None else scale, DTYPE_TO_CODE[q_dtype])
+    nbytes = int(_lib.ckh_window_attention_workspace_bytes(batch, queries, keys, heads, kv_heads, dim, window, sinks))
+    return ((batch, queries, keys, heads, kv_heads, dim, _strides(*q_stride[:3], *k_stride[:3], *v_stride[:3]), window, sinks,
+             dim ** -0.5 if scale is None else scale, DTYPE_TO_CODE[q_dtype]), nbytes)
 
 
 def _own_rows16(t: torch.Tensor) -> torch.Tensor:
@@ -678,8 +680,11 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
         plan = _window_plan(q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, *rest)
     if lengths is not None:
         lengths = lengths.contiguous()
+    sizes, nbytes = plan
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _launch("ckh_window_attention", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(lengths), out.data_ptr(), *plan)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _launch("ckh_window_attention", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(lengths), out.data_ptr(), *sizes,
+            _ptr(ws), nbytes)
     return out
 
 

@@ -15,7 +15,14 @@
 //   - V is stored by token, its operand holds 4 + 4 tokens of one d: the transposing LDS read
 //     delivers that (16 lanes give 4 tokens by 16 d).  16-byte pieces are placed so that neither
 //     it nor K's reads meet on a bank.
-//   - Tiles without a visible pair are not visited; only tiles with masked pairs pay for masks.
+//   - Tiles without a visible pair are not visited; only tiles with masked pairs pay for masks, and
+//     only for the bounds that cut them (777 tokens of 24 heads, head_dim 64, window 256: 13.1 us,
+//     16.8 with one test of the whole condition).
+//   - Where there are fewer workgroups than CUs, a workgroup's tiles are split over several, which
+//     leave their fp32 sums to a second launch that joins them in order (2 x 3 queries of 40 heads
+//     over 6000 keys: 28 us, 150 by one workgroup a block).
+//   - A third buffer of tiles, the compiler's wait for the next tile before V is read taken away:
+//     slower (4096 tokens, 16 heads: 152 us against 129).
 //   - The maximum is only raised when a score passes it by 2^8 (P stays below 2^8), P is rounded to
 //     the 16-bit type for the second product after its fp32 sum was taken.
 //   - A masked pair's weight is zero, but zero times an infinity is not: if a result is not
@@ -44,6 +51,9 @@ struct WindowArgs {
     int queries, keys, heads, kv_heads, group;
     int window, sinks;  // window INT32_MAX: none
     int row_blocks;     // blocks of rows of a key-value head
+    int splits;         // workgroups that share a block's tiles
+    float* part;        // their unnormalised outputs [splits][row][D], then maxima and sums [splits][row][2]
+    int64_t all_rows;   // rows of the call
     float scale;
     FastDiv by_group;
 };
@@ -99,7 +109,8 @@ __global__ __launch_bounds__(kWinWaves * 64, D == 256 ? 1 : 2) void window_kerne
     const int win_from = max(0, g_lo - a.window + 1) / kTileKeys;
     const int win_to = (max(key_end, 0) + kTileKeys - 1) / kTileKeys;
     const int sink_tiles = min((min(a.sinks, max(key_end, 0)) + kTileKeys - 1) / kTileKeys, win_from);
-    const int tiles = sink_tiles + max(0, win_to - win_from);
+    const int all = sink_tiles + max(0, win_to - win_from);
+    const int tile0 = all * blockIdx.y / gridDim.y, tiles = all * (blockIdx.y + 1) / gridDim.y;  // this workgroup's
 
     float c = a.scale * kLog2e;
     const uint32_t flip = c < 0.0f ? 0x80008000u : 0u;
@@ -158,14 +169,24 @@ __global__ __launch_bounds__(kWinWaves * 64, D == 256 ? 1 : 2) void window_kerne
         const bool edge = k0 + kTileKeys - 1 > w_lo || k0 + kTileKeys > len ||
                           !(k0 > w_hi - a.window || k0 + kTileKeys <= a.sinks);
         if (edge) {
+            // element e's key is at + its constant place: compared with the lane's bounds from there
+            const int at = k0 + 4 * g;
+            const int high = min(pos, len - 1) - at, low = pos - a.window + 1 - at, sink = a.sinks - at;
+            if (k0 + kTileKeys - 1 > w_lo || k0 + kTileKeys > len) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int j = k0 + h * 32 + 8 * (e >> 2) + 4 * g + (e & 3);
-                    const bool see = j <= pos && j < len && (pos - j < a.window || j < a.sinks);
-                    s[h][e] = see ? s[h][e] : -__builtin_inff();
-                }
+                    for (int e = 0; e < 16; ++e) s[h][e] = h * 32 + 8 * (e >> 2) + (e & 3) <= high ? s[h][e] : -__builtin_inff();
+            }
+            if (k0 <= w_hi - a.window) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int j = h * 32 + 8 * (e >> 2) + (e & 3);
+                        s[h][e] = j >= low || j < sink ? s[h][e] : -__builtin_inff();
+                    }
+            }
         }
         float top = s[0][0];
 #pragma unroll
@@ -262,9 +283,9 @@ __global__ __launch_bounds__(kWinWaves * 64, D == 256 ? 1 : 2) void window_kerne
         // (The buffers change hands as pointers: where the compiler sees which part of LDS a load
         // writes, it waits for the load before the next LDS read.)
         uint8_t *cur = lds, *next = lds + 2 * kTile;
-        if (tiles > 0) stage(0, cur);
+        if (tile0 < tiles) stage(tile0, cur);
 #pragma unroll 1
-        for (int i = 0; i < tiles; ++i) {
+        for (int i = tile0; i < tiles; ++i) {
             __asm__ volatile("" ::: "memory");
             __builtin_amdgcn_s_waitcnt(0);  // this wave's part of tile i has arrived
             __builtin_amdgcn_s_barrier();   // everyone's has, and nobody reads the other buffer
@@ -290,8 +311,21 @@ __global__ __launch_bounds__(kWinWaves * 64, D == 256 ? 1 : 2) void window_kerne
     if (redo) run(std::true_type{});
 
     if (row0 + r32 >= rows) return;
+    const int64_t out_row = (static_cast<int64_t>(b) * a.queries + qi) * a.heads + hq;
+    if (a.splits > 1) {
+        const int64_t at = blockIdx.y * a.all_rows + out_row;
+        float* op = a.part + at * D + g * 4;
+#pragma unroll
+        for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                *reinterpret_cast<v4f*>(op + n * 32 + e * 8) = v4f{acc[n][4 * e], acc[n][4 * e + 1], acc[n][4 * e + 2], acc[n][4 * e + 3]};
+        float* ml = a.part + a.splits * a.all_rows * D + at * 2;
+        if (g == 0) ml[0] = m, ml[1] = l;
+        return;
+    }
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
-    uint8_t* op = a.out + ((static_cast<int64_t>(b) * a.queries + qi) * a.heads + hq) * (D * 2) + g * 8;
+    uint8_t* op = a.out + out_row * (D * 2) + g * 8;
 #pragma unroll
     for (int n = 0; n < D / 32; ++n)
 #pragma unroll
@@ -301,12 +335,48 @@ __global__ __launch_bounds__(kWinWaves * 64, D == 256 ? 1 : 2) void window_kerne
         }
 }
 
+// Joins a row's splits: D / 4 lanes a row, four d a lane.
+template <int C, int D>
+__global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
+    constexpr int kLanes = D / 4, kRows = 256 / kLanes;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kLanes;
+    if (threadIdx.x >= kRows * kLanes || row >= a.all_rows) return;
+    const int d = threadIdx.x % kLanes * 4;
+    const float* ml = a.part + a.splits * a.all_rows * D;
+    float top = -1e30f, sum = 0.0f;
+    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[(s * a.all_rows + row) * 2]);
+    v4f o = v4f{0, 0, 0, 0};
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) {
+        const int64_t at = s * a.all_rows + row;
+        const float f = exp2_hw(ml[at * 2] - top);
+        sum += f * ml[at * 2 + 1];
+        o += f * *reinterpret_cast<const v4f*>(a.part + at * D + d);
+    }
+    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+    *reinterpret_cast<v2u*>(a.out + (row * D + d) * 2) = v2u{pack2<C>(o[0] * f, o[1] * f), pack2<C>(o[2] * f, o[3] * f)};
+}
+
+// Workgroups that share a block's tiles: enough for two a CU, of four tiles at least.
+int window_splits(int64_t batch, int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads, int64_t window, int64_t sinks) {
+    const int64_t group = heads / kv_heads, grid = batch * kv_heads * cdiv(queries * group, kWinWaves * 32);
+    const int64_t span = std::min(queries, cdiv(kWinWaves * 32, group) + 1);  // positions of a workgroup's rows
+    const int64_t seen = window > 0 ? std::min(keys, window + span + std::min(sinks, keys)) : keys;
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({32, 2 * device_cus() / grid, seen / (4 * kTileKeys)})));
+}
+
+template <int C, int D>
+void launch_window(const WindowArgs& a, unsigned grid, hipStream_t st) {
+    window_kernel<C, D><<<dim3(grid, a.splits), kWinWaves * 64, 0, st>>>(a);
+    if (a.splits > 1) window_join_kernel<C, D><<<static_cast<unsigned>(cdiv(a.all_rows, 256 / (D / 4))), 256, 0, st>>>(a);
+}
+
 template <int C>
 void launch_window(int dim, const WindowArgs& a, unsigned grid, hipStream_t st) {
-    if (dim == 64) window_kernel<C, 64><<<grid, kWinWaves * 64, 0, st>>>(a);
-    else if (dim == 96) window_kernel<C, 96><<<grid, kWinWaves * 64, 0, st>>>(a);
-    else if (dim == 128) window_kernel<C, 128><<<grid, kWinWaves * 64, 0, st>>>(a);
-    else window_kernel<C, 256><<<grid, kWinWaves * 64, 0, st>>>(a);
+    if (dim == 64) launch_window<C, 64>(a, grid, st);
+    else if (dim == 96) launch_window<C, 96>(a, grid, st);
+    else if (dim == 128) launch_window<C, 128>(a, grid, st);
+    else launch_window<C, 256>(a, grid, st);
 }
 
 }  // namespace attn
@@ -314,10 +384,17 @@ void launch_window(int dim, const WindowArgs& a, unsigned grid, hipStream_t st) 
 
 using namespace ckh;
 
+extern "C" int64_t ckh_window_attention_workspace_bytes(int64_t batch, int64_t queries, int64_t keys, int64_t heads,
+                                                        int64_t kv_heads, int64_t dim, int64_t window, int64_t sinks) {
+    if (batch <= 0 || queries <= 0 || keys <= 0 || kv_heads <= 0 || heads < kv_heads || dim <= 0) return 0;
+    const int64_t s = attn::window_splits(batch, queries, keys, heads, kv_heads, window, sinks);
+    return s > 1 ? s * batch * queries * heads * (dim + 2) * 4 : 0;
+}
+
 extern "C" int ckh_window_attention(const void* q, const void* k, const void* v, const void* lengths, void* out,
                                     int64_t batch, int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads,
                                     int64_t dim, const int64_t* strides, int64_t window, int64_t sinks, float scale,
-                                    int code, uintptr_t stream) {
+                                    int code, void* workspace, int64_t workspace_bytes, uintptr_t stream) {
     CKH_REQUIRE(code == CKH_F16 || code == CKH_BF16, "window_attention: unsupported dtype %d", code);
     CKH_REQUIRE(dim == 64 || dim == 96 || dim == 128 || dim == 256, "window_attention: head_dim %lld is not 64, 96, 128 or 256",
                 static_cast<long long>(dim));
@@ -354,6 +431,11 @@ extern "C" int ckh_window_attention(const void* q, const void* k, const void* v,
     a.by_group = attn::fast_div(static_cast<uint32_t>(a.group));
     const int64_t grid = batch * kv_heads * a.row_blocks;
     CKH_REQUIRE(grid <= INT32_MAX, "window_attention: too many rows");
+    const int64_t need = ckh_window_attention_workspace_bytes(batch, queries, keys, heads, kv_heads, dim, window, sinks);
+    a.splits = need > 0 && workspace && workspace_bytes >= need && aligned(workspace, 16)
+                   ? attn::window_splits(batch, queries, keys, heads, kv_heads, window, sinks) : 1;
+    a.part = static_cast<float*>(workspace);
+    a.all_rows = batch * queries * heads;
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (code == CKH_BF16) attn::launch_window<CKH_BF16>(static_cast<int>(dim), a, static_cast<unsigned>(grid), st);
     else attn::launch_window<CKH_F16>(static_cast<int>(dim), a, static_cast<unsigned>(grid), st);

@@ -364,11 +364,15 @@ int ckh_paged_copy(void* k_cache, void* v_cache, const void* src, const void* ds
  * keys), and p - j < window or j < sinks; window 0: no window.  A query that sees nothing gives
  * zeros.  What a pair that is not visible holds has no influence, infinities and NaN included.
  * heads % kv_heads == 0; dim 64, 96, 128 or 256.  strides: q, k, v: batch, token, head each.
+ * The workspace of ckh_window_attention_workspace_bytes lets few rows' keys be split over the GPU (0:
+ * they are not); NULL or a short one is no error.
  */
+int64_t ckh_window_attention_workspace_bytes(int64_t batch, int64_t queries, int64_t keys, int64_t heads,
+                                             int64_t kv_heads, int64_t dim, int64_t window, int64_t sinks);
 int ckh_window_attention(const void* q, const void* k, const void* v, const void* lengths, void* out, int64_t batch,
                          int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim,
                          const int64_t* strides, int64_t window, int64_t sinks, float scale, int code,
-                         uintptr_t stream);
+                         void* workspace, int64_t workspace_bytes, uintptr_t stream);
 
 #ifdef __cplusplus
 }

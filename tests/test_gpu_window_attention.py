@@ -95,6 +95,21 @@ def test_long(hip):
     same(*inputs(1, 2500, 4100, 2, 2, 64, "f16"))
 
 
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+def test_few_rows_over_many_keys(d, hip):
+    """Keys split over workgroups: ranges without a visible pair, sinks in the first, rows that see
+    nothing, values that are not finite where they are not seen."""
+    same(*inputs(1, 1, 5000, 4, 2, d, "bf16"))
+    same(*inputs(2, 3, 3333, 5, 1, d, "f16"), window=2000, sinks=40)
+    same(*inputs(3, 7, 2100, 4, 4, d, "bf16"), window=0, sinks=0, lengths=[0, 900, 2098])
+    q, k, v = inputs(1, 40, 4000, 2, 1, d, "bf16")
+    w, bound = want(q, k, v, 1500, 0)
+    v[0, 3980] = float("inf")
+    got = ck.window_attention(q.cuda(), k.cuda(), v.cuda(), 1500).cpu()
+    check(got[:, :20], w[:, :20], bound[:, :20])
+    assert bool((got[:, 20:] == float("inf")).all())
+
+
 def test_large_scores_and_scales(hip):
     same(*inputs(1, 200, 200, 4, 2, 64, "bf16", spread=20.0))
     same(*inputs(1, 200, 200, 4, 2, 64, "f16", spread=8.0), window=100)
