@@ -417,22 +417,16 @@ def quantize_int4(w: torch.Tensor, group_size: int) -> tuple[torch.Tensor, torch
     return codes, scales
 
 
-def _int4_weight(name: str, codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None,
-                 group_size: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None, int, int]:
-    """The weight's tensors, contiguous and of the shapes that the codes ask for, with N and K."""
-    n, half = codes.shape
-    k = 2 * half
+def _check_groups(name: str, codes_shape, scales_shape, zeros_shape, group_size: int) -> None:
+    """Scales and zero points of the shape that the codes ask for."""
     if group_size < 32 or group_size % 32:
         raise ValueError(f"{name}: group_size must be a positive multiple of 32, got {group_size}")
-    shape = (n, -(-k // group_size))
-    if scales.shape != shape:
-        raise ValueError(f"{name}: scales must be {list(shape)} for codes {list(codes.shape)} and group_size "
-                         f"{group_size}, got {list(scales.shape)}")
-    if zeros is not None:
-        if zeros.shape != shape:
-            raise ValueError(f"{name}: zeros must be {list(shape)}, got {list(zeros.shape)}")
-        zeros = zeros.contiguous()
-    return _aligned(codes), scales.contiguous(), zeros, n, k
+    shape = (codes_shape[0], -(-2 * codes_shape[1] // group_size))
+    if scales_shape != shape:
+        raise ValueError(f"{name}: scales must be {list(shape)} for codes {list(codes_shape)} and group_size "
+                         f"{group_size}, got {list(scales_shape)}")
+    if zeros_shape is not None and zeros_shape != shape:
+        raise ValueError(f"{name}: zeros must be {list(shape)}, got {list(zeros_shape)}")
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -451,39 +445,67 @@ def _same_device(name: str, first: torch.Tensor, *others: torch.Tensor | None) -
 def dequantize_int4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None, group_size: int,
                     output_type: torch.dtype = torch.bfloat16) -> torch.Tensor:
     _same_device("dequantize_int4", codes, scales, zeros)
-    codes, scales, zeros, n, k = _int4_weight("dequantize_int4", codes, scales, zeros, group_size)
+    _check_groups("dequantize_int4", codes.shape, scales.shape, None if zeros is None else zeros.shape, group_size)
+    codes, scales = _aligned(codes), scales.contiguous()
+    zeros = None if zeros is None else zeros.contiguous()
+    n, k = codes.shape[0], 2 * codes.shape[1]
     out = torch.empty((n, k), dtype=output_type, device=codes.device)
     _launch("ckh_dequantize_int4", codes, codes.data_ptr(), scales.data_ptr(), _ptr(zeros), out.data_ptr(), n, k,
             group_size, DTYPE_TO_CODE[scales.dtype], DTYPE_TO_CODE[output_type])
     return out
 
 
-@functools.lru_cache(maxsize=256)
-def _int4_workspace_bytes(m: int, n: int, k: int, group: int) -> int:
-    return int(_lib.ckh_linear_int4_workspace_bytes(m, n, k, group))
+@functools.lru_cache(maxsize=512)
+def _linear_plan(x_shape, x_stride, x_dtype, codes_shape, scales_shape, scales_dtype, zeros_shape, group_size):
+    """The call's checks, and its sizes as the C side takes them: (out's shape, sizes, codes behind
+    them, workspace bytes), or None where x has to be copied."""
+    n, half = codes_shape
+    k = 2 * half
+    _check_groups("linear_int4", codes_shape, scales_shape, zeros_shape, group_size)
+    if x_shape[-1] != k:
+        raise ValueError(f"linear_int4: x has {x_shape[-1]} inputs, the weight {k}")
+    m = 1
+    for size in x_shape[:-1]:
+        m *= size
+    stride = k
+    if len(x_shape) == 2 and m > 1:
+        stride = x_stride[0]
+    elif len(x_shape) > 2 and m > 0:  # rows of one step, or a copy
+        step = 1
+        for size, s in zip(x_shape[-2::-1], x_stride[-2::-1]):
+            if size == 1:
+                continue
+            if step == 1:
+                stride, step = s, size
+            elif s != stride * step:
+                return None
+            else:
+                step *= size
+    if x_stride[-1] != 1 or stride % 8 or stride < k:
+        return None
+    nbytes = int(_lib.ckh_linear_int4_workspace_bytes(m, n, k, group_size))
+    return ((*x_shape[:-1], n), (m, n, k, stride, group_size, DTYPE_TO_CODE[x_dtype], DTYPE_TO_CODE[scales_dtype]), nbytes)
 
 
 def linear_int4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None,
                 bias: torch.Tensor | None = None, group_size: int = 128) -> torch.Tensor:
     _same_device("linear_int4", x, codes, scales, zeros, bias)
-    codes, scales, zeros, n, k = _int4_weight("linear_int4", codes, scales, zeros, group_size)
-    if x.shape[-1] != k:
-        raise ValueError(f"linear_int4: x has {x.shape[-1]} inputs, the weight {k}")
-    rows = x if x.dim() == 2 else x.reshape(-1, k)
-    m = rows.shape[0]
-    stride = rows.stride(0)
-    if rows.stride(1) != 1 or rows.data_ptr() % 16 or (m > 1 and (stride % 8 or stride < k)):
-        rows = rows.contiguous()
-        if rows.data_ptr() % 16:
-            rows = rows.clone()
-        stride = k
-    bias, bias_code = _bias_args(bias, n, x.device)
-    out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
-    nbytes = _int4_workspace_bytes(m, n, k, group_size) if m > 16 else 0
+    rest = (codes.shape, scales.shape, scales.dtype, None if zeros is None else zeros.shape, group_size)
+    plan = _linear_plan(x.shape, x.stride(), x.dtype, *rest)
+    if plan is None or x.data_ptr() % 16:
+        x = _aligned(x)
+        plan = _linear_plan(x.shape, x.stride(), x.dtype, *rest)
+    shape, sizes, nbytes = plan
+    codes, scales = _aligned(codes), scales.contiguous()
+    if zeros is not None:
+        zeros = zeros.contiguous()
+    bias_code = 0
+    if bias is not None:
+        bias, bias_code = _bias_args(bias, codes.shape[0], x.device)
+    out = torch.empty(shape, dtype=x.dtype, device=x.device)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-    _launch("ckh_linear_int4", rows, rows.data_ptr(), codes.data_ptr(), scales.data_ptr(), _ptr(zeros), _ptr(bias),
-            out.data_ptr(), m, n, k, stride if m > 1 else k, group_size, DTYPE_TO_CODE[x.dtype],
-            DTYPE_TO_CODE[scales.dtype], bias_code, _ptr(ws), nbytes)
+    _launch("ckh_linear_int4", x, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), _ptr(zeros), _ptr(bias),
+            out.data_ptr(), *sizes, bias_code, _ptr(ws), nbytes)
     return out
 
 
