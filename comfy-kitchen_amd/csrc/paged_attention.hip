@@ -31,7 +31,6 @@ namespace ckh {
 namespace attn {
 
 constexpr int kWaves = 4;
-constexpr int kMinTiles = 16;  // least tiles of a chunk where there are more chunks than one
 constexpr uint32_t kOut = 0x80000000u;
 
 struct PagedArgs {
@@ -46,7 +45,8 @@ struct PagedArgs {
     int64_t table_stride;
     int batch, heads, kv_heads, group, head_tiles;  // group: query heads of a key-value head
     int pages, page_size, max_pages, window, sinks;
-    int target;  // chunks wanted
+    int target;     // chunks wanted; 1: no splitting
+    int min_tiles;  // least tiles of a chunk, where a unit has several
     float scale;
     FastDiv by_page;
 };
@@ -95,7 +95,7 @@ __device__ __forceinline__ Place find_chunk(const PagedArgs& a, int at, int unit
     for (int i = 64; i < a.batch; i += 64)
         total += __shfl(wave_scan(i + lane < a.batch ? Visible(a, a.lengths[i + lane]).tiles : 0, lane), 63, 64);
     const int64_t want = (total * units + a.target - 1) / a.target;
-    p.size = static_cast<int>(min(max(want, static_cast<int64_t>(kMinTiles)), static_cast<int64_t>(1) << 30));
+    p.size = static_cast<int>(min(max(want, static_cast<int64_t>(a.min_tiles)), static_cast<int64_t>(1) << 30));
     int before = 0;
     for (int i = 0; i < a.batch; i += 64) {
         const int n = i == 0 ? length : i + lane < a.batch ? a.lengths[i + lane] : 0;
@@ -482,15 +482,24 @@ __global__ __launch_bounds__(256) void join_kernel(PagedArgs a) {
     }
 }
 
-// Workgroups that a call may need: the chunks wanted, one more a unit for their ragged ends, and
-// no more than the cache has chunks.
-int64_t paged_slots(int64_t units, int64_t capacity, int target) {
-    const int64_t most = cdiv(cdiv(capacity, 32) + 2, kMinTiles);  // a unit's, with the sinks' tiles
-    return std::min(units * most, units + target);
+// How a call is split, from what the host knows: the units and the tokens their tables can hold.
+struct Split {
+    int target, min_tiles;  // as in PagedArgs
+    int64_t slots;          // workgroups that the call may need
+};
+Split paged_split(int64_t units, int64_t capacity) {
+    const int64_t tiles = cdiv(capacity, 32) + 2;  // a unit's at most, with the sinks'
+    // Chunks of 16 tiles at least, four a wave: with 8 the joins cost more than the shorter chunks
+    // gain (4 x 30000 tokens of one head 24.5 us against 23.1) unless even chunks of 16 leave most of
+    // the CUs idle (4000 tokens of 8 heads: 11.9 against 15.5).
+    const int min_tiles = units * tiles < 8 * device_cus() && tiles > 32 ? 8 : 16;
+    if (tiles <= min_tiles) return {1, min_tiles, units};
+    // Two or three workgroups are resident on a CU; four a CU even out their ends (48 ragged
+    // sequences in bf16: 168 us; three 175; eight 165, but 64 windows of 1024 tokens 68 for 60).
+    // Each unit may have one chunk more for its ragged end.
+    const int target = std::max(2, 4 * device_cus());
+    return {target, min_tiles, std::min(units * cdiv(tiles, min_tiles), units + target)};
 }
-
-// Chunks wanted: two workgroups are resident on a CU, and four rounds of them even out the ends.
-int paged_target() { return 4 * device_cus(); }
 
 template <int QC, int D, bool F8>
 void launch_paged(const PagedArgs& a, int64_t slots, bool join, hipStream_t st) {
@@ -519,9 +528,9 @@ static int64_t paged_units(int64_t batch, int64_t heads, int64_t kv_heads) {
 extern "C" int64_t ckh_paged_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim,
                                                        int64_t page_size, int64_t max_pages) {
     if (batch <= 0 || heads <= 0 || kv_heads <= 0 || dim <= 0 || page_size <= 0 || max_pages < 0) return 0;
-    const int64_t units = paged_units(batch, heads, kv_heads), capacity = page_size * max_pages;
-    if (cdiv(cdiv(capacity, 32) + 2, attn::kMinTiles) <= 1) return 0;  // always one chunk
-    return attn::paged_slots(units, capacity, attn::paged_target()) * 16 * (dim + 2) * 4 + units * 8;
+    const int64_t units = paged_units(batch, heads, kv_heads);
+    const attn::Split split = attn::paged_split(units, page_size * max_pages);
+    return split.target == 1 ? 0 : split.slots * 16 * (dim + 2) * 4 + units * 8;
 }
 
 extern "C" int ckh_paged_attention(const void* q, const void* k_cache, const void* v_cache, const void* page_table,
@@ -555,11 +564,12 @@ extern "C" int ckh_paged_attention(const void* q, const void* k_cache, const voi
     CKH_REQUIRE(aligned(q, 16) && aligned(k_cache, 16) && aligned(v_cache, 16) && aligned(out, 2) && aligned(page_table, 4) &&
                     aligned(lengths, 4) && aligned(k_scale, 4) && aligned(v_scale, 4),
                 "paged_attention: misaligned pointer");
-    const int64_t units = paged_units(batch, heads, kv_heads), capacity = page_size * max_pages;
+    const int64_t units = paged_units(batch, heads, kv_heads);
     CKH_REQUIRE(units <= (1 << 28), "paged_attention: too many heads and sequences");
     const int64_t need = ckh_paged_attention_workspace_bytes(batch, heads, kv_heads, dim, page_size, max_pages);
     // without a workspace every sequence is one chunk
-    const bool split = need > 0 && workspace && workspace_bytes >= need && aligned(workspace, 8);
+    attn::Split split = attn::paged_split(units, page_size * max_pages);
+    if (need > 0 && !(workspace && workspace_bytes >= need && aligned(workspace, 8))) split = {1, 16, units};
     attn::PagedArgs a{};
     a.q = static_cast<const uint8_t*>(q);
     a.k = static_cast<const uint8_t*>(k_cache);
@@ -578,19 +588,20 @@ extern "C" int ckh_paged_attention(const void* q, const void* k_cache, const voi
     a.group = static_cast<int>(heads / kv_heads), a.head_tiles = static_cast<int>(cdiv(a.group, 16));
     a.pages = static_cast<int>(pages), a.page_size = static_cast<int>(page_size), a.max_pages = static_cast<int>(max_pages);
     a.window = static_cast<int>(window), a.sinks = static_cast<int>(sinks);
-    a.target = split ? std::max(2, attn::paged_target()) : 1;
+    a.target = split.target, a.min_tiles = split.min_tiles;
     a.scale = scale;
     a.by_page = attn::fast_div(static_cast<uint32_t>(page_size));
-    const int64_t slots = split ? attn::paged_slots(units, capacity, a.target) : units;
-    if (split) a.plan = reinterpret_cast<int2*>(static_cast<uint8_t*>(workspace) + slots * 16 * (dim + 2) * 4);
+    const int64_t slots = split.slots;
+    const bool join = split.target > 1;
+    if (join) a.plan = reinterpret_cast<int2*>(static_cast<uint8_t*>(workspace) + slots * 16 * (dim + 2) * 4);
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const int d = static_cast<int>(dim);
     if (q_code == CKH_BF16) {
-        if (es == 1) attn::launch_paged<CKH_BF16, true>(d, a, slots, split, st);
-        else attn::launch_paged<CKH_BF16, false>(d, a, slots, split, st);
+        if (es == 1) attn::launch_paged<CKH_BF16, true>(d, a, slots, join, st);
+        else attn::launch_paged<CKH_BF16, false>(d, a, slots, join, st);
     } else {
-        if (es == 1) attn::launch_paged<CKH_F16, true>(d, a, slots, split, st);
-        else attn::launch_paged<CKH_F16, false>(d, a, slots, split, st);
+        if (es == 1) attn::launch_paged<CKH_F16, true>(d, a, slots, join, st);
+        else attn::launch_paged<CKH_F16, false>(d, a, slots, join, st);
     }
     return check_launch("paged_attention");
 }
