@@ -19,6 +19,7 @@
 //   - A workgroup owns 16 R weight rows; its waves split K and add their sums in LDS in wave
 //     order, so results do not depend on timing.
 #include <algorithm>
+#include <type_traits>
 
 #include "ckh_common.h"
 
@@ -65,12 +66,19 @@ __device__ __forceinline__ v4f mfma(v4u a, v4u b, v4f c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
-// The 8 codes of a word as B + q, in the order (k0 k4)(k1 k5)(k2 k6)(k3 k7).
+// The exponent bits of B for two values, held in a vector register: one and-or instruction takes a
+// constant from there and the mask from a scalar one, where two scalars would cost two instructions.
 template <int XC>
-__device__ __forceinline__ v4u widen(uint32_t w) {
-    constexpr uint32_t magic = XC == CKH_BF16 ? 0x43004300u : 0x64006400u;
-    return v4u{(w & 0x000f000fu) | magic, ((w >> 4) & 0x000f000fu) | magic, ((w >> 8) & 0x000f000fu) | magic,
-               ((w >> 12) & 0x000f000fu) | magic};
+__device__ __forceinline__ uint32_t base_bits() {
+    uint32_t v = XC == CKH_BF16 ? 0x43004300u : 0x64006400u;
+    __asm__("" : "+v"(v));
+    return v;
+}
+
+// The 8 codes of a word as B + q, in the order (k0 k4)(k1 k5)(k2 k6)(k3 k7).
+__device__ __forceinline__ v4u widen(uint32_t w, uint32_t base) {
+    return v4u{(w & 0x000f000fu) | base, ((w >> 4) & 0x000f000fu) | base, ((w >> 8) & 0x000f000fu) | base,
+               ((w >> 12) & 0x000f000fu) | base};
 }
 
 // 8 consecutive 16-bit activations in widen()'s order.
@@ -201,6 +209,7 @@ __global__ __launch_bounds__(W * 64) void linear_kernel(LinearArgs a) {
     for (int t = 0; t < T; ++t)
         ox[t] = static_cast<uint32_t>((min(t * 16 + r16, toks - 1) * a.x_stride + quarter * 8) * 2);
 
+    const uint32_t base = base_bits<XC>();
     const v4u ones = XC == CKH_BF16 ? v4u{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}
                                     : v4u{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
 
@@ -242,7 +251,7 @@ __global__ __launch_bounds__(W * 64) void linear_kernel(LinearArgs a) {
                 }
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    const v4u b = widen<XC>(d.w[r][j]);
+                    const v4u b = widen(d.w[r][j], base);
 #pragma unroll
                     for (int t = 0; t < T; ++t) acc[r][t] = mfma<XC>(d.x[t][j], b, fresh ? v4f{0, 0, 0, 0} : acc[r][t]);
                 }
@@ -347,6 +356,7 @@ __global__ __launch_bounds__(W * 64, MT > 1 && GB == 1 ? 3 : 4) void matvec_kern
 #pragma unroll
     for (int r = 0; r < R; ++r) ow[r] = min(r * 16 + r16, rows - 1) * pitch + quarter * 16;
 
+    const uint32_t base = base_bits<XC>();
     const v4u ones = XC == CKH_BF16 ? v4u{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}
                                     : v4u{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
 
@@ -367,7 +377,7 @@ __global__ __launch_bounds__(W * 64, MT > 1 && GB == 1 ? 3 : 4) void matvec_kern
                 const v4u x = xp[j * 4 * MT];
                 sum = mfma<XC>(x, ones, fresh ? v4f{0, 0, 0, 0} : sum);
 #pragma unroll
-                for (int r = 0; r < R; ++r) acc[r] = mfma<XC>(x, widen<XC>(w[r][j]), fresh ? v4f{0, 0, 0, 0} : acc[r]);
+                for (int r = 0; r < R; ++r) acc[r] = mfma<XC>(x, widen(w[r][j], base), fresh ? v4f{0, 0, 0, 0} : acc[r]);
             }
             if (j % GB == GB - 1 && j - (GB - 1) < blocks) {
                 const int g = a.group_of(s * 4 + j - (GB - 1)) - g0;
@@ -509,6 +519,7 @@ __global__ __launch_bounds__(256, 4) void tile_kernel(LinearArgs a) {
         for (int i = 0; i < kPer; ++i) xs[(s & 1) * kUnits + threadIdx.x + i * 256] = pair_order(d[i]);
     };
 
+    const uint32_t base = base_bits<XC>();
     const v4u ones = XC == CKH_BF16 ? v4u{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}
                                     : v4u{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
     v4f total[R][T];
@@ -517,7 +528,7 @@ __global__ __launch_bounds__(256, 4) void tile_kernel(LinearArgs a) {
 #pragma unroll
         for (int t = 0; t < T; ++t) total[r][t] = v4f{0, 0, 0, 0};
     const int g0 = a.group_of(first * 4);
-    const auto use = [&](const v4u (&codes)[R], int s, int blocks) __attribute__((always_inline)) {
+    const auto use = [&](const v4u (&codes)[R], int s, auto blocks) __attribute__((always_inline)) {
         v4f acc[R][T], sum[T];
         v4u c[R];
 #pragma unroll
@@ -529,7 +540,7 @@ __global__ __launch_bounds__(256, 4) void tile_kernel(LinearArgs a) {
                 const bool fresh = j % GB == 0;
                 v4u b[R];
 #pragma unroll
-                for (int r = 0; r < R; ++r) b[r] = widen<XC>(c[r][j]);
+                for (int r = 0; r < R; ++r) b[r] = widen(c[r][j], base);
 #pragma unroll
                 for (int t = 0; t < T; ++t) {
                     const v4u f = xp[(j * T + t) * 64];
@@ -570,7 +581,8 @@ __global__ __launch_bounds__(256, 4) void tile_kernel(LinearArgs a) {
             const int s = s0 + u;
             if (s >= last) break;
             load_x(x[u], s + D);  // past the range: unused, within the operand or zeros
-            use(w[u], s, min(4, (a.k >> 5) - s * 4));
+            if (s < a.k >> 7) use(w[u], s, std::integral_constant<int, 4>{});
+            else use(w[u], s, (a.k >> 5) - s * 4);
             load_codes(w[u], s + D);
             store_x(x[(u + 1) % D], s + 1);
             __syncthreads();
