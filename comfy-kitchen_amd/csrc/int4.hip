@@ -34,7 +34,9 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr int kScaleGroups = 128;  // groups whose scales are in LDS at a time
-constexpr int kTileRows = 32;       // activation rows of a workgroup of tile_kernel
+constexpr int kTileRows = 32;       // tile_kernel: activation rows of a workgroup
+constexpr int kTileWaves = 8;       // and its waves, of 16 weight rows each
+constexpr int kTileTarget = 3;      // half-workgroups wanted a CU
 constexpr int kMaxSplits = 16;
 constexpr int kVecCodes = 8192;    // matvec_kernel: codes whose activations are in LDS at a time, half as many for 4 rows
 
@@ -459,20 +461,24 @@ __global__ __launch_bounds__(W * 64, MT > 1 && GB == 1 ? 3 : 4) void matvec_kern
     }
 }
 
-// More rows: a workgroup takes 32 activation rows, 64 weight rows (four waves of 16) and one of
+// More rows: a workgroup takes 32 activation rows, 128 weight rows (eight waves of 16) and one of
 // `splits` ranges of K, and its waves share the activations, which go through LDS in the operand's
 // order (two buffers, a barrier a step): read by every wave itself they would cost more than the
 // codes.  Where K is split, the sums go to memory in fp32 and reduce_kernel adds them in order.
-// 24 rows, N = 5120, K = 13824: 24.7 us with 12 ranges, 26.9 with 6; linear_kernel 31.  No one unit
-// bounds it: codes, LDS, MFMAs (half of them the sums of x) and VALU take 4-6 us each, and the
-// second launch as much.  32 weight rows a wave, or a third step in flight, measured no better.
+// 24 rows, N = 5120, K = 13824 (35 MB of codes): 23.3 us, 1.6 TB/s.  Some 5 of them are the second
+// launch, 6 the way to the first step and back, the rest is bound by the loads: with the products
+// taken out it takes as long, without the activations' loads 5 us less, without the codes' 3.
+// 64 weight rows a workgroup 26 (64 rows, N = 13824, K = 5120: 42 against 34), six steps of codes in
+// flight 24.4, two 23.7; 256-byte runs of an activation row a load (whole lines) 25.1, for their
+// writes to LDS meet on banks; two or four workgroups' halves a CU 27.
 template <int XC, int GB>
-__global__ __launch_bounds__(256, 4) void tile_kernel(LinearArgs a) {
+__global__ __launch_bounds__(kTileWaves * 64, GB == 1 ? 3 : 4) void tile_kernel(LinearArgs a) {
     constexpr int T = kTileRows / 16, R = 1;  // 16-row tiles of activations, and of a wave's weight rows
-    constexpr int W = 4, D = 2;               // waves; steps in flight
+    constexpr int W = kTileWaves, D = 4, DX = 2;  // waves; steps of codes, of activations in flight
+    static_assert(D % DX == 0 && D % 2 == 0, "a step's registers and buffer are known by its place in the loop");
     constexpr int kRows = 16 * R * W;
     constexpr int kUnits = T * 256;       // 16-byte pieces of a step's activations
-    constexpr int kPer = kUnits / 256;    // a thread's
+    constexpr int kPer = kUnits / (W * 64);  // a thread's
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     v4u* xs = reinterpret_cast<v4u*>(lds);  // [2][block][tile][quarter][row]
     v2f(*sp)[16 * R * W + 1] = reinterpret_cast<v2f(*)[16 * R * W + 1]>(lds + 2 * kUnits * 16);
@@ -496,14 +502,14 @@ __global__ __launch_bounds__(256, 4) void tile_kernel(LinearArgs a) {
     uint32_t ow[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) ow[r] = min((wave * R + r) * 16 + r16, rows - 1) * pitch + quarter * 16;
-    // piece e of a step: block e / (64 T), tile, then quarter and row as the operand's lanes
+    // piece e of a step: its block and tile by the wave, its quarter and row as the operand's lanes
     uint32_t ox[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        const int e = threadIdx.x + i * 256, l = e & 63, t = (e >> 6) % T, j = (e >> 6) / T;
+        const int e = threadIdx.x + i * W * 64, l = e & 63, t = (e >> 6) % T, j = (e >> 6) / T;
         ox[i] = static_cast<uint32_t>((min(t * 16 + (l & 15), toks - 1) * a.x_stride + j * 32 + (l >> 4) * 8) * 2);
     }
-    v4u w[D][R], x[D][kPer];
+    v4u w[D][R], x[DX][kPer];
     const auto load_codes = [&](v4u (&d)[R], int s) __attribute__((always_inline)) {
 #pragma unroll
         for (int r = 0; r < R; ++r)
@@ -514,9 +520,9 @@ __global__ __launch_bounds__(256, 4) void tile_kernel(LinearArgs a) {
         for (int i = 0; i < kPer; ++i)
             d[i] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rx, ox[i], s * 256, 0));
     };
-    const auto store_x = [&](const v4u (&d)[kPer], int s) __attribute__((always_inline)) {
+    const auto store_x = [&](const v4u (&d)[kPer], int buffer) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) xs[(s & 1) * kUnits + threadIdx.x + i * 256] = pair_order(d[i]);
+        for (int i = 0; i < kPer; ++i) xs[buffer * kUnits + threadIdx.x + i * W * 64] = pair_order(d[i]);
     };
 
     const uint32_t base = base_bits<XC>();
@@ -528,12 +534,12 @@ __global__ __launch_bounds__(256, 4) void tile_kernel(LinearArgs a) {
 #pragma unroll
         for (int t = 0; t < T; ++t) total[r][t] = v4f{0, 0, 0, 0};
     const int g0 = a.group_of(first * 4);
-    const auto use = [&](const v4u (&codes)[R], int s, auto blocks) __attribute__((always_inline)) {
+    const auto use = [&](const v4u (&codes)[R], int s, int buffer, auto blocks) __attribute__((always_inline)) {
         v4f acc[R][T], sum[T];
         v4u c[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) c[r] = transpose_quarters(codes[r]);
-        const v4u* xp = xs + (s & 1) * kUnits + lane;
+        const v4u* xp = xs + buffer * kUnits + lane;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (j < blocks) {
@@ -569,24 +575,28 @@ __global__ __launch_bounds__(256, 4) void tile_kernel(LinearArgs a) {
     load_x(x[0], first);
     sl.load(a, n0, rows, wave, lane, g0, gn);
 #pragma unroll
-    for (int u = 0; u < D; ++u) load_codes(w[u], first + u);
+    for (int u = 1; u < DX; ++u) load_x(x[u], first + u);
 #pragma unroll
-    for (int u = 1; u < D; ++u) load_x(x[u], first + u);
-    store_x(x[0], first);
+    for (int u = 0; u < D; ++u) load_codes(w[u], first + u);
+    store_x(x[0], 0);
     sl.store(a, sp, rows, wave, lane, gn);
     __syncthreads();
-    for (int s0 = first; s0 < last; s0 += D) {
+    const int full = min(last, a.k >> 7);  // whole steps; K may end inside the last
+    for (int s0 = first; s0 < full; s0 += D) {
 #pragma unroll
         for (int u = 0; u < D; ++u) {
             const int s = s0 + u;
-            if (s >= last) break;
-            load_x(x[u], s + D);  // past the range: unused, within the operand or zeros
-            if (s < a.k >> 7) use(w[u], s, std::integral_constant<int, 4>{});
-            else use(w[u], s, (a.k >> 5) - s * 4);
+            if (s >= full) break;
+            load_x(x[u % DX], s + DX);  // past the range: unused, within the operand or zeros
+            use(w[u], s, u & 1, std::integral_constant<int, 4>{});
             load_codes(w[u], s + D);
-            store_x(x[(u + 1) % D], s + 1);
+            store_x(x[(u + 1) % DX], (u + 1) & 1);
             __syncthreads();
         }
+    }
+    if (full < last) {
+        load_codes(w[0], full);
+        use(w[0], full, (full - first) & 1, (a.k >> 5) - full * 4);
     }
 
 #pragma unroll
@@ -649,26 +659,27 @@ void launch_matvec(const LinearArgs& a, hipStream_t st) {
 }
 
 // Ranges of K for a call (1: not split), 0 where tile_kernel does not serve it: few rows, rows that
-// linear_kernel's 64-row workgroups serve better (32 rows, N = 13824: 25.9 against 27.7), or more
-// groups in a range than LDS holds.  Three workgroups a CU are wanted, of four steps at least.
+// linear_kernel's 64-row workgroups serve better (32 rows, N = 13824, K = 5120: 22.5 against 24), or
+// more groups in a range than LDS holds.  Three workgroups for two CUs are wanted, of four steps at
+// least.
 int tile_splits(int64_t m, int64_t n, int64_t k, int64_t group, bool may_split) {
     const int cus = device_cus();
     if (m <= 16 || (m <= 32 && n > 48 * cus)) return 0;
-    const int64_t blocks = cdiv(n, 64) * cdiv(m, kTileRows), steps = cdiv(k, 128);
-    int64_t s = std::min<int64_t>({kMaxSplits, cdiv(3 * cus, blocks), std::max<int64_t>(1, steps / 4)});
+    const int64_t blocks = cdiv(n, 16 * kTileWaves) * cdiv(m, kTileRows), steps = cdiv(k, 128);
+    int64_t s = std::min<int64_t>({kMaxSplits, cdiv(kTileTarget * cus, 2 * blocks), std::max<int64_t>(1, steps / 4)});
     s = may_split ? std::max(s, cdiv(steps, chunk_steps(group))) : 1;
     return s <= kMaxSplits && cdiv(steps, s) <= chunk_steps(group) ? static_cast<int>(s) : 0;
 }
 
 template <int XC>
 void launch_tile(const LinearArgs& a, hipStream_t st) {
-    const dim3 grid(static_cast<unsigned>(cdiv(a.n, 64)), static_cast<unsigned>(a.splits), static_cast<unsigned>(cdiv(a.m, kTileRows)));
+    const dim3 grid(static_cast<unsigned>(cdiv(a.n, 16 * kTileWaves)), static_cast<unsigned>(a.splits), static_cast<unsigned>(cdiv(a.m, kTileRows)));
     const int64_t codes = cdiv(cdiv(a.k, 128), a.splits) * 128;
     const int64_t groups = std::min<int64_t>({a.groups, kScaleGroups, codes / a.group + 2});
-    const size_t lds = 2 * kTileRows * 256 + groups * 65 * 8;  // two steps' activations, the scales
-    if (a.group % 128 == 0) tile_kernel<XC, 4><<<grid, 256, lds, st>>>(a);
-    else if (a.group % 64 == 0) tile_kernel<XC, 2><<<grid, 256, lds, st>>>(a);
-    else tile_kernel<XC, 1><<<grid, 256, lds, st>>>(a);
+    const size_t lds = 2 * kTileRows * 256 + groups * (16 * kTileWaves + 1) * 8;  // two steps' activations, the scales
+    if (a.group % 128 == 0) tile_kernel<XC, 4><<<grid, kTileWaves * 64, lds, st>>>(a);
+    else if (a.group % 64 == 0) tile_kernel<XC, 2><<<grid, kTileWaves * 64, lds, st>>>(a);
+    else tile_kernel<XC, 1><<<grid, kTileWaves * 64, lds, st>>>(a);
     if (a.splits > 1) reduce_kernel<XC><<<static_cast<unsigned>(cdiv(static_cast<int64_t>(a.m) * a.n, 256)), 256, 0, st>>>(a);
 }
 
@@ -680,8 +691,8 @@ void launch_tile(const LinearArgs& a, hipStream_t st) {
 //              under 128 (their scales would not fit the registers), 16
 //   5-16 rows  32 weight rows, 8 waves (16.7; 16 rows 19.9), 16 waves where there are fewer
 //              workgroups than CUs (N = K = 5120, 16 rows: 12.0 against 13.6)
-//   more       tile_kernel (64 rows: 39; 45 with 64 weight rows and 8 waves of linear_kernel), but
-//              linear_kernel for up to 32 rows of wide layers, and where tile_splits says so
+//   more       tile_kernel (64 rows: 34; linear_kernel 45), but linear_kernel, 64 weight rows a
+//              workgroup, for up to 32 rows of wide layers, and where tile_splits says so
 template <int XC>
 void linear(const LinearArgs& a, hipStream_t st) {
     const int cus = device_cus();
