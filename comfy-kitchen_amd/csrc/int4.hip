@@ -219,17 +219,18 @@ __global__ __launch_bounds__(W * 64) void linear_kernel(LinearArgs a) {
         v4u w[R], x[T][4];
     };
     // Step s's loads.  Where K ends inside the step, words of later codes (of the next row, or
-    // zeros past the operand) arrive, which use() leaves alone.
+    // zeros past the operand) arrive, which use() leaves alone.  (A step's place is part of the offset
+    // that the descriptor's bounds are checked for; the instruction's scalar offset is not.)
     const auto load = [&](Step& d, int s) {
         const int kq = s * 128;
 #pragma unroll
         for (int r = 0; r < R; ++r)
-            d.w[r] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rw, ow[r], kq >> 1, 0));
+            d.w[r] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rw, ow[r] + (kq >> 1), 0, 0));
 #pragma unroll
         for (int t = 0; t < T; ++t)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                d.x[t][j] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rx, ox[t] + j * 64, kq * 2, 0));
+                d.x[t][j] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rx, ox[t] + kq * 2 + j * 64, 0, 0));
     };
     v4f total[R][T];
 #pragma unroll
@@ -405,7 +406,7 @@ __global__ __launch_bounds__(W * 64, MT > 1 && GB == 1 ? 3 : 4) void matvec_kern
         const auto load = [&](v4u (&d)[R], int s) {
 #pragma unroll
             for (int r = 0; r < R; ++r)
-                d[r] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(s < last ? rw : none, ow[r], s * 64, 0));
+                d[r] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(s < last ? rw : none, ow[r] + s * 64, 0, 0));
         };
         // activations and scales first, codes behind them
         g0 = a.group_of(c0 * 4);
@@ -513,12 +514,12 @@ __global__ __launch_bounds__(kTileWaves * 64, GB == 1 ? 3 : 4) void tile_kernel(
     const auto load_codes = [&](v4u (&d)[R], int s) __attribute__((always_inline)) {
 #pragma unroll
         for (int r = 0; r < R; ++r)
-            d[r] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(s < last ? rw : none, ow[r], s * 64, 0));
+            d[r] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(s < last ? rw : none, ow[r] + s * 64, 0, 0));
     };
     const auto load_x = [&](v4u (&d)[kPer], int s) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
-            d[i] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rx, ox[i], s * 256, 0));
+            d[i] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rx, ox[i] + s * 256, 0, 0));
     };
     const auto store_x = [&](const v4u (&d)[kPer], int buffer) __attribute__((always_inline)) {
 #pragma unroll
