@@ -82,7 +82,7 @@ class PagedKVCache:
 
     def _on_device(self, values, dtype=torch.int32) -> torch.Tensor:
         t = torch.tensor(values, dtype=dtype)
-        if self.k.is_cuda:
+        if self.k.is_cuda and t.numel():
             t = t.pin_memory()
         return t.to(self.k.device, non_blocking=True)
 

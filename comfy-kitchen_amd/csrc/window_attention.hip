@@ -18,6 +18,8 @@
 //   - Tiles without a visible pair are not visited; only tiles with masked pairs pay for masks, and
 //     only for the bounds that cut them (777 tokens of 24 heads, head_dim 64, window 256: 13.1 us,
 //     16.8 with one test of the whole condition).
+//     16384 tokens of 40 heads over 8, head_dim 128, window 4096: 1.18-1.34 ms (the clock varies),
+//     0.9-1.03 PF, against 1.33 PF of a 16384^3 product.
 //   - Where there are fewer workgroups than CUs, a workgroup's tiles are split over several, which
 //     leave their fp32 sums to a second launch that joins them in order (2 x 3 queries of 40 heads
 //     over 6000 keys: 28 us, 150 by one workgroup a block).

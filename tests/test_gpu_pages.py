@@ -191,3 +191,21 @@ def test_sequences_end_to_end(dtype, page, hip):
     for s in (a, b, c, e, f):
         cache.free(s)
     assert cache.free_pages == 60
+
+
+def test_sequences_of_no_tokens(hip):
+    cache = ck.PagedKVCache(1, 4, 16, 2, 64)
+    a, b = cache.add(), cache.add()
+    q = torch.randn(2, 4, 64, device="cuda").bfloat16()
+    assert cache.append([a, b], [0, 0]).shape == (0,)
+    out = cache.attend(0, q, *cache.tables([a, b]))  # a table without a column
+    assert out.shape == q.shape and bool((out == 0).all())
+    slots = cache.append([b], [1])
+    row = torch.randn(1, 2, 64, device="cuda").bfloat16()
+    cache.write(0, row, row, slots)
+    out = cache.attend(0, q, *cache.tables([a, b]))
+    assert bool((out[0] == 0).all()) and torch.equal(out[1], row[0].repeat_interleave(2, 0))
+    assert cache.attend(0, q[:0], *cache.tables([])).shape == (0, 4, 64)
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    ck.paged_write(row[:0], row[:0], cache.k[0], cache.v[0], none)
+    ck.paged_copy(cache.k, cache.v, none, none)
