@@ -206,14 +206,32 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void paged_kernel(Pa
         uint32_t k[2][L::NK * L::KD], v[8][L::VD];
         int base, lo, hi;  // tokens base .. base + 31, of which lo .. hi - 1 are visible
     };
-    // Tile i's loads; past the chunk's end they read nothing (or the last tile again).
-    const auto load = [&](Tile& t, int i) {
-        const bool live = i < t1;
+    const auto place_tile = [&](Tile& t, int i) {
         const int j = min(i, t1 - 1);
         const bool sink = j < vis.sink_tiles;
         t.base = (sink ? j : (vis.start >> 5) + j - vis.sink_tiles) * 32;
         t.lo = sink ? 0 : vis.start;
         t.hi = sink ? vis.sink_end : vis.len;
+    };
+    // Without whole pages: a lane's tokens in a tile (two of K, eight of V), taken into the visible
+    // ones, and their pages, which are looked up a tile ahead of the rows they lead to.
+    const auto token = [&](const Tile& t, int n) {
+        const int tk = t.base + (n < 2 ? n * 16 + r16 : ((n - 2) >> 2) * 16 + 4 * c + ((n - 2) & 3));
+        return max(t.lo, min(tk, t.hi - 1));
+    };
+    int page_of[WHOLE ? 1 : 10];
+    const auto look_up = [&](int i) {
+        if constexpr (!WHOLE) {
+            Tile t;
+            place_tile(t, i);
+#pragma unroll
+            for (int n = 0; n < 10; ++n) page_of[n] = table[a.by_page.div(token(t, n))];
+        }
+    };
+    // Tile i's loads; past the chunk's end they read nothing (or the last tile again).
+    const auto load = [&](Tile& t, int i) {
+        const bool live = i < t1;
+        place_tile(t, i);
         if constexpr (WHOLE) {
             __amdgpu_buffer_rsrc_t rk[2], rv[2];
             uint32_t ko[2], vo[8];
@@ -253,26 +271,25 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void paged_kernel(Pa
                                                               vo[e] + (L::base(1) + r16 * L::width(1)) * ES);
             }
         } else {
-            const auto row = [&](int token, const uint8_t* base, int64_t page_stride, int64_t tok_stride) {
-                const int tk = max(t.lo, min(token, t.hi - 1));  // visible tokens only
-                const int pi = a.by_page.div(tk), slot = tk - pi * a.page_size;
-                const int64_t page = min(static_cast<uint32_t>(table[pi]), static_cast<uint32_t>(a.pages - 1));
+            const auto row = [&](int n, const uint8_t* base, int64_t page_stride, int64_t tok_stride) {
+                const int tk = token(t, n), slot = tk - a.by_page.div(tk) * a.page_size;
+                const int64_t page = min(static_cast<uint32_t>(page_of[n]), static_cast<uint32_t>(a.pages - 1));
                 return base + (page * page_stride + slot * tok_stride) * ES;
             };
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint8_t* p = row(t.base + h * 16 + r16, kbase, a.k_page, a.k_tok) + c * L::KW * ES;
+                const uint8_t* p = row(h, kbase, a.k_page, a.k_tok) + c * L::KW * ES;
 #pragma unroll
                 for (int n = 0; n < L::NK; ++n) fetch<L::KD, false>(t.k[h] + n * L::KD, p + n * 4 * L::KW * ES);
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int tv = t.base + (e >> 2) * 16 + 4 * c + (e & 3);
-                const uint8_t* p = row(tv, vbase, a.v_page, a.v_tok);
+                const uint8_t* p = row(2 + e, vbase, a.v_page, a.v_tok);
                 fetch<L::words(0), L::width(0) * ES == 2>(t.v[e], p + r16 * L::width(0) * ES);
                 if constexpr (L::SETS > 1)
                     fetch<L::words(1), L::width(1) * ES == 2>(t.v[e] + L::at(1), p + (L::base(1) + r16 * L::width(1)) * ES);
             }
+            look_up(i + kWaves);
         }
     };
 
@@ -372,6 +389,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void paged_kernel(Pa
     if (t0 + wave < t1) {
         Tile x, y;
         int i = t0 + wave;
+        look_up(i);
         load(x, i);
         for (;;) {
             load(y, i + kWaves);
