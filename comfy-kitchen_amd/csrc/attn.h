@@ -23,6 +23,11 @@ typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// The power of two that the largest weight is held at, at least: f16 has no normal numbers under 2^-14,
+// and many far weights under that may together outweigh the near ones, so its weights sit at 2^7 .. 2^15.
+template <int C>
+constexpr float kLift = C == CKH_F16 ? 7.0f : 0.0f;
+
 template <int C>
 __device__ __forceinline__ v4f mfma16(v4u a, v4u b, v4f c) {
     if constexpr (C == CKH_BF16)

@@ -25,7 +25,7 @@
 //     over 6000 keys: 28 us, 150 by one workgroup a block).
 //   - A third buffer of tiles, the compiler's wait for the next tile before V is read taken away:
 //     slower (4096 tokens, 16 heads: 152 us against 129).
-//   - The maximum is only raised when a score passes it by 2^8 (P stays below 2^8), P is rounded to
+//   - The maximum is only raised when a weight would pass 2^8 (in f16 2^15, attn.h), P is rounded to
 //     the 16-bit type for the second product after its fp32 sum was taken.
 //   - A masked pair's weight is zero, but zero times an infinity is not: if a result is not
 //     finite, the workgroup runs again and keeps values that are not finite out of the
@@ -196,9 +196,9 @@ __global__ __launch_bounds__(W * 64, D == 256 ? 1 : 2) void window_kernel(Window
 #pragma unroll
         for (int e = 0; e < 16; ++e) top = fmaxf(top, s[1][e]);
         top *= c;
-        if (__any(top > m + 8.0f)) {
+        if (__any(top > m + kLift<C> + 8.0f)) {
             top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float to = fmaxf(m, top);
+            const float to = fmaxf(m, top - kLift<C>);
             const float f = exp2_hw(m - to);
             m = to;
             l *= f;
@@ -206,13 +206,15 @@ __global__ __launch_bounds__(W * 64, D == 256 ? 1 : 2) void window_kernel(Window
             for (int n = 0; n < D / 32; ++n) acc[n] *= f;
         }
         v4u p[4];
+        float sum = 0.0f;  // the tile's own: single small weights would be lost in a large l
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 s[h][e] = exp2_hw(__fmaf_rn(s[h][e], c, -m));
-                l += s[h][e];
+                sum += s[h][e];
             }
+        l += sum;
 #pragma unroll
         for (int w = 0; w < 4; ++w)
 #pragma unroll

@@ -11,8 +11,9 @@ import torch
 UNIT = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 
 
-def attend(q, k, v, scale, dtype):
-    """q [..., d], k and v [n, d] in 64 bits -> (o, bound); no keys give zeros."""
+def attend(q, k, v, scale, dtype, largest=1.0):
+    """q [..., d], k and v [n, d] in 64 bits -> (o, bound); no keys give zeros.  largest: what the
+    largest weight is held at, at least."""
     if k.shape[0] == 0:
         return torch.zeros_like(q), torch.zeros_like(q)
     s = q @ k.t() * scale
@@ -23,7 +24,7 @@ def attend(q, k, v, scale, dtype):
     size = (q.abs() @ k.abs().t()).amax(-1, keepdim=True) * abs(scale)
     bound = 1.01 * UNIT[dtype] * (o.abs() + mass) + 2.0 ** -16 * (1 + size) * mass + 1e-7
     if dtype == torch.float16:
-        bound = bound + k.shape[0] * 2.0 ** -25 * v.abs().amax() / total
+        bound = bound + k.shape[0] * 2.0 ** -25 / largest * v.abs().amax() / total
     return o, bound
 
 

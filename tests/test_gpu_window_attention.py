@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import comfy_kitchen as ck
-from attention_ref import UNIT, check
+from attention_ref import UNIT, attend, check
 
 pytestmark = pytest.mark.gpu
 
@@ -116,6 +116,23 @@ def test_large_scores_and_scales(hip):
     q, k, v = inputs(1, 100, 130, 2, 1, 128, "bf16")
     same(q, k, v, scale=-0.3)
     same(q, k, v, scale=0.0)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_many_small_weights(dtype, hip):
+    """One near key among far ones whose weights e^-far add up; f16 has 2^-24 for e^-16.25 = 1.47 2^-24,
+    so its weights are held 2^7 larger."""
+    g = torch.Generator().manual_seed(2)
+    n, d, heads, rows = 400000, 64, 64, 512
+    k = torch.zeros(n, d)
+    k[100, 0] = 16.25
+    v = torch.randn(n, d, generator=g) + 1
+    v[100] = -3.0
+    q = torch.zeros(1, rows, heads, d)
+    q[..., 0] = 8.0  # scale 1/8
+    k, v, q = (x.to(DT[dtype]) for x in (k, v, q))
+    got = ck.window_attention(q.cuda(), k.cuda()[None, :, None], v.cuda()[None, :, None])[0, -1]
+    check(got, *attend(q[0, -1].double(), k.double(), v.double(), 0.125, DT[dtype], 2.0 ** 7))
 
 
 def test_strides(hip):
