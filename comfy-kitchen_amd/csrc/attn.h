@@ -60,18 +60,5 @@ __device__ __forceinline__ uint32_t widen_e4m3(uint32_t w) {
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// n / d for n < 2^31 and the d >= 1 that made the constants.
-struct FastDiv {
-    uint32_t mul, shift;  // mul 0: d is 1
-    __device__ __forceinline__ uint32_t div(uint32_t n) const {
-        return mul ? static_cast<uint32_t>((static_cast<uint64_t>(n) * mul) >> 32) >> shift : n;
-    }
-};
-inline FastDiv fast_div(uint32_t d) {
-    if (d <= 1) return {0u, 0u};
-    uint32_t s = 31 - __builtin_clz(d - 1);  // ceil(log2 d) - 1
-    return {static_cast<uint32_t>(((uint64_t(1) << (32 + s)) + d - 1) / d), s};
-}
-
 }  // namespace attn
 }  // namespace ckh

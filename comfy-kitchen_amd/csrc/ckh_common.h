@@ -32,6 +32,21 @@ inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintp
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t rup(int64_t a, int64_t b) { return cdiv(a, b) * b; }
 
+// n / d, exactly, for n < 2^31 and the d >= 1 that made the constants: with l = ceil(log2 d) and
+// mul = ceil(2^(31 + l) / d), mul d exceeds 2^(31 + l) by less than 2^l, so n mul / 2^(31 + l) is less
+// than 1 / d above n / d.
+struct FastDiv {
+    uint32_t mul, shift;  // mul 0: d is 1
+    __host__ __device__ __forceinline__ uint32_t div(uint32_t n) const {
+        return mul ? static_cast<uint32_t>((static_cast<uint64_t>(n) * mul) >> 32) >> shift : n;
+    }
+};
+inline FastDiv fast_div(uint32_t d) {
+    if (d <= 1) return {0u, 0u};
+    uint32_t s = 31 - __builtin_clz(d - 1);  // ceil(log2 d) - 1
+    return {static_cast<uint32_t>(((uint64_t(1) << (32 + s)) + d - 1) / d), s};
+}
+
 // --------------------------------------------------------- bit reinterpret
 __device__ __forceinline__ float as_f(uint32_t u) { return __uint_as_float(u); }
 __device__ __forceinline__ uint32_t as_u(float f) { return __float_as_uint(f); }

@@ -49,14 +49,14 @@ struct LinearArgs {
     void* y;
     int64_t x_stride;  // elements between activation rows
     int m, n, k, groups, group;
-    uint32_t per_group;  // ceil(2^32 / (group / 32)): block b of 32 codes is in group (b * per_group) >> 32
+    FastDiv by_group;  // by the blocks of 32 codes of a group
     int chunk;  // steps of 128 codes whose groups fit kScaleGroups
     int scale_code, bias_code;
     int splits;   // tile_kernel: ranges of K
     float* part;  // their sums, [splits][m][n]
 
     __device__ __forceinline__ int group_of(uint32_t block) const {
-        return per_group ? static_cast<int>((static_cast<uint64_t>(block) * per_group) >> 32) : static_cast<int>(block);
+        return static_cast<int>(by_group.div(block));
     }
 };
 
@@ -876,7 +876,7 @@ extern "C" int ckh_linear_int4(const void* x, const void* codes, const void* sca
     a.bias = bias, a.y = y, a.x_stride = m == 1 ? k : x_stride;
     a.m = static_cast<int>(m), a.n = static_cast<int>(n), a.k = static_cast<int>(k);
     a.groups = static_cast<int>(cdiv(k, group)), a.group = static_cast<int>(group);
-    a.per_group = group == 32 ? 0u : static_cast<uint32_t>(cdiv(int64_t(1) << 32, group / 32));
+    a.by_group = fast_div(static_cast<uint32_t>(group / 32));
     a.chunk = i4::chunk_steps(group);
     a.scale_code = scale_code, a.bias_code = bias_code;
     a.splits = i4::tile_splits(m, n, k, group, split);

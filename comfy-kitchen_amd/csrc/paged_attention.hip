@@ -614,7 +614,7 @@ extern "C" int ckh_paged_attention(const void* q, const void* k_cache, const voi
     a.window = static_cast<int>(window), a.sinks = static_cast<int>(sinks);
     a.target = split.target, a.min_tiles = split.min_tiles;
     a.scale = scale;
-    a.by_page = attn::fast_div(static_cast<uint32_t>(page_size));
+    a.by_page = fast_div(static_cast<uint32_t>(page_size));
     const int64_t slots = split.slots;
     const bool join = split.target > 1;
     if (join) a.plan = reinterpret_cast<int2*>(static_cast<uint8_t*>(workspace) + slots * 16 * (dim + 2) * 4);

@@ -15,12 +15,11 @@
 // ordinary accesses.  write stores past the caches too (32000 tokens, 262 MB: 48.3 us, 51.3 without)
 // but reads its keys and values through them, where the prompt's attention finds them.  More pieces a thread are slower (two layers' 187, four pieces of a row's
 // K or V 185).
-#include "attn.h"
+#include "ckh_common.h"
 
 namespace ckh {
 namespace pages {
 
-using attn::FastDiv;
 typedef unsigned v4u __attribute__((ext_vector_type(4)));
 typedef unsigned v2u __attribute__((ext_vector_type(2)));
 
@@ -154,10 +153,10 @@ extern "C" int ckh_paged_write(const void* key, const void* value, void* k_cache
         a.x_tok[n] = strides[2 * n] * 2, a.x_head[n] = strides[2 * n + 1] * 2;
         a.to[n] = {strides[4 + 3 * n] * es, strides[5 + 3 * n] * es, strides[6 + 3 * n] * es};
     }
-    a.slots = {slots, wide_slots != 0, pages * page_size, attn::fast_div(static_cast<uint32_t>(page_size)), static_cast<int>(page_size)};
+    a.slots = {slots, wide_slots != 0, pages * page_size, fast_div(static_cast<uint32_t>(page_size)), static_cast<int>(page_size)};
     a.pieces = tokens * row;
     a.row = static_cast<int>(row), a.head = static_cast<int>(dim / 8);
-    a.by_row = attn::fast_div(a.row), a.by_head = attn::fast_div(a.head);
+    a.by_row = fast_div(a.row), a.by_head = fast_div(a.head);
     const unsigned grid = static_cast<unsigned>(cdiv(a.pieces, 256));
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (es == 2) pages::write_kernel<CKH_BF16, false><<<grid, 256, 0, st>>>(a);  // 16 bits are moved as they are
@@ -192,12 +191,12 @@ extern "C" int ckh_paged_copy(void* k_cache, void* v_cache, const void* src, con
         a.layer[n] = strides[4 * n] * element_bytes;
         a.st[n] = {strides[4 * n + 1] * element_bytes, strides[4 * n + 2] * element_bytes, strides[4 * n + 3] * element_bytes};
     }
-    a.src = {src, wide_slots != 0, pages * page_size, attn::fast_div(static_cast<uint32_t>(page_size)), static_cast<int>(page_size)};
+    a.src = {src, wide_slots != 0, pages * page_size, fast_div(static_cast<uint32_t>(page_size)), static_cast<int>(page_size)};
     a.dst = a.src;
     a.dst.at = dst;
     a.pieces = static_cast<uint32_t>(rows * row);
     a.row = static_cast<int>(row), a.head = static_cast<int>(head);
-    a.by_row = attn::fast_div(a.row), a.by_head = attn::fast_div(a.head);
+    a.by_row = fast_div(a.row), a.by_head = fast_div(a.head);
     const dim3 grid(static_cast<unsigned>(cdiv(a.pieces, 256)), static_cast<unsigned>(layers));
     pages::copy_kernel<<<grid, 256, 0, reinterpret_cast<hipStream_t>(stream)>>>(a);
     return check_launch("paged_copy");

@@ -442,7 +442,7 @@ extern "C" int ckh_window_attention(const void* q, const void* k, const void* v,
     const int waves = attn::window_waves(batch, queries, heads, kv_heads);
     a.row_blocks = static_cast<int>(cdiv(queries * a.group, waves * 32));
     a.scale = scale;
-    a.by_group = attn::fast_div(static_cast<uint32_t>(a.group));
+    a.by_group = fast_div(static_cast<uint32_t>(a.group));
     const int64_t grid = batch * kv_heads * a.row_blocks;
     CKH_REQUIRE(grid <= INT32_MAX, "window_attention: too many rows");
     const int64_t need = ckh_window_attention_workspace_bytes(batch, queries, keys, heads, kv_heads, dim, window, sinks);

@@ -89,3 +89,6 @@ extern "C" int ckh_skinny_forms(int nv) {
 extern "C" int ckh_nv_quantize_fast_rows(int64_t rows, int64_t orig_rows, int64_t cols) {
     return nv_quantize_fast_rows(rows, orig_rows, cols);
 }
+
+// n / d as the kernels divide.
+extern "C" uint32_t ckh_fast_div(uint32_t n, uint32_t d) { return fast_div(d).div(n); }

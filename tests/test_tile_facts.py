@@ -74,3 +74,15 @@ def test_nvfp4_quantize_of_padded_rows(rows, cols, fast):
     f = library().ckh_nv_quantize_fast_rows
     f.argtypes = [ctypes.c_int64] * 3
     assert f(-(-rows // 16) * 16, rows, cols) == fast
+
+
+def test_division_by_constants():
+    """n / d as the kernels divide is exact for n < 2^31, next to multiples of d above all."""
+    f = library().ckh_fast_div
+    f.argtypes, f.restype = [ctypes.c_uint32] * 2, ctypes.c_uint32
+    top = 2 ** 31 - 1
+    for d in (1, 2, 3, 5, 7, 32, 33, 1000, 4097, 40001, 65535, 65537, 131073, 2 ** 18, 2 ** 30 - 1, 2 ** 30 + 1, top):
+        multiples = {top // d, *range(1, 6), *(top // d // j for j in (2, 3, 7, 1000))}
+        for n in {0, top, *(q * d + r for q in multiples for r in (-1, 0, 1))}:
+            if 0 <= n <= top:
+                assert f(n, d) == n // d, (n, d)
