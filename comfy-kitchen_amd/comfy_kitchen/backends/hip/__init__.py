@@ -455,12 +455,25 @@ def dequantize_int4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tens
     return out
 
 
+def _used_strides(shape: tuple, stride: tuple) -> tuple:
+    """stride, where it places elements: 0 (the last: 1) for dimensions of one element and row-major
+    for a tensor of none, whose own may be anything, and stay so in what contiguous() returns."""
+    if 0 in shape:
+        stride, step = [], 1
+        for size in reversed(shape):
+            stride.insert(0, step)
+            step *= max(size, 1)
+    *outer, last = (s if size != 1 else None for size, s in zip(shape, stride))
+    return (*(s or 0 for s in outer), 1 if last is None else last)
+
+
 @functools.lru_cache(maxsize=512)
 def _linear_plan(x_shape, x_stride, x_dtype, codes_shape, scales_shape, scales_dtype, zeros_shape, group_size):
     """The call's checks, and its sizes as the C side takes them: (out's shape, sizes, codes behind
     them, workspace bytes), or None where x has to be copied."""
     n, half = codes_shape
     k = 2 * half
+    x_stride = _used_strides(x_shape, x_stride)
     _check_groups("linear_int4", codes_shape, scales_shape, zeros_shape, group_size)
     if x_shape[-1] != k:
         raise ValueError(f"linear_int4: x has {x_shape[-1]} inputs, the weight {k}")
@@ -523,14 +536,16 @@ def _on_rows16(stride: tuple, size: int) -> bool:
     return stride[-1] == 1 and not any(s * size % 16 for s in stride[:-1])
 
 
-def _cache_pair(name: str, k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype) -> None:
+def _cache_pair(name: str, k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype) -> tuple[tuple, tuple]:
     """What every call asks of the two caches: one shape and dtype, rows that 16-byte pieces fit.
-    They are used in place, so nothing is copied to fit."""
+    They are used in place, so nothing is copied to fit.  Returns their strides."""
     if k_shape != v_shape or k_dtype != v_dtype:
         raise ValueError(f"{name}: k_cache {list(k_shape)} {k_dtype} and v_cache {list(v_shape)} {v_dtype} differ")
-    for stride in (k_stride, v_stride):
+    strides = _used_strides(k_shape, k_stride), _used_strides(v_shape, v_stride)
+    for stride in strides:
         if not _on_rows16(stride, k_dtype.itemsize):
             raise ValueError(f"{name}: a cache of strides {stride} is not 16-byte aligned with head_dim contiguous")
+    return strides
 
 
 def _cache_pointers(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int]:
@@ -542,7 +557,7 @@ def _cache_pointers(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor) -> 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """t, its last dimension contiguous and its rows on 16-byte boundaries (copied where they are not)."""
-    if not t.data_ptr() % 16 and _on_rows16(t.stride(), t.element_size()):
+    if not t.data_ptr() % 16 and _on_rows16(_used_strides(t.shape, t.stride()), t.element_size()):
         return t
     t = t.contiguous()
     return t.clone() if t.data_ptr() % 16 else t
@@ -551,7 +566,7 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
 @functools.lru_cache(maxsize=512)
 def _attention_plan(q_shape, q_stride, q_dtype, k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype, table_shape,
                     table_stride, sequences, window, sinks, scale):
-    _cache_pair("paged_attention", k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype)
+    k_stride, v_stride = _cache_pair("paged_attention", k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype)
     batch, heads, dim = q_shape
     pages, page_size, kv_heads, cache_dim = k_shape
     if dim != cache_dim or kv_heads == 0 or heads % kv_heads:
@@ -564,6 +579,7 @@ def _attention_plan(q_shape, q_stride, q_dtype, k_shape, k_stride, k_dtype, v_sh
         raise ValueError(f"paged_attention: page_table {list(table_shape)} and {sequences} lengths for {batch} sequences")
     if window < 0 or sinks < 0:
         raise ValueError(f"paged_attention: window ({window}) and sinks ({sinks}) must not be negative")
+    q_stride = _used_strides(q_shape, q_stride)
     if not _on_rows16(q_stride, 2):
         return None
     max_pages = table_shape[1]
@@ -602,7 +618,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 @functools.lru_cache(maxsize=512)
 def _write_plan(key_shape, key_stride, key_dtype, value_shape, value_stride, value_dtype, k_shape, k_stride, k_dtype, v_shape,
                 v_stride, v_dtype, slots, slots_dtype):
-    _cache_pair("paged_write", k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype)
+    k_stride, v_stride = _cache_pair("paged_write", k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype)
     tokens, kv_heads, dim = key_shape
     pages, page_size = k_shape[:2]
     if value_shape != key_shape or value_dtype != key_dtype or k_shape[2:] != key_shape[1:]:
@@ -614,6 +630,7 @@ def _write_plan(key_shape, key_stride, key_dtype, value_shape, value_stride, val
         raise ValueError(f"paged_write: head_dim {dim} is not a multiple of 16")
     if slots != tokens:
         raise ValueError(f"paged_write: {slots} slots for {tokens} tokens")
+    key_stride, value_stride = _used_strides(key_shape, key_stride), _used_strides(value_shape, value_stride)
     if not (_on_rows16(key_stride, 2) and _on_rows16(value_stride, 2)):
         return None
     return (tokens, kv_heads, dim, pages, page_size, _strides(*key_stride[:2], *value_stride[:2], *k_stride[:3], *v_stride[:3]),
@@ -640,7 +657,7 @@ def paged_write(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v
 
 @functools.lru_cache(maxsize=512)
 def _copy_plan(k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype, src_shape, src_dtype, dst_shape, dst_dtype):
-    _cache_pair("paged_copy", k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype)
+    k_stride, v_stride = _cache_pair("paged_copy", k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype)
     if len(k_shape) not in (4, 5):
         raise ValueError(f"paged_copy: a cache has 4 dimensions, or 5 with the layers first, got {len(k_shape)}")
     if src_shape != dst_shape or src_dtype != dst_dtype:
@@ -679,6 +696,7 @@ def _window_plan(q_shape, q_stride, q_dtype, k_shape, k_stride, k_dtype, v_shape
         raise ValueError(f"window_attention: window ({window}) and sinks ({sinks}) must not be negative")
     if sequences is not None and sequences != batch:
         raise ValueError(f"window_attention: {sequences} lengths for a batch of {batch}")
+    q_stride, k_stride, v_stride = (_used_strides(k_shape if i else q_shape, s) for i, s in enumerate((q_stride, k_stride, v_stride)))
     overlap = keys > 1 and min(k_stride[1], v_stride[1]) < dim  # broadcast keys have no rows of their own
     if overlap or not (_on_rows16(q_stride, 2) and _on_rows16(k_stride, 2) and _on_rows16(v_stride, 2)):
         return None
