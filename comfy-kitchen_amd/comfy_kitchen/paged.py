@@ -62,6 +62,10 @@ class PagedKVCache:
         """The sequence's page numbers in order; -1 for pages given back by `trim`."""
         return list(self._sequences[sequence].pages)
 
+    def _next_free(self, count: int) -> list[int]:
+        """The pages that `_take` of as many will take."""
+        return self._free[:-count - 1:-1]
+
     def _take(self, count: int) -> list[int]:
         taken = [self._free.pop() for _ in range(count)]
         for page in taken:
@@ -123,22 +127,34 @@ class PagedKVCache:
             need += -(-(owner.length + count) // size) - len(owner.pages) + copy
         if need > len(self._free):
             raise OutOfPages(f"append needs {need} pages, {len(self._free)} are free")
-        src, dst, slots = [], [], []
+        # What the device is asked for may be refused, so it comes before any change here.
+        fresh = iter(self._next_free(need))
+        src, dst, slots, after = [], [], [], []
         for sequence, count, copy in zip(sequences, counts, shared):
             owner = self._sequences[sequence]
+            first, fill = divmod(owner.length, size)
+            pages = owner.pages[first:]  # those that the new tokens are in
             if copy:
-                old, (new,) = owner.pages[-1], self._take(1)
-                fill = owner.length % size
+                old, new = pages[0], next(fresh)
                 src.extend(range(old * size, old * size + fill))
                 dst.extend(range(new * size, new * size + fill))
-                owner.pages[-1] = new
-                self._drop([old])
-            begin, owner.length = owner.length, owner.length + count
-            owner.pages.extend(self._take(-(-owner.length // size) - len(owner.pages)))
-            slots.extend(owner.pages[t // size] * size + t % size for t in range(begin, owner.length))
+                pages = [new]
+            while len(pages) * size < fill + count:
+                pages.append(next(fresh))
+            after.append((owner, first, pages, owner.length + count, copy))
+            for page in pages:
+                begin, end = page * size + fill, page * size + min(size, fill + count)
+                slots.extend(range(begin, end))
+                fill, count = 0, count - (end - begin)
+        placed = self._on_device(slots)
         if src:
             self._copy(src, dst)
-        return self._on_device(slots)
+        self._take(need)
+        for owner, first, pages, end, copy in after:
+            if copy:
+                self._drop(owner.pages[first:])
+            owner.pages[first:], owner.length = pages, end
+        return placed
 
     def trim(self, sequence: int, window: int, sinks: int = 0) -> int:
         """Give back the pages that hold neither one of the last `window` tokens nor one of the first
@@ -164,10 +180,11 @@ class PagedKVCache:
         need = -(-len(keep) // size)
         if need > len(self._free):
             raise OutOfPages(f"compact needs {need} pages, {len(self._free)} are free")
-        new = self._take(need)
+        new = self._next_free(need)
         if keep:
             self._copy([owner.pages[t // size] * size + t % size for t in keep],
                        [new[i // size] * size + i % size for i in range(len(keep))])
+        self._take(need)
         self._drop(owner.pages)
         owner.pages, owner.length = new, len(keep)
 
