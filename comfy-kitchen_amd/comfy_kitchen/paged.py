@@ -29,13 +29,20 @@ class PagedKVCache:
     """K and V of `layers` layers, [layers, pages, page_size, kv_heads, head_dim], and their sequences.
 
     dtype: of the rows, f16 / bf16, or float8_e4m3fn, whose codes stand for value / k_scale and
-    value / v_scale (floats; kept as one-element tensors on the device)."""
+    value / v_scale (floats; kept as one-element tensors on the device).
+    head_dim: a multiple of 16; `attend` takes 64, 96, 128 and 256."""
 
     def __init__(self, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int,
                  dtype: torch.dtype = torch.bfloat16, device: torch.device | str = "cuda",
                  k_scale: float | None = None, v_scale: float | None = None):
         if min(layers, pages, page_size, kv_heads, head_dim) < 1:
             raise ValueError("layers, pages, page_size, kv_heads and head_dim must be positive")
+        if dtype not in (torch.float16, torch.bfloat16, torch.float8_e4m3fn):
+            raise ValueError(f"a cache holds float16, bfloat16 or float8_e4m3fn, not {dtype}")
+        if head_dim % 16:
+            raise ValueError(f"head_dim {head_dim} is not a multiple of 16, which `write` needs")
+        if pages * page_size > 2 ** 31 - 1:
+            raise ValueError(f"{pages} pages of {page_size} tokens: slots must fit 32 bits")
         shape = (layers, pages, page_size, kv_heads, head_dim)
         self.page_size = page_size
         self.k = torch.zeros(shape, dtype=dtype, device=device)

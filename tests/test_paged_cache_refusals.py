@@ -43,3 +43,12 @@ def test_a_refused_call_changes_nothing(broken, monkeypatch):
     c.free(a)
     c.free(b)
     assert c.free_pages == 8 and not any(c._owners)
+
+
+def test_a_cache_that_no_call_takes():
+    for change, match in ((dict(head_dim=72), "multiple of 16"), (dict(dtype=torch.float32), "float32"),
+                          (dict(dtype=torch.float8_e5m2), "e5m2"), (dict(pages=2 ** 27, page_size=16), "32 bits")):
+        args = dict(layers=1, pages=4, page_size=4, kv_heads=1, head_dim=16, dtype=torch.float16, device="meta")
+        args.update(change)
+        with pytest.raises(ValueError, match=match):
+            ck.PagedKVCache(**args)
