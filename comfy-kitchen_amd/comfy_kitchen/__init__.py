@@ -243,8 +243,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     held in pages; the result has q's shape and dtype.
 
     k_cache, v_cache: [pages, page_size, kv_heads, head_dim], in q's dtype or as E4M3 codes of
-    value / k_scale, value / v_scale (one-element fp32 tensors; None: 1); any strides that are
-    multiples of 16 bytes with head_dim contiguous, so [pages, kv_heads, page_size, head_dim] is a
+    value / k_scale, value / v_scale (one-element fp32 tensors, which multiply what either kind of cache
+    holds; None: 1); any strides that are multiples of 16 bytes with head_dim contiguous, so [pages, kv_heads, page_size, head_dim] is a
     permuted view away.  heads is a multiple of kv_heads; head_dim 64, 96, 128 or 256.
     page_table: int32 [B, n]; token t of sequence b is row t % page_size of page
     page_table[b, t // page_size].  lengths: int32 [B], the tokens of each sequence, the new one
@@ -265,8 +265,9 @@ def paged_write(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v
     a cache held in pages, in place: slot page * page_size + row for each token (int32 or int64,
     on the device; a slot outside the cache, such as -1, skips its token; slots are distinct).
 
-    The caches are [pages, page_size, kv_heads, head_dim] of key's dtype, or E4M3, which take
-    the codes of clamp(x / scale, +-448).  head_dim is a multiple of 16."""
+    The caches are [pages, page_size, kv_heads, head_dim] of key's dtype, which take the rows as they
+    are (no scales), or E4M3, which take the codes of clamp(x / scale, +-448).  head_dim is a
+    multiple of 16."""
     if direct(key, value, k_cache, v_cache, slots, k_scale, v_scale) and untouched("paged_write"):
         _dispatch("paged_write", key=key, value=value, k_cache=k_cache, v_cache=v_cache, slots=slots,
                   k_scale=k_scale, v_scale=v_scale)

@@ -651,6 +651,8 @@ def paged_write(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v
         k_scale = _scalar_on(k_scale, key.device, "k_scale")
     if v_scale is not None:
         v_scale = _scalar_on(v_scale, key.device, "v_scale")
+    if (k_scale is not None or v_scale is not None) and k_cache.dtype != torch.float8_e4m3fn:
+        raise ValueError(f"paged_write: k_scale and v_scale are for a cache of float8_e4m3fn, not {k_cache.dtype}")
     slots = slots.contiguous()
     _launch("ckh_paged_write", key, key.data_ptr(), value.data_ptr(), k, v, slots.data_ptr(), _ptr(k_scale), _ptr(v_scale), *plan)
 

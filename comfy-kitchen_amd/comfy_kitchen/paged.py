@@ -39,6 +39,8 @@ class PagedKVCache:
             raise ValueError("layers, pages, page_size, kv_heads and head_dim must be positive")
         if dtype not in (torch.float16, torch.bfloat16, torch.float8_e4m3fn):
             raise ValueError(f"a cache holds float16, bfloat16 or float8_e4m3fn, not {dtype}")
+        if dtype != torch.float8_e4m3fn and (k_scale is not None or v_scale is not None):
+            raise ValueError(f"k_scale and v_scale are for a cache of float8_e4m3fn, not {dtype}")
         if head_dim % 16:
             raise ValueError(f"head_dim {head_dim} is not a multiple of 16, which `write` needs")
         if pages * page_size > 2 ** 31 - 1:

@@ -133,6 +133,7 @@ extern "C" int ckh_paged_write(const void* key, const void* value, void* k_cache
                 static_cast<long long>(dim));
     CKH_REQUIRE(pages > 0 && page_size > 0 && pages <= INT32_MAX && page_size <= INT32_MAX && pages * page_size <= INT32_MAX,
                 "paged_write: %lld pages of %lld tokens", static_cast<long long>(pages), static_cast<long long>(page_size));
+    CKH_REQUIRE(cache_code == CKH_E4M3 || (!k_scale && !v_scale), "paged_write: scales with a cache of dtype %d", cache_code);
     const int64_t row = kv_heads * dim / 8;
     CKH_REQUIRE(kv_heads <= 65535 && dim <= 65536 && tokens * row < INT32_MAX, "paged_write: too many elements");
     if (tokens * row == 0) return CKH_OK;

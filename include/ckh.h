@@ -324,8 +324,8 @@ int ckh_linear_int4(const void* x, const void* codes, const void* scales, const 
  * ckh_paged_attention: one query token per sequence.  out[b, h] = softmax(scale q[b, h] K^T) V over
  * sequence b's visible tokens: its lengths[b] tokens (int32, taken into 0 .. max_pages * page_size),
  * or with window > 0 its last `window` and its first `sinks`.  q [batch, heads, dim] and out
- * (contiguous) of q_code (f16/bf16); cache_code the same, or e4m3 with values code * *k_scale,
- * code * *v_scale (device f32, NULL: 1).  heads % kv_heads == 0; dim 64, 96, 128 or 256.  Query head h
+ * (contiguous) of q_code (f16/bf16); cache_code the same or e4m3, and what the cache holds is
+ * multiplied by *k_scale, *v_scale (device f32, NULL: 1).  heads % kv_heads == 0; dim 64, 96, 128 or 256.  Query head h
  * reads key-value head h / (heads / kv_heads).  A sequence without visible tokens gives zeros.
  * page_table: int32 [batch, max_pages], table_stride elements a row; entries that no visible token
  * needs are not read, others outside 0 .. pages-1 are read as the last page.
@@ -334,7 +334,7 @@ int ckh_linear_int4(const void* x, const void* codes, const void* scales, const 
  * split); with NULL or a short one every sequence is read by one workgroup per key-value head.
  *
  * ckh_paged_write: key, value [tokens, kv_heads, dim] of x_code (f16/bf16) to slots[tokens] of K and
- * V, as they are (cache_code == x_code) or as e4m3 codes of clamp(x / *scale, +-448).  dim % 16 == 0.
+ * V, as they are (cache_code == x_code; no scales) or as e4m3 codes of clamp(x / *scale, +-448).  dim % 16 == 0.
  * strides: key token, head; value token, head; k page, token, head; v page, token, head.
  *
  * ckh_paged_copy: rows src[i] to dst[i], i < rows, of K and V in each of `layers` caches; no slot of

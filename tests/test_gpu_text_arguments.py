@@ -1,4 +1,5 @@
-"""One sequence, token or head cut from something wider gives what a copy of it gives."""
+"""Arguments of the text-generation calls: one sequence, token or head cut from something wider gives what
+a copy of it gives, and scales are taken where they mean something."""
 import pytest
 import torch
 
@@ -62,3 +63,15 @@ def test_nothing_to_do(hip):
     assert ck.linear_int4(x[:0].unflatten(0, (0, 3)), codes, scales).shape == (0, 3, 8)
     k = torch.zeros(2, 9, 2, 64, dtype=torch.bfloat16, device="cuda")
     assert ck.window_attention(x[:0, :64].reshape(0, 64)[None, :, None].expand(2, 0, 4, 64), k, k).shape == (2, 0, 4, 64)
+
+
+def test_scales_of_16_bit_caches(hip):
+    """Rows are written as they are there: a scale is refused; attention multiplies by it."""
+    k, v = (torch.randn(2, 16, 2, 64, device="cuda").bfloat16() for _ in range(2))
+    row, slot, two = k[0, :1], torch.zeros(1, dtype=torch.int32, device="cuda"), torch.tensor(2.0, device="cuda")
+    for scales in (dict(k_scale=two), dict(v_scale=two)):
+        with pytest.raises(ValueError, match="float8_e4m3fn"):
+            ck.paged_write(row, row, k, v, slot, **scales)
+    q = torch.randn(1, 2, 64, device="cuda").bfloat16()
+    args = (torch.tensor([[0, 1]], dtype=torch.int32, device="cuda"), torch.tensor([20], dtype=torch.int32, device="cuda"))
+    assert torch.equal(ck.paged_attention(q, k, v, *args, k_scale=two, v_scale=two), ck.paged_attention(q, k * 2, v * 2, *args))

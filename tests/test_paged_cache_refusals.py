@@ -52,3 +52,10 @@ def test_a_cache_that_no_call_takes():
         args.update(change)
         with pytest.raises(ValueError, match=match):
             ck.PagedKVCache(**args)
+
+
+def test_scales_of_a_cache_that_is_not_scaled():
+    """write leaves 16-bit rows as they are, so attend must not multiply them."""
+    for scales in (dict(k_scale=0.5), dict(v_scale=2.0)):
+        with pytest.raises(ValueError, match="float8_e4m3fn"):
+            cache(**scales)

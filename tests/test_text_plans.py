@@ -83,3 +83,15 @@ def test_nothing_to_do():
     cache = torch.zeros(3, 16, 2, 64, dtype=torch.bfloat16)
     assert hb._write_plan(*described(none, none, cache, cache), 0, torch.int64) is not None
     assert hb._attention_plan(*described(none, cache, cache), (0, 0), (1, 1), 0, 0, 0, None) is not None
+
+
+def test_writes_with_scales_into_16_bits():
+    """They are not scaled, so a scale there is refused (without a GPU: before any HIP call)."""
+    import ctypes
+
+    buf = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(buf) + 255) // 256 * 256
+    strides = (ctypes.c_int64 * 10)(128, 64, 128, 64, 2048, 128, 64, 2048, 128, 64)
+    for scales in ((p, None), (None, p)):
+        assert hb._lib.ckh_paged_write(p, p, p, p, p, *scales, 2, 2, 64, 3, 16, strides, 2, 2, 0, 0) == 1
+        assert b"scales" in hb._lib.ckh_last_error()
