@@ -61,8 +61,9 @@ class _Kernels(dict):
 
 _kernels = _Kernels()
 # What this module's own definitions put in torch's list (set behind them): an op that changes its
-# arguments has a kernel that counts the change.
+# arguments has a kernel that counts the change.  What a program put there before is its own.
 _defined: frozenset = frozenset()
+_before = frozenset(_registered) if _OBSERVABLE else frozenset()
 
 
 def changed(*tensors: torch.Tensor) -> None:
@@ -384,4 +385,4 @@ def _(x, freqs_cis):
 
 
 if _OBSERVABLE:
-    _defined = frozenset(entry for entry in _registered if entry.startswith("comfy_kitchen/"))
+    _defined = frozenset(_registered) - _before
