@@ -101,13 +101,19 @@ class BaseLayoutParams:
 
     def copy_from(self, src: BaseLayoutParams, non_blocking: bool = False) -> None:
         """Take src's values in place: tensors are copied into this object's own tensors
-        (their memory is reused), every other field is rebound."""
-        tensors = set(self._tensor_fields())
+        (their memory is reused), every other field is rebound.  An optional tensor that only
+        src has is copied to this object's device, one that only this object has is dropped;
+        tensors that do not fit are refused before anything changes."""
+        both = set(self._tensor_fields()) & set(src._tensor_fields())
+        for name in both:
+            getattr(src, name).expand_as(getattr(self, name))
         for f in dataclasses.fields(self):
             value = getattr(src, f.name)
-            if f.name in tensors:
+            if f.name in both:
                 getattr(self, f.name).copy_(value, non_blocking=non_blocking)
             else:
+                if isinstance(value, torch.Tensor):
+                    value = value.to(device=self.scale.device, copy=True)
                 object.__setattr__(self, f.name, value)
 
 
@@ -348,8 +354,9 @@ class QuantizedTensor(torch.Tensor):
             raise TypeError(f"Layout mismatch: {self._layout_cls} vs {src._layout_cls}")
         non_blocking = bool(a.get("non_blocking", False))
         keep = self._params.orig_dtype  # the destination keeps its logical dtype
-        self._qdata.copy_(src._qdata, non_blocking=non_blocking)
+        src._qdata.expand_as(self._qdata)  # refused before anything changes, as copy_from's
         self._params.copy_from(src._params, non_blocking=non_blocking)
+        self._qdata.copy_(src._qdata, non_blocking=non_blocking)
         self._params = dataclasses.replace(self._params, orig_dtype=keep)
         return self
 
