@@ -38,6 +38,7 @@ constexpr int kTileRows = 32;       // tile_kernel: activation rows of a workgro
 constexpr int kTileWaves = 8;       // and its waves, of 16 weight rows each
 constexpr int kTileTarget = 3;      // half-workgroups wanted a CU
 constexpr int kMaxSplits = 16;
+constexpr int64_t kSplitBytes = 64 << 20;  // of the sums of ranges that only their groups ask for
 constexpr int kVecCodes = 8192;    // matvec_kernel: codes whose activations are in LDS at a time, half as many for 4 rows
 
 struct LinearArgs {
@@ -194,14 +195,12 @@ __global__ __launch_bounds__(W * 64) void linear_kernel(LinearArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, quarter = lane >> 4;
     const int n0 = blockIdx.x * kRows;
-    const int m0 = blockIdx.y * 16 * T;
-    const int rows = min(kRows, a.n - n0), toks = min(16 * T, a.m - m0);
+    const int rows = min(kRows, a.n - n0), toks = a.m;  // at most 16 T
     const int pitch = a.k >> 1;  // code bytes per weight row
 
     const __amdgpu_buffer_rsrc_t rw = buffer_rsrc(a.codes + static_cast<int64_t>(n0) * pitch, rows * pitch);
     const __amdgpu_buffer_rsrc_t rx =
-        buffer_rsrc(static_cast<const uint16_t*>(a.x) + m0 * a.x_stride,
-                    static_cast<uint32_t>(((toks - 1) * a.x_stride + a.k) * 2));
+        buffer_rsrc(a.x, static_cast<uint32_t>(((toks - 1) * a.x_stride + a.k) * 2));
 
     // Weight rows past N and activation rows past M repeat the last one: what they give is not stored.
     uint32_t ow[R], ox[T];
@@ -327,7 +326,7 @@ __global__ __launch_bounds__(W * 64) void linear_kernel(LinearArgs a) {
         for (int w = 1; w < W; ++w) v += red[w][slot][l];
         const int row = slot / (4 * T) * 16 + (l & 15);
         const int tok = slot / 4 % T * 16 + (l >> 4) * 4 + (slot & 3);
-        if (row < rows && tok < toks) store_result<XC>(a, m0 + tok, n0 + row, v);
+        if (row < rows && tok < toks) store_result<XC>(a, tok, n0 + row, v);
     }
 }
 
@@ -466,13 +465,14 @@ __global__ __launch_bounds__(W * 64, MT > 1 && GB == 1 ? 3 : 4) void matvec_kern
 // `splits` ranges of K, and its waves share the activations, which go through LDS in the operand's
 // order (two buffers, a barrier a step): read by every wave itself they would cost more than the
 // codes.  Where K is split, the sums go to memory in fp32 and reduce_kernel adds them in order.
+// ROUNDS: a range has more groups than LDS holds, and is taken in equal parts that stage theirs.
 // 24 rows, N = 5120, K = 13824 (35 MB of codes): 23.3 us, 1.6 TB/s.  Some 5 of them are the second
 // launch, 6 the way to the first step and back, the rest is bound by the loads: with the products
 // taken out it takes as long, without the activations' loads 5 us less, without the codes' 3.
 // 64 weight rows a workgroup 26 (64 rows, N = 13824, K = 5120: 42 against 34), six steps of codes in
 // flight 24.4, two 23.7; 256-byte runs of an activation row a load (whole lines) 25.1, for their
 // writes to LDS meet on banks; two or four workgroups' halves a CU 27.
-template <int XC, int GB>
+template <int XC, int GB, bool ROUNDS>
 __global__ __launch_bounds__(kTileWaves * 64, GB == 1 ? 3 : 4) void tile_kernel(LinearArgs a) {
     constexpr int T = kTileRows / 16, R = 1;  // 16-row tiles of activations, and of a wave's weight rows
     constexpr int W = kTileWaves, D = 4, DX = 2;  // waves; steps of codes, of activations in flight
@@ -511,10 +511,10 @@ __global__ __launch_bounds__(kTileWaves * 64, GB == 1 ? 3 : 4) void tile_kernel(
         ox[i] = static_cast<uint32_t>((min(t * 16 + (l & 15), toks - 1) * a.x_stride + j * 32 + (l >> 4) * 8) * 2);
     }
     v4u w[D][R], x[DX][kPer];
-    const auto load_codes = [&](v4u (&d)[R], int s) __attribute__((always_inline)) {
+    const auto load_codes = [&](v4u (&d)[R], int s, int end) __attribute__((always_inline)) {
 #pragma unroll
         for (int r = 0; r < R; ++r)
-            d[r] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(s < last ? rw : none, ow[r] + s * 64, 0, 0));
+            d[r] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(s < end ? rw : none, ow[r] + s * 64, 0, 0));
     };
     const auto load_x = [&](v4u (&d)[kPer], int s) __attribute__((always_inline)) {
 #pragma unroll
@@ -534,7 +534,7 @@ __global__ __launch_bounds__(kTileWaves * 64, GB == 1 ? 3 : 4) void tile_kernel(
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int t = 0; t < T; ++t) total[r][t] = v4f{0, 0, 0, 0};
-    const int g0 = a.group_of(first * 4);
+    int g0 = 0;  // the staged groups' first
     const auto use = [&](const v4u (&codes)[R], int s, int buffer, auto blocks) __attribute__((always_inline)) {
         v4f acc[R][T], sum[T];
         v4u c[R];
@@ -571,33 +571,51 @@ __global__ __launch_bounds__(kTileWaves * 64, GB == 1 ? 3 : 4) void tile_kernel(
         }
     };
 
-    const int gn = min(a.groups, a.group_of(last * 4 - 1) + 1) - g0;
-    ScaleLoads<XC, R * W, W> sl;
-    load_x(x[0], first);
-    sl.load(a, n0, rows, wave, lane, g0, gn);
-#pragma unroll
-    for (int u = 1; u < DX; ++u) load_x(x[u], first + u);
-#pragma unroll
-    for (int u = 0; u < D; ++u) load_codes(w[u], first + u);
-    store_x(x[0], 0);
-    sl.store(a, sp, rows, wave, lane, gn);
-    __syncthreads();
-    const int full = min(last, a.k >> 7);  // whole steps; K may end inside the last
-    for (int s0 = first; s0 < full; s0 += D) {
-#pragma unroll
-        for (int u = 0; u < D; ++u) {
-            const int s = s0 + u;
-            if (s >= full) break;
-            load_x(x[u % DX], s + DX);  // past the range: unused, within the operand or zeros
-            use(w[u], s, u & 1, std::integral_constant<int, 4>{});
-            load_codes(w[u], s + D);
-            store_x(x[(u + 1) % DX], (u + 1) & 1);
-            __syncthreads();
+    // Steps c0 .. c1 - 1, whose groups LDS holds.  The last barrier of a round before K's end frees what the
+    // next one stages.
+    const auto round = [&](int c0, int c1) __attribute__((always_inline)) {
+        g0 = a.group_of(c0 * 4);
+        const int gn = min(a.groups, a.group_of(c1 * 4 - 1) + 1) - g0;
+        int at = lane;
+        if constexpr (ROUNDS) __asm__ volatile("" : "+v"(at));  // else its places are kept in registers for the next
+        ScaleLoads<XC, R * W, W> sl;
+        if constexpr (ROUNDS) {  // beside the sums, registers do not hold scales and codes on their way
+            sl.load(a, n0, rows, wave, at, g0, gn);
+            sl.store(a, sp, rows, wave, at, gn);
         }
-    }
-    if (full < last) {
-        load_codes(w[0], full);
-        use(w[0], full, (full - first) & 1, (a.k >> 5) - full * 4);
+        load_x(x[0], c0);
+        if constexpr (!ROUNDS) sl.load(a, n0, rows, wave, at, g0, gn);
+#pragma unroll
+        for (int u = 1; u < DX; ++u) load_x(x[u], c0 + u);
+#pragma unroll
+        for (int u = 0; u < D; ++u) load_codes(w[u], c0 + u, c1);
+        store_x(x[0], 0);
+        if constexpr (!ROUNDS) sl.store(a, sp, rows, wave, at, gn);
+        __syncthreads();
+        const int full = min(c1, a.k >> 7);  // whole steps; K may end inside the last
+        for (int s0 = c0; s0 < full; s0 += D) {
+#pragma unroll
+            for (int u = 0; u < D; ++u) {
+                const int s = s0 + u;
+                if (s >= full) break;
+                load_x(x[u % DX], s + DX);  // past the round: unused, within the operand or zeros
+                use(w[u], s, u & 1, std::integral_constant<int, 4>{});
+                load_codes(w[u], s + D, c1);
+                store_x(x[(u + 1) % DX], (u + 1) & 1);
+                __syncthreads();
+            }
+        }
+        if (full < c1) {
+            load_codes(w[0], full, c1);
+            use(w[0], full, (full - c0) & 1, (a.k >> 5) - full * 4);
+        }
+    };
+    if constexpr (ROUNDS) {
+        const int rounds = (last - first + a.chunk - 1) / a.chunk, per = (last - first + rounds - 1) / rounds;
+#pragma unroll 1
+        for (int c0 = first; c0 < last; c0 += per) round(c0, min(last, c0 + per));
+    } else {
+        round(first, last);
     }
 
 #pragma unroll
@@ -634,7 +652,7 @@ int chunk_steps(int64_t group) {
 
 template <int XC, int T, int R, int W, int U>
 void launch_linear(const LinearArgs& a, hipStream_t st) {
-    const dim3 grid(static_cast<unsigned>(cdiv(a.n, 16 * R)), static_cast<unsigned>(cdiv(a.m, 16 * T)));
+    const unsigned grid = static_cast<unsigned>(cdiv(a.n, 16 * R));
     if (a.group % 128 == 0)
         linear_kernel<XC, T, R, W, U, 4><<<grid, W * 64, 0, st>>>(a);
     else if (a.group % 64 == 0)
@@ -659,28 +677,38 @@ void launch_matvec(const LinearArgs& a, hipStream_t st) {
     else launch_matvec<XC, MT, R, W, D, 1>(a, st);
 }
 
-// Ranges of K for a call (1: not split), 0 where tile_kernel does not serve it: few rows, rows that
-// linear_kernel's 64-row workgroups serve better (32 rows, N = 13824, K = 5120: 22.5 against 24), or
-// more groups in a range than LDS holds.  Three workgroups for two CUs are wanted, of four steps at
-// least.
+// Ranges of K for a call (1: not split), 0 where tile_kernel does not serve it: few rows, or rows that
+// linear_kernel's 64-row workgroups serve better (32 rows, N = 13824, K = 5120: 22.5 against 24).
+// Three workgroups for two CUs are wanted, of four steps at least.  Where that leaves a range more
+// groups than LDS holds, K is split further while the ranges' sums stay within kSplitBytes (groups of
+// 32, N = 5120, K = 13824: 256 rows 138 us, in rounds 162; 512 rows 270 against 305), and else
+// the range goes in rounds (1024 rows 507, in ranges 535; 4096 rows 1988 against 2120), so that
+// a prompt's workspace does not grow with its rows.
 int tile_splits(int64_t m, int64_t n, int64_t k, int64_t group, bool may_split) {
     const int cus = device_cus();
     if (m <= 16 || (m <= 32 && n > 48 * cus)) return 0;
     const int64_t blocks = cdiv(n, 16 * kTileWaves) * cdiv(m, kTileRows), steps = cdiv(k, 128);
-    int64_t s = std::min<int64_t>({kMaxSplits, cdiv(kTileTarget * cus, 2 * blocks), std::max<int64_t>(1, steps / 4)});
-    s = may_split ? std::max(s, cdiv(steps, chunk_steps(group))) : 1;
-    return s <= kMaxSplits && cdiv(steps, s) <= chunk_steps(group) ? static_cast<int>(s) : 0;
+    if (!may_split) return 1;
+    const int64_t s = std::min<int64_t>({kMaxSplits, cdiv(kTileTarget * cus, 2 * blocks), std::max<int64_t>(1, steps / 4)});
+    const int64_t whole = std::min<int64_t>(kMaxSplits, cdiv(steps, chunk_steps(group)));  // ranges of one round
+    return static_cast<int>(whole > s && whole * m * n * 4 <= kSplitBytes ? whole : s);
+}
+
+template <int XC, bool ROUNDS>
+void launch_tile(const LinearArgs& a, dim3 grid, size_t lds, hipStream_t st) {
+    if (a.group % 128 == 0) tile_kernel<XC, 4, ROUNDS><<<grid, kTileWaves * 64, lds, st>>>(a);
+    else if (a.group % 64 == 0) tile_kernel<XC, 2, ROUNDS><<<grid, kTileWaves * 64, lds, st>>>(a);
+    else tile_kernel<XC, 1, ROUNDS><<<grid, kTileWaves * 64, lds, st>>>(a);
 }
 
 template <int XC>
 void launch_tile(const LinearArgs& a, hipStream_t st) {
     const dim3 grid(static_cast<unsigned>(cdiv(a.n, 16 * kTileWaves)), static_cast<unsigned>(a.splits), static_cast<unsigned>(cdiv(a.m, kTileRows)));
-    const int64_t codes = cdiv(cdiv(a.k, 128), a.splits) * 128;
+    const int64_t range = cdiv(cdiv(a.k, 128), a.splits), codes = std::min<int64_t>(a.chunk, range) * 128;
     const int64_t groups = std::min<int64_t>({a.groups, kScaleGroups, codes / a.group + 2});
     const size_t lds = 2 * kTileRows * 256 + groups * (16 * kTileWaves + 1) * 8;  // two steps' activations, the scales
-    if (a.group % 128 == 0) tile_kernel<XC, 4><<<grid, kTileWaves * 64, lds, st>>>(a);
-    else if (a.group % 64 == 0) tile_kernel<XC, 2><<<grid, kTileWaves * 64, lds, st>>>(a);
-    else tile_kernel<XC, 1><<<grid, kTileWaves * 64, lds, st>>>(a);
+    if (range <= a.chunk) launch_tile<XC, false>(a, grid, lds, st);
+    else launch_tile<XC, true>(a, grid, lds, st);
     if (a.splits > 1) reduce_kernel<XC><<<static_cast<unsigned>(cdiv(static_cast<int64_t>(a.m) * a.n, 256)), 256, 0, st>>>(a);
 }
 
@@ -693,7 +721,7 @@ void launch_tile(const LinearArgs& a, hipStream_t st) {
 //   5-16 rows  32 weight rows, 8 waves (16.7; 16 rows 19.9), 16 waves where there are fewer
 //              workgroups than CUs (N = K = 5120, 16 rows: 12.0 against 13.6)
 //   more       tile_kernel (64 rows: 34; linear_kernel 45), but linear_kernel, 64 weight rows a
-//              workgroup, for up to 32 rows of wide layers, and where tile_splits says so
+//              workgroup, for up to 32 rows of wide layers (tile_splits)
 template <int XC>
 void linear(const LinearArgs& a, hipStream_t st) {
     const int cus = device_cus();

@@ -23,3 +23,24 @@ def same(c: Linear):
 def test_groups_of_millions(k, group, m, dtype, hip):
     """The last 32 inputs of a long group have its scale and zero point, not the next one's."""
     same(Linear(m, 5, k, group, DT[dtype], True, False))
+
+
+# more groups than LDS holds at a time: K in more ranges, or scales staged in rounds (many rows, or
+# more groups in each of the ranges)
+MANY_GROUPS = [(400, 5000, 12224, 96), (4000, 500, 4224, 32), (2100, 1024, 13824, 32), (33, 30000, 8224, 64),
+               (3001, 2999, 8224, 64), (3000, 3000, 12224, 96), (3000, 3000, 20000, 128), (9000, 1000, 4224, 32), (100, 70, 70016, 32)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("m,n,k,group", MANY_GROUPS)
+def test_many_groups_and_rows(m, n, k, group, dtype, hip):
+    same(Linear(m, n, k, group, DT[dtype], False, True))
+    same(Linear(m, n, k, group, DT[dtype], True, False, seed=1))
+
+
+def test_many_groups_without_a_workspace(hip):
+    c = Linear(40, 96, 6144, 32, torch.bfloat16, True, False)
+    d = [t.cuda() for t in (c.x, c.codes, c.scales, c.zeros)]
+    y = torch.empty(40, 96, dtype=torch.bfloat16, device="cuda")
+    hip._launch("ckh_linear_int4", y, *(t.data_ptr() for t in d), None, y.data_ptr(), 40, 96, 6144, 6144, 32, 2, 2, 0, None, 0)
+    assert torch.equal(y.cpu(), c.want())

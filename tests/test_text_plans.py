@@ -95,3 +95,14 @@ def test_writes_with_scales_into_16_bits():
     for scales in ((p, None), (None, p)):
         assert hb._lib.ckh_paged_write(p, p, p, p, p, *scales, 2, 2, 64, 3, 16, strides, 2, 2, 0, 0) == 1
         assert b"scales" in hb._lib.ckh_last_error()
+
+
+def test_workspace_of_linears_does_not_grow_with_the_prompt():
+    """Tiles that fill the GPU need no ranges of K, however many groups it has."""
+    f = hb._lib.ckh_linear_int4_workspace_bytes
+    for group in (32, 64, 96, 128, 1024):
+        for k in (1024, 5120, 13824, 70016):
+            for n in (256, 1024, 5120, 13824, 60000):
+                sizes = [f(m, n, k, group) for m in (1, 16, 17, 24, 64, 100, 512, 2000, 16384, 100000)]
+                assert max(sizes) <= 64 * 2 ** 20 and sizes[:2] == [0, 0] and sizes[-1] == 0, (group, k, n, sizes)
+    assert f(16384, 5120, 13824, 32) == 0 < f(24, 5120, 13824, 32)
