@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import comfy_kitchen as ck
-from int4_exact import LONG_GROUPS, Linear
+from int4_exact import LONG_GROUPS, MANY_GROUPS, SHAPES, Linear, dense, far
 
 pytestmark = pytest.mark.gpu
 
@@ -18,17 +18,25 @@ def same(c: Linear):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("m,n,k,group", SHAPES)
+def test_linear(m, n, k, group, dtype, hip):
+    for seed, (zeros, bias) in enumerate(((False, True), (True, False), (True, True))):
+        same(Linear(m, n, k, group, DT[dtype], zeros, bias, seed))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("m,n,k,group", SHAPES[1:])
+def test_dense(m, n, k, group, dtype, hip):
+    (x, codes, scales, zeros), want = dense(m, n, k, group, DT[dtype], device="cuda")
+    assert far(ck.linear_int4(x, codes, scales, zeros, group_size=group), want, DT[dtype]) < 1
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("m", [1, 3, 9, 20])
 @pytest.mark.parametrize("k,group", LONG_GROUPS)
 def test_groups_of_millions(k, group, m, dtype, hip):
     """The last 32 inputs of a long group have its scale and zero point, not the next one's."""
     same(Linear(m, 5, k, group, DT[dtype], True, False))
-
-
-# more groups than LDS holds at a time: K in more ranges, or scales staged in rounds (many rows, or
-# more groups in each of the ranges)
-MANY_GROUPS = [(400, 5000, 12224, 96), (4000, 500, 4224, 32), (2100, 1024, 13824, 32), (33, 30000, 8224, 64),
-               (3001, 2999, 8224, 64), (3000, 3000, 12224, 96), (3000, 3000, 20000, 128), (9000, 1000, 4224, 32), (100, 70, 70016, 32)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
