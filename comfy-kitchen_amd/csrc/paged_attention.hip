@@ -34,6 +34,7 @@ namespace ckh {
 namespace attn {
 
 constexpr int kWaves = 4;
+constexpr int kMaxChunks = 1024;  // of a unit: the join's factors are in LDS
 constexpr uint32_t kOut = 0x80000000u;
 
 struct PagedArgs {
@@ -48,7 +49,7 @@ struct PagedArgs {
     int64_t table_stride;
     int batch, heads, kv_heads, group, head_tiles;  // group: query heads of a key-value head
     int pages, page_size, max_pages, window, sinks;
-    int target;     // chunks wanted; 1: no splitting
+    int target;     // chunks wanted, at most kMaxChunks, which no unit then passes; 1: no splitting
     int min_tiles;  // least tiles of a chunk, where a unit has several
     float scale;
     FastDiv by_page;
@@ -455,9 +456,8 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) void paged_kernel(Pa
 // The chunks' factors go to LDS first, so that their outputs are read without waiting for them.
 template <int QC, int D>
 __global__ __launch_bounds__(256) void join_kernel(PagedArgs a) {
-    constexpr int N = 256 / D;    // chunks taken at a time
-    constexpr int kAtOnce = 1024;  // chunks whose factors LDS holds
-    __shared__ float so[N][D], factor[kAtOnce], red[8];
+    constexpr int N = 256 / D;  // chunks taken at a time
+    __shared__ float so[N][D], factor[kMaxChunks], red[8];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int b = blockIdx.y, h = blockIdx.x;
     const int units = a.kv_heads * a.head_tiles;
@@ -476,19 +476,15 @@ __global__ __launch_bounds__(256) void join_kernel(PagedArgs a) {
     top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     const int d = threadIdx.x % D, g = threadIdx.x / D;
     float o = 0.0f, sum = 0.0f;
-    for (int first = 0; first < count; first += kAtOnce) {
-        const int last = min(count, first + kAtOnce);
-        if (first > 0) __syncthreads();
-        for (int i = first + threadIdx.x; i < last; i += 256) {
-            const float f = exp2_hw(part[i * step + D] - top);
-            factor[i - first] = f;
-            sum += f * part[i * step + D + 1];
-        }
-        __syncthreads();
-        if (g < N) {
+    for (int i = threadIdx.x; i < count; i += 256) {
+        const float f = exp2_hw(part[i * step + D] - top);
+        factor[i] = f;
+        sum += f * part[i * step + D + 1];
+    }
+    __syncthreads();
+    if (g < N) {
 #pragma unroll 8
-            for (int i = first + g; i < last; i += N) o += factor[i - first] * part[i * step + d];
-        }
+        for (int i = g; i < count; i += N) o += factor[i] * part[i * step + d];
     }
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) sum += __shfl_xor(sum, s, 64);
@@ -521,7 +517,7 @@ Split paged_split(int64_t units, int64_t capacity) {
     // Two or three workgroups are resident on a CU; four a CU even out their ends (48 ragged
     // sequences in bf16: 168 us; three 175; eight 165, but 64 windows of 1024 tokens 68 for 60).
     // Each unit may have one chunk more for its ragged end.
-    const int target = std::max(2, 4 * device_cus());
+    const int target = std::clamp(4 * device_cus(), 2, kMaxChunks);
     return {target, min_tiles, std::min(units * cdiv(tiles, min_tiles), units + target)};
 }
 
