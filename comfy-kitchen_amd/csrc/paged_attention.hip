@@ -568,9 +568,13 @@ extern "C" int ckh_paged_attention(const void* q, const void* k_cache, const voi
                 "paged_attention: %lld heads over %lld key-value heads, batch %lld", static_cast<long long>(heads),
                 static_cast<long long>(kv_heads), static_cast<long long>(batch));
     CKH_REQUIRE(pages > 0 && pages <= INT32_MAX && page_size > 0 && max_pages >= 0 && page_size <= INT32_MAX &&
-                    max_pages * page_size <= INT32_MAX - 64 && max_pages <= INT32_MAX,
+                    max_pages <= INT32_MAX && max_pages * page_size <= INT32_MAX - 64,
                 "paged_attention: %lld pages of %lld tokens, %lld a sequence", static_cast<long long>(pages),
                 static_cast<long long>(page_size), static_cast<long long>(max_pages));
+    // find_chunk sums the tiles of 64 sequences in 32 bits
+    CKH_REQUIRE(std::min<int64_t>(batch, 64) * (cdiv(max_pages * page_size, 32) + 1) <= INT32_MAX,
+                "paged_attention: page tables of %lld tokens for %lld sequences", static_cast<long long>(max_pages * page_size),
+                static_cast<long long>(batch));
     CKH_REQUIRE(window >= 0 && window <= INT32_MAX && sinks >= 0 && sinks <= INT32_MAX, "paged_attention: window %lld, sinks %lld",
                 static_cast<long long>(window), static_cast<long long>(sinks));
     if (batch == 0 || heads == 0) return CKH_OK;

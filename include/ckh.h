@@ -327,7 +327,8 @@ int ckh_linear_int4(const void* x, const void* codes, const void* scales, const 
  * (contiguous) of q_code (f16/bf16); cache_code the same or e4m3, and what the cache holds is
  * multiplied by *k_scale, *v_scale (device f32, NULL: 1).  heads % kv_heads == 0; dim 64, 96, 128 or 256.  Query head h
  * reads key-value head h / (heads / kv_heads).  A sequence without visible tokens gives zeros.
- * page_table: int32 [batch, max_pages], table_stride elements a row; entries that no visible token
+ * page_table: int32 [batch, max_pages], table_stride elements a row, of under 2^31 tokens each (and 64
+ * rows of under 2^36); entries that no visible token
  * needs are not read, others outside 0 .. pages-1 are read as the last page.
  * strides: q batch, head; k page, token, head; v page, token, head.
  * The workspace of ckh_paged_attention_workspace_bytes lets long sequences be split (0: never

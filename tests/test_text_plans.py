@@ -106,3 +106,21 @@ def test_workspace_of_linears_does_not_grow_with_the_prompt():
                 sizes = [f(m, n, k, group) for m in (1, 16, 17, 24, 64, 100, 512, 2000, 16384, 100000)]
                 assert max(sizes) <= 64 * 2 ** 20 and sizes[:2] == [0, 0] and sizes[-1] == 0, (group, k, n, sizes)
     assert f(16384, 5120, 13824, 32) == 0 < f(24, 5120, 13824, 32)
+
+
+def test_page_tables_whose_tiles_pass_32_bits():
+    """The kernel adds the tiles of 64 sequences in 32 bits; one sequence may have all that a table holds."""
+    import ctypes
+
+    buf = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(buf) + 255) // 256 * 256
+    strides = (ctypes.c_int64 * 8)(256, 64, 2 ** 26, 64, 64, 2 ** 26, 64, 64)
+
+    def call(batch, most, q=p):
+        return hb._lib.ckh_paged_attention(q, p, p, p, p, None, None, p, batch, 4, 1, 64, 3, 2 ** 20, most, most, strides, 0, 0, 1.0, 2, 2,
+                                           None, 0, 0)
+
+    for batch, most in ((64, 1024), (1000, 1024), (33, 2047)):
+        assert call(batch, most) == 1 and b"page tables of" in hb._lib.ckh_last_error()
+    for batch, most in ((64, 1023), (60000, 1000), (32, 2047), (1, 2047)):  # as far as the null pointer
+        assert call(batch, most, None) == 1 and b"null pointer" in hb._lib.ckh_last_error()
