@@ -20,9 +20,10 @@
 //     unlike lengths load the chip evenly and one long sequence fills it.  A sequence in several
 //     chunks leaves fp32 partial results, which a second small launch joins in chunk order:
 //     results do not depend on timing.
-//   - Measured: 80003 tokens of 30 heads, f16 (1.23 GB): 216 us, 5.7 TB/s; 48 sequences of 8192 tokens
-//     and fewer, 8 heads, bf16 (823 MB): 168 us, 4.9 TB/s; the same as E4M3 (412 MB): 107 us, 3.9
-//     TB/s, for its rows are 128 bytes; 333 tokens: 7.3 us, loads that wait for each other.
+//   - Measured: 80003 tokens of 30 heads, f16 (1.23 GB): 211-220 us by card, 5.6-5.8 TB/s; 48
+//     sequences of 8192 tokens and fewer, 8 heads, bf16 (823 MB): 168 us, 4.9 TB/s; the same as E4M3
+//     (412 MB): 107 us, 3.9 TB/s, for its rows are 128 bytes; 333 tokens: 7.3-8.2 us, loads that
+//     wait for each other.
 //   - The maximum is only raised when a weight would pass 2^8 (in f16 2^15, attn.h): that costs
 //     fp32 sums nothing and saves most rescaling.  P is rounded to the 16-bit type for the
 //     second product, as its other operand is; its sum is taken before that.

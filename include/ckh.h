@@ -325,17 +325,19 @@ int ckh_linear_int4(const void* x, const void* codes, const void* scales, const 
  * sequence b's visible tokens: its lengths[b] tokens (int32, taken into 0 .. max_pages * page_size),
  * or with window > 0 its last `window` and its first `sinks`.  q [batch, heads, dim] and out
  * (contiguous) of q_code (f16/bf16); cache_code the same or e4m3, and what the cache holds is
- * multiplied by *k_scale, *v_scale (device f32, NULL: 1).  heads % kv_heads == 0; dim 64, 96, 128 or 256.  Query head h
- * reads key-value head h / (heads / kv_heads).  A sequence without visible tokens gives zeros.
+ * multiplied by *k_scale, *v_scale (device f32, NULL: 1).  heads % kv_heads == 0; dim 64, 96, 128 or
+ * 256.  Query head h reads key-value head h / (heads / kv_heads).  A sequence without visible tokens
+ * gives zeros.
  * page_table: int32 [batch, max_pages], table_stride elements a row, of under 2^31 tokens each (and 64
- * rows of under 2^36); entries that no visible token
- * needs are not read, others outside 0 .. pages-1 are read as the last page.
+ * rows of under 2^36); entries that no visible token needs are not read, others outside 0 .. pages-1
+ * are read as the last page.
  * strides: q batch, head; k page, token, head; v page, token, head.
  * The workspace of ckh_paged_attention_workspace_bytes lets long sequences be split (0: never
  * split); with NULL or a short one every sequence is read by one workgroup per key-value head.
  *
  * ckh_paged_write: key, value [tokens, kv_heads, dim] of x_code (f16/bf16) to slots[tokens] of K and
- * V, as they are (cache_code == x_code; no scales) or as e4m3 codes of clamp(x / *scale, +-448).  dim % 16 == 0.
+ * V, as they are (cache_code == x_code; no scales) or as e4m3 codes of clamp(x / *scale, +-448).
+ * dim % 16 == 0.
  * strides: key token, head; value token, head; k page, token, head; v page, token, head.
  *
  * ckh_paged_copy: rows src[i] to dst[i], i < rows, of K and V in each of `layers` caches; no slot of
