@@ -19,6 +19,7 @@ from .float_utils import from_blocked, swap_nibbles, to_blocked
 from .ops import DTYPE_TO_CODE, _dispatch, _quantize_fp8_dynamic, changed, direct, untouched
 from .paged import OutOfPages, PagedKVCache
 from .registry import registry
+from .rope import rope_rates
 
 __version__ = "0.1.0"
 
@@ -39,7 +40,14 @@ __all__ = [
     "paged_attention",
     "paged_write",
     "paged_copy",
+    "paged_write_rope",
+    "rope_rates",
     "window_attention",
+    "shared_attention",
+    "rms_norm",
+    "rms_norm_fp8",
+    "rms_norm_mxfp8",
+    "sample_tokens",
     "PagedKVCache",
     "OutOfPages",
     "apply_rope",
@@ -304,6 +312,112 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     if direct(q, k, v, lengths) and untouched("window_attention"):
         return _dispatch("window_attention", q=q, k=k, v=v, window=window, sinks=sinks, lengths=lengths, scale=scale)
     return torch.ops.comfy_kitchen.window_attention(q, k, v, window, sinks, lengths, scale)
+
+
+def shared_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                     lengths: torch.Tensor, groups: torch.Tensor, shared: torch.Tensor, scale: float | None = None,
+                     k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> torch.Tensor:
+    """paged_attention, without a window, for sequences that begin with the same tokens (several
+    answers to one prompt, PagedKVCache.fork): what they share is read once for all of them.
+
+    groups: int32 [G + 1], ascending; sequences groups[g] .. groups[g + 1] - 1 are group g, and a sequence in
+    none of them shares nothing.  shared: int32 [G]; the first shared[g] tokens of a group's sequences have the
+    same keys and values, which are found by the page table of the group's first sequence (of more than
+    its shortest sequence holds, that many).  PagedKVCache.groups gives both.  All else, and the result, as for
+    paged_attention.
+    At most 4096 sequences and groups together."""
+    if (direct(q, k_cache, v_cache, page_table, lengths, groups, shared, k_scale, v_scale)
+            and untouched("shared_attention")):
+        return _dispatch("shared_attention", q=q, k_cache=k_cache, v_cache=v_cache, page_table=page_table,
+                         lengths=lengths, groups=groups, shared=shared, scale=scale, k_scale=k_scale, v_scale=v_scale)
+    return torch.ops.comfy_kitchen.shared_attention(q, k_cache, v_cache, page_table, lengths, groups, shared, scale,
+                                                    k_scale, v_scale)
+
+
+def paged_write_rope(q: torch.Tensor, key: torch.Tensor, value: torch.Tensor, positions: torch.Tensor,
+                     rates: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
+                     interleaved: bool = True, magnitude: float = 1.0, k_scale: torch.Tensor | None = None,
+                     v_scale: torch.Tensor | None = None,
+                     keep_key: bool = False) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """Turn the queries [T, heads, head_dim] and keys [T, kv_heads, head_dim] of new tokens to their positions
+    (int32 or int64 [T]) and store the keys, and the values as they are, as paged_write does.  Returns the
+    turned queries, or (queries, keys) with keep_key (a prompt's attention reads them again).
+
+    rates: fp32 [n], from rope_rates: pair i of the first 2n elements of a head turns by position * rates[i]
+    (in 64 bits, so far positions are exact) and is multiplied by magnitude; the rest of the head stays as it is.
+    Pairs are neighbours (2i, 2i + 1) as in apply_rope, or with interleaved=False (i, i + n).
+    A token whose slot is outside the cache is turned and not stored."""
+    if (type(interleaved) is bool and type(keep_key) is bool
+            and direct(q, key, value, positions, rates, k_cache, v_cache, slots, k_scale, v_scale)
+            and untouched("paged_write_rope")):
+        turned, kept = _dispatch("paged_write_rope", q=q, key=key, value=value, positions=positions, rates=rates,
+                                 k_cache=k_cache, v_cache=v_cache, slots=slots, interleaved=interleaved,
+                                 magnitude=magnitude, k_scale=k_scale, v_scale=v_scale, keep_key=keep_key)
+        changed(k_cache, v_cache)
+    else:
+        turned, kept = torch.ops.comfy_kitchen.paged_write_rope(
+            q, key, value, positions, rates, k_cache, v_cache, slots, interleaved, magnitude, k_scale, v_scale, keep_key)
+    return (turned, kept) if keep_key else turned
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+             eps: float = 1e-6) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """y = h / sqrt(mean(h^2) + eps) * weight over the last dimension, h = x, in x's dtype (f32 / f16 / bf16).
+    With a residual of x's shape and dtype h is x + residual, rounded to x's dtype, and (y, h) is returned.
+
+    At most 65536 elements a row; any strides (rows that are not one step apart are copied)."""
+    if direct(x, weight, residual) and untouched("rms_norm"):
+        y, h = _dispatch("rms_norm", x=x, weight=weight, residual=residual, eps=eps)
+    else:
+        y, h = torch.ops.comfy_kitchen.rms_norm(x, weight, residual, eps)
+    return y if residual is None else (y, h)
+
+
+def rms_norm_fp8(x: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor | None = None,
+                 residual: torch.Tensor | None = None, eps: float = 1e-6,
+                 output_type: torch.dtype = torch.float8_e4m3fn) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """quantize_per_tensor_fp8(rms_norm(x, ...), scale, output_type) in one call, bit for bit: codes, or
+    (codes, h) with a residual."""
+    code = DTYPE_TO_CODE[output_type]
+    if direct(x, scale, weight, residual) and untouched("rms_norm_fp8"):
+        codes, h = _dispatch("rms_norm_fp8", x=x, scale=scale, weight=weight, residual=residual, eps=eps,
+                             output_type=output_type)
+    else:
+        codes, h = torch.ops.comfy_kitchen.rms_norm_fp8(x, scale, weight, residual, eps, code)
+    return codes if residual is None else (codes, h)
+
+
+def rms_norm_mxfp8(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+                   eps: float = 1e-6, pad_32x: bool = False) -> tuple[torch.Tensor, ...]:
+    """quantize_mxfp8(rms_norm(x, ...), pad_32x) of a 2-D x in one call, bit for bit: (codes, scales), or
+    (codes, scales, h) with a residual."""
+    if type(pad_32x) is bool and direct(x, weight, residual) and untouched("rms_norm_mxfp8"):
+        codes, scales, h = _dispatch("rms_norm_mxfp8", x=x, weight=weight, residual=residual, eps=eps, pad_32x=pad_32x)
+    else:
+        codes, scales, h = torch.ops.comfy_kitchen.rms_norm_mxfp8(x, weight, residual, eps, pad_32x)
+    return (codes, scales) if residual is None else (codes, scales, h)
+
+
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: float | torch.Tensor = 1.0,
+                  top_k: int | torch.Tensor = 0, top_p: float | torch.Tensor = 1.0,
+                  min_p: float | torch.Tensor = 0.0) -> torch.Tensor:
+    """The next token of each row of logits [B, vocab] (f32 / f16 / bf16), int64 [B], drawn with the random
+    numbers u (fp32 [B], 0 <= u < 1): the same inputs give the same tokens.
+
+    Tokens stand in the order of their logits, the largest first, equal ones by number, and weigh
+    w = exp((logit - max) / temperature).  Kept are those that are among the first top_k (0: all), and of these
+    the first that together reach top_p of their weight, and of these the ones with w >= min_p; the first
+    always is.  The result is the first token whose running weight in that order exceeds u times the weight of
+    all that are kept.  temperature 0 takes the first of the largest logits.
+    Each of the four is a number or a tensor on the device of one a row (fp32; top_k int32).
+    -inf (a masked token) and NaN are never drawn, nor is a token over 32 temperatures under the largest; a
+    row that holds nothing else gives -1."""
+    given = [v if isinstance(v, torch.Tensor) else None for v in (temperature, top_k, top_p, min_p)]
+    if direct(logits, u, *given) and untouched("sample_tokens"):
+        return _dispatch("sample_tokens", logits=logits, u=u, temperature=temperature, top_k=top_k, top_p=top_p,
+                         min_p=min_p)
+    common = [v if t is None else 0 for v, t in zip((temperature, top_k, top_p, min_p), given)]
+    return torch.ops.comfy_kitchen.sample_tokens(logits, u, *common, *given)
 
 
 def apply_rope(xq: torch.Tensor, xk: torch.Tensor,

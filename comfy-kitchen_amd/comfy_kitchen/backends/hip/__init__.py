@@ -36,15 +36,21 @@ __all__ = [
     "paged_attention",
     "paged_copy",
     "paged_write",
+    "paged_write_rope",
     "quantize_fp8_dynamic",
     "quantize_int4",
     "quantize_mxfp8",
     "quantize_nvfp4",
     "quantize_nvfp4_dynamic",
     "quantize_per_tensor_fp8",
+    "rms_norm",
+    "rms_norm_fp8",
+    "rms_norm_mxfp8",
+    "sample_tokens",
     "scaled_mm_fp8",
     "scaled_mm_mxfp8",
     "scaled_mm_nvfp4",
+    "shared_attention",
     "window_attention",
 ]
 
@@ -52,6 +58,7 @@ LIB_PATH = Path(os.environ.get("CKH_LIBRARY", Path(__file__).with_name("libckh.s
 REQUIRED_ARCH = ("gfx950",)
 
 _p, _i64, _i32, _f32, _u64 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_uint64
+_f64 = ctypes.c_double
 
 # C signatures, exactly as declared in include/ckh.h
 SIGNATURES: dict[str, tuple] = {
@@ -84,6 +91,12 @@ SIGNATURES: dict[str, tuple] = {
     "ckh_paged_copy": (_i32, [_p] * 4 + [_i64] * 6 + [_p] + [_i32] * 2 + [_u64]),
     "ckh_window_attention_workspace_bytes": (_i64, [_i64] * 8),
     "ckh_window_attention": (_i32, [_p] * 5 + [_i64] * 6 + [_p] + [_i64] * 2 + [_f32, _i32, _p, _i64, _u64]),
+    "ckh_rms_norm": (_i32, [_p] * 7 + [_i64] * 6 + [_f32] + [_i32] * 4 + [_u64]),
+    "ckh_paged_write_rope": (_i32, [_p] * 12 + [_i64] * 7 + [_p, _i32, _f32] + [_i32] * 4 + [_u64]),
+    "ckh_sample_workspace_bytes": (_i64, [_i64] * 2),
+    "ckh_sample": (_i32, [_p] * 6 + [_f64, _i64, _f64, _f64, _p] + [_i64] * 3 + [_i32, _p, _i64, _u64]),
+    "ckh_shared_attention_workspace_bytes": (_i64, [_i64] * 7),
+    "ckh_shared_attention": (_i32, [_p] * 10 + [_i64] * 9 + [_p, _f32, _i32, _i32, _p, _i64, _u64]),
 }
 ABI_VERSION = 8
 # CKH_AMAX_WORKSPACE_BYTES of include/ckh.h: the workspace ckh_amax_scale takes
@@ -730,6 +743,223 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     return out
 
 
+@functools.lru_cache(maxsize=512)
+def _rope_write_plan(q_shape, q_stride, q_dtype, key_shape, key_stride, key_dtype, value_shape, value_stride, value_dtype, k_shape,
+                     k_stride, k_dtype, v_shape, v_stride, v_dtype, positions, positions_dtype, slots, slots_dtype, rates, interleaved,
+                     magnitude):
+    k_stride, v_stride = _cache_pair("paged_write_rope", k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype)
+    tokens, heads, dim = q_shape
+    kv_heads = key_shape[1]
+    pages, page_size = k_shape[:2]
+    if (value_shape != key_shape or key_shape[0] != tokens or key_shape[2] != dim or k_shape[2:] != key_shape[1:]
+            or not q_dtype == key_dtype == value_dtype):
+        raise ValueError(f"paged_write_rope: q {list(q_shape)} {q_dtype}, key {list(key_shape)} {key_dtype}, value {list(value_shape)} "
+                         f"{value_dtype} and a cache {list(k_shape)} do not fit")
+    if k_dtype not in (key_dtype, torch.float8_e4m3fn):
+        raise ValueError(f"paged_write_rope: {key_dtype} into a cache of {k_dtype}")
+    if dim % 16:
+        raise ValueError(f"paged_write_rope: head_dim {dim} is not a multiple of 16")
+    if 2 * rates > dim:
+        raise ValueError(f"paged_write_rope: {rates} rates turn more than head_dim {dim}")
+    if positions != tokens or slots != tokens:
+        raise ValueError(f"paged_write_rope: {positions} positions and {slots} slots for {tokens} tokens")
+    strides = [_used_strides(*t) for t in ((q_shape, q_stride), (key_shape, key_stride), (value_shape, value_stride))]
+    if not all(_on_rows16(s, 2) for s in strides):
+        return None
+    return (tokens, heads, kv_heads, dim, 2 * rates, pages, page_size,
+            _strides(*(s for t in strides for s in t[:2]), *k_stride[:3], *v_stride[:3]), int(interleaved), magnitude,
+            DTYPE_TO_CODE[key_dtype], DTYPE_TO_CODE[k_dtype], int(positions_dtype == torch.int64), int(slots_dtype == torch.int64))
+
+
+def paged_write_rope(q: torch.Tensor, key: torch.Tensor, value: torch.Tensor, positions: torch.Tensor, rates: torch.Tensor,
+                     k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, interleaved: bool = True,
+                     magnitude: float = 1.0, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                     keep_key: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """(q', key'); key' has no tokens where it is not kept."""
+    _same_device("paged_write_rope", q, key, value, positions, rates, k_cache, v_cache, slots)
+    rest = (k_cache.shape, k_cache.stride(), k_cache.dtype, v_cache.shape, v_cache.stride(), v_cache.dtype, positions.shape[0],
+            positions.dtype, slots.shape[0], slots.dtype, rates.shape[0], interleaved, magnitude)
+    plan = _rope_write_plan(q.shape, q.stride(), q.dtype, key.shape, key.stride(), key.dtype, value.shape, value.stride(), value.dtype,
+                            *rest)
+    if plan is None or (q.data_ptr() | key.data_ptr() | value.data_ptr()) & 15:
+        q, key, value = _rows16(q), _rows16(key), _rows16(value)
+        plan = _rope_write_plan(q.shape, q.stride(), q.dtype, key.shape, key.stride(), key.dtype, value.shape, value.stride(),
+                                value.dtype, *rest)
+    k, v = _cache_pointers("paged_write_rope", k_cache, v_cache)
+    if k_scale is not None:
+        k_scale = _scalar_on(k_scale, key.device, "k_scale")
+    if v_scale is not None:
+        v_scale = _scalar_on(v_scale, key.device, "v_scale")
+    if (k_scale is not None or v_scale is not None) and k_cache.dtype != torch.float8_e4m3fn:
+        raise ValueError(f"paged_write_rope: k_scale and v_scale are for a cache of float8_e4m3fn, not {k_cache.dtype}")
+    positions, rates, slots = positions.contiguous(), rates.contiguous(), slots.contiguous()
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    key_out = torch.empty(key.shape if keep_key else (0, *key.shape[1:]), dtype=q.dtype, device=q.device)
+    _launch("ckh_paged_write_rope", q, q.data_ptr(), key.data_ptr(), value.data_ptr(), positions.data_ptr(), rates.data_ptr(),
+            out.data_ptr(), key_out.data_ptr() if keep_key else None, k, v, slots.data_ptr(), _ptr(k_scale), _ptr(v_scale), *plan)
+    return out, key_out
+
+
+@functools.lru_cache(maxsize=512)
+def _shared_plan(q_shape, q_stride, q_dtype, k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype, table_shape, table_stride,
+                 sequences, starts, shared, scale):
+    k_stride, v_stride = _cache_pair("shared_attention", k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype)
+    batch, heads, dim = q_shape
+    pages, page_size, kv_heads, cache_dim = k_shape
+    if dim != cache_dim or kv_heads == 0 or heads % kv_heads:
+        raise ValueError(f"shared_attention: q {list(q_shape)} does not fit a cache of {kv_heads} heads of {cache_dim}")
+    if dim not in (64, 96, 128, 256):
+        raise ValueError(f"shared_attention: head_dim {dim} is not 64, 96, 128 or 256")
+    if k_dtype not in (q_dtype, torch.float8_e4m3fn):
+        raise ValueError(f"shared_attention: a cache of {k_dtype} with queries of {q_dtype}")
+    if table_shape[0] != batch or sequences != batch:
+        raise ValueError(f"shared_attention: page_table {list(table_shape)} and {sequences} lengths for {batch} sequences")
+    if starts != shared + 1:
+        raise ValueError(f"shared_attention: {starts} group bounds for {shared} groups, which need one more than that")
+    q_stride = _used_strides(q_shape, q_stride)
+    if not _on_rows16(q_stride, 2):
+        return None
+    nbytes = int(_lib.ckh_shared_attention_workspace_bytes(batch, heads, kv_heads, dim, shared, page_size, table_shape[1]))
+    return ((batch, heads, kv_heads, dim, shared, pages, page_size, table_shape[1], table_stride[0],
+             _strides(*q_stride[:2], *k_stride[:3], *v_stride[:3]), dim ** -0.5 if scale is None else scale,
+             DTYPE_TO_CODE[q_dtype], DTYPE_TO_CODE[k_dtype]), nbytes)
+
+
+def shared_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                     groups: torch.Tensor, shared: torch.Tensor, scale: float | None = None, k_scale: torch.Tensor | None = None,
+                     v_scale: torch.Tensor | None = None) -> torch.Tensor:
+    _same_device("shared_attention", q, k_cache, v_cache, page_table, lengths, groups, shared)
+    lengths, groups, shared = lengths.contiguous(), groups.contiguous(), shared.contiguous()
+    if page_table.stride(1) != 1 and page_table.shape[1] > 1:
+        page_table = page_table.contiguous()
+    rest = (k_cache.shape, k_cache.stride(), k_cache.dtype, v_cache.shape, v_cache.stride(), v_cache.dtype, page_table.shape,
+            page_table.stride(), lengths.shape[0], groups.shape[0], shared.shape[0], scale)
+    plan = _shared_plan(q.shape, q.stride(), q.dtype, *rest)
+    if plan is None or q.data_ptr() % 16:
+        q = _rows16(q)
+        plan = _shared_plan(q.shape, q.stride(), q.dtype, *rest)
+    sizes, nbytes = plan
+    k, v = _cache_pointers("shared_attention", k_cache, v_cache)
+    if k_scale is not None:
+        k_scale = _scalar_on(k_scale, q.device, "k_scale")
+    if v_scale is not None:
+        v_scale = _scalar_on(v_scale, q.device, "v_scale")
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _launch("ckh_shared_attention", q, q.data_ptr(), k, v, page_table.data_ptr(), lengths.data_ptr(), groups.data_ptr(),
+            shared.data_ptr(), _ptr(k_scale), _ptr(v_scale), out.data_ptr(), *sizes, _ptr(ws), nbytes)
+    return out
+
+
+# ------------------------------------------------------------------------------- norms
+def _norm_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """t [..., cols] and the elements between its rows, copied where they are not one step apart."""
+    if t.dim() > 2:
+        t = t.reshape(-1, t.shape[-1])
+    rows, cols = t.shape if t.dim() == 2 else (1, t.shape[0])
+    if cols > 1 and t.stride(-1) != 1:
+        t = t.contiguous()
+    return t, t.stride(0) if rows > 1 and t.dim() == 2 else cols
+
+
+def _rms_norm(name: str, x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Tensor | None, eps: float, scale, y, scales,
+              out_rows: int, out_cols: int, mx: int) -> torch.Tensor:
+    cols = x.shape[-1]
+    rows = x.numel() // cols if cols else 0
+    h = torch.empty(x.shape if residual is not None else (0,), dtype=x.dtype, device=x.device)
+    if rows == 0 and not mx:
+        return h
+    flat, step = _norm_rows(x)
+    r_step, r = 0, residual
+    if residual is not None:
+        r, r_step = _norm_rows(residual)
+    if weight is not None:
+        weight = weight.contiguous()
+    _launch("ckh_rms_norm", x, flat.data_ptr(), _ptr(r), _ptr(weight), _ptr(scale), y.data_ptr(), _ptr(scales),
+            None if r is None else h.data_ptr(), rows, cols, out_rows, out_cols, step, r_step, eps, DTYPE_TO_CODE[x.dtype],
+            0 if weight is None else DTYPE_TO_CODE[weight.dtype], DTYPE_TO_CODE[y.dtype], mx)
+    return h
+
+
+def _check_norm(name: str, x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Tensor | None) -> None:
+    _same_device(name, x, weight, residual)
+    if weight is not None and weight.shape[0] != x.shape[-1]:
+        raise ValueError(f"{name}: {weight.shape[0]} weights for rows of {x.shape[-1]}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError(f"{name}: x {list(x.shape)} {x.dtype} and residual {list(residual.shape)} {residual.dtype} differ")
+    if x.shape[-1] > 65536:
+        raise ValueError(f"{name}: rows of {x.shape[-1]} elements, 65536 at most")
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+             eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    """(y, h); h has no elements where there is no residual."""
+    _check_norm("rms_norm", x, weight, residual)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    cols = x.shape[-1]
+    rows = x.numel() // cols if cols else 0
+    return y, _rms_norm("rms_norm", x, weight, residual, eps, None, y, None, rows, cols, 0)
+
+
+def rms_norm_fp8(x: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+                 eps: float = 1e-6, output_type: torch.dtype = torch.float8_e4m3fn) -> tuple[torch.Tensor, torch.Tensor]:
+    _check_norm("rms_norm_fp8", x, weight, residual)
+    scale = _scalar_on(scale, x.device, "scale")
+    y = torch.empty(x.shape, dtype=output_type, device=x.device)
+    cols = x.shape[-1]
+    rows = x.numel() // cols if cols else 0
+    return y, _rms_norm("rms_norm_fp8", x, weight, residual, eps, scale, y, None, rows, cols, 0)
+
+
+def rms_norm_mxfp8(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torch.Tensor | None = None, eps: float = 1e-6,
+                   pad_32x: bool = False) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    _check_norm("rms_norm_mxfp8", x, weight, residual)
+    rows, cols = x.shape
+    out_rows, out_cols = (roundup(rows, 32), roundup(cols, 32)) if pad_32x else (rows, cols)
+    if out_cols % 32:
+        raise ValueError(f"K dimension must be divisible by 32 (got {cols}); pass pad_32x=True")
+    y = torch.empty((out_rows, out_cols), dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty((roundup(rows, 128), roundup(out_cols // 32, 4)), dtype=torch.float8_e8m0fnu, device=x.device)
+    return y, scales, _rms_norm("rms_norm_mxfp8", x, weight, residual, eps, None, y, scales, out_rows, out_cols, 1)
+
+
+# ---------------------------------------------------------------------------- sampling
+@functools.lru_cache(maxsize=256)
+def _sample_workspace_bytes(rows: int, vocab: int) -> int:
+    return int(_lib.ckh_sample_workspace_bytes(rows, vocab))
+
+
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor | float = 1.0, top_k: torch.Tensor | int = 0,
+                  top_p: torch.Tensor | float = 1.0, min_p: torch.Tensor | float = 0.0) -> torch.Tensor:
+    """Each of the four is a number for all rows, or a tensor of one a row."""
+    rows, vocab = logits.shape
+    if u.shape[0] != rows:
+        raise ValueError(f"sample_tokens: {u.shape[0]} random numbers for {rows} rows")
+    if vocab == 0:
+        raise ValueError("sample_tokens: no logits")
+    per_row, common = [], []
+    for name, value, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                               ("min_p", min_p, torch.float32)):
+        if isinstance(value, torch.Tensor):
+            if value.shape != (rows,) or value.dtype != dtype:
+                raise ValueError(f"sample_tokens: {name} {list(value.shape)} {value.dtype} is not one {dtype} for each of {rows} rows")
+            per_row.append(value.contiguous())
+            common.append(0)
+        else:
+            per_row.append(None)
+            common.append(value)
+    _same_device("sample_tokens", logits, u, *per_row)
+    if vocab > 1 and logits.stride(1) != 1:
+        logits = logits.contiguous()
+    u = u.contiguous()
+    out = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    nbytes = _sample_workspace_bytes(rows, vocab)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
+    _launch("ckh_sample", logits, logits.data_ptr(), u.data_ptr(), *(_ptr(t) for t in per_row), common[0], common[1], common[2], common[3],
+            out.data_ptr(), rows, vocab, logits.stride(0) if rows > 1 else vocab, DTYPE_TO_CODE[logits.dtype], ws.data_ptr(), nbytes)
+    return out
+
+
 # ----------------------------------------------------------------------------- RoPE
 def _rope_call(xq: torch.Tensor, xk: torch.Tensor | None, freqs_cis: torch.Tensor):
     if xq.dim() != 4 or freqs_cis.dim() != 6:
@@ -860,6 +1090,37 @@ def _build_constraints() -> dict:
                                k=ParamConstraint(dtypes=half, shape_rules=(ExactDims(4),)),
                                v=ParamConstraint(dtypes=half, shape_rules=(ExactDims(4),)),
                                lengths=ParamConstraint(dtypes=i32, shape_rules=(ExactDims(1),))),
+        "shared_attention": fc(q=ParamConstraint(dtypes=half, shape_rules=(ExactDims(3),)),
+                               k_cache=ParamConstraint(dtypes=half | e4m3, shape_rules=(ExactDims(4),)),
+                               v_cache=ParamConstraint(dtypes=half | e4m3, shape_rules=(ExactDims(4),)),
+                               page_table=ParamConstraint(dtypes=i32, shape_rules=two_d),
+                               lengths=ParamConstraint(dtypes=i32, shape_rules=(ExactDims(1),)),
+                               groups=ParamConstraint(dtypes=i32, shape_rules=(ExactDims(1),)),
+                               shared=ParamConstraint(dtypes=i32, shape_rules=(ExactDims(1),)),
+                               k_scale=ParamConstraint(dtypes=f32, devices=frozenset({"cuda", "cpu"})),
+                               v_scale=ParamConstraint(dtypes=f32, devices=frozenset({"cuda", "cpu"}))),
+        "paged_write_rope": fc(q=ParamConstraint(dtypes=half, shape_rules=(ExactDims(3),)),
+                               key=ParamConstraint(dtypes=half, shape_rules=(ExactDims(3),)),
+                               value=ParamConstraint(dtypes=half, shape_rules=(ExactDims(3),)),
+                               positions=ParamConstraint(dtypes=ints, shape_rules=(ExactDims(1),)),
+                               rates=ParamConstraint(dtypes=f32, shape_rules=(ExactDims(1),)),
+                               k_cache=ParamConstraint(dtypes=half | e4m3, shape_rules=(ExactDims(4),)),
+                               v_cache=ParamConstraint(dtypes=half | e4m3, shape_rules=(ExactDims(4),)),
+                               slots=ParamConstraint(dtypes=ints, shape_rules=(ExactDims(1),)),
+                               k_scale=ParamConstraint(dtypes=f32, devices=frozenset({"cuda", "cpu"})),
+                               v_scale=ParamConstraint(dtypes=f32, devices=frozenset({"cuda", "cpu"}))),
+        "rms_norm": fc(x=ParamConstraint(dtypes=floats, shape_rules=(MinDims(1),)),
+                       weight=ParamConstraint(dtypes=floats, shape_rules=(ExactDims(1),)),
+                       residual=ParamConstraint(dtypes=floats)),
+        "rms_norm_fp8": fc(x=ParamConstraint(dtypes=floats, shape_rules=(MinDims(1),)),
+                           scale=ParamConstraint(dtypes=f32, devices=frozenset({"cuda", "cpu"})),
+                           weight=ParamConstraint(dtypes=floats, shape_rules=(ExactDims(1),)),
+                           residual=ParamConstraint(dtypes=floats), output_type=ParamConstraint(dtypes=fp8)),
+        "rms_norm_mxfp8": fc(x=ParamConstraint(dtypes=floats, shape_rules=two_d),
+                             weight=ParamConstraint(dtypes=floats, shape_rules=(ExactDims(1),)),
+                             residual=ParamConstraint(dtypes=floats)),
+        "sample_tokens": fc(logits=ParamConstraint(dtypes=floats, shape_rules=two_d),
+                            u=ParamConstraint(dtypes=f32, shape_rules=(ExactDims(1),))),
         "apply_rope1": fc(x=ParamConstraint(dtypes=floats, shape_rules=(ExactDims(4),)),
                           freqs_cis=ParamConstraint(dtypes=floats, shape_rules=(ExactDims(6),))),
         "apply_rope": fc(xq=ParamConstraint(dtypes=floats, shape_rules=(ExactDims(4),)),

@@ -363,6 +363,93 @@ def _(q, k, v, window, sinks, lengths, scale):
     return q.new_empty(q.shape)
 
 
+@torch.library.custom_op("comfy_kitchen::shared_attention", mutates_args=())
+def shared_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                     lengths: torch.Tensor, groups: torch.Tensor, shared: torch.Tensor, scale: float | None,
+                     k_scale: torch.Tensor | None, v_scale: torch.Tensor | None) -> torch.Tensor:
+    return _dispatch("shared_attention", q=q, k_cache=k_cache, v_cache=v_cache, page_table=page_table, lengths=lengths,
+                     groups=groups, shared=shared, scale=scale, k_scale=k_scale, v_scale=v_scale)
+
+
+@shared_attention.register_fake
+def _(q, k_cache, v_cache, page_table, lengths, groups, shared, scale, k_scale, v_scale):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("comfy_kitchen::paged_write_rope", mutates_args=("k_cache", "v_cache"))
+def paged_write_rope(q: torch.Tensor, key: torch.Tensor, value: torch.Tensor, positions: torch.Tensor,
+                     rates: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
+                     interleaved: bool, magnitude: float, k_scale: torch.Tensor | None, v_scale: torch.Tensor | None,
+                     keep_key: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    return _dispatch("paged_write_rope", q=q, key=key, value=value, positions=positions, rates=rates, k_cache=k_cache,
+                     v_cache=v_cache, slots=slots, interleaved=interleaved, magnitude=magnitude, k_scale=k_scale,
+                     v_scale=v_scale, keep_key=keep_key)
+
+
+@paged_write_rope.register_fake
+def _(q, key, value, positions, rates, k_cache, v_cache, slots, interleaved, magnitude, k_scale, v_scale, keep_key):
+    return q.new_empty(q.shape), key.new_empty(key.shape if keep_key else (0, *key.shape[1:]))
+
+
+# ---------------------------------------------------------------- norms, sampling
+@torch.library.custom_op("comfy_kitchen::rms_norm", mutates_args=())
+def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Tensor | None,
+             eps: float) -> tuple[torch.Tensor, torch.Tensor]:
+    return _dispatch("rms_norm", x=x, weight=weight, residual=residual, eps=eps)
+
+
+def _fake_sum(x, residual):
+    return x.new_empty(x.shape if residual is not None else (0,))
+
+
+@rms_norm.register_fake
+def _(x, weight, residual, eps):
+    return x.new_empty(x.shape), _fake_sum(x, residual)
+
+
+@torch.library.custom_op("comfy_kitchen::rms_norm_fp8", mutates_args=())
+def rms_norm_fp8(x: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor | None, residual: torch.Tensor | None,
+                 eps: float, output_dtype_code: int) -> tuple[torch.Tensor, torch.Tensor]:
+    return _dispatch("rms_norm_fp8", x=x, scale=scale, weight=weight, residual=residual, eps=eps,
+                     output_type=DTYPE_CODE_TO_DTYPE[output_dtype_code])
+
+
+@rms_norm_fp8.register_fake
+def _(x, scale, weight, residual, eps, output_dtype_code):
+    return x.new_empty(x.shape, dtype=DTYPE_CODE_TO_DTYPE[output_dtype_code]), _fake_sum(x, residual)
+
+
+@torch.library.custom_op("comfy_kitchen::rms_norm_mxfp8", mutates_args=())
+def rms_norm_mxfp8(x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Tensor | None, eps: float,
+                   pad_32x: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _dispatch("rms_norm_mxfp8", x=x, weight=weight, residual=residual, eps=eps, pad_32x=pad_32x)
+
+
+@rms_norm_mxfp8.register_fake
+def _(x, weight, residual, eps, pad_32x):
+    rows, cols = x.shape
+    if pad_32x:
+        rows, cols = roundup(rows, 32), roundup(cols, 32)
+    q = torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device=x.device)
+    s = torch.empty((roundup(x.shape[0], 128), roundup(cols // 32, 4)), dtype=torch.float8_e8m0fnu, device=x.device)
+    return q, s, _fake_sum(x, residual)
+
+
+@torch.library.custom_op("comfy_kitchen::sample_tokens", mutates_args=())
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: float, top_k: int, top_p: float, min_p: float,
+                  temperatures: torch.Tensor | None, top_ks: torch.Tensor | None, top_ps: torch.Tensor | None,
+                  min_ps: torch.Tensor | None) -> torch.Tensor:
+    """The values hold for all rows where there is no tensor of one for each."""
+    return _dispatch("sample_tokens", logits=logits, u=u, temperature=temperature if temperatures is None else temperatures,
+                     top_k=top_k if top_ks is None else top_ks, top_p=top_p if top_ps is None else top_ps,
+                     min_p=min_p if min_ps is None else min_ps)
+
+
+@sample_tokens.register_fake
+def _(logits, u, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps):
+    return logits.new_empty(logits.shape[0], dtype=torch.int64)
+
+
 # ------------------------------------------------------------------------- RoPE
 @torch.library.custom_op("comfy_kitchen::apply_rope", mutates_args=())
 def apply_rope(xq: torch.Tensor, xk: torch.Tensor, freqs_cis: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:

@@ -22,43 +22,6 @@ namespace ckh {
 constexpr int kThreads = 128;
 constexpr int kPerThread = 16;
 
-template <int OUT>
-__device__ __forceinline__ uint32_t encode_fp8(float t) {
-    if constexpr (OUT == CKH_E4M3) {
-        t = t > 448.0f ? 448.0f : (t < -448.0f ? -448.0f : t);  // NaN passes through
-        return f_to_e4m3(t);
-    } else {
-        t = t > 57344.0f ? 57344.0f : (t < -57344.0f ? -57344.0f : t);
-        return f_to_e5m2(t);
-    }
-}
-
-// The code of a NaN product t = x * r, as the reference's eager arithmetic writes it
-// (torch's vectorised CPU kernels on x86; the c10 E4M3/E5M2 cast is 0x7F | sign for NaN):
-//  - bf16: the bf16 narrowing of the product (vec512_bfloat16.h cvtfp32_bf16) turns every
-//    NaN into 0xFFFF, so every NaN code is 0xFF.  (Eager's scalar remainder, the < 64
-//    elements of each thread's chunk past its last whole vector pair, narrows through
-//    c10::BFloat16 instead, whose NaN is 0x7FC0: 0x7F there.)
-//  - f16 / f32: the NaN keeps its sign through the multiply, clamp and narrowing.  The
-//    product's NaN is r's when r = 1/scale is NaN (scale NaN, r keeps its sign), else x's,
-//    else x86's default NaN, which is negative (0 * inf).
-template <int IN>
-__device__ __forceinline__ uint32_t fp8_nan_code(float x, float scale) {
-    if constexpr (IN == CKH_BF16) {
-        return 0xffu;
-    } else {
-        const uint32_t s = is_nan(scale) ? as_u(scale) : (is_nan(x) ? as_u(x) : 0x80000000u);
-        return 0x7fu | ((s >> 24) & 0x80u);
-    }
-}
-
-// One element through the reference's steps (software converts), NaN bytes included.
-template <int IN, int OUT>
-__device__ __forceinline__ uint32_t quantize_one(float x, float r, float scale) {
-    const float t = round_to<IN>(x * r);
-    return is_nan(t) ? fp8_nan_code<IN>(x, scale) : encode_fp8<OUT>(t);
-}
-
 template <int IN, int OUT, bool VEC>
 __global__ __launch_bounds__(kThreads) void quantize_fp8_kernel(const void* __restrict__ x,
                                                                 const float* __restrict__ scale,

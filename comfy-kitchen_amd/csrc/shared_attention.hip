@@ -1,0 +1,594 @@
+// Attention of one new token per sequence over a key-value cache held in pages, for sequences that begin
+// with the same tokens, for gfx950:
+//   out[b, h] = sum_t softmax_t(scale q[b, h] . k_t) v_t,  t < lengths[b],
+// where the first shared[g] tokens of a group's sequences are the same rows of the cache.
+//
+// A span is a run of tokens that some sequences see: what a group shares, seen by all its sequences, and what
+// lies behind it, seen by one.  Its rows are these sequences' query heads of a key-value head; so the common
+// tokens are a matrix product of many rows, read once for each 128 of them, and bound by the matrix units
+// from some 300 rows on, by HBM below.
+//   - A small first launch turns lengths and groups, which only the device knows, into a list of pieces of work: a
+//     span's tokens in chunks of one size for the whole call, chosen so that there are about two a CU,
+//     times its blocks of 128 rows and the key-value heads.
+//   - The second works on one piece a workgroup, as prompts are (attn.h): a wave owns 32 rows, the columns of
+//     32x32x16 MFMAs, with running maximum and sum; tiles of 64 tokens go to LDS, the next while this
+//     one is used, each token's row found by its page, which is looked up a tile before.  A 16-bit cache goes there
+//     without passing registers; E4M3 codes are widened on the way, once for all rows.
+//   - The third joins each row's chunks, those of its group and its own, in their order: results do not
+//     depend on timing.
+#include <algorithm>
+
+#include "attn.h"
+
+namespace ckh {
+namespace attn {
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(1))) void global_void;
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s lds_v4s;
+
+constexpr int kTileTokens = 64;
+constexpr int kBlockRows = 128;
+constexpr int kMinTiles = 4;    // of a chunk, where a span has several
+constexpr int kMaxSpans = 4096; // sequences and groups of a call
+constexpr int kPlanThreads = 1024;
+
+struct Span {
+    int first, chunks;   // its first piece of work; chunks of each row
+    int seq, sequences;  // the sequences that see it
+    int from, to;        // tokens
+    int group;           // of a sequence's own span: its group's span, or -1
+    int pad;
+    int64_t part;        // row of the partial results that chunk 0 of its first row has
+};
+
+struct Piece {
+    int span, kv_head, row0, chunk;  // span -1: nothing to do
+    int from, to;                    // tokens
+    int seq, rows;                   // the span's first sequence; its rows
+    int64_t part;                    // of the span's row 0 in this chunk and head
+    int64_t pad;
+};
+
+struct SharedArgs {
+    const uint8_t *q, *k, *v;
+    const int *table, *lengths, *starts, *shared;
+    const float *k_scale, *v_scale;
+    uint8_t* out;
+    Span* spans;     // [groups + batch]
+    Piece* pieces;   // [slots]
+    float *part, *stat;  // [row][D], [row][2]: unnormalised outputs; maxima and sums
+    int64_t q_b, q_h, k_page, k_tok, k_head, v_page, v_tok, v_head;  // bytes
+    int64_t table_stride;
+    int batch, heads, kv_heads, group, groups;  // group: query heads of a key-value head
+    int pages, page_size, capacity, slots, target;
+    float scale;
+    FastDiv by_page, by_group;
+};
+
+// Inclusive sum over the plan's threads; `total` of all.
+template <typename T>
+__device__ __forceinline__ T plan_scan(T v, T* wave_sums, T& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const T u = __shfl_up(v, d, 64);
+        if (lane >= d) v += u;
+    }
+    __syncthreads();
+    if (lane == 63) wave_sums[wave] = v;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 64; ++w) {
+        if (w < wave) v += wave_sums[w];
+        total += wave_sums[w];
+    }
+    return v;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(SharedArgs a) {
+    __shared__ int start[kMaxSpans + 1], common[kMaxSpans], first[kMaxSpans + 1];
+    __shared__ int64_t sums[kPlanThreads / 64];
+    __shared__ int top[kPlanThreads / 64];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int spans = a.groups + a.batch;
+    const auto length = [&](int b) { return max(0, min(a.lengths[b], a.capacity)); };
+
+    // group bounds, within the batch and ascending (whatever they are, groups do not overlap)
+    int before = 0;
+    for (int i0 = 0; i0 <= a.groups; i0 += kPlanThreads) {
+        int v = i0 + t <= a.groups ? max(0, min(a.starts[i0 + t], a.batch)) : 0;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int u = __shfl_up(v, d, 64);
+            if (lane >= d) v = max(v, u);
+        }
+        __syncthreads();
+        if (lane == 63) top[wave] = v;
+        __syncthreads();
+        v = max(v, before);
+        for (int w = 0; w < kPlanThreads / 64; ++w) {
+            if (w < wave) v = max(v, top[w]);
+            before = max(before, top[w]);
+        }
+        if (i0 + t <= a.groups) start[i0 + t] = v;
+    }
+    for (int g = t; g < a.groups; g += kPlanThreads) common[g] = max(0, a.shared[g]);
+    __syncthreads();
+    const auto group_of = [&](int b) {  // the last group that begins at or before b, if b is in it
+        int lo = 0, hi = a.groups;      // groups lo .. hi - 1
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (start[mid] <= b) lo = mid + 1;
+            else hi = mid;
+        }
+        return lo > 0 && b < start[lo] ? lo - 1 : -1;
+    };
+    for (int b = t; b < a.batch; b += kPlanThreads) {
+        const int g = group_of(b);
+        if (g >= 0) atomicMin(&common[g], start[g + 1] - start[g] > 1 ? length(b) : 0);
+    }
+    __syncthreads();
+
+    const auto span = [&](int i) {
+        Span s{};
+        if (i < a.groups) {
+            s.seq = start[i], s.sequences = start[i + 1] - start[i];
+            s.to = s.sequences ? common[i] : 0;
+            s.group = -1;
+        } else {
+            s.seq = i - a.groups, s.sequences = 1;
+            s.group = group_of(s.seq);
+            s.from = s.group < 0 ? 0 : common[s.group];
+            s.to = length(s.seq);
+        }
+        return s;
+    };
+    const auto tiles_of = [&](const Span& s) { return (s.to - s.from + kTileTokens - 1) / kTileTokens; };
+    const auto units_of = [&](const Span& s) {  // pieces of a chunk of all its rows
+        return static_cast<int64_t>((static_cast<int64_t>(s.sequences) * a.group + kBlockRows - 1) / kBlockRows) * a.kv_heads;
+    };
+    int64_t tiles = 0, units = 0;
+    for (int i0 = 0; i0 < spans; i0 += kPlanThreads) {
+        int64_t work = 0, some = 0, total;
+        if (i0 + t < spans) {
+            const Span s = span(i0 + t);
+            const int n = tiles_of(s);
+            some = n ? units_of(s) : 0;
+            work = some * n;
+        }
+        plan_scan(work, sums, total);
+        tiles += total;
+        plan_scan(some, sums, total);
+        units += total;
+    }
+    // every span has a ragged end of its own
+    const int64_t room = max(a.target - units, static_cast<int64_t>(a.target / 2));
+    const int64_t size = max((tiles + room - 1) / room, static_cast<int64_t>(kMinTiles));
+
+    int64_t slot = 0, row = 0;
+    for (int i0 = 0; i0 < spans; i0 += kPlanThreads) {
+        int64_t n = 0, rows = 0, total;
+        Span s{};
+        if (i0 + t < spans) {
+            s = span(i0 + t);
+            s.chunks = static_cast<int>((tiles_of(s) + size - 1) / size);
+            n = s.chunks * units_of(s);
+            rows = static_cast<int64_t>(s.chunks) * a.kv_heads * s.sequences * a.group;
+        }
+        const int64_t end = plan_scan(n, sums, total);
+        s.first = static_cast<int>(slot + end - n);
+        slot += total;
+        const int64_t row_end = plan_scan(rows, sums, total);
+        s.part = row + row_end - rows;
+        row += total;
+        if (i0 + t < spans) {
+            first[i0 + t] = s.first;
+            a.spans[i0 + t] = s;
+        }
+    }
+    if (t == 0) first[spans] = static_cast<int>(slot);
+    __threadfence_block();
+    __syncthreads();
+    for (int i = t; i < a.slots; i += kPlanThreads) {
+        Piece p{};
+        p.span = -1;
+        if (i < static_cast<int>(slot)) {
+            int lo = 0, hi = spans;  // the last span that begins at or before i
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (first[mid] <= i) lo = mid;
+                else hi = mid;
+            }
+            const Span s = a.spans[lo];
+            // chunk by chunk, block of rows by block, and the heads of a token's rows side by side
+            const int blocks = static_cast<int>(units_of(s)) / a.kv_heads, in = i - s.first;
+            const int at = in / a.kv_heads;
+            p.span = lo;
+            p.kv_head = in - at * a.kv_heads;
+            p.chunk = at / blocks;
+            p.row0 = (at - p.chunk * blocks) * kBlockRows;
+            p.from = static_cast<int>(s.from + p.chunk * size * kTileTokens);
+            p.to = static_cast<int>(min(static_cast<int64_t>(s.to), p.from + size * kTileTokens));
+            p.seq = s.seq;
+            p.rows = s.sequences * a.group;
+            p.part = s.part + (static_cast<int64_t>(p.chunk) * a.kv_heads + p.kv_head) * p.rows;
+        }
+        a.pieces[i] = p;
+    }
+}
+
+// LDS rows are D (96: 128) values of 16 bits; 16-byte piece c of token t's row is at piece c ^ swizzle(t).
+template <int D>
+struct TileRows {
+    static constexpr int kPieces = D == 96 ? 16 : D / 8;
+    static constexpr int kBytes = kPieces * 16;
+    static constexpr int kMask = kPieces < 16 ? kPieces - 1 : 15;
+    static __device__ __forceinline__ int k_swizzle(int t) { return t & 7; }
+    static __device__ __forceinline__ int v_swizzle(int t) { return (2 * t) & kMask; }
+};
+
+template <int C, int D, bool F8>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void shared_kernel(SharedArgs a) {
+    using R = TileRows<D>;
+    constexpr int kTile = kTileTokens * R::kBytes;
+    // loads of a thread for a tile of K or V: 16 bytes, of a row's kRow
+    constexpr int kRow = F8 ? D / 16 : R::kPieces;
+    constexpr int kLoads = (kTileTokens * kRow + 255) / 256;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * kTile];  // two buffers of K, V
+
+    const Piece piece = a.pieces[blockIdx.x];
+    if (piece.span < 0) return;  // the whole workgroup
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r32 = lane & 31, g = lane >> 5;
+    const int from = __builtin_amdgcn_readfirstlane(piece.from), to = __builtin_amdgcn_readfirstlane(piece.to);
+    const int kvh = __builtin_amdgcn_readfirstlane(piece.kv_head), rows = __builtin_amdgcn_readfirstlane(piece.rows);
+    const int seq = __builtin_amdgcn_readfirstlane(piece.seq);
+    const int row0 = __builtin_amdgcn_readfirstlane(piece.row0) + wave * 32;
+    const int tiles = (to - from + kTileTokens - 1) / kTileTokens;
+    const int* table = a.table + seq * a.table_stride;
+    const bool busy = row0 < rows;  // this wave has rows
+
+    float c = a.scale * kLog2e * (a.k_scale ? *a.k_scale : 1.0f);
+    const uint32_t flip = c < 0.0f ? 0x80008000u : 0u;
+    c = fmaxf(fabsf(c), 1e-37f);
+    v4u q[D / 16];
+    {
+        const int row = min(row0 + r32, rows - 1), s = a.by_group.div(row);
+        const uint8_t* qp = a.q + (seq + s) * a.q_b + (kvh * a.group + row - s * a.group) * a.q_h + g * 16;
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) q[n] = *reinterpret_cast<const v4u*>(qp + n * 32) ^ flip;
+    }
+
+    // a thread's places in the loads of a tile
+    const auto place = [&](int n) { return F8 ? static_cast<int>(threadIdx.x) + n * 256 : (wave * kLoads + n) * 64 + lane; };
+    const uint8_t* kb = a.k + kvh * a.k_head;
+    const uint8_t* vb = a.v + kvh * a.v_head;
+    int page_of[kLoads];  // of the next tile's tokens
+    const auto token = [&](int i, int n) { return min(from + i * kTileTokens + min(place(n) / kRow, kTileTokens - 1), to - 1); };
+    const auto look_up = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < kLoads; ++n) page_of[n] = table[a.by_page.div(token(i, n))];
+    };
+    v4u held[F8 ? 2 * kLoads : 1];  // codes on their way to LDS
+    // Begins to fetch tile i; its tokens from the chunk's end on are copies of the last.
+    const auto fetch = [&](int i, uint8_t* at) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < kLoads; ++n) {
+            const int tk = token(i, n), slot = tk - a.by_page.div(tk) * a.page_size;
+            const int64_t page = min(static_cast<uint32_t>(page_of[n]), static_cast<uint32_t>(a.pages - 1));
+            const int t = min(place(n) / kRow, kTileTokens - 1), p = place(n) % kRow;
+            const uint8_t* kp = kb + page * a.k_page + slot * a.k_tok;
+            const uint8_t* vp = vb + page * a.v_page + slot * a.v_tok;
+            if constexpr (F8) {
+                held[n] = *reinterpret_cast<const v4u*>(kp + p * 16);
+                held[kLoads + n] = *reinterpret_cast<const v4u*>(vp + p * 16);
+            } else {
+                const int kc = min(p ^ R::k_swizzle(t), D / 8 - 1), vc = min(p ^ R::v_swizzle(t), D / 8 - 1);
+                __builtin_amdgcn_global_load_lds((global_void*)(kp + kc * 16), (lds_void*)(at + (wave * kLoads + n) * 1024), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((global_void*)(vp + vc * 16), (lds_void*)(at + kTile + (wave * kLoads + n) * 1024), 16, 0, 0);
+            }
+        }
+    };
+    // Tile i is in LDS at `at` when this wave and the others are through here; values from the end on are zeros.
+    const auto settle = [&](int i, uint8_t* at) __attribute__((always_inline)) {
+        const int left = to - from - i * kTileTokens;
+#pragma unroll
+        for (int n = 0; n < kLoads; ++n) {
+            const int t = place(n) / kRow, p = place(n) % kRow;
+            if constexpr (F8) {
+                if (kTileTokens * kRow % 256 != 0 && place(n) >= kTileTokens * kRow) continue;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t k0 = held[n][2 * half], k1 = held[n][2 * half + 1];
+                    uint32_t v0 = held[kLoads + n][2 * half], v1 = held[kLoads + n][2 * half + 1];
+                    if (t >= left) v0 = v1 = 0u;
+                    const int piece = 2 * p + half;
+                    *reinterpret_cast<v4u*>(at + t * R::kBytes + ((piece ^ R::k_swizzle(t)) << 4)) =
+                        v4u{widen_e4m3<C, false>(k0), widen_e4m3<C, true>(k0), widen_e4m3<C, false>(k1), widen_e4m3<C, true>(k1)};
+                    *reinterpret_cast<v4u*>(at + kTile + t * R::kBytes + ((piece ^ R::v_swizzle(t)) << 4)) =
+                        v4u{widen_e4m3<C, false>(v0), widen_e4m3<C, true>(v0), widen_e4m3<C, false>(v1), widen_e4m3<C, true>(v1)};
+                }
+            } else {
+                if (left < kTileTokens && t >= left)
+                    *reinterpret_cast<v4u*>(at + kTile + (wave * kLoads + n) * 1024 + lane * 16) = v4u{0u, 0u, 0u, 0u};
+            }
+        }
+    };
+
+    v16f acc[D / 32];
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[n][e] = 0.0f;
+    float m = -1e30f, l = 0.0f;
+
+    const auto use = [&](int i, const uint8_t* kt, const uint8_t* vt) __attribute__((always_inline)) {
+        v16f s[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[h][e] = 0.0f;
+            const int t = h * 32 + r32;
+            const uint8_t* kr = kt + t * R::kBytes;
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n)
+                s[h] = mfma32<C>(*reinterpret_cast<const v4u*>(kr + (((2 * n + g) ^ R::k_swizzle(t)) << 4)), q[n], s[h]);
+        }
+        const int left = to - from - i * kTileTokens;
+        if (left < kTileTokens) {
+            const int high = left - 4 * g;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[h][e] = h * 32 + 8 * (e >> 2) + (e & 3) < high ? s[h][e] : -__builtin_inff();
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) top = fmaxf(top, s[0][e]);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, s[1][e]);
+        top *= c;
+        if (__any(top > m + kLift<C> + 8.0f)) {
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float high = fmaxf(m, top - kLift<C>);
+            const float f = exp2_hw(m - high);
+            m = high;
+            l *= f;
+#pragma unroll
+            for (int n = 0; n < D / 32; ++n) acc[n] *= f;
+        }
+        v4u p[4];
+        float sum = 0.0f;  // the tile's own: single small weights would be lost in a large l
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[h][e] = exp2_hw(__fmaf_rn(s[h][e], c, -m));
+                sum += s[h][e];
+            }
+        l += sum;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                p[w][e] = pack2<C>(s[w >> 1][(w & 1) * 8 + 2 * e], s[w >> 1][(w & 1) * 8 + 2 * e + 1]);
+        // tokens w * 16 + half * 8 + 4 g + 0..3: the lane gives a piece of one token and 4 d, and
+        // gets one d of the four tokens
+        const int sub = lane & 15, db = (lane >> 4) & 1;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+#pragma unroll
+            for (int n = 0; n < D / 32; ++n) {
+                v4u f;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int t = w * 16 + half * 8 + 4 * g + (sub >> 2);
+                    const int piece = n * 4 + db * 2 + ((sub >> 1) & 1);
+                    const uint8_t* at = vt + t * R::kBytes + ((piece ^ R::v_swizzle(t)) << 4) + (sub & 1) * 8;
+                    const v2u two = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at)));
+                    f[half * 2] = two[0];
+                    f[half * 2 + 1] = two[1];
+                }
+                acc[n] = mfma32<C>(f, p[w], acc[n]);
+            }
+        }
+    };
+
+    // (The buffers change hands as pointers: where the compiler sees which part of LDS a load
+    // writes, it waits for the load before the next LDS read.)
+    uint8_t *cur = lds, *next = lds + 2 * kTile;
+    look_up(0);
+    fetch(0, cur);
+    if (tiles > 1) look_up(1);
+    if constexpr (F8) settle(0, cur);
+#pragma unroll 1
+    for (int i = 0; i < tiles; ++i) {
+        __asm__ volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0);  // this wave's part of tile i has arrived
+        if constexpr (!F8) {
+            if (i + 1 == tiles) {
+                __asm__ volatile("" ::: "memory");
+                settle(i, cur);
+                __asm__ volatile("" ::: "memory");
+                __builtin_amdgcn_s_waitcnt(0);
+            }
+        }
+        __builtin_amdgcn_s_barrier();   // everyone's has, and nobody reads the other buffer
+        __asm__ volatile("" ::: "memory");
+        if (i + 1 < tiles) {
+            fetch(i + 1, next);
+            if (i + 2 < tiles) look_up(i + 2);
+        }
+        if (busy) use(i, cur, cur + kTile);
+        if constexpr (F8) {
+            if (i + 1 < tiles) settle(i + 1, next);
+        }
+        uint8_t* const t = cur;
+        cur = next;
+        next = t;
+    }
+    l += __shfl_xor(l, 32, 64);
+
+    if (row0 + r32 >= rows) return;
+    const int64_t at = piece.part + row0 + r32;
+    float* op = a.part + at * D + g * 4;
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<v4f*>(op + n * 32 + e * 8) = v4f{acc[n][4 * e], acc[n][4 * e + 1], acc[n][4 * e + 2], acc[n][4 * e + 3]};
+    if (g == 0) *reinterpret_cast<float2*>(a.stat + at * 2) = make_float2(m, l);
+}
+
+// A row's chunks: D / 4 lanes a row, four d a lane.
+template <int C, int D>
+__global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
+    constexpr int kLanes = D / 4, kRows = 256 / kLanes;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kLanes;
+    if (threadIdx.x >= kRows * kLanes || row >= static_cast<int64_t>(a.batch) * a.heads) return;
+    const int b = static_cast<int>(row / a.heads), h = static_cast<int>(row - static_cast<int64_t>(b) * a.heads);
+    const int kvh = h / a.group, in = h - kvh * a.group, d = threadIdx.x % kLanes * 4;
+    const Span own = a.spans[a.groups + b];
+    Span group{};
+    if (own.group >= 0) group = a.spans[own.group];
+    int64_t at[2], step[2];
+    const Span* both[2] = {&group, &own};
+    float top = -1e30f;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const Span& s = *both[n];
+        step[n] = static_cast<int64_t>(a.kv_heads) * s.sequences * a.group;
+        at[n] = s.part + static_cast<int64_t>(kvh) * s.sequences * a.group + static_cast<int64_t>(b - s.seq) * a.group + in;
+        for (int i = 0; i < s.chunks; ++i) top = fmaxf(top, a.stat[(at[n] + i * step[n]) * 2]);
+    }
+    float sum = 0.0f;
+    v4f o = v4f{0, 0, 0, 0};
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+#pragma unroll 4
+        for (int i = 0; i < both[n]->chunks; ++i) {
+            const int64_t r = at[n] + i * step[n];
+            const float2 st = *reinterpret_cast<const float2*>(a.stat + r * 2);
+            const float f = exp2_hw(st.x - top);
+            sum += f * st.y;
+            o += f * *reinterpret_cast<const v4f*>(a.part + r * D + d);
+        }
+    }
+    const float f = sum == 0.0f ? 0.0f : (a.v_scale ? *a.v_scale : 1.0f) / sum;
+    *reinterpret_cast<v2u*>(a.out + (row * D + d) * 2) = v2u{pack2<C>(o[0] * f, o[1] * f), pack2<C>(o[2] * f, o[3] * f)};
+}
+
+template <int C, int D>
+void launch_shared(const SharedArgs& a, bool f8, hipStream_t st) {
+    plan_kernel<<<1, kPlanThreads, 0, st>>>(a);
+    if (f8) shared_kernel<C, D, true><<<a.slots, 256, 0, st>>>(a);
+    else shared_kernel<C, D, false><<<a.slots, 256, 0, st>>>(a);
+    const int64_t rows = static_cast<int64_t>(a.batch) * a.heads;
+    shared_join_kernel<C, D><<<static_cast<unsigned>(cdiv(rows, 256 / (D / 4))), 256, 0, st>>>(a);
+}
+
+template <int C>
+void launch_shared(int dim, const SharedArgs& a, bool f8, hipStream_t st) {
+    if (dim == 64) launch_shared<C, 64>(a, f8, st);
+    else if (dim == 96) launch_shared<C, 96>(a, f8, st);
+    else if (dim == 128) launch_shared<C, 128>(a, f8, st);
+    else launch_shared<C, 256>(a, f8, st);
+}
+
+// Places in the workspace.
+struct SharedSpace {
+    int64_t target, slots, rows, pieces, part, stat, bytes;  // slots: pieces of work at most; rows: of partial results
+    SharedSpace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t groups) {
+        const int64_t all = batch * (heads / kv_heads);  // rows of a key-value head
+        target = 2 * device_cus();
+        // units: blocks of each sequence's rows and of each group's
+        const int64_t units = kv_heads * (batch * cdiv(heads / kv_heads, kBlockRows) + groups + all / kBlockRows);
+        slots = target + units;
+        rows = target * std::min<int64_t>(kBlockRows, all) + 2 * kv_heads * all;
+        pieces = rup((batch + groups) * sizeof(Span), 256);
+        part = pieces + rup(slots * sizeof(Piece), 256);
+        stat = part + rup(rows * dim * 4, 256);
+        bytes = stat + rows * 8;
+    }
+};
+
+}  // namespace attn
+}  // namespace ckh
+
+using namespace ckh;
+
+extern "C" int64_t ckh_shared_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t groups,
+                                                        int64_t page_size, int64_t max_pages) {
+    if (batch <= 0 || kv_heads <= 0 || heads < kv_heads || dim <= 0 || groups < 0 || page_size <= 0 || max_pages < 0) return 0;
+    return attn::SharedSpace(batch, heads, kv_heads, dim, groups).bytes;
+}
+
+extern "C" int ckh_shared_attention(const void* q, const void* k_cache, const void* v_cache, const void* page_table,
+                                    const void* lengths, const void* group_starts, const void* shared, const void* k_scale,
+                                    const void* v_scale, void* out, int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim,
+                                    int64_t groups, int64_t pages, int64_t page_size, int64_t max_pages, int64_t table_stride,
+                                    const int64_t* strides, float scale, int q_code, int cache_code, void* workspace,
+                                    int64_t workspace_bytes, uintptr_t stream) {
+    CKH_REQUIRE(q_code == CKH_F16 || q_code == CKH_BF16, "shared_attention: unsupported query dtype %d", q_code);
+    CKH_REQUIRE(cache_code == q_code || cache_code == CKH_E4M3, "shared_attention: cache dtype %d with query dtype %d",
+                cache_code, q_code);
+    CKH_REQUIRE(dim == 64 || dim == 96 || dim == 128 || dim == 256, "shared_attention: head_dim %lld is not 64, 96, 128 or 256",
+                static_cast<long long>(dim));
+    CKH_REQUIRE(batch >= 0 && heads >= 0 && kv_heads > 0 && heads % kv_heads == 0 && heads <= 65535,
+                "shared_attention: %lld heads over %lld key-value heads", static_cast<long long>(heads),
+                static_cast<long long>(kv_heads));
+    CKH_REQUIRE(groups >= 0 && batch + groups <= attn::kMaxSpans, "shared_attention: %lld sequences in %lld groups (%d together at most)",
+                static_cast<long long>(batch), static_cast<long long>(groups), attn::kMaxSpans);
+    CKH_REQUIRE(pages > 0 && pages <= INT32_MAX && page_size > 0 && max_pages >= 0 && page_size <= INT32_MAX &&
+                    max_pages <= INT32_MAX && max_pages * page_size <= INT32_MAX - 64,
+                "shared_attention: %lld pages of %lld tokens, %lld a sequence", static_cast<long long>(pages),
+                static_cast<long long>(page_size), static_cast<long long>(max_pages));
+    if (batch == 0 || heads == 0) return CKH_OK;
+    CKH_REQUIRE(q && k_cache && v_cache && (page_table || max_pages == 0) && lengths && group_starts && (shared || groups == 0) && out &&
+                    strides && workspace,
+                "shared_attention: null pointer");
+    const int es = cache_code == CKH_E4M3 ? 1 : 2;
+    // q: batch, head; k: page, token, head; v: page, token, head (elements)
+    for (int i = 0; i < 8; ++i)
+        CKH_REQUIRE(strides[i] >= 0 && strides[i] * (i < 2 ? 2 : es) % 16 == 0, "shared_attention: stride %d (%lld) is not a multiple of 16 bytes",
+                    i, static_cast<long long>(strides[i]));
+    CKH_REQUIRE(aligned(q, 16) && aligned(k_cache, 16) && aligned(v_cache, 16) && aligned(out, 8) && aligned(page_table, 4) &&
+                    aligned(lengths, 4) && aligned(group_starts, 4) && aligned(shared, 4) && aligned(k_scale, 4) && aligned(v_scale, 4) &&
+                    aligned(workspace, 16),
+                "shared_attention: misaligned pointer");
+    const attn::SharedSpace space(batch, heads, kv_heads, dim, groups);
+    CKH_REQUIRE(space.slots <= (1 << 24), "shared_attention: too many heads and sequences");
+    CKH_REQUIRE(workspace_bytes >= space.bytes, "shared_attention: a workspace of %lld bytes, needs %lld",
+                static_cast<long long>(workspace_bytes), static_cast<long long>(space.bytes));
+    attn::SharedArgs a{};
+    a.q = static_cast<const uint8_t*>(q);
+    a.k = static_cast<const uint8_t*>(k_cache), a.v = static_cast<const uint8_t*>(v_cache);
+    a.table = static_cast<const int*>(page_table), a.lengths = static_cast<const int*>(lengths);
+    a.starts = static_cast<const int*>(group_starts), a.shared = static_cast<const int*>(shared);
+    a.k_scale = static_cast<const float*>(k_scale), a.v_scale = static_cast<const float*>(v_scale);
+    a.out = static_cast<uint8_t*>(out);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    a.spans = reinterpret_cast<attn::Span*>(ws);
+    a.pieces = reinterpret_cast<attn::Piece*>(ws + space.pieces);
+    a.part = reinterpret_cast<float*>(ws + space.part);
+    a.stat = reinterpret_cast<float*>(ws + space.stat);
+    a.q_b = strides[0] * 2, a.q_h = strides[1] * 2;
+    a.k_page = strides[2] * es, a.k_tok = strides[3] * es, a.k_head = strides[4] * es;
+    a.v_page = strides[5] * es, a.v_tok = strides[6] * es, a.v_head = strides[7] * es;
+    a.table_stride = table_stride;
+    a.batch = static_cast<int>(batch), a.heads = static_cast<int>(heads), a.kv_heads = static_cast<int>(kv_heads);
+    a.group = static_cast<int>(heads / kv_heads), a.groups = static_cast<int>(groups);
+    a.pages = static_cast<int>(pages), a.page_size = static_cast<int>(page_size);
+    a.capacity = static_cast<int>(max_pages * page_size);
+    a.slots = static_cast<int>(space.slots), a.target = static_cast<int>(space.target);
+    a.scale = scale;
+    a.by_page = fast_div(static_cast<uint32_t>(page_size)), a.by_group = fast_div(static_cast<uint32_t>(a.group));
+    const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    if (q_code == CKH_BF16) attn::launch_shared<CKH_BF16>(static_cast<int>(dim), a, es == 1, st);
+    else attn::launch_shared<CKH_F16>(static_cast<int>(dim), a, es == 1, st);
+    return check_launch("shared_attention");
+}

@@ -377,6 +377,72 @@ int ckh_window_attention(const void* q, const void* k, const void* v, const void
                          const int64_t* strides, int64_t window, int64_t sinks, float scale, int code,
                          void* workspace, int64_t workspace_bytes, uintptr_t stream);
 
+/*
+ * Root-mean-square norm with the residual's addition.  With T the rounding to x's type:
+ *   h = T(x + residual) (x without one),  y = T(h rsqrt(mean(h^2) + eps) weight)
+ * for x [rows, cols] of x_code (f32/f16/bf16), x_stride elements between rows; residual the same with
+ * residual_stride, or NULL; weight [cols] of weight_code (f32/f16/bf16) or NULL (ones); h contiguous, written
+ * where there is a residual.  cols up to 65536; squares are summed in fp32.
+ * The result: y itself (out_code == x_code), contiguous; or the codes that ckh_quantize_fp8 gives for y and
+ * *scale (out_code e4m3 / e5m2); or with mx != 0 the codes [out_rows, out_cols] and swizzled scales that
+ * ckh_quantize_mxfp8 gives for y (out_code e4m3; out_cols % 32 == 0, out_rows at most rows rounded up to 128;
+ * padding is zeros).  out_rows and out_cols are rows and cols where mx is 0.
+ */
+int ckh_rms_norm(const void* x, const void* residual, const void* weight, const void* scale, void* y, void* scales,
+                 void* h, int64_t rows, int64_t cols, int64_t out_rows, int64_t out_cols, int64_t x_stride,
+                 int64_t residual_stride, float eps, int x_code, int weight_code, int out_code, int mx,
+                 uintptr_t stream);
+
+/*
+ * ckh_paged_write of keys that are turned to their positions first, and queries with them.  Pair i of the
+ * first `rotary` elements of a head turns by position * rates[i] (rates: f32 [rotary / 2]; the product in 64
+ * bits), (x, y) -> magnitude (x cos - y sin, x sin + y cos): neighbours (2i, 2i + 1) where interleaved != 0,
+ * else (i, i + rotary / 2).  q [tokens, heads, dim] -> q_out, key -> its slots, rounded once, and key_out
+ * (NULL: not kept), value -> its slots; q_out and key_out contiguous, of x_code.  positions [tokens]: int32, or
+ * int64 where wide_positions != 0.  The rest as for ckh_paged_write; rotary is even, 0 .. dim.
+ * strides: q token, head; key token, head; value token, head; k page, token, head; v page, token, head.
+ */
+int ckh_paged_write_rope(const void* q, const void* key, const void* value, const void* positions, const void* rates,
+                         void* q_out, void* key_out, void* k_cache, void* v_cache, const void* slots,
+                         const void* k_scale, const void* v_scale, int64_t tokens, int64_t heads, int64_t kv_heads,
+                         int64_t dim, int64_t rotary, int64_t pages, int64_t page_size, const int64_t* strides,
+                         int interleaved, float magnitude, int x_code, int cache_code, int wide_positions,
+                         int wide_slots, uintptr_t stream);
+
+/*
+ * The next token of each row of logits [rows, vocab] (code f32/f16/bf16, row_stride elements between rows),
+ * drawn with u [rows] (f32, 0 <= u < 1).  Tokens stand in the order of their logits, the largest first, equal
+ * ones by number; w = exp((logit - max) / temperature).  Kept are the first tokens of that order that are among
+ * the first top_k (0: all), and needed to reach top_p of the weight of those (1 and over: all), and have
+ * w >= min_p; the first always is.  out [rows] (int64) is the first token whose running weight exceeds u times
+ * the weight of all kept.  Temperature 0: the first of the largest logits.  -inf and NaN are never drawn, nor
+ * what lies over 32 temperatures under the largest; a row of nothing else gives -1.
+ * temperature, top_p, min_p (f32) and top_k (int32): device arrays of one a row, or NULL, then the *_all
+ * values hold.  In an array, a temperature that is not over 0 counts as 0, a top_k under 1 as all, a min_p over
+ * 1 as 1.  vocab up to 2^24.  The workspace is needed.
+ */
+int64_t ckh_sample_workspace_bytes(int64_t rows, int64_t vocab);
+int ckh_sample(const void* logits, const void* u, const void* temperature, const void* top_k, const void* top_p,
+               const void* min_p, double temperature_all, int64_t top_k_all, double top_p_all, double min_p_all,
+               void* out, int64_t rows, int64_t vocab, int64_t row_stride, int code, void* workspace,
+               int64_t workspace_bytes, uintptr_t stream);
+
+/*
+ * ckh_paged_attention (without a window) for sequences that begin with the same tokens, which are read once.
+ * Sequences group_starts[g] .. group_starts[g + 1] - 1 form group g (int32 [groups + 1], ascending; a sequence
+ * outside all groups shares nothing), and the first shared[g] of their tokens (int32 [groups]; at most the shortest's length
+ * counts) have the same rows, found by the table of the group's first sequence: what is read for each of
+ * the others are its tokens behind them.  Everything else as for ckh_paged_attention.  The workspace is needed.
+ */
+int64_t ckh_shared_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t groups,
+                                             int64_t page_size, int64_t max_pages);
+int ckh_shared_attention(const void* q, const void* k_cache, const void* v_cache, const void* page_table,
+                         const void* lengths, const void* group_starts, const void* shared, const void* k_scale,
+                         const void* v_scale, void* out, int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim,
+                         int64_t groups, int64_t pages, int64_t page_size, int64_t max_pages, int64_t table_stride,
+                         const int64_t* strides, float scale, int q_code, int cache_code, void* workspace,
+                         int64_t workspace_bytes, uintptr_t stream);
+
 #ifdef __cplusplus
 }
 #endif
