@@ -13,9 +13,11 @@
 //     weights of its logits by bin, from its own largest logit down;
 //   - a second (a workgroup a row) adds these up, which gives the bins that the borders of top_k, top_p,
 //     min_p and the drawn token lie in; reads the row again for the few logits of those bins; and finds
-//     the places in them by counting over ever narrower ranges of (logit, number).
-// Both read the row once (the second mostly from a cache), whatever is asked of them; a bin that does not fit
-// LDS is narrowed over the row in memory.
+//     the places in them: one wave where there are at most 64, else by counting over ever narrower ranges of
+//     (logit, number).  Bins that do not fit LDS are narrowed over the row in memory.
+// What bounds them: the first, instructions and LDS atomics, 18 of 64 bits for a logit (256 rows of 128000 in f32, 131 MB:
+// 29 us); the second, one CU's loads and instructions for a row, and some 8 us of steps that wait for each other (41 us of
+// that case; 64 rows of 150001 in bf16: 12 + 27; one row of 32000: 4.4 + 12.8).
 //
 // A weight is a 32-bit fixed-point number relative to its bin's upper end, taken from the logit in 64 bits;
 // sums of them are whole numbers, so they do not depend on the order in which atomics add them.  The
@@ -30,9 +32,11 @@ constexpr int kBins = 512;
 constexpr double kPer = 16.0;     // bins of a temperature
 constexpr int kChunk = 8192;      // logits of a workgroup of the first launch
 constexpr int kFirst = 512;       // its threads
-constexpr int kThreads = 1024;    // of the second launch's workgroup
+constexpr int kThreads = 512;     // of the second launch's workgroup
 constexpr int kList = 4096;       // logits that it holds
-constexpr int kSub = kThreads;    // ranges that it counts by
+constexpr int kQueue = 3072;      // 16-byte pieces of the row that it looks at twice
+constexpr int kSubBits = 9, kSub = 1 << kSubBits;  // ranges that it counts by
+static_assert(kSub == kThreads && kBins <= kThreads, "a range and a bin a thread");
 constexpr int kMaxChunks = 2048;
 constexpr double kSlack = 0x1p-36;
 
@@ -57,33 +61,35 @@ struct __attribute__((packed, aligned(2))) Piece16 {
     uint32_t w[4];
 };
 
-// The 8 logits from i on (i a multiple of 8) of a row; NaN, and what lies past the row's end, as -inf.
+// 8 logits of a row from the place `begin` on.
 template <int C>
-__device__ __forceinline__ void load_logits(const uint8_t* row, int i, int vocab, float (&v)[8]) {
-    const float none = -__builtin_inff();
-    if (i + 8 <= vocab) {
-        if constexpr (C == CKH_F32) {
-            struct __attribute__((packed, aligned(4))) Piece32 {
-                float f[8];
-            };
-            const Piece32 p = *reinterpret_cast<const Piece32*>(row + static_cast<int64_t>(i) * 4);
+__device__ __forceinline__ void load_logits(const uint8_t* row, int begin, float (&v)[8]) {
+    if constexpr (C == CKH_F32) {
+        struct __attribute__((packed, aligned(4))) Piece32 {
+            float f[8];
+        };
+        const Piece32 p = *reinterpret_cast<const Piece32*>(row + static_cast<int64_t>(begin) * 4);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = p.f[e];
-        } else {
-            const Piece16 p = *reinterpret_cast<const Piece16*>(row + static_cast<int64_t>(i) * 2);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t h = (p.w[e >> 1] >> (16 * (e & 1))) & 0xffffu;
-                v[e] = C == CKH_BF16 ? bf16_to_f(h) : f16_to_f(h);
-            }
-        }
+        for (int e = 0; e < 8; ++e) v[e] = p.f[e];
     } else {
+        const Piece16 p = *reinterpret_cast<const Piece16*>(row + static_cast<int64_t>(begin) * 2);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = i + e < vocab ? load1<C>(row, i + e) : none;
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t h = (p.w[e >> 1] >> (16 * (e & 1))) & 0xffffu;
+            v[e] = C == CKH_BF16 ? bf16_to_f(h) : f16_to_f(h);
+        }
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = v[e] == v[e] ? v[e] : none;
 }
+
+// A row of 8 logits or more in pieces of 8: the one from i on begins at begin(i), and what it holds before i is another's.
+// (Where the row ends inside a piece, the piece lies at the row's end, so that all loads are whole ones.)
+template <int C>
+struct Pieces {
+    const uint8_t* row;
+    int vocab;
+    __device__ __forceinline__ int begin(int i) const { return min(i, vocab - 8); }
+    __device__ __forceinline__ void load(int i, float (&v)[8]) const { load_logits<C>(row, begin(i), v); }
+};
 
 // Bins under a largest logit `top`.
 struct Scale {
@@ -94,29 +100,36 @@ struct Scale {
         top_at = t == __builtin_inff() ? 0.0 : static_cast<double>(t) * per;
         top_bin = floor(top_at);
     }
-    // A logit's bin, counted down from the top's, or kBins; x: how far under its bin's upper end, in bins.
-    __device__ __forceinline__ int bin(float l, double& x) const {
+    // A finite logit's bin, counted down from the top's (or kBins and more); y: its place in the bin, 0 .. 1.
+    __device__ __forceinline__ uint32_t finite_bin(float l, double& y) const {
         const double at = static_cast<double>(l) * per, b = floor(at);
-        x = b + 1.0 - at;
+        y = at - b;
+        return static_cast<uint32_t>(fmin(top_bin - b, static_cast<double>(kBins)));
+    }
+    __device__ __forceinline__ int bin(float l, double& y) const {
         if (top == __builtin_inff()) {  // infinities alone count, all alike
-            x = 1.0;
+            y = 0.0;
             return l == top ? 0 : kBins;
         }
-        const double rel = top_bin - b;
-        return rel < kBins ? static_cast<int>(rel) : kBins;
+        return static_cast<int>(finite_bin(l, y));
     }
 };
 
-// 2^32 exp(-x / 16), 0 <= x <= 1, as a whole number: the terms up to the sixth power, 10^-12 off.
-__device__ __forceinline__ uint64_t weight(double x) {
-    const double y = x * (-1.0 / kPer);
-    double e = __fma_rn(y, 1.0 / 720.0, 1.0 / 120.0);
-    e = __fma_rn(y, e, 1.0 / 24.0);
-    e = __fma_rn(y, e, 1.0 / 6.0);
-    e = __fma_rn(y, e, 0.5);
-    e = __fma_rn(y, e, 1.0);
-    e = __fma_rn(y, e, 1.0);
-    return static_cast<uint64_t>(e * 0x1p32 + 0.5);
+// a b + c with c in scalar registers (left to itself the compiler copies every constant to vector ones first).
+__device__ __forceinline__ double fma_const(double a, double b, double c) {
+    double r;
+    __asm__("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+    return r;
+}
+
+// 2^32 exp((y - 1) / 16), 0 <= y <= 1, as a whole number: a polynomial through five Chebyshev points, 2^-35 off.
+__device__ __forceinline__ uint64_t weight(double y) {
+    double e = __fma_rn(y, 6.162469714203124e-07, 3.820811450174273e-05);
+    e = fma_const(y, e, 0.0018347971173092148);
+    e = fma_const(y, e, 0.05871331567765126);
+    e = fma_const(y, e, 0.9394130628284427);
+    // 2^20 has steps of 2^-32: the sum's low bits are the rounded number
+    return static_cast<uint64_t>(__double_as_longlong(e + 0x1p20)) & 0x1ffffffffull;
 }
 
 // ---------------------------------------------------------------- first launch
@@ -125,167 +138,359 @@ __global__ __launch_bounds__(kFirst) void bins_kernel(Args a) {
     constexpr int N = kChunk / (kFirst * 8);
     __shared__ uint64_t bins[kBins];
     __shared__ float top_of[kFirst / 64];
-    __shared__ int at_of[kFirst / 64];
+    __shared__ int first;
     const int chunk = blockIdx.x, row = blockIdx.y;
-    const uint8_t* logits = a.logits + row * a.row_bytes;
+    const Pieces<C> pieces{a.logits + row * a.row_bytes, a.vocab};
     float v[N][8];
     float top = -__builtin_inff();
-    int at = INT32_MAX;
+    const auto place = [&](int n) { return chunk * kChunk + (n * kFirst + static_cast<int>(threadIdx.x)) * 8; };
+    const bool whole = a.vocab >= 8;
+    if (whole) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) load_logits<C>(logits, chunk * kChunk + (n * kFirst + threadIdx.x) * 8, a.vocab, v[n]);
+        for (int n = 0; n < N; ++n) pieces.load(place(n), v[n]);
+    } else {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[n][e] = place(n) + e < a.vocab ? load1<C>(pieces.row, place(n) + e) : -__builtin_inff();
+    }
     for (int i = threadIdx.x; i < kBins; i += kFirst) bins[i] = 0;
+    if (whole && (chunk + 1) * kChunk > a.vocab) {  // the row's end: what a piece there holds of another's does not count
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < place(n) - pieces.begin(place(n))) v[n][e] = -__builtin_inff();
+    }
 #pragma unroll
     for (int n = 0; n < N; ++n)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (v[n][e] > top) {
-                top = v[n][e];
-                at = chunk * kChunk + (n * kFirst + threadIdx.x) * 8 + e;
-            }
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, v[n][e]);  // a NaN is not taken
 #pragma unroll
-    for (int s = 32; s >= 1; s >>= 1) {
-        const float t = __shfl_xor(top, s, 64);
-        const int i = __shfl_xor(at, s, 64);
-        if (t > top || (t == top && i < at)) top = t, at = i;
-    }
-    if ((threadIdx.x & 63) == 0) {
-        top_of[threadIdx.x >> 6] = top;
-        at_of[threadIdx.x >> 6] = at;
-    }
+    for (int s = 32; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
+    if ((threadIdx.x & 63) == 0) top_of[threadIdx.x >> 6] = top;
+    if (threadIdx.x == 0) first = INT32_MAX;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kFirst / 64; ++w)
-        if (top_of[w] > top || (top_of[w] == top && at_of[w] < at)) top = top_of[w], at = at_of[w];
-    const int64_t place = static_cast<int64_t>(row) * a.chunks + chunk;
-    if (threadIdx.x == 0) a.top[place] = make_int2(static_cast<int>(as_u(top)), at);
-    if (a.greedy(row) || top == -__builtin_inff()) return;
+    for (int w = 0; w < kFirst / 64; ++w) top = fmaxf(top, top_of[w]);
+    bool here = false;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) here |= v[n][e] == top;
+    if (here && top > -__builtin_inff()) {
+        int at = INT32_MAX;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (v[n][e] == top) at = min(at, (whole ? pieces.begin(place(n)) : place(n)) + e);
+        atomicMin(&first, at);
+    }
+    const int64_t slot = static_cast<int64_t>(row) * a.chunks + chunk;
+    if (a.greedy(row) || top == -__builtin_inff()) {
+        __syncthreads();
+        if (threadIdx.x == 0) a.top[slot] = make_int2(static_cast<int>(as_u(top)), first);
+        return;
+    }
+    const float largest = top;
+    if (top == __builtin_inff()) {  // infinities alone count, all alike
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[n][e] = v[n][e] == top ? 0.0f : -__builtin_inff();
+        top = 0.0f;
+    }
     const Scale scale(top, a.temperature_of(row));
 #pragma unroll
     for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            if (v[n][e] == -__builtin_inff()) continue;
-            double x;
-            const int b = scale.bin(v[n][e], x);
-            if (b < kBins) atomicAdd(reinterpret_cast<unsigned long long*>(&bins[b]), (1ull << 48) | weight(x));
+            double y;
+            const uint32_t b = scale.finite_bin(v[n][e], y);  // -inf: kBins
+            const uint64_t one = (1ull << 48) | weight(y);
+            if (b < kBins) atomicAdd(reinterpret_cast<unsigned long long*>(&bins[b]), static_cast<unsigned long long>(one));
         }
     __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += kFirst) a.bins[place * kBins + i] = bins[i];
+    if (threadIdx.x == 0) a.top[slot] = make_int2(static_cast<int>(as_u(largest)), first);
+    for (int i = threadIdx.x; i < kBins; i += kFirst) a.bins[slot * kBins + i] = bins[i];
 }
 
 // --------------------------------------------------------------- second launch
-// Orders tokens: the larger logit first, then the smaller number.
-__device__ __forceinline__ uint64_t order_of(float l, int i) {
-    const uint32_t u = as_u(l + 0.0f);  // one zero
-    const uint32_t up = u & 0x80000000u ? u : ~u & 0x7fffffffu;
-    return static_cast<uint64_t>(up) << 32 | static_cast<uint32_t>(i);
-}
-__device__ __forceinline__ float logit_of(uint64_t order) {
-    const uint32_t up = static_cast<uint32_t>(order >> 32);
-    return as_f(up & 0x80000000u ? up : ~up & 0x7fffffffu);
-}
-
-struct Shared {
-    double below[kBins];     // weight of the bins up to and with this one
-    uint32_t count[kBins], sum_count[kBins];
-    uint64_t list[kList];
-    uint64_t sub_weight[kSub];
-    uint32_t sub_count[kSub];
-    uint8_t wanted[kBins];
-    uint16_t under[kMaxChunks];  // by how many bins a chunk's largest logit is under the row's
-    double wave_weight[kThreads / 64];
-    uint64_t wave_sum[kThreads / 64];
-    uint32_t wave_count[kThreads / 64];
-    unsigned long long lo, hi, above_weight;
-    uint32_t above_count, listed;
-    int found, first;
+// A token's place in the order as one number: its logit's bits, turned so that the larger logit is the
+// smaller number (16-bit types have no more bits than that), then the token's own number.
+template <int C>
+struct Order {
+    static constexpr int kDrop = C == CKH_F32 ? 0 : C == CKH_F16 ? 13 : 16;  // zeros in a widened logit
+    int bits;  // of a token's number
+    __device__ __forceinline__ uint64_t key(float l) const {
+        const uint32_t u = as_u(l + 0.0f);  // one zero
+        return (u & 0x80000000u ? u : ~u & 0x7fffffffu) >> kDrop;
+    }
+    __device__ __forceinline__ uint64_t of(float l, int token) const { return key(l) << bits | static_cast<uint32_t>(token); }
+    __device__ __forceinline__ float logit(uint64_t order) const {
+        const uint32_t up = static_cast<uint32_t>(order >> bits) << kDrop;
+        return as_f(up & 0x80000000u ? up : ~up & 0x7fffffffu & ~((1u << kDrop) - 1u));
+    }
+    __device__ __forceinline__ int64_t token(uint64_t order) const { return static_cast<int64_t>(order & ((1ull << bits) - 1)); }
 };
 
 enum Ask { kRank, kReach, kPass };  // the r-th token; the first whose running weight reaches, or passes, a target
 
-// All threads of the workgroup call its members together.
+// What the bins' sums tell of the borders.
+struct Found {
+    double low_k, high_k, low, high;  // the weight that top_k leaves, that is kept: at least and at most
+    int bin_k, bin_m;                 // the bins of top_k's and min_p's borders
+    bool by_k, by_p, by_min;          // which borders have to be looked for
+};
+
+struct Shared {
+    double below[kBins];          // weight of the bins up to and with this one
+    uint32_t counts[kBins];       // their tokens
+    uint16_t under[kMaxChunks];   // by how many bins a chunk's largest logit is under the row's
+    int queue[kQueue];            // pieces of the row that hold some of them
+    uint64_t list[kList];         // places of the tokens of the bins that are looked into
+    uint64_t sub_weight[kSub], few[64];
+    uint32_t sub_count[kSub];
+    float low[3], high[3];        // logits of these bins: of top_k's border, of the tighter of top_p's and min_p's, of the draw
+    uint32_t listed, queued, fews;
+    int bin, sub;
+    Found found;
+    unsigned long long above_weight, sum;
+    uint32_t above_count, sub_n;
+    double running;
+    uint64_t place;
+};
+
 template <int C>
 struct Row {
     const Args& a;
     Shared& s;
-    const uint8_t* logits;
+    Pieces<C> pieces;
     Scale scale;
-    bool whole;  // the list does not hold the bins that are asked for: the row itself is read
+    Order<C> order;
+    int lane;
+    bool whole;  // the list does not hold the bins that are looked into: the row itself is read
 
-    __device__ __forceinline__ double unit(int bin) const {  // weight of a bin's upper end / 2^32, relative to the largest logit's
+    __device__ __forceinline__ double unit(int bin) const {  // a weight's 2^-32 in this bin, relative to the largest logit's weight
         return exp((scale.top_bin - scale.top_at + 1.0 - bin) * (1.0 / kPer)) * 0x1p-32;
     }
     __device__ __forceinline__ bool is(Ask ask, double running, double target) const {
         return ask == kPass ? running > target * (1.0 + kSlack) : running >= target * (1.0 - kSlack);
     }
-    // f(order, fixed-point weight) for the tokens of a bin
+    __device__ __forceinline__ double base(int bin) const { return bin ? s.below[bin - 1] : 0.0; }
+
+    // Logits that a bin's lie between (a little more than the bin).
+    __device__ __forceinline__ float lower(int bin) const {
+        if (scale.top == __builtin_inff()) return scale.top;
+        const float f = static_cast<float>((scale.top_bin - bin) / scale.per);
+        return fmaxf(f - fabsf(f) * 0x1p-22f - 1e-37f, -3.402823466e38f);
+    }
+    __device__ __forceinline__ float upper(int bin) const {
+        if (scale.top == __builtin_inff()) return scale.top;
+        const float f = static_cast<float>((scale.top_bin - bin + 1.0) / scale.per);
+        return fminf(f + fabsf(f) * 0x1p-22f + 1e-37f, scale.top);
+    }
+
+    // The workgroup: lists the tokens whose logits lie in one of the ranges low .. high.  What bounds it is instructions, so
+    // 16-byte pieces are looked at as they lie in memory: a range of logits of one sign is a range of their bits, and x is
+    // in it where x - first, as an unsigned number, is at most its width; the least of these over a piece tells of the piece,
+    // and the few pieces that hold something are looked at again logit by logit.  (Widened and compared as floats the row
+    // took three times as long: 64 rows of 150001 in bf16 24 us of the launch.)
+    static constexpr int kPiece = C == CKH_F32 ? 4 : 8;  // logits of a piece
+    static __device__ __forceinline__ uint32_t code(float l) {  // a logit's bits in its own type, rounded towards zero
+        if constexpr (C == CKH_F32) return as_u(l);
+        else if constexpr (C == CKH_BF16) return as_u(l) >> 16;
+        else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(l, 0.0f)) & 0xffffu;
+    }
+    // Q ranges of bits at most.
+    template <int Q>
+    __device__ __forceinline__ void scan(const uint32_t (&first)[6], const uint32_t (&width)[6]) const {
+        constexpr int U = 8;  // pieces of a thread in flight
+        typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+        struct __attribute__((packed, aligned(C == CKH_F32 ? 4 : 2))) Words {
+            uint32_t w[4];
+        };
+        const auto load = [&](Words (&x)[U], int i0) {
+#pragma unroll
+            for (int n = 0; n < U; ++n) {
+                const int i = min(i0 + (n * kThreads + static_cast<int>(threadIdx.x)) * kPiece, a.vocab - kPiece);
+                x[n] = *reinterpret_cast<const Words*>(pieces.row + static_cast<int64_t>(i) * (16 / kPiece));
+            }
+        };
+        Words x[U], next[U];
+        load(x, 0);
+        constexpr int kStep = kThreads * kPiece * U;
+        for (int i0 = 0; i0 < a.vocab; i0 += kStep) {
+            if (i0 + kStep < a.vocab) load(next, i0 + kStep);
+#pragma unroll
+            for (int n = 0; n < U; ++n) {
+                bool hit = false;
+#pragma unroll
+                for (int q = 0; q < Q; ++q) {
+                    if constexpr (C == CKH_F32) {
+                        uint32_t least = x[n].w[0] - first[q];
+#pragma unroll
+                        for (int e = 1; e < 4; ++e) {
+                            const uint32_t d = x[n].w[e] - first[q];
+                            least = d < least ? d : least;
+                        }
+                        hit |= least <= width[q];
+                    } else {
+                        const u16x2 from = __builtin_bit_cast(u16x2, first[q] * 0x10001u);
+                        u16x2 least = __builtin_bit_cast(u16x2, x[n].w[0]) - from;
+#pragma unroll
+                        for (int e = 1; e < 4; ++e) least = __builtin_elementwise_min(least, static_cast<u16x2>(__builtin_bit_cast(u16x2, x[n].w[e]) - from));
+                        hit |= (least.x < least.y ? least.x : least.y) <= width[q];
+                    }
+                }
+                const int i = i0 + (n * kThreads + static_cast<int>(threadIdx.x)) * kPiece;
+                if (hit && i < a.vocab) {
+                    const uint32_t place = atomicAdd(&s.queued, 1u);
+                    if (place < kQueue) s.queue[place] = i;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < U; ++n) x[n] = next[n];
+        }
+    }
+    __device__ __forceinline__ void gather() const {
+        const float low0 = s.low[0], high0 = s.high[0], low1 = s.low[1], high1 = s.high[1], low2 = s.low[2], high2 = s.high[2];
+        const auto wanted = [&](float l) { return (l >= low0 && l <= high0) || (l >= low1 && l <= high1) || (l >= low2 && l <= high2); };
+        const auto list = [&](float l, int token) {
+            if (!wanted(l)) return;
+            const uint32_t place = atomicAdd(&s.listed, 1u);
+            if (place < kList) s.list[place] = order.of(l, token);
+        };
+        if (a.vocab < 8) {
+            if (static_cast<int>(threadIdx.x) < a.vocab) list(load1<C>(pieces.row, threadIdx.x), threadIdx.x);
+            return;
+        }
+        uint32_t first[6], width[6];
+        int ranges = 0;
+#pragma unroll
+        for (int n = 0; n < 6; ++n) first[n] = code(-__builtin_nanf("")) | (C == CKH_F32 ? 0x7fffffu : 0x7fu), width[n] = 0;  // NaN
+        const auto add = [&](uint32_t from, uint32_t to) {
+#pragma unroll
+            for (int n = 0; n < 6; ++n)
+                if (n == ranges) first[n] = from, width[n] = to - from;
+            ++ranges;
+        };
+#pragma unroll
+        for (int n = 0; n < 3; ++n) {
+            const float lo = s.low[n], hi = s.high[n];
+            if (lo > hi) continue;
+            if (lo <= 0.0f) add(code(hi < 0.0f ? hi : -0.0f), code(lo < 0.0f ? lo : -0.0f));
+            if (hi >= 0.0f) add(code(lo > 0.0f ? lo : 0.0f), code(hi > 0.0f ? hi : 0.0f));
+        }
+        if (ranges == 1) scan<1>(first, width);
+        else if (ranges == 2) scan<2>(first, width);
+        else if (ranges == 3) scan<3>(first, width);
+        else scan<6>(first, width);
+        __syncthreads();
+        const int n = min(s.queued, static_cast<uint32_t>(kQueue));
+        for (int j = threadIdx.x; j < n; j += kThreads) {
+            const int i = s.queue[j], begin = min(i, a.vocab - kPiece);
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e)
+                if (begin + e >= i) list(load1<C>(pieces.row, begin + e), begin + e);
+        }
+    }
+
+    // f(place in the order, fixed-point weight) for the tokens of a bin
     template <typename F>
     __device__ __forceinline__ void each(int bin, F f) const {
         if (!whole) {
-            for (uint32_t i = threadIdx.x; i < min(s.listed, static_cast<uint32_t>(kList)); i += kThreads) {
+            const uint32_t n = min(s.listed, static_cast<uint32_t>(kList));
+            for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
                 const uint64_t o = s.list[i];
-                double x;
-                if (scale.bin(logit_of(o), x) == bin) f(o, weight(x));
+                double y;
+                if (scale.bin(order.logit(o), y) == bin) f(o, weight(y));
             }
         } else {
             for (int i = threadIdx.x * 8; i < a.vocab; i += kThreads * 8) {
                 float v[8];
-                load_logits<C>(logits, i, a.vocab, v);
+                pieces.load(i, v);
+                const int begin = pieces.begin(i);
                 for (int e = 0; e < 8; ++e) {
-                    double x;
-                    if (v[e] != -__builtin_inff() && scale.bin(v[e], x) == bin) f(order_of(v[e], i + e), weight(x));
+                    double y;
+                    if (v[e] > -__builtin_inff() && begin + e >= i && scale.bin(v[e], y) == bin) f(order.of(v[e], begin + e), weight(y));
                 }
             }
         }
     }
 
-    // The first bin whose running weight is (or count reaches) what is asked, or the last that is not empty.
-    __device__ int find(Ask ask, double target, uint32_t rank) {
-        __syncthreads();
-        if (threadIdx.x == 0) s.first = 0;
-        __syncthreads();
-        const int i = threadIdx.x;
-        if (i < kBins && s.count[i]) {
-            const bool here = ask == kRank ? s.sum_count[i] >= rank : is(ask, s.below[i], target);
-            const bool before = i > 0 && (ask == kRank ? s.sum_count[i - 1] >= rank : s.sum_count[i - 1] > 0 && is(ask, s.below[i - 1], target));
-            // an order of its own for the last one: it stands where nothing is found
-            if (!before && (here || s.sum_count[i] == s.sum_count[kBins - 1])) s.first = i;
+    // One wave: the first bin that is not empty and whose running weight is (or count reaches) what is asked, or the
+    // last that is not empty.
+    __device__ __forceinline__ int find(Ask ask, double target, uint32_t rank) const {
+        // the first of 64 runs of bins that ends there, then the bin in it
+        constexpr int N = kBins / 64;
+        const uint32_t all = s.counts[kBins - 1];
+        uint64_t hit = 0;
+        int i = lane * N + N - 1;
+#pragma unroll
+        for (int step = 0; step < 2; ++step) {
+            const uint32_t n = s.counts[i];
+            const double w = s.below[i];
+            hit = __ballot(ask == kRank ? n >= rank : is(ask, w, target));
+            if (!hit) hit = __ballot(n >= all);
+            if (step == 0) i = __builtin_ctzll(hit) * N + min(lane, N - 1);
         }
-        __syncthreads();
-        return s.first;
+        return (i - min(lane, N - 1)) + min(static_cast<int>(__builtin_ctzll(hit)), N - 1);
     }
 
-    // The token that is asked for within a bin that holds it: its order, and the weight of the tokens up to and with it.
-    __device__ uint64_t within(int bin, Ask ask, double target, uint32_t rank, double& running) {
-        const double base = bin ? s.below[bin - 1] : 0.0, one = unit(bin);
-        const uint32_t rank_base = bin ? s.sum_count[bin - 1] : 0;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            s.lo = 0, s.hi = ~0ull;
-            s.above_weight = 0, s.above_count = 0;
+    // One wave, a token a lane (n of them): the one that is asked for, with `above` weight and tokens of its bin before these.
+    __device__ __forceinline__ uint64_t pick(uint64_t o, uint64_t w, bool live, int bin, Ask ask, double target, uint32_t rank,
+                                             uint64_t above_weight, uint32_t above_count, double& running) const {
+        uint64_t sum = 0;
+        uint32_t n = 0;
+        for (uint64_t left = __ballot(live); left; left &= left - 1) {
+            const int j = __builtin_ctzll(left);
+            const uint64_t oj = lane_of(o, j), wj = lane_of(w, j);
+            if (oj <= o) sum += wj, ++n;
         }
-        __syncthreads();
-        for (;;) {
-            // the range's first and last token
-            const uint64_t lo = s.lo, hi = s.hi;
-            uint64_t least = ~0ull, most = 0;
-            __syncthreads();
-            if (threadIdx.x == 0) s.lo = ~0ull, s.hi = 0;
+        const double begin = base(bin), one = unit(bin);
+        const uint32_t count = (bin ? s.counts[bin - 1] : 0) + above_count + n;
+        const double to = begin + static_cast<double>(above_weight + sum) * one;
+        const bool here = live && (ask == kRank ? count >= rank : is(ask, to, target));
+        // the first of these in the order, or the last of all
+        const uint64_t all = __ballot(live), those = __ballot(here);
+        uint64_t best = 0;
+        int lane_at = -1;
+        for (uint64_t left = those ? those : all; left; left &= left - 1) {
+            const int j = __builtin_ctzll(left);
+            const uint64_t oj = lane_of(o, j);
+            if (lane_at < 0 || (those ? oj < best : oj > best)) best = oj, lane_at = j;
+        }
+        running = __shfl(to, lane_at < 0 ? 0 : lane_at, 64);
+        return best;
+    }
+    static __device__ __forceinline__ uint64_t lane_of(uint64_t v, int j) {
+        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), j);
+        const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), j);
+        return static_cast<uint64_t>(hi) << 32 | lo;
+    }
+
+    // One wave, where the list has at most 64 tokens: the one that is asked for in a bin.
+    __device__ __forceinline__ uint64_t in_wave(int bin, Ask ask, double target, uint32_t rank, double& running) const {
+        const uint64_t o = lane < static_cast<int>(s.listed) ? s.list[lane] : 0;
+        double y = 0.0;
+        const bool live = lane < static_cast<int>(s.listed) && scale.bin(order.logit(o), y) == bin;
+        return pick(o, weight(y), live, bin, ask, target, rank, 0, 0, running);
+    }
+
+    // The workgroup: the same in a bin of any size.
+    __device__ uint64_t in_group(int bin, Ask ask, double target, uint32_t rank, double& running) {
+        uint64_t from = order.of(upper(bin), 0), to = order.of(lower(bin), 0) | ((1ull << order.bits) - 1);
+        uint64_t above_weight = 0;
+        uint32_t above_count = 0, n = s.counts[bin] - (bin ? s.counts[bin - 1] : 0);
+        const uint32_t rank_base = bin ? s.counts[bin - 1] : 0;
+        const double begin = base(bin), one = unit(bin);
+        while (n > 64) {
+            const int shift = max(0, 64 - __clzll(static_cast<long long>(to - from)) - kSubBits);
             s.sub_weight[threadIdx.x] = 0;
             s.sub_count[threadIdx.x] = 0;
             __syncthreads();
-            each(bin, [&](uint64_t o, uint64_t) {
-                if (o >= lo && o <= hi) least = o < least ? o : least, most = o > most ? o : most;
-            });
-            if (least <= most) {
-                atomicMin(&s.lo, static_cast<unsigned long long>(least));
-                atomicMax(&s.hi, static_cast<unsigned long long>(most));
-            }
-            __syncthreads();
-            const uint64_t from = s.lo, to = s.hi;
-            if (from >= to) break;
-            const uint64_t span = to - from;
-            const int shift = max(0, 64 - __clzll(static_cast<long long>(span)) - 10);
             each(bin, [&](uint64_t o, uint64_t w) {
                 if (o >= from && o <= to) {
                     const uint32_t i = static_cast<uint32_t>((o - from) >> shift);
@@ -294,55 +499,81 @@ struct Row {
                 }
             });
             __syncthreads();
-            uint64_t w = s.sub_weight[threadIdx.x];
-            uint32_t n = s.sub_count[threadIdx.x];
-            const uint64_t own_w = w;
-            const uint32_t own_n = n;
-            scan(w, n);
-            w += s.above_weight;
-            n += s.above_count;
-            const bool here = ask == kRank ? rank_base + n >= rank : is(ask, base + static_cast<double>(w) * one, target);
-            const bool before = ask == kRank ? rank_base + n - own_n >= rank
-                                             : n - own_n > s.above_count && is(ask, base + static_cast<double>(w - own_w) * one, target);
-            __syncthreads();
-            const int last = static_cast<int>(span >> shift);
-            const bool mine = own_n && !before && (here || static_cast<int>(threadIdx.x) == last);
-            if (mine) {
-                const uint64_t begin = from + (static_cast<uint64_t>(threadIdx.x) << shift);
-                s.lo = begin;
-                s.hi = (to - begin) >> shift ? begin + ((1ull << shift) - 1) : to;
-                s.above_weight = w - own_w;
-                s.above_count = n - own_n;
+            if (threadIdx.x < 64) {  // a lane's ranges one after the other
+                constexpr int N = kSub / 64;
+                uint64_t w = 0;
+                uint32_t c = 0;
+#pragma unroll
+                for (int e = 0; e < N; ++e) w += s.sub_weight[lane * N + e], c += s.sub_count[lane * N + e];
+                uint64_t end_w = w;
+                uint32_t end_c = c;
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) {
+                    const uint64_t u = __shfl_up(static_cast<unsigned long long>(end_w), d, 64);
+                    const uint32_t m = __shfl_up(end_c, d, 64);
+                    if (lane >= d) end_w += u, end_c += m;
+                }
+                w = above_weight + end_w - w;
+                c = above_count + end_c - c;
+                int at = kSub, last = -1;
+                uint64_t at_w = 0, last_w = 0;
+                uint32_t at_c = 0, last_c = 0;
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const int i = lane * N + e;
+                    const uint64_t ow = s.sub_weight[i];
+                    const uint32_t oc = s.sub_count[i];
+                    if (oc) {
+                        last = i, last_w = w, last_c = c;
+                        if (at == kSub && (ask == kRank ? rank_base + c + oc >= rank : is(ask, begin + static_cast<double>(w + ow) * one, target)))
+                            at = i, at_w = w, at_c = c;
+                    }
+                    w += ow, c += oc;
+                }
+                const uint64_t found = __ballot(at < kSub), any = __ballot(last >= 0);
+                const int l = found ? __builtin_ctzll(found) : 63 - __builtin_clzll(any | 1);
+                if (lane == l) {
+                    s.sub = found ? at : last;
+                    s.above_weight = found ? at_w : last_w;
+                    s.above_count = found ? at_c : last_c;
+                    s.sub_n = s.sub < 0 ? 0 : s.sub_count[s.sub];
+                }
             }
             __syncthreads();
+            above_weight = s.above_weight, above_count = s.above_count, n = s.sub_n;
+            from += static_cast<uint64_t>(max(s.sub, 0)) << shift;
+            if ((to - from) >> shift) to = from + ((1ull << shift) - 1);
+            __syncthreads();
         }
-        const uint64_t o = s.lo;
-        double x;
-        scale.bin(logit_of(o), x);
-        running = base + static_cast<double>(s.above_weight + weight(x)) * one;
-        return o;
-    }
-
-    // inclusive sums over the workgroup's threads
-    __device__ __forceinline__ void scan(uint64_t& w, uint32_t& n) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint64_t u = __shfl_up(static_cast<unsigned long long>(w), d, 64);
-            const uint32_t m = __shfl_up(n, d, 64);
-            if (lane >= d) w += u, n += m;
+        if (threadIdx.x == 0) s.fews = 0;
+        __syncthreads();
+        each(bin, [&](uint64_t o, uint64_t) {
+            if (o >= from && o <= to) {
+                const uint32_t i = atomicAdd(&s.fews, 1u);
+                if (i < 64) s.few[i] = o;
+            }
+        });
+        __syncthreads();
+        if (threadIdx.x < 64) {
+            const bool live = lane < static_cast<int>(s.fews);
+            const uint64_t o = live ? s.few[lane] : 0;
+            double y = 0.0, r;
+            if (live) scale.bin(order.logit(o), y);
+            const uint64_t place = pick(o, weight(y), live, bin, ask, target, rank, above_weight, above_count, r);
+            if (lane == 0) s.place = place, s.running = r;
         }
-        if (lane == 63) s.wave_sum[wave] = w, s.wave_count[wave] = n;
         __syncthreads();
-        for (int i = 0; i < wave; ++i) w += s.wave_sum[i], n += s.wave_count[i];
+        running = s.running;
+        const uint64_t place = s.place;
         __syncthreads();
+        return place;
     }
 };
 
 template <int C>
 __global__ __launch_bounds__(kThreads) void pick_kernel(Args a) {
     __shared__ Shared s;
-    const int row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int row = blockIdx.x, lane = threadIdx.x & 63;
     const int2* tops = a.top + static_cast<int64_t>(row) * a.chunks;
 
     // the row's largest logit, the first of equal ones
@@ -364,9 +595,9 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(Args a) {
         return;
     }
     const double temperature = a.temperature_of(row);
-    Row<C> r{a, s, a.logits + row * a.row_bytes, Scale(top, temperature), false};
+    Row<C> r{a, s, {a.logits + row * a.row_bytes, a.vocab}, Scale(top, temperature), Order<C>{32 - __clz(a.vocab - 1 | 1)}, lane, false};
 
-    // counts and weights of the bins, and their running sums
+    // weights and counts of the bins
     for (int c = threadIdx.x; c < a.chunks; c += kThreads) {
         const float t = as_f(tops[c].x);
         double under = kBins;
@@ -374,10 +605,11 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(Args a) {
         else if (t > -__builtin_inff() && top < __builtin_inff()) under = fmin(under, r.scale.top_bin - Scale(t, temperature).top_bin);
         s.under[c] = static_cast<uint16_t>(under);
     }
+    if (threadIdx.x == 0) s.listed = s.queued = 0;
     __syncthreads();
-    uint64_t w = 0;
-    uint32_t n = 0;
     if (threadIdx.x < kBins) {
+        uint64_t w = 0;
+        uint32_t n = 0;
         const uint64_t* bins = a.bins + static_cast<int64_t>(row) * a.chunks * kBins;
 #pragma unroll 8
         for (int c = 0; c < a.chunks; ++c) {
@@ -386,114 +618,137 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(Args a) {
             w += x & 0xffffffffffffull;
             n += static_cast<uint32_t>(x >> 48);
         }
+        s.below[threadIdx.x] = static_cast<double>(w) * r.unit(threadIdx.x);
+        s.counts[threadIdx.x] = n;
     }
-    double f = static_cast<double>(w) * r.unit(threadIdx.x);
-    uint32_t m = n;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const double g = __shfl_up(f, d, 64);
-        const uint32_t k = __shfl_up(m, d, 64);
-        if (lane >= d) f += g, m += k;
-    }
-    if (lane == 63) s.wave_weight[wave] = f, s.wave_count[wave] = m;
-    __syncthreads();
-    for (int i = wave - 1; i >= 0; --i) f += s.wave_weight[i], m += s.wave_count[i];
-    if (threadIdx.x < kBins) {
-        s.count[threadIdx.x] = n;
-        s.sum_count[threadIdx.x] = m;
-        s.below[threadIdx.x] = f;
-        s.wanted[threadIdx.x] = 0;
-    }
-    if (threadIdx.x == 0) s.listed = 0;
     __syncthreads();
 
     const int top_k = a.top_k_of(row);
     const double top_p = a.top_p ? a.top_p[row] : a.top_p_all;
     const double min_p = fmin(a.min_p ? a.min_p[row] : a.min_p_all, 1.0);
     const double u = fmin(fmax(static_cast<double>(a.u[row]), 0.0), 1.0 - 0x1p-25);
-    const uint32_t all = s.sum_count[kBins - 1];
-    const bool by_k = top_k > 0 && static_cast<uint32_t>(top_k) < all, by_p = top_p < 1.0, by_min = min_p > 0.0;
-
-    // the bins in which the borders can lie: each border's range follows from the one before it
-    double low = s.below[kBins - 1], high = low;  // weight that is kept, at least and at most
-    double low_k = low, high_k = high;            // the same of top_k alone
-    int bin_k = -1, bin_m = -1;
-    const auto want = [&](int from, int to) {
-        if (static_cast<int>(threadIdx.x) >= from && static_cast<int>(threadIdx.x) <= to) s.wanted[threadIdx.x] = 1;
-    };
-    if (by_k) {
-        bin_k = r.find(kRank, 0.0, top_k);
-        low = low_k = bin_k ? s.below[bin_k - 1] : 0.0, high = high_k = s.below[bin_k];
-        want(bin_k, bin_k);
-    }
-    if (by_p) {
-        const int from = r.find(kReach, top_p * low, 0), to = r.find(kReach, top_p * high, 0);
-        low = fmin(low, from ? s.below[from - 1] : 0.0), high = fmin(high, s.below[to]);
-        want(from, to);
-    }
-    if (by_min) {
-        // the last bin with a part at min_p or over it (the one behind that, by rounding, does no harm)
-        const double under = ceil(r.scale.top_bin - r.scale.top_at - log(min_p) * kPer);
-        bin_m = static_cast<int>(fmin(fmax(under, 0.0), kBins - 1.0));
-        low = fmin(low, bin_m ? s.below[bin_m - 1] : 0.0), high = fmin(high, s.below[bin_m]);
-        want(bin_m, bin_m);
-    }
-    want(r.find(kPass, u * low, 0), r.find(kPass, u * high, 0));
-    __syncthreads();
-
-    // their tokens
-    uint32_t wanted = threadIdx.x < kBins && s.wanted[threadIdx.x] ? n : 0;
-    uint64_t unused = 0;
-    r.scan(unused, wanted);
-    if (threadIdx.x == kThreads - 1) s.above_count = wanted;
-    __syncthreads();
-    r.whole = s.above_count > kList;
-    if (!r.whole) {
-        for (int i = threadIdx.x * 8; i < a.vocab; i += kThreads * 8) {
-            float v[8];
-            load_logits<C>(r.logits, i, a.vocab, v);
+    const bool by_p = top_p < 1.0, by_min = min_p > 0.0;
+    if (threadIdx.x < 64) {
+        // running sums
+        constexpr int N = kBins / 64;
+        double f[N], sum = 0.0;
+        uint32_t c[N], count = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if (v[e] == -__builtin_inff()) continue;
-                double x;
-                const int b = r.scale.bin(v[e], x);
-                if (b < kBins && s.wanted[b]) {
-                    const uint32_t place = atomicAdd(&s.listed, 1u);
-                    if (place < kList) s.list[place] = order_of(v[e], i + e);
-                }
+        for (int e = 0; e < N; ++e) {
+            f[e] = sum += s.below[lane * N + e];
+            c[e] = count += s.counts[lane * N + e];
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const double g = __shfl_up(sum, d, 64);
+            const uint32_t k = __shfl_up(count, d, 64);
+            if (lane >= d) sum += g, count += k;
+        }
+        const double before = sum - f[N - 1];
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            s.below[lane * N + e] = e + 1 < N ? before + f[e] : sum;
+            s.counts[lane * N + e] = count - c[N - 1] + c[e];
+        }
+        __asm__ volatile("" ::: "memory");  // (one wave: LDS keeps its order)
+        // the bins in which the borders can lie: each border's range follows from the one before it
+        const double all = s.below[kBins - 1];
+        const bool by_k = top_k > 0 && static_cast<uint32_t>(top_k) < s.counts[kBins - 1];
+        Found f0{};
+        f0.low_k = f0.high_k = all;
+        int from[3] = {0, 0, 0}, to[3] = {-1, -1, -1};
+        if (by_k) {
+            f0.bin_k = r.find(kRank, 0.0, top_k);
+            f0.low_k = r.base(f0.bin_k), f0.high_k = s.below[f0.bin_k];
+        }
+        f0.low = f0.low_k, f0.high = f0.high_k;
+        f0.by_k = by_k, f0.by_p = by_p, f0.by_min = by_min;
+        if (by_p) {
+            from[1] = r.find(kReach, top_p * f0.low_k, 0), to[1] = r.find(kReach, top_p * f0.high_k, 0);
+            f0.low = fmin(f0.low, r.base(from[1])), f0.high = fmin(f0.high, s.below[to[1]]);
+        }
+        if (by_min) {
+            // the last bin with a part at min_p or over it (the one behind that, by rounding, does no harm)
+            const double under = ceil(r.scale.top_bin - r.scale.top_at - log(min_p) * kPer);
+            f0.bin_m = static_cast<int>(fmin(fmax(under, 0.0), kBins - 1.0));
+            f0.low = fmin(f0.low, r.base(f0.bin_m)), f0.high = fmin(f0.high, s.below[f0.bin_m]);
+            // a border that lies behind another does not count
+            if (by_p && f0.bin_m < from[1]) f0.by_p = false;
+            if ((by_p && f0.bin_m > to[1]) || (by_k && f0.bin_m > f0.bin_k)) f0.by_min = false;
+            if (f0.by_min && !f0.by_p) from[1] = to[1] = f0.bin_m;
+            if (by_k && f0.by_min && !f0.by_p && f0.bin_m < f0.bin_k) f0.by_k = false;
+        }
+        if (f0.by_k) from[0] = to[0] = f0.bin_k;
+        from[2] = r.find(kPass, u * f0.low, 0), to[2] = r.find(kPass, u * f0.high, 0);
+        if (lane == 0) {
+            s.found = f0;
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                s.low[i] = to[i] < 0 ? __builtin_inff() : r.lower(to[i]);
+                s.high[i] = to[i] < 0 ? -__builtin_inff() : r.upper(from[i]);
             }
         }
     }
     __syncthreads();
 
-    double kept = s.below[kBins - 1];
-    if (by_k) {
-        double running;
-        r.within(bin_k, kRank, 0.0, top_k, running);
-        kept = fmin(fmax(running, low_k), high_k);  // (sums of the same in another order)
+    // their tokens
+    r.gather();
+    __syncthreads();
+
+    // the places of the borders, and the token
+    r.whole = s.listed > kList || s.queued > kQueue;
+    const bool few = !r.whole && s.listed <= 64;
+    if (few && threadIdx.x >= 64) return;
+    const Found f = s.found;
+    const auto find = [&](Ask ask, double target) {
+        if (few) return r.find(ask, target, 0);
+        if (threadIdx.x < 64) {
+            const int bin = r.find(ask, target, 0);
+            if (lane == 0) s.bin = bin;
+        }
+        __syncthreads();
+        return s.bin;  // (in_group has barriers before the next write)
+    };
+    const auto look = [&](int bin, Ask ask, double target, double& running) {
+        return few ? r.in_wave(bin, ask, target, top_k, running) : r.in_group(bin, ask, target, top_k, running);
+    };
+    double kept = s.below[kBins - 1], running;
+    if (f.by_k) {
+        look(f.bin_k, kRank, 0.0, running);
+        kept = fmin(fmax(running, f.low_k), f.high_k);  // (sums of the same in another order)
     }
-    const double target = top_p * kept;
-    if (by_p) {
-        double running;
-        r.within(r.find(kReach, target, 0), kReach, target, 0, running);
+    if (f.by_p) {
+        const double target = top_p * kept;
+        look(find(kReach, target), kReach, target, running);
         kept = fmin(kept, running);
     }
-    if (by_min) {
-        __syncthreads();
-        if (threadIdx.x == 0) s.above_weight = 0;
-        __syncthreads();
-        r.each(bin_m, [&](uint64_t o, uint64_t weight) {
-            const double l = logit_of(o);
-            if (o >> 32 == order_of(top, 0) >> 32 || exp((l - static_cast<double>(top)) / temperature) >= min_p)
-                atomicAdd(&s.above_weight, static_cast<unsigned long long>(weight));
-        });
-        __syncthreads();
-        kept = fmin(kept, (bin_m ? s.below[bin_m - 1] : 0.0) + static_cast<double>(s.above_weight) * r.unit(bin_m));
+    if (f.by_min) {
+        uint64_t sum = 0;
+        const auto add = [&](uint64_t o, uint64_t w) {
+            const float l = r.order.logit(o);
+            if (r.order.key(l) == r.order.key(top) || exp((static_cast<double>(l) - static_cast<double>(top)) / temperature) >= min_p) sum += w;
+        };
+        if (few) {
+            const uint64_t o = lane < static_cast<int>(s.listed) ? s.list[lane] : 0;
+            double y;
+            if (lane < static_cast<int>(s.listed) && r.scale.bin(r.order.logit(o), y) == f.bin_m) add(o, weight(y));
+        } else {
+            if (threadIdx.x == 0) s.sum = 0;
+            __syncthreads();
+            r.each(f.bin_m, add);
+        }
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(static_cast<unsigned long long>(sum), d, 64);
+        if (!few) {
+            if (lane == 0) atomicAdd(&s.sum, static_cast<unsigned long long>(sum));
+            __syncthreads();
+            sum = s.sum;
+        }
+        kept = fmin(kept, r.base(f.bin_m) + static_cast<double>(sum) * r.unit(f.bin_m));
     }
-    kept = fmin(fmax(kept, low), high);
-    double running;
-    const uint64_t o = r.within(r.find(kPass, u * kept, 0), kPass, u * kept, 0, running);
-    if (threadIdx.x == 0) a.out[row] = static_cast<int64_t>(o & 0xffffffffu);
+    kept = fmin(fmax(kept, f.low), f.high);
+    const uint64_t o = look(find(kPass, u * kept), kPass, u * kept, running);
+    if (threadIdx.x == 0) a.out[row] = r.order.token(o);
 }
 
 template <int C>
