@@ -18,7 +18,7 @@
 //     depend on timing.
 #include <algorithm>
 
-#include "attn.h"
+#include "paged_tiles.h"
 
 namespace ckh {
 namespace attn {
@@ -29,26 +29,18 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s lds_v4s;
 
 constexpr int kTileTokens = 64;
-constexpr int kBlockRows = 128;
+constexpr int kWideRows = 128;  // of a piece
+constexpr int kThinRows = 16;
 constexpr int kMinTiles = 4;    // of a chunk, where a span has several
 constexpr int kMaxSpans = 4096; // sequences and groups of a call
-constexpr int kPlanThreads = 1024;
 
 struct Span {
     int first, chunks;   // its first piece of work; chunks of each row
     int seq, sequences;  // the sequences that see it
     int from, to;        // tokens
     int group;           // of a sequence's own span: its group's span, or -1
-    int pad;
+    int size;            // tiles of a chunk
     int64_t part;        // row of the partial results that chunk 0 of its first row has
-};
-
-struct Piece {
-    int span, kv_head, row0, chunk;  // span -1: nothing to do
-    int from, to;                    // tokens
-    int seq, rows;                   // the span's first sequence; its rows
-    int64_t part;                    // of the span's row 0 in this chunk and head
-    int64_t pad;
 };
 
 struct SharedArgs {
@@ -56,49 +48,62 @@ struct SharedArgs {
     const int *table, *lengths, *starts, *shared;
     const float *k_scale, *v_scale;
     uint8_t* out;
-    Span* spans;     // [groups + batch]
-    Piece* pieces;   // [slots]
+    Span* spans;  // [groups + batch]
+    int* firsts;  // [groups + batch + 1]: their first pieces, the pieces of all
     float *part, *stat;  // [row][D], [row][2]: unnormalised outputs; maxima and sums
     int64_t q_b, q_h, k_page, k_tok, k_head, v_page, v_tok, v_head;  // bytes
     int64_t table_stride;
     int batch, heads, kv_heads, group, groups;  // group: query heads of a key-value head
-    int pages, page_size, capacity, slots, target;
+    int pages, page_size, capacity, target;
     float scale;
     FastDiv by_page, by_group;
 };
 
-// Inclusive sum over the plan's threads; `total` of all.
-template <typename T>
-__device__ __forceinline__ T plan_scan(T v, T* wave_sums, T& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const T u = __shfl_up(v, d, 64);
-        if (lane >= d) v += u;
-    }
-    __syncthreads();
-    if (lane == 63) wave_sums[wave] = v;
-    __syncthreads();
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kPlanThreads / 64; ++w) {
-        if (w < wave) v += wave_sums[w];
-        total += wave_sums[w];
-    }
-    return v;
+// Pieces of work that a chunk of `sequences` sequences' rows makes for each key-value head.
+__host__ __device__ __forceinline__ int64_t blocks_of(int64_t rows) {
+    return rows <= kThinRows ? (rows > 0) : (rows + kWideRows - 1) / kWideRows;
 }
 
-__global__ __launch_bounds__(kPlanThreads) void plan_kernel(SharedArgs a) {
-    __shared__ int start[kMaxSpans + 1], common[kMaxSpans], first[kMaxSpans + 1];
-    __shared__ int64_t sums[kPlanThreads / 64];
-    __shared__ int top[kPlanThreads / 64];
+// Inclusive sums over the T threads of the workgroup; `total`: of all.
+template <int T>
+__device__ __forceinline__ void plan_scan(int64_t (&v)[2], int64_t (&total)[2], int64_t (*sums)[2]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const int64_t u = __shfl_up(static_cast<long long>(v[n]), d, 64);
+            if (lane >= d) v[n] += u;
+        }
+    __syncthreads();
+    if (lane == 63) sums[wave][0] = v[0], sums[wave][1] = v[1];
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        total[n] = 0;
+#pragma unroll
+        for (int w = 0; w < T / 64; ++w) {
+            if (w < wave) v[n] += sums[w][n];
+            total[n] += sums[w][n];
+        }
+    }
+}
+
+template <int T>
+__global__ __launch_bounds__(T) void plan_kernel(SharedArgs a) {
+    constexpr int kSpans = T == 256 ? 256 : kMaxSpans;
+    __shared__ int start[kSpans + 1], common[kSpans];
+    __shared__ int64_t sums[T / 64][2];
+    __shared__ int top[T / 64];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int spans = a.groups + a.batch;
     const auto length = [&](int b) { return max(0, min(a.lengths[b], a.capacity)); };
+    const int own_length = t < a.batch ? length(t) : 0;  // (the first T sequences': read ahead)
 
+    for (int g = t; g < a.groups; g += T) common[g] = max(0, a.shared[g]);
     // group bounds, within the batch and ascending (whatever they are, groups do not overlap)
     int before = 0;
-    for (int i0 = 0; i0 <= a.groups; i0 += kPlanThreads) {
+    for (int i0 = 0; i0 <= a.groups; i0 += T) {
         int v = i0 + t <= a.groups ? max(0, min(a.starts[i0 + t], a.batch)) : 0;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -109,13 +114,12 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(SharedArgs a) {
         if (lane == 63) top[wave] = v;
         __syncthreads();
         v = max(v, before);
-        for (int w = 0; w < kPlanThreads / 64; ++w) {
+        for (int w = 0; w < T / 64; ++w) {
             if (w < wave) v = max(v, top[w]);
             before = max(before, top[w]);
         }
         if (i0 + t <= a.groups) start[i0 + t] = v;
     }
-    for (int g = t; g < a.groups; g += kPlanThreads) common[g] = max(0, a.shared[g]);
     __syncthreads();
     const auto group_of = [&](int b) {  // the last group that begins at or before b, if b is in it
         int lo = 0, hi = a.groups;      // groups lo .. hi - 1
@@ -126,9 +130,9 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(SharedArgs a) {
         }
         return lo > 0 && b < start[lo] ? lo - 1 : -1;
     };
-    for (int b = t; b < a.batch; b += kPlanThreads) {
+    for (int b = t; b < a.batch; b += T) {
         const int g = group_of(b);
-        if (g >= 0) atomicMin(&common[g], start[g + 1] - start[g] > 1 ? length(b) : 0);
+        if (g >= 0) atomicMin(&common[g], start[g + 1] - start[g] > 1 ? (b == t ? own_length : length(b)) : 0);
     }
     __syncthreads();
 
@@ -146,78 +150,47 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(SharedArgs a) {
         }
         return s;
     };
-    const auto tiles_of = [&](const Span& s) { return (s.to - s.from + kTileTokens - 1) / kTileTokens; };
-    const auto units_of = [&](const Span& s) {  // pieces of a chunk of all its rows
-        return static_cast<int64_t>((static_cast<int64_t>(s.sequences) * a.group + kBlockRows - 1) / kBlockRows) * a.kv_heads;
-    };
-    int64_t tiles = 0, units = 0;
-    for (int i0 = 0; i0 < spans; i0 += kPlanThreads) {
-        int64_t work = 0, some = 0, total;
+    // chunks begin at multiples of a tile
+    const auto tiles_of = [&](const Span& s) { return s.to > s.from ? (s.to + kTileTokens - 1) / kTileTokens - s.from / kTileTokens : 0; };
+    const auto rows_of = [&](const Span& s) { return static_cast<int64_t>(s.sequences) * a.group; };
+    int64_t tiles = 0;
+    Span held{};  // the thread's span, where there are no more than threads
+    for (int i0 = 0; i0 < spans; i0 += T) {
+        int64_t work[2] = {0, 0}, total[2];
         if (i0 + t < spans) {
             const Span s = span(i0 + t);
-            const int n = tiles_of(s);
-            some = n ? units_of(s) : 0;
-            work = some * n;
+            if (i0 == 0) held = s;
+            work[0] = tiles_of(s) * blocks_of(rows_of(s)) * a.kv_heads;
         }
-        plan_scan(work, sums, total);
-        tiles += total;
-        plan_scan(some, sums, total);
-        units += total;
+        plan_scan<T>(work, total, sums);
+        tiles += total[0];
     }
-    // every span has a ragged end of its own
-    const int64_t room = max(a.target - units, static_cast<int64_t>(a.target / 2));
-    const int64_t size = max((tiles + room - 1) / room, static_cast<int64_t>(kMinTiles));
+    // (no span has 2^26 tiles)
+    const int64_t size = min(max((tiles + a.target - 1) / a.target, static_cast<int64_t>(kMinTiles)), static_cast<int64_t>(1) << 26);
 
     int64_t slot = 0, row = 0;
-    for (int i0 = 0; i0 < spans; i0 += kPlanThreads) {
-        int64_t n = 0, rows = 0, total;
+    for (int i0 = 0; i0 < spans; i0 += T) {
+        int64_t n[2] = {0, 0}, total[2];  // pieces, rows of partial results
         Span s{};
         if (i0 + t < spans) {
-            s = span(i0 + t);
+            s = i0 == 0 ? held : span(i0 + t);
+            s.size = static_cast<int>(size);
             s.chunks = static_cast<int>((tiles_of(s) + size - 1) / size);
-            n = s.chunks * units_of(s);
-            rows = static_cast<int64_t>(s.chunks) * a.kv_heads * s.sequences * a.group;
+            n[0] = s.chunks * blocks_of(rows_of(s)) * a.kv_heads;
+            n[1] = s.chunks * rows_of(s) * a.kv_heads;
         }
-        const int64_t end = plan_scan(n, sums, total);
-        s.first = static_cast<int>(slot + end - n);
-        slot += total;
-        const int64_t row_end = plan_scan(rows, sums, total);
-        s.part = row + row_end - rows;
-        row += total;
+        int64_t end[2] = {n[0], n[1]};
+        plan_scan<T>(end, total, sums);
+        s.first = static_cast<int>(slot + end[0] - n[0]);
+        s.part = row + end[1] - n[1];
+        slot += total[0];
+        row += total[1];
         if (i0 + t < spans) {
-            first[i0 + t] = s.first;
+            a.firsts[i0 + t] = s.first;
             a.spans[i0 + t] = s;
         }
     }
-    if (t == 0) first[spans] = static_cast<int>(slot);
-    __threadfence_block();
-    __syncthreads();
-    for (int i = t; i < a.slots; i += kPlanThreads) {
-        Piece p{};
-        p.span = -1;
-        if (i < static_cast<int>(slot)) {
-            int lo = 0, hi = spans;  // the last span that begins at or before i
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (first[mid] <= i) lo = mid;
-                else hi = mid;
-            }
-            const Span s = a.spans[lo];
-            // chunk by chunk, block of rows by block, and the heads of a token's rows side by side
-            const int blocks = static_cast<int>(units_of(s)) / a.kv_heads, in = i - s.first;
-            const int at = in / a.kv_heads;
-            p.span = lo;
-            p.kv_head = in - at * a.kv_heads;
-            p.chunk = at / blocks;
-            p.row0 = (at - p.chunk * blocks) * kBlockRows;
-            p.from = static_cast<int>(s.from + p.chunk * size * kTileTokens);
-            p.to = static_cast<int>(min(static_cast<int64_t>(s.to), p.from + size * kTileTokens));
-            p.seq = s.seq;
-            p.rows = s.sequences * a.group;
-            p.part = s.part + (static_cast<int64_t>(p.chunk) * a.kv_heads + p.kv_head) * p.rows;
-        }
-        a.pieces[i] = p;
-    }
+    if (t == 0) a.firsts[spans] = static_cast<int>(slot);
 }
 
 // LDS rows are D (96: 128) values of 16 bits; 16-byte piece c of token t's row is at piece c ^ swizzle(t).
@@ -230,24 +203,67 @@ struct TileRows {
     static __device__ __forceinline__ int v_swizzle(int t) { return (2 * t) & kMask; }
 };
 
+// What a workgroup works on.
+struct Piece {
+    int kv_head, row0, rows;  // its first row, the span's rows
+    int from, to, seq;        // tokens; the span's first sequence
+    int64_t part;             // of the span's row 0 in this chunk and head
+};
+
+// Up to 16 rows: their tokens are read once, and what counts is loads in flight.
+template <int C, int D, bool F8, bool WHOLE>
+__device__ __forceinline__ void thin_piece(const SharedArgs& a, const Piece& p, uint8_t* lds) {
+    using L = Lay<D, F8>;
+    auto& lo = *reinterpret_cast<float(*)[kWaves][D][17]>(lds);
+    auto& lm = *reinterpret_cast<float(*)[kWaves][16]>(lds + sizeof(lo));
+    auto& ll = *reinterpret_cast<float(*)[kWaves][16]>(lds + sizeof(lo) + sizeof(lm));
+    const int lane = threadIdx.x & 63, r16 = lane & 15, c = lane >> 4;
+    v4u q[D / 32];
+    {
+        const int row = min(r16, p.rows - 1), s = a.by_group.div(row);
+        const uint8_t* qp = a.q + (p.seq + s) * a.q_b + (p.kv_head * a.group + row - s * a.group) * a.q_h;
+#pragma unroll
+        for (int n = 0; n < D / 32; ++n) {
+            const int d = L::KW == 8 ? n * 32 + c * 8 : (n >> 1) * 64 + c * 16 + (n & 1) * 8;
+            q[n] = *reinterpret_cast<const v4u*>(qp + d * 2);
+        }
+    }
+    const float to_log2 = a.scale * kLog2e * (a.k_scale ? *a.k_scale : 1.0f);
+    constexpr int ES = L::ES;
+    const PagedRows rows{a.k + p.kv_head * a.k_head, a.v + p.kv_head * a.v_head, a.table + p.seq * a.table_stride,
+                         a.k_page / ES, a.k_tok / ES, a.v_page / ES, a.v_tok / ES, a.pages, a.page_size, a.by_page};
+    paged_tiles<C, D, F8, WHOLE>(rows, PagedTiles{0, 0, p.from, p.to, 0, ((p.to + 31) >> 5) - (p.from >> 5)}, q, to_log2, lo, lm, ll);
+    __syncthreads();
+    for (int e = threadIdx.x; e < p.rows * D; e += kWaves * 64) {
+        const int h = e / D, d = e % D;
+        float top = lm[0][h];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, lm[w][h]);
+        float o = 0.0f, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float f = exp2_hw(lm[w][h] - top);
+            o += f * lo[w][d][h];
+            sum += f * ll[w][h];
+        }
+        a.part[(p.part + h) * D + d] = o;
+        if (d == 0) *reinterpret_cast<float2*>(a.stat + (p.part + h) * 2) = make_float2(top, sum);
+    }
+}
+
+// Up to 128 of more rows.
 template <int C, int D, bool F8>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void shared_kernel(SharedArgs a) {
+__device__ __forceinline__ void wide_piece(const SharedArgs& a, const Piece& piece, uint8_t* lds) {
     using R = TileRows<D>;
-    constexpr int kTile = kTileTokens * R::kBytes;
+    constexpr int kTile = kTileTokens * R::kBytes;  // two buffers of K, V
     // loads of a thread for a tile of K or V: 16 bytes, of a row's kRow
     constexpr int kRow = F8 ? D / 16 : R::kPieces;
     constexpr int kLoads = (kTileTokens * kRow + 255) / 256;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * kTile];  // two buffers of K, V
-
-    const Piece piece = a.pieces[blockIdx.x];
-    if (piece.span < 0) return;  // the whole workgroup
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r32 = lane & 31, g = lane >> 5;
-    const int from = __builtin_amdgcn_readfirstlane(piece.from), to = __builtin_amdgcn_readfirstlane(piece.to);
-    const int kvh = __builtin_amdgcn_readfirstlane(piece.kv_head), rows = __builtin_amdgcn_readfirstlane(piece.rows);
-    const int seq = __builtin_amdgcn_readfirstlane(piece.seq);
-    const int row0 = __builtin_amdgcn_readfirstlane(piece.row0) + wave * 32;
+    const int from = piece.from, to = piece.to, kvh = piece.kv_head, rows = piece.rows, seq = piece.seq;
+    const int row0 = piece.row0 + wave * 32;
     const int tiles = (to - from + kTileTokens - 1) / kTileTokens;
     const int* table = a.table + seq * a.table_stride;
     const bool busy = row0 < rows;  // this wave has rows
@@ -444,6 +460,37 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void shared_kernel(SharedArg
     if (g == 0) *reinterpret_cast<float2*>(a.stat + at * 2) = make_float2(m, l);
 }
 
+template <int C, int D, bool F8, bool WHOLE>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void shared_kernel(SharedArgs a) {
+    constexpr int kLds = std::max<int>(4 * kTileTokens * TileRows<D>::kBytes, kWaves * (D * 17 + 32) * 4);
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
+    // the span of this piece: the last that begins at or before it
+    const int spans = a.groups + a.batch, id = blockIdx.x;
+    if (id >= a.firsts[spans]) return;
+    int before = 0;
+    for (int i0 = 0; i0 < spans; i0 += 64) {
+        const int i = i0 + static_cast<int>(threadIdx.x & 63);
+        const uint64_t here = __ballot(i < spans && a.firsts[i] <= id);
+        before += __popcll(here);
+        if (here != ~0ull) break;
+    }
+    const int span = __builtin_amdgcn_readfirstlane(before) - 1;
+    const Span s = a.spans[span];
+    Piece p;
+    p.rows = s.sequences * a.group;
+    // chunk by chunk, block of rows by block, and the heads of a token's rows side by side
+    const int blocks = static_cast<int>(blocks_of(p.rows)), in = id - s.first, at = in / a.kv_heads;
+    const int chunk = at / blocks, first_tile = s.from / kTileTokens + chunk * s.size;
+    p.kv_head = in - at * a.kv_heads;
+    p.row0 = (at - chunk * blocks) * kWideRows;
+    p.from = max(s.from, first_tile * kTileTokens);
+    p.to = static_cast<int>(min(static_cast<int64_t>(s.to), (static_cast<int64_t>(first_tile) + s.size) * kTileTokens));
+    p.seq = s.seq;
+    p.part = s.part + (static_cast<int64_t>(chunk) * a.kv_heads + p.kv_head) * p.rows;
+    if (p.rows <= kThinRows) thin_piece<C, D, F8, WHOLE>(a, p, lds);
+    else wide_piece<C, D, F8>(a, p, lds);
+}
+
 // A row's chunks: D / 4 lanes a row, four d a lane.
 template <int C, int D>
 __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
@@ -483,34 +530,38 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
 }
 
 template <int C, int D>
-void launch_shared(const SharedArgs& a, bool f8, hipStream_t st) {
-    plan_kernel<<<1, kPlanThreads, 0, st>>>(a);
-    if (f8) shared_kernel<C, D, true><<<a.slots, 256, 0, st>>>(a);
-    else shared_kernel<C, D, false><<<a.slots, 256, 0, st>>>(a);
+void launch_shared(const SharedArgs& a, int64_t slots, bool f8, hipStream_t st) {
+    if (a.batch + a.groups <= 256) plan_kernel<256><<<1, 256, 0, st>>>(a);
+    else plan_kernel<1024><<<1, 1024, 0, st>>>(a);
+    const bool whole = a.page_size % 16 == 0;
+    const unsigned grid = static_cast<unsigned>(slots);
+    if (f8 && whole) shared_kernel<C, D, true, true><<<grid, 256, 0, st>>>(a);
+    else if (f8) shared_kernel<C, D, true, false><<<grid, 256, 0, st>>>(a);
+    else if (whole) shared_kernel<C, D, false, true><<<grid, 256, 0, st>>>(a);
+    else shared_kernel<C, D, false, false><<<grid, 256, 0, st>>>(a);
     const int64_t rows = static_cast<int64_t>(a.batch) * a.heads;
     shared_join_kernel<C, D><<<static_cast<unsigned>(cdiv(rows, 256 / (D / 4))), 256, 0, st>>>(a);
 }
 
 template <int C>
-void launch_shared(int dim, const SharedArgs& a, bool f8, hipStream_t st) {
-    if (dim == 64) launch_shared<C, 64>(a, f8, st);
-    else if (dim == 96) launch_shared<C, 96>(a, f8, st);
-    else if (dim == 128) launch_shared<C, 128>(a, f8, st);
-    else launch_shared<C, 256>(a, f8, st);
+void launch_shared(int dim, const SharedArgs& a, int64_t slots, bool f8, hipStream_t st) {
+    if (dim == 64) launch_shared<C, 64>(a, slots, f8, st);
+    else if (dim == 96) launch_shared<C, 96>(a, slots, f8, st);
+    else if (dim == 128) launch_shared<C, 128>(a, slots, f8, st);
+    else launch_shared<C, 256>(a, slots, f8, st);
 }
 
 // Places in the workspace.
 struct SharedSpace {
-    int64_t target, slots, rows, pieces, part, stat, bytes;  // slots: pieces of work at most; rows: of partial results
+    int64_t target, slots, rows, firsts, part, stat, bytes;  // slots: pieces of work at most; rows: of partial results
     SharedSpace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t groups) {
-        const int64_t all = batch * (heads / kv_heads);  // rows of a key-value head
+        const int64_t group = heads / kv_heads, all = batch * group;  // rows of a key-value head
         target = 2 * device_cus();
-        // units: blocks of each sequence's rows and of each group's
-        const int64_t units = kv_heads * (batch * cdiv(heads / kv_heads, kBlockRows) + groups + all / kBlockRows);
-        slots = target + units;
-        rows = target * std::min<int64_t>(kBlockRows, all) + 2 * kv_heads * all;
-        pieces = rup((batch + groups) * sizeof(Span), 256);
-        part = pieces + rup(slots * sizeof(Piece), 256);
+        // a chunk of every span, and `target` for those that have several: the plan's chunks are at least tiles / target long
+        slots = target + kv_heads * (batch * blocks_of(group) + groups + all / kWideRows);
+        rows = target * std::min<int64_t>(kWideRows, all) + 2 * kv_heads * all;
+        firsts = rup((batch + groups) * sizeof(Span), 256);
+        part = firsts + rup((batch + groups + 1) * 4, 256);
         stat = part + rup(rows * dim * 4, 256);
         bytes = stat + rows * 8;
     }
@@ -556,6 +607,7 @@ extern "C" int ckh_shared_attention(const void* q, const void* k_cache, const vo
     for (int i = 0; i < 8; ++i)
         CKH_REQUIRE(strides[i] >= 0 && strides[i] * (i < 2 ? 2 : es) % 16 == 0, "shared_attention: stride %d (%lld) is not a multiple of 16 bytes",
                     i, static_cast<long long>(strides[i]));
+    CKH_REQUIRE(strides[3] * es < (int64_t(1) << 25) && strides[6] * es < (int64_t(1) << 25), "shared_attention: token stride too large");
     CKH_REQUIRE(aligned(q, 16) && aligned(k_cache, 16) && aligned(v_cache, 16) && aligned(out, 8) && aligned(page_table, 4) &&
                     aligned(lengths, 4) && aligned(group_starts, 4) && aligned(shared, 4) && aligned(k_scale, 4) && aligned(v_scale, 4) &&
                     aligned(workspace, 16),
@@ -573,7 +625,7 @@ extern "C" int ckh_shared_attention(const void* q, const void* k_cache, const vo
     a.out = static_cast<uint8_t*>(out);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     a.spans = reinterpret_cast<attn::Span*>(ws);
-    a.pieces = reinterpret_cast<attn::Piece*>(ws + space.pieces);
+    a.firsts = reinterpret_cast<int*>(ws + space.firsts);
     a.part = reinterpret_cast<float*>(ws + space.part);
     a.stat = reinterpret_cast<float*>(ws + space.stat);
     a.q_b = strides[0] * 2, a.q_h = strides[1] * 2;
@@ -584,11 +636,11 @@ extern "C" int ckh_shared_attention(const void* q, const void* k_cache, const vo
     a.group = static_cast<int>(heads / kv_heads), a.groups = static_cast<int>(groups);
     a.pages = static_cast<int>(pages), a.page_size = static_cast<int>(page_size);
     a.capacity = static_cast<int>(max_pages * page_size);
-    a.slots = static_cast<int>(space.slots), a.target = static_cast<int>(space.target);
+    a.target = static_cast<int>(space.target);
     a.scale = scale;
     a.by_page = fast_div(static_cast<uint32_t>(page_size)), a.by_group = fast_div(static_cast<uint32_t>(a.group));
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    if (q_code == CKH_BF16) attn::launch_shared<CKH_BF16>(static_cast<int>(dim), a, es == 1, st);
-    else attn::launch_shared<CKH_F16>(static_cast<int>(dim), a, es == 1, st);
+    if (q_code == CKH_BF16) attn::launch_shared<CKH_BF16>(static_cast<int>(dim), a, space.slots, es == 1, st);
+    else attn::launch_shared<CKH_F16>(static_cast<int>(dim), a, space.slots, es == 1, st);
     return check_launch("shared_attention");
 }

@@ -96,7 +96,8 @@ def test_shared_attention(lib, mem):
                          (dict(kv_heads=0), "heads"), (dict(pages=0), "pages"), (dict(page=0), "pages"), (dict(most=1 << 30), "pages"), (dict(groups=-1), "groups"),
                          (dict(batch=4096), "4096"), (dict(q=None), "null pointer"), (dict(shared=None), "null pointer"), (dict(ws=None), "null pointer"),
                          (dict(q=p + 4), "misaligned"), (dict(ws=p + 8), "misaligned"), (dict(nbytes=1000), "workspace"),
-                         (dict(s=strides(256, 64, 2048, 126, 64, 2048, 128, 64)), "stride 3"), (dict(heads=65532, kv_heads=65532, batch=4000), "too many")):
+                         (dict(s=strides(256, 64, 2048, 126, 64, 2048, 128, 64)), "stride 3"),
+                         (dict(s=strides(256, 64, 2048, 1 << 25, 64, 2048, 128, 64)), "too large"), (dict(heads=65532, kv_heads=65532, batch=4000), "too many")):
         refused(lib, call(**kwargs), text)
     assert call(batch=0) == 0 and call(heads=0) == 0
     f = lib.ckh_shared_attention_workspace_bytes
