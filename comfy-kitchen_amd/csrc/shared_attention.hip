@@ -491,42 +491,67 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void shared_kernel(SharedArg
     else wide_piece<C, D, F8>(a, p, lds);
 }
 
-// A row's chunks: D / 4 lanes a row, four d a lane.
+// A row a wave: its chunks' maxima and sums first, 64 at a time, then four d a lane of as many chunks at once as lanes allow.
 template <int C, int D>
 __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
-    constexpr int kLanes = D / 4, kRows = 256 / kLanes;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kLanes;
-    if (threadIdx.x >= kRows * kLanes || row >= static_cast<int64_t>(a.batch) * a.heads) return;
+    constexpr int kLanes = D / 4, kSets = 64 / kLanes;  // lanes of a chunk's row; chunks at once
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    if (row >= static_cast<int64_t>(a.batch) * a.heads) return;
+    const int lane = threadIdx.x & 63, set = lane / kLanes, d = (lane - set * kLanes) * 4;
     const int b = static_cast<int>(row / a.heads), h = static_cast<int>(row - static_cast<int64_t>(b) * a.heads);
-    const int kvh = h / a.group, in = h - kvh * a.group, d = threadIdx.x % kLanes * 4;
+    const int kvh = h / a.group, in = h - kvh * a.group;
     const Span own = a.spans[a.groups + b];
-    Span group{};
-    if (own.group >= 0) group = a.spans[own.group];
-    int64_t at[2], step[2];
-    const Span* both[2] = {&group, &own};
-    float top = -1e30f;
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-        const Span& s = *both[n];
-        step[n] = static_cast<int64_t>(a.kv_heads) * s.sequences * a.group;
-        at[n] = s.part + static_cast<int64_t>(kvh) * s.sequences * a.group + static_cast<int64_t>(b - s.seq) * a.group + in;
-        for (int i = 0; i < s.chunks; ++i) top = fmaxf(top, a.stat[(at[n] + i * step[n]) * 2]);
-    }
-    float sum = 0.0f;
+    const Span group = own.group >= 0 ? a.spans[own.group] : Span{};
+    // chunk i of the group's, then of the sequence's own: its row of the partial results
+    const int64_t group_step = static_cast<int64_t>(a.kv_heads) * group.sequences * a.group, own_step = static_cast<int64_t>(a.kv_heads) * a.group;
+    const int64_t group_at = group.part + (static_cast<int64_t>(kvh) * group.sequences + (b - group.seq)) * a.group + in;
+    const int64_t own_at = own.part + static_cast<int64_t>(kvh) * a.group + in;
+    const int chunks = group.chunks + own.chunks;
+    const auto place = [&](int i) { return i < group.chunks ? group_at + i * group_step : own_at + (i - group.chunks) * own_step; };
+
+    float top = -1e30f, sum = 0.0f;
     v4f o = v4f{0, 0, 0, 0};
+    for (int i0 = 0; i0 < chunks; i0 += 64) {
+        const int i = i0 + lane;
+        float2 st = make_float2(-1e30f, 0.0f);
+        if (i < chunks) st = *reinterpret_cast<const float2*>(a.stat + place(i) * 2);
+        float high = st.x;
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-#pragma unroll 4
-        for (int i = 0; i < both[n]->chunks; ++i) {
-            const int64_t r = at[n] + i * step[n];
-            const float2 st = *reinterpret_cast<const float2*>(a.stat + r * 2);
-            const float f = exp2_hw(st.x - top);
-            sum += f * st.y;
-            o += f * *reinterpret_cast<const v4f*>(a.part + r * D + d);
+        for (int s = 32; s >= 1; s >>= 1) high = fmaxf(high, __shfl_xor(high, s, 64));
+        high = fmaxf(high, top);
+        const float f = exp2_hw(st.x - high), old = exp2_hw(top - high);
+        top = high;
+        float part = f * st.y;
+#pragma unroll
+        for (int s = 32; s >= 1; s >>= 1) part += __shfl_xor(part, s, 64);
+        sum = sum * old + part;
+        o *= old;
+        const int n = min(64, chunks - i0);
+        constexpr int U = 4;  // loads of a lane in flight
+        for (int j0 = 0; j0 < n; j0 += U * kSets) {
+            v4f x[U];
+            float g[U];
+#pragma unroll
+            for (int e = 0; e < U; ++e) {  // past the last chunk (and in lanes without a set): the last one again, with no weight
+                const int j = j0 + e * kSets + set;
+                const bool live = set < kSets && j < n;
+                x[e] = *reinterpret_cast<const v4f*>(a.part + place(i0 + min(j, n - 1)) * D + d);
+                g[e] = __shfl(f, live ? j : 0, 64);
+                g[e] = live ? g[e] : 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < U; ++e) o += g[e] != 0.0f ? g[e] * x[e] : v4f{0, 0, 0, 0};
         }
     }
+    // the sets' sums, in order
+    v4f all = o;
+#pragma unroll
+    for (int n = 1; n < kSets; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) all[e] += __shfl(o[e], lane + n * kLanes, 64);
+    if (set != 0) return;
     const float f = sum == 0.0f ? 0.0f : (a.v_scale ? *a.v_scale : 1.0f) / sum;
-    *reinterpret_cast<v2u*>(a.out + (row * D + d) * 2) = v2u{pack2<C>(o[0] * f, o[1] * f), pack2<C>(o[2] * f, o[3] * f)};
+    *reinterpret_cast<v2u*>(a.out + (row * D + d) * 2) = v2u{pack2<C>(all[0] * f, all[1] * f), pack2<C>(all[2] * f, all[3] * f)};
 }
 
 template <int C, int D>
@@ -540,7 +565,7 @@ void launch_shared(const SharedArgs& a, int64_t slots, bool f8, hipStream_t st) 
     else if (whole) shared_kernel<C, D, false, true><<<grid, 256, 0, st>>>(a);
     else shared_kernel<C, D, false, false><<<grid, 256, 0, st>>>(a);
     const int64_t rows = static_cast<int64_t>(a.batch) * a.heads;
-    shared_join_kernel<C, D><<<static_cast<unsigned>(cdiv(rows, 256 / (D / 4))), 256, 0, st>>>(a);
+    shared_join_kernel<C, D><<<static_cast<unsigned>(cdiv(rows, 4)), 256, 0, st>>>(a);
 }
 
 template <int C>
