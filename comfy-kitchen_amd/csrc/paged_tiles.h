@@ -66,11 +66,11 @@ struct PagedTiles {
     int sink_tiles, sink_end, start, len, t0, t1;
 };
 
-// A workgroup of kWaves waves: every wave's unnormalised output, maxima and sums to lo, lm and ll.  A wave's query
-// columns are q (column lane & 15; d as Lay has K's).  QC: type of q.  F8: the cache holds E4M3 codes
-// (else QC).  WHOLE: 16 consecutive tokens are always on one page (page_size % 16 == 0), so a tile needs
+// Every wave's unnormalised output, maxima and sums to lo, lm and ll.  A wave's query columns are q (column
+// lane & 15; d as Lay has K's).  STEP: kWaves where the waves of the workgroup share the tiles, 1 where each has its
+// own (and arguments of its own).  QC: type of q.  F8: the cache holds E4M3 codes (else QC).  WHOLE: 16 consecutive tokens are always on one page (page_size % 16 == 0), so a tile needs
 // two page numbers, which are the wave's (scalar); else every lane looks up the pages of its tokens, a tile ahead.
-template <int QC, int D, bool F8, bool WHOLE>
+template <int QC, int D, bool F8, bool WHOLE, int STEP = kWaves>
 __device__ __forceinline__ void paged_tiles(const PagedRows& a, const PagedTiles& vis, const v4u (&q)[D / 32], float to_log2,
                                             float (&lo)[kWaves][D][17], float (&lm)[kWaves][16], float (&ll)[kWaves][16]) {
     using L = Lay<D, F8>;
@@ -169,7 +169,7 @@ __device__ __forceinline__ void paged_tiles(const PagedRows& a, const PagedTiles
                 if constexpr (L::SETS > 1)
                     fetch<L::words(1), L::width(1) * ES == 2>(t.v[e] + L::at(1), p + (L::base(1) + r16 * L::width(1)) * ES);
             }
-            look_up(i + kWaves);
+            look_up(i + STEP);
         }
     };
 
@@ -267,19 +267,19 @@ __device__ __forceinline__ void paged_tiles(const PagedRows& a, const PagedTiles
         }
     };
 
-    if (t0 + wave < t1) {
+    int i = t0 + (STEP > 1 ? wave : 0);
+    if (i < t1) {
         Tile x, y;
-        int i = t0 + wave;
         look_up(i);
         load(x, i);
         for (;;) {
-            load(y, i + kWaves);
+            load(y, i + STEP);
             use(x);
-            i += kWaves;
+            i += STEP;
             if (i >= t1) break;
-            load(x, i + kWaves);
+            load(x, i + STEP);
             use(y);
-            i += kWaves;
+            i += STEP;
             if (i >= t1) break;
         }
     }

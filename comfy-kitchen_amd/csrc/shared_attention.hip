@@ -25,6 +25,7 @@ namespace attn {
 
 typedef __attribute__((address_space(3))) void lds_void;
 typedef const __attribute__((address_space(1))) void global_void;
+typedef const __attribute__((address_space(4))) int constant_int;
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s lds_v4s;
 
@@ -32,14 +33,17 @@ constexpr int kTileTokens = 64;
 constexpr int kWideRows = 128;  // of a piece
 constexpr int kThinRows = 16;
 constexpr int kMinTiles = 4;    // of a chunk, where a span has several
+constexpr int kMinThinTiles = 2;
 constexpr int kMaxSpans = 4096; // sequences and groups of a call
 
 struct Span {
-    int first, chunks;   // its first piece of work; chunks of each row
+    int first, chunks;   // its first workgroup; chunks of each row
     int seq, sequences;  // the sequences that see it
     int from, to;        // tokens
     int group;           // of a sequence's own span: its group's span, or -1
     int size;            // tiles of a chunk
+    int pieces;          // of work
+    int pad;
     int64_t part;        // row of the partial results that chunk 0 of its first row has
 };
 
@@ -49,7 +53,7 @@ struct SharedArgs {
     const float *k_scale, *v_scale;
     uint8_t* out;
     Span* spans;  // [groups + batch]
-    int* firsts;  // [groups + batch + 1]: their first pieces, the pieces of all
+    int* firsts;  // [groups + batch + 1]: their first workgroups, the workgroups of all
     float *part, *stat;  // [row][D], [row][2]: unnormalised outputs; maxima and sums
     int64_t q_b, q_h, k_page, k_tok, k_head, v_page, v_tok, v_head;  // bytes
     int64_t table_stride;
@@ -59,7 +63,7 @@ struct SharedArgs {
     FastDiv by_page, by_group;
 };
 
-// Pieces of work that a chunk of `sequences` sequences' rows makes for each key-value head.
+// Blocks of rows.
 __host__ __device__ __forceinline__ int64_t blocks_of(int64_t rows) {
     return rows <= kThinRows ? (rows > 0) : (rows + kWideRows - 1) / kWideRows;
 }
@@ -174,9 +178,13 @@ __global__ __launch_bounds__(T) void plan_kernel(SharedArgs a) {
         Span s{};
         if (i0 + t < spans) {
             s = i0 == 0 ? held : span(i0 + t);
-            s.size = static_cast<int>(size);
-            s.chunks = static_cast<int>((tiles_of(s) + size - 1) / size);
+            // a workgroup works on one block of many rows, or on the few rows of kWaves chunks or heads
+            const bool thin = rows_of(s) <= kThinRows;
+            s.size = static_cast<int>(thin ? max((size + kWaves - 1) / kWaves, static_cast<int64_t>(kMinThinTiles)) : size);
+            s.chunks = (tiles_of(s) + s.size - 1) / s.size;
             n[0] = s.chunks * blocks_of(rows_of(s)) * a.kv_heads;
+            s.pieces = static_cast<int>(n[0]);
+            if (thin) n[0] = (n[0] + kWaves - 1) / kWaves;
             n[1] = s.chunks * rows_of(s) * a.kv_heads;
         }
         int64_t end[2] = {n[0], n[1]};
@@ -193,24 +201,36 @@ __global__ __launch_bounds__(T) void plan_kernel(SharedArgs a) {
     if (t == 0) a.firsts[spans] = static_cast<int>(slot);
 }
 
-// LDS rows are D (96: 128) values of 16 bits; 16-byte piece c of token t's row is at piece c ^ swizzle(t).
+// LDS rows are D (96: 128) values of 16 bits; 16-byte piece c of token t's row is at piece c ^ swizzle(t), so that the
+// 16 lanes that read K at once (16 tokens' pieces), and the 32 that read V (4 tokens', 4 pieces of each), touch all 64 banks.
 template <int D>
 struct TileRows {
     static constexpr int kPieces = D == 96 ? 16 : D / 8;
     static constexpr int kBytes = kPieces * 16;
-    static constexpr int kMask = kPieces < 16 ? kPieces - 1 : 15;
-    static __device__ __forceinline__ int k_swizzle(int t) { return t & 7; }
-    static __device__ __forceinline__ int v_swizzle(int t) { return (2 * t) & kMask; }
+    static __device__ __forceinline__ int k_swizzle(int t) { return D == 64 ? (t >> 1) & 7 : t & 15; }
+    static __device__ __forceinline__ int v_swizzle(int t) { return D == 64 ? (t & 2) * 2 : (t & 3) * 4; }
 };
 
-// What a workgroup works on.
+// What a workgroup, or a wave of one, works on.
 struct Piece {
     int kv_head, row0, rows;  // its first row, the span's rows
     int from, to, seq;        // tokens; the span's first sequence
     int64_t part;             // of the span's row 0 in this chunk and head
+    // The at-th of the span's: chunk by chunk, block of rows by block, and the heads of a token's rows side by side.
+    __device__ __forceinline__ Piece(const SharedArgs& a, const Span& s, int at) {
+        rows = s.sequences * a.group;
+        const int blocks = static_cast<int>(blocks_of(rows)), in = at / a.kv_heads, chunk = in / blocks;
+        const int64_t tile = s.from / kTileTokens + static_cast<int64_t>(chunk) * s.size;
+        kv_head = at - in * a.kv_heads;
+        row0 = (in - chunk * blocks) * kWideRows;
+        from = static_cast<int>(max(static_cast<int64_t>(s.from), tile * kTileTokens));
+        to = static_cast<int>(min(static_cast<int64_t>(s.to), (tile + s.size) * kTileTokens));
+        seq = s.seq;
+        part = s.part + (static_cast<int64_t>(chunk) * a.kv_heads + kv_head) * rows;
+    }
 };
 
-// Up to 16 rows: their tokens are read once, and what counts is loads in flight.
+// A wave, up to 16 rows: their tokens are read once, and what counts is loads in flight.
 template <int C, int D, bool F8, bool WHOLE>
 __device__ __forceinline__ void thin_piece(const SharedArgs& a, const Piece& p, uint8_t* lds) {
     using L = Lay<D, F8>;
@@ -218,6 +238,7 @@ __device__ __forceinline__ void thin_piece(const SharedArgs& a, const Piece& p, 
     auto& lm = *reinterpret_cast<float(*)[kWaves][16]>(lds + sizeof(lo));
     auto& ll = *reinterpret_cast<float(*)[kWaves][16]>(lds + sizeof(lo) + sizeof(lm));
     const int lane = threadIdx.x & 63, r16 = lane & 15, c = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     v4u q[D / 32];
     {
         const int row = min(r16, p.rows - 1), s = a.by_group.div(row);
@@ -232,39 +253,29 @@ __device__ __forceinline__ void thin_piece(const SharedArgs& a, const Piece& p, 
     constexpr int ES = L::ES;
     const PagedRows rows{a.k + p.kv_head * a.k_head, a.v + p.kv_head * a.v_head, a.table + p.seq * a.table_stride,
                          a.k_page / ES, a.k_tok / ES, a.v_page / ES, a.v_tok / ES, a.pages, a.page_size, a.by_page};
-    paged_tiles<C, D, F8, WHOLE>(rows, PagedTiles{0, 0, p.from, p.to, 0, ((p.to + 31) >> 5) - (p.from >> 5)}, q, to_log2, lo, lm, ll);
-    __syncthreads();
-    for (int e = threadIdx.x; e < p.rows * D; e += kWaves * 64) {
-        const int h = e / D, d = e % D;
-        float top = lm[0][h];
-#pragma unroll
-        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, lm[w][h]);
-        float o = 0.0f, sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const float f = exp2_hw(lm[w][h] - top);
-            o += f * lo[w][d][h];
-            sum += f * ll[w][h];
-        }
-        a.part[(p.part + h) * D + d] = o;
-        if (d == 0) *reinterpret_cast<float2*>(a.stat + (p.part + h) * 2) = make_float2(top, sum);
-    }
+    paged_tiles<C, D, F8, WHOLE, 1>(rows, PagedTiles{0, 0, p.from, p.to, 0, ((p.to + 31) >> 5) - (p.from >> 5)}, q, to_log2, lo, lm, ll);
+    __asm__ volatile("" ::: "memory");  // (one wave: LDS keeps its order)
+    for (int e = lane; e < p.rows * D; e += 64) a.part[p.part * D + e] = lo[wave][e % D][e / D];
+    if (lane < p.rows) *reinterpret_cast<float2*>(a.stat + (p.part + lane) * 2) = make_float2(lm[wave][lane], ll[wave][lane]);
 }
 
-// Up to 128 of more rows.
-template <int C, int D, bool F8>
+// A workgroup, up to 128 of more rows.  A wave fetches 16 tokens of a tile: with WHOLE they lie on one page, whose number
+// and place are the wave's (scalar), and what is not to be seen is out of the buffer's bounds, which arrives as zeros;
+// else every lane finds its tokens' places.
+template <int C, int D, bool F8, bool WHOLE>
 __device__ __forceinline__ void wide_piece(const SharedArgs& a, const Piece& piece, uint8_t* lds) {
     using R = TileRows<D>;
     constexpr int kTile = kTileTokens * R::kBytes;  // two buffers of K, V
-    // loads of a thread for a tile of K or V: 16 bytes, of a row's kRow
+    // loads of a lane for a tile of K or V: 16 bytes, of a row's kRow
     constexpr int kRow = F8 ? D / 16 : R::kPieces;
-    constexpr int kLoads = (kTileTokens * kRow + 255) / 256;
+    constexpr int kLoads = (16 * kRow + 63) / 64;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r32 = lane & 31, g = lane >> 5;
     const int from = piece.from, to = piece.to, kvh = piece.kv_head, rows = piece.rows, seq = piece.seq;
     const int row0 = piece.row0 + wave * 32;
-    const int tiles = (to - from + kTileTokens - 1) / kTileTokens;
+    const int first = from / kTileTokens * kTileTokens;  // of the first tile
+    const int tiles = (to - first + kTileTokens - 1) / kTileTokens;
     const int* table = a.table + seq * a.table_stride;
     const bool busy = row0 < rows;  // this wave has rows
 
@@ -279,58 +290,94 @@ __device__ __forceinline__ void wide_piece(const SharedArgs& a, const Piece& pie
         for (int n = 0; n < D / 16; ++n) q[n] = *reinterpret_cast<const v4u*>(qp + n * 32) ^ flip;
     }
 
-    // a thread's places in the loads of a tile
-    const auto place = [&](int n) { return F8 ? static_cast<int>(threadIdx.x) + n * 256 : (wave * kLoads + n) * 64 + lane; };
+    // a lane's load n of a tile: piece (n * 64 + lane) % kRow of the wave's token (n * 64 + lane) / kRow
+    const auto tok = [&](int n) { return min((n * 64 + lane) / kRow, 15); };
+    const auto col = [&](int n) { return (n * 64 + lane) % kRow; };
+    const auto k_at = [&](int n) { return F8 ? col(n) : min(col(n) ^ R::k_swizzle(wave * 16 + tok(n)), D / 8 - 1); };
+    const auto v_at = [&](int n) { return F8 ? col(n) : min(col(n) ^ R::v_swizzle(wave * 16 + tok(n)), D / 8 - 1); };
     const uint8_t* kb = a.k + kvh * a.k_head;
     const uint8_t* vb = a.v + kvh * a.v_head;
-    int page_of[kLoads];  // of the next tile's tokens
-    const auto token = [&](int i, int n) { return min(from + i * kTileTokens + min(place(n) / kRow, kTileTokens - 1), to - 1); };
+    // Whether any of the wave's tokens of tile i are to be seen.
+    const auto some = [&](int i) { return first + i * kTileTokens + wave * 16 < to && first + i * kTileTokens + wave * 16 + 16 > from; };
+    const auto token = [&](int i, int n) { return max(from, min(first + i * kTileTokens + wave * 16 + tok(n), to - 1)); };
+    int page_of[WHOLE ? 1 : kLoads];  // of the next tile's tokens
     const auto look_up = [&](int i) __attribute__((always_inline)) {
+        if constexpr (WHOLE) {
+            // (a scalar load: a vector one would be waited for, and with it the fetches before it)
+            page_of[0] = some(i) ? ((constant_int*)table)[a.by_page.div(first + i * kTileTokens + wave * 16)] : 0;
+        } else {
 #pragma unroll
-        for (int n = 0; n < kLoads; ++n) page_of[n] = table[a.by_page.div(token(i, n))];
+            for (int n = 0; n < kLoads; ++n) page_of[n] = table[a.by_page.div(token(i, n))];
+        }
     };
     v4u held[F8 ? 2 * kLoads : 1];  // codes on their way to LDS
-    // Begins to fetch tile i; its tokens from the chunk's end on are copies of the last.
-    const auto fetch = [&](int i, uint8_t* at) __attribute__((always_inline)) {
+    uint32_t ko[WHOLE ? kLoads : 1], vo[WHOLE ? kLoads : 1];
+    if constexpr (WHOLE) {
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
-            const int tk = token(i, n), slot = tk - a.by_page.div(tk) * a.page_size;
-            const int64_t page = min(static_cast<uint32_t>(page_of[n]), static_cast<uint32_t>(a.pages - 1));
-            const int t = min(place(n) / kRow, kTileTokens - 1), p = place(n) % kRow;
-            const uint8_t* kp = kb + page * a.k_page + slot * a.k_tok;
-            const uint8_t* vp = vb + page * a.v_page + slot * a.v_tok;
-            if constexpr (F8) {
-                held[n] = *reinterpret_cast<const v4u*>(kp + p * 16);
-                held[kLoads + n] = *reinterpret_cast<const v4u*>(vp + p * 16);
-            } else {
-                const int kc = min(p ^ R::k_swizzle(t), D / 8 - 1), vc = min(p ^ R::v_swizzle(t), D / 8 - 1);
-                __builtin_amdgcn_global_load_lds((global_void*)(kp + kc * 16), (lds_void*)(at + (wave * kLoads + n) * 1024), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((global_void*)(vp + vc * 16), (lds_void*)(at + kTile + (wave * kLoads + n) * 1024), 16, 0, 0);
+            ko[n] = tok(n) * static_cast<uint32_t>(a.k_tok) + k_at(n) * 16;
+            vo[n] = tok(n) * static_cast<uint32_t>(a.v_tok) + v_at(n) * 16;
+        }
+    }
+    // Begins to fetch tile i.
+    const auto fetch = [&](int i, uint8_t* at) __attribute__((always_inline)) {
+        if constexpr (WHOLE) {
+            const int t0 = first + i * kTileTokens + wave * 16, slot = t0 - a.by_page.div(t0) * a.page_size;
+            const int64_t page = min(static_cast<uint32_t>(page_of[0]), static_cast<uint32_t>(a.pages - 1));
+            const __amdgpu_buffer_rsrc_t rk = buffer_rsrc(kb + page * a.k_page + slot * a.k_tok, some(i) ? 0x7fffffffu : 0u);
+            const __amdgpu_buffer_rsrc_t rv = buffer_rsrc(vb + page * a.v_page + slot * a.v_tok, some(i) ? 0x7fffffffu : 0u);
+            const bool edge = first + i * kTileTokens < from || first + (i + 1) * kTileTokens > to;
+#pragma unroll
+            for (int n = 0; n < kLoads; ++n) {
+                uint32_t kn = ko[n], vn = vo[n];
+                if (edge && (t0 + tok(n) < from || t0 + tok(n) >= to)) kn = vn = kOut;
+                if constexpr (F8) {
+                    held[n] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rk, kn, 0, 0));
+                    held[kLoads + n] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rv, vn, 0, 0));
+                } else {
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void*)(at + (wave * kLoads + n) * 1024), 16, kn, 0, 0, 0);
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void*)(at + kTile + (wave * kLoads + n) * 1024), 16, vn, 0, 0, 0);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < kLoads; ++n) {
+                const int tk = token(i, n), slot = tk - a.by_page.div(tk) * a.page_size;
+                const int64_t page = min(static_cast<uint32_t>(page_of[n]), static_cast<uint32_t>(a.pages - 1));
+                const uint8_t* kp = kb + page * a.k_page + slot * a.k_tok + k_at(n) * 16;
+                const uint8_t* vp = vb + page * a.v_page + slot * a.v_tok + v_at(n) * 16;
+                if constexpr (F8) {
+                    held[n] = *reinterpret_cast<const v4u*>(kp);
+                    held[kLoads + n] = *reinterpret_cast<const v4u*>(vp);
+                } else {
+                    __builtin_amdgcn_global_load_lds((global_void*)kp, (lds_void*)(at + (wave * kLoads + n) * 1024), 16, 0, 0);
+                    __builtin_amdgcn_global_load_lds((global_void*)vp, (lds_void*)(at + kTile + (wave * kLoads + n) * 1024), 16, 0, 0);
+                }
             }
         }
     };
-    // Tile i is in LDS at `at` when this wave and the others are through here; values from the end on are zeros.
+    // What of tile i the fetch does not bring to LDS at `at` by itself: widened codes; zeros for values that are not to be seen.
     const auto settle = [&](int i, uint8_t* at) __attribute__((always_inline)) {
-        const int left = to - from - i * kTileTokens;
+        const int t0 = first + i * kTileTokens;
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
-            const int t = place(n) / kRow, p = place(n) % kRow;
+            const int t = wave * 16 + tok(n);
+            const bool out = !WHOLE && (t0 + t < from || t0 + t >= to);
             if constexpr (F8) {
-                if (kTileTokens * kRow % 256 != 0 && place(n) >= kTileTokens * kRow) continue;
+                if (16 * kRow % 64 != 0 && n * 64 + lane >= 16 * kRow) continue;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const uint32_t k0 = held[n][2 * half], k1 = held[n][2 * half + 1];
                     uint32_t v0 = held[kLoads + n][2 * half], v1 = held[kLoads + n][2 * half + 1];
-                    if (t >= left) v0 = v1 = 0u;
-                    const int piece = 2 * p + half;
+                    if (out) v0 = v1 = 0u;
+                    const int piece = 2 * col(n) + half;
                     *reinterpret_cast<v4u*>(at + t * R::kBytes + ((piece ^ R::k_swizzle(t)) << 4)) =
                         v4u{widen_e4m3<C, false>(k0), widen_e4m3<C, true>(k0), widen_e4m3<C, false>(k1), widen_e4m3<C, true>(k1)};
                     *reinterpret_cast<v4u*>(at + kTile + t * R::kBytes + ((piece ^ R::v_swizzle(t)) << 4)) =
                         v4u{widen_e4m3<C, false>(v0), widen_e4m3<C, true>(v0), widen_e4m3<C, false>(v1), widen_e4m3<C, true>(v1)};
                 }
-            } else {
-                if (left < kTileTokens && t >= left)
-                    *reinterpret_cast<v4u*>(at + kTile + (wave * kLoads + n) * 1024 + lane * 16) = v4u{0u, 0u, 0u, 0u};
+            } else if (out) {
+                *reinterpret_cast<v4u*>(at + kTile + (wave * kLoads + n) * 1024 + lane * 16) = v4u{0u, 0u, 0u, 0u};
             }
         }
     };
@@ -343,24 +390,30 @@ __device__ __forceinline__ void wide_piece(const SharedArgs& a, const Piece& pie
     float m = -1e30f, l = 0.0f;
 
     const auto use = [&](int i, const uint8_t* kt, const uint8_t* vt) __attribute__((always_inline)) {
+        // (the two halves in turn: a product that adds to the one before it waits for it)
         v16f s[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[h][e] = 0.0f;
-            const int t = h * 32 + r32;
-            const uint8_t* kr = kt + t * R::kBytes;
 #pragma unroll
-            for (int n = 0; n < D / 16; ++n)
+        for (int n = 0; n < D / 16; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int t = h * 32 + r32;
+                const uint8_t* kr = kt + t * R::kBytes;
                 s[h] = mfma32<C>(*reinterpret_cast<const v4u*>(kr + (((2 * n + g) ^ R::k_swizzle(t)) << 4)), q[n], s[h]);
-        }
-        const int left = to - from - i * kTileTokens;
-        if (left < kTileTokens) {
-            const int high = left - 4 * g;
+            }
+        const int t0 = first + i * kTileTokens;
+        if (t0 < from || t0 + kTileTokens > to) {
+            const int low = from - t0 - 4 * g, high = to - t0 - 4 * g;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[h][e] = h * 32 + 8 * (e >> 2) + (e & 3) < high ? s[h][e] : -__builtin_inff();
+                for (int e = 0; e < 16; ++e) {
+                    const int j = h * 32 + 8 * (e >> 2) + (e & 3);
+                    s[h][e] = j >= low && j < high ? s[h][e] : -__builtin_inff();
+                }
         }
         float top = s[0][0];
 #pragma unroll
@@ -377,41 +430,45 @@ __device__ __forceinline__ void wide_piece(const SharedArgs& a, const Piece& pie
 #pragma unroll
             for (int n = 0; n < D / 32; ++n) acc[n] *= f;
         }
-        v4u p[4];
+        // The weights of 16 tokens are made while the matrix units multiply those of the 16 before with their values.
         float sum = 0.0f;  // the tile's own: single small weights would be lost in a large l
+        const auto weigh = [&](int w) __attribute__((always_inline)) {
+            float x[8];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                s[h][e] = exp2_hw(__fmaf_rn(s[h][e], c, -m));
-                sum += s[h][e];
+            for (int e = 0; e < 8; ++e) {
+                x[e] = exp2_hw(__fmaf_rn(s[w >> 1][(w & 1) * 8 + e], c, -m));
+                sum += x[e];
             }
-        l += sum;
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                p[w][e] = pack2<C>(s[w >> 1][(w & 1) * 8 + 2 * e], s[w >> 1][(w & 1) * 8 + 2 * e + 1]);
+            return v4u{pack2<C>(x[0], x[1]), pack2<C>(x[2], x[3]), pack2<C>(x[4], x[5]), pack2<C>(x[6], x[7])};
+        };
         // tokens w * 16 + half * 8 + 4 g + 0..3: the lane gives a piece of one token and 4 d, and
         // gets one d of the four tokens
         const int sub = lane & 15, db = (lane >> 4) & 1;
+        const auto values = [&](int w, v4u (&f)[D / 32]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-#pragma unroll
-            for (int n = 0; n < D / 32; ++n) {
-                v4u f;
+            for (int n = 0; n < D / 32; ++n)
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const int t = w * 16 + half * 8 + 4 * g + (sub >> 2);
                     const int piece = n * 4 + db * 2 + ((sub >> 1) & 1);
                     const uint8_t* at = vt + t * R::kBytes + ((piece ^ R::v_swizzle(t)) << 4) + (sub & 1) * 8;
                     const v2u two = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at)));
-                    f[half * 2] = two[0];
-                    f[half * 2 + 1] = two[1];
+                    f[n][half * 2] = two[0];
+                    f[n][half * 2 + 1] = two[1];
                 }
-                acc[n] = mfma32<C>(f, p[w], acc[n]);
-            }
+        };
+        v4u f[D / 32], p = weigh(0);
+        values(0, f);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            v4u next = p;
+            if (w < 3) next = weigh(w + 1);
+#pragma unroll
+            for (int n = 0; n < D / 32; ++n) acc[n] = mfma32<C>(f[n], p, acc[n]);
+            if (w < 3) values(w + 1, f);
+            p = next;
         }
+        l += sum;
     };
 
     // (The buffers change hands as pointers: where the compiler sees which part of LDS a load
@@ -425,8 +482,8 @@ __device__ __forceinline__ void wide_piece(const SharedArgs& a, const Piece& pie
     for (int i = 0; i < tiles; ++i) {
         __asm__ volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(0);  // this wave's part of tile i has arrived
-        if constexpr (!F8) {
-            if (i + 1 == tiles) {
+        if constexpr (!F8 && !WHOLE) {
+            if (i == 0 || i + 1 == tiles) {
                 __asm__ volatile("" ::: "memory");
                 settle(i, cur);
                 __asm__ volatile("" ::: "memory");
@@ -464,7 +521,7 @@ template <int C, int D, bool F8, bool WHOLE>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void shared_kernel(SharedArgs a) {
     constexpr int kLds = std::max<int>(4 * kTileTokens * TileRows<D>::kBytes, kWaves * (D * 17 + 32) * 4);
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
-    // the span of this piece: the last that begins at or before it
+    // the span of this workgroup: the last that begins at or before it
     const int spans = a.groups + a.batch, id = blockIdx.x;
     if (id >= a.firsts[spans]) return;
     int before = 0;
@@ -474,21 +531,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void shared_kernel(SharedArg
         before += __popcll(here);
         if (here != ~0ull) break;
     }
-    const int span = __builtin_amdgcn_readfirstlane(before) - 1;
-    const Span s = a.spans[span];
-    Piece p;
-    p.rows = s.sequences * a.group;
-    // chunk by chunk, block of rows by block, and the heads of a token's rows side by side
-    const int blocks = static_cast<int>(blocks_of(p.rows)), in = id - s.first, at = in / a.kv_heads;
-    const int chunk = at / blocks, first_tile = s.from / kTileTokens + chunk * s.size;
-    p.kv_head = in - at * a.kv_heads;
-    p.row0 = (at - chunk * blocks) * kWideRows;
-    p.from = max(s.from, first_tile * kTileTokens);
-    p.to = static_cast<int>(min(static_cast<int64_t>(s.to), (static_cast<int64_t>(first_tile) + s.size) * kTileTokens));
-    p.seq = s.seq;
-    p.part = s.part + (static_cast<int64_t>(chunk) * a.kv_heads + p.kv_head) * p.rows;
-    if (p.rows <= kThinRows) thin_piece<C, D, F8, WHOLE>(a, p, lds);
-    else wide_piece<C, D, F8>(a, p, lds);
+    const Span s = a.spans[__builtin_amdgcn_readfirstlane(before) - 1];
+    if (s.sequences * a.group <= kThinRows) {
+        const int at = (id - s.first) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        if (at < s.pieces) thin_piece<C, D, F8, WHOLE>(a, Piece(a, s, at), lds);
+    } else {
+        wide_piece<C, D, F8, WHOLE>(a, Piece(a, s, id - s.first), lds);
+    }
 }
 
 // A row a wave: its chunks' maxima and sums first, 64 at a time, then four d a lane of as many chunks at once as lanes allow.
@@ -582,9 +631,10 @@ struct SharedSpace {
     SharedSpace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t groups) {
         const int64_t group = heads / kv_heads, all = batch * group;  // rows of a key-value head
         target = 2 * device_cus();
-        // a chunk of every span, and `target` for those that have several: the plan's chunks are at least tiles / target long
-        slots = target + kv_heads * (batch * blocks_of(group) + groups + all / kWideRows);
-        rows = target * std::min<int64_t>(kWideRows, all) + 2 * kv_heads * all;
+        // workgroups for a chunk of every span (one more where they share it out), and `target` for those that have several: the
+        // plan's chunks are at least tiles / target long, those of few rows a quarter of that
+        slots = target + kv_heads * (batch * blocks_of(group) + groups + all / kWideRows) + 2 * (batch + groups);
+        rows = target * std::max(std::min<int64_t>(kWideRows, all), kWaves * std::min<int64_t>(kThinRows, all)) + 2 * kv_heads * all;
         firsts = rup((batch + groups) * sizeof(Span), 256);
         part = firsts + rup((batch + groups + 1) * 4, 256);
         stat = part + rup(rows * dim * 4, 256);
