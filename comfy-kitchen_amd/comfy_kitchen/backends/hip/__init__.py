@@ -774,8 +774,8 @@ def _rope_write_plan(q_shape, q_stride, q_dtype, key_shape, key_stride, key_dtyp
 def paged_write_rope(q: torch.Tensor, key: torch.Tensor, value: torch.Tensor, positions: torch.Tensor, rates: torch.Tensor,
                      k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, interleaved: bool = True,
                      magnitude: float = 1.0, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
-                     keep_key: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
-    """(q', key'); key' has no tokens where it is not kept."""
+                     keep_key: bool = False) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """(q', key'); key' is None where it is not kept."""
     _same_device("paged_write_rope", q, key, value, positions, rates, k_cache, v_cache, slots)
     rest = (k_cache.shape, k_cache.stride(), k_cache.dtype, v_cache.shape, v_cache.stride(), v_cache.dtype, positions.shape[0],
             positions.dtype, slots.shape[0], slots.dtype, rates.shape[0], interleaved, magnitude)
@@ -793,10 +793,10 @@ def paged_write_rope(q: torch.Tensor, key: torch.Tensor, value: torch.Tensor, po
     if (k_scale is not None or v_scale is not None) and k_cache.dtype != torch.float8_e4m3fn:
         raise ValueError(f"paged_write_rope: k_scale and v_scale are for a cache of float8_e4m3fn, not {k_cache.dtype}")
     positions, rates, slots = positions.contiguous(), rates.contiguous(), slots.contiguous()
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    key_out = torch.empty(key.shape if keep_key else (0, *key.shape[1:]), dtype=q.dtype, device=q.device)
+    out = q.new_empty(q.shape)
+    key_out = key.new_empty(key.shape) if keep_key else None
     _launch("ckh_paged_write_rope", q, q.data_ptr(), key.data_ptr(), value.data_ptr(), positions.data_ptr(), rates.data_ptr(),
-            out.data_ptr(), key_out.data_ptr() if keep_key else None, k, v, slots.data_ptr(), _ptr(k_scale), _ptr(v_scale), *plan)
+            out.data_ptr(), _ptr(key_out), k, v, slots.data_ptr(), _ptr(k_scale), _ptr(v_scale), *plan)
     return out, key_out
 
 
@@ -844,7 +844,7 @@ def shared_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         k_scale = _scalar_on(k_scale, q.device, "k_scale")
     if v_scale is not None:
         v_scale = _scalar_on(v_scale, q.device, "v_scale")
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = q.new_empty(q.shape)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     _launch("ckh_shared_attention", q, q.data_ptr(), k, v, page_table.data_ptr(), lengths.data_ptr(), groups.data_ptr(),
             shared.data_ptr(), _ptr(k_scale), _ptr(v_scale), out.data_ptr(), *sizes, _ptr(ws), nbytes)
@@ -852,75 +852,99 @@ def shared_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 
 
 # ------------------------------------------------------------------------------- norms
-def _norm_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
-    """t [..., cols] and the elements between its rows, copied where they are not one step apart."""
-    if t.dim() > 2:
-        t = t.reshape(-1, t.shape[-1])
-    rows, cols = t.shape if t.dim() == 2 else (1, t.shape[0])
-    if cols > 1 and t.stride(-1) != 1:
-        t = t.contiguous()
-    return t, t.stride(0) if rows > 1 and t.dim() == 2 else cols
+def _row_step(shape: tuple, stride: tuple) -> int | None:
+    """The elements between the rows of [..., cols], or None where they are not one step apart (or cols not contiguous)."""
+    if 0 in shape:
+        return shape[-1]
+    *outer, last = _used_strides(shape, stride)
+    if last != 1:
+        return None
+    step, run = shape[-1], None
+    for size, s in zip(shape[-2::-1], outer[::-1]):
+        if size == 1:
+            continue
+        if run is None:
+            step, run = s, size
+        elif s != step * run:
+            return None
+        else:
+            run *= size
+    return step
 
 
-def _rms_norm(name: str, x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Tensor | None, eps: float, scale, y, scales,
-              out_rows: int, out_cols: int, mx: int) -> torch.Tensor:
-    cols = x.shape[-1]
-    rows = x.numel() // cols if cols else 0
-    h = torch.empty(x.shape if residual is not None else (0,), dtype=x.dtype, device=x.device)
-    if rows == 0 and not mx:
-        return h
-    flat, step = _norm_rows(x)
-    r_step, r = 0, residual
-    if residual is not None:
-        r, r_step = _norm_rows(residual)
-    if weight is not None:
-        weight = weight.contiguous()
-    _launch("ckh_rms_norm", x, flat.data_ptr(), _ptr(r), _ptr(weight), _ptr(scale), y.data_ptr(), _ptr(scales),
-            None if r is None else h.data_ptr(), rows, cols, out_rows, out_cols, step, r_step, eps, DTYPE_TO_CODE[x.dtype],
-            0 if weight is None else DTYPE_TO_CODE[weight.dtype], DTYPE_TO_CODE[y.dtype], mx)
-    return h
+@functools.lru_cache(maxsize=512)
+def _norm_plan(name, x_shape, x_stride, x_dtype, weight_shape, weight_dtype, residual_shape, residual_stride, residual_dtype, output_type,
+               pad_32x):
+    """The call's checks, and its sizes as the C side takes them (result's shape, scales' shape, sizes, the codes of the
+    dtypes), or None where x or the residual has to be copied."""
+    cols = x_shape[-1]
+    if weight_shape is not None and weight_shape[0] != cols:
+        raise ValueError(f"{name}: {weight_shape[0]} weights for rows of {cols}")
+    if residual_shape is not None and (residual_shape != x_shape or residual_dtype != x_dtype):
+        raise ValueError(f"{name}: x {list(x_shape)} {x_dtype} and residual {list(residual_shape)} {residual_dtype} differ")
+    if cols > 65536:
+        raise ValueError(f"{name}: rows of {cols} elements, 65536 at most")
+    rows = 1
+    for size in x_shape[:-1]:
+        rows *= size
+    mx = pad_32x is not None
+    out_rows, out_cols = (roundup(rows, 32), roundup(cols, 32)) if pad_32x else (rows, cols)
+    if mx and out_cols % 32:
+        raise ValueError(f"K dimension must be divisible by 32 (got {cols}); pass pad_32x=True")
+    x_step = _row_step(x_shape, x_stride)
+    r_step = 0 if residual_shape is None else _row_step(residual_shape, residual_stride)
+    if x_step is None or r_step is None:
+        return None
+    return ((out_rows, out_cols) if mx else x_shape, (roundup(rows, 128), roundup(out_cols // 32, 4)),
+            (rows, cols, out_rows, out_cols, x_step, r_step),
+            (DTYPE_TO_CODE[x_dtype], 0 if weight_dtype is None else DTYPE_TO_CODE[weight_dtype], DTYPE_TO_CODE[output_type], int(mx)))
 
 
-def _check_norm(name: str, x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Tensor | None) -> None:
+def _rms_norm(name: str, x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Tensor | None, eps: float,
+              scale: torch.Tensor | None, output_type: torch.dtype, pad_32x: bool | None):
+    """(result, scales or None, h or None)."""
     _same_device(name, x, weight, residual)
-    if weight is not None and weight.shape[0] != x.shape[-1]:
-        raise ValueError(f"{name}: {weight.shape[0]} weights for rows of {x.shape[-1]}")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
-        raise ValueError(f"{name}: x {list(x.shape)} {x.dtype} and residual {list(residual.shape)} {residual.dtype} differ")
-    if x.shape[-1] > 65536:
-        raise ValueError(f"{name}: rows of {x.shape[-1]} elements, 65536 at most")
+    w = (None, None) if weight is None else (weight.shape, weight.dtype)
+    r = (None, None, None) if residual is None else (residual.shape, residual.stride(), residual.dtype)
+    plan = _norm_plan(name, x.shape, x.stride(), x.dtype, *w, *r, output_type, pad_32x)
+    if plan is None:
+        x = x.contiguous()
+        if residual is not None:
+            residual = residual.contiguous()
+            r = (residual.shape, residual.stride(), residual.dtype)
+        plan = _norm_plan(name, x.shape, x.stride(), x.dtype, *w, *r, output_type, pad_32x)
+    shape, scales_shape, sizes, codes = plan
+    plain = x.is_contiguous()  # empty_like takes half of empty's time
+    same = plain and shape == x.shape
+    y = torch.empty_like(x, dtype=output_type) if same else torch.empty(shape, dtype=output_type, device=x.device)
+    scales = torch.empty(scales_shape, dtype=torch.float8_e8m0fnu, device=x.device) if codes[3] else None
+    h = None
+    if residual is not None:
+        h = torch.empty_like(x) if plain else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if sizes[0] and sizes[1]:
+        if weight is not None:
+            weight = weight.contiguous()
+        _launch("ckh_rms_norm", x, x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(scale), y.data_ptr(), _ptr(scales), _ptr(h), *sizes, eps,
+                *codes)
+    return y, scales, h
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torch.Tensor | None = None,
-             eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
-    """(y, h); h has no elements where there is no residual."""
-    _check_norm("rms_norm", x, weight, residual)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    cols = x.shape[-1]
-    rows = x.numel() // cols if cols else 0
-    return y, _rms_norm("rms_norm", x, weight, residual, eps, None, y, None, rows, cols, 0)
+             eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """(y, h); h is None where there is no residual."""
+    y, _, h = _rms_norm("rms_norm", x, weight, residual, eps, None, x.dtype, None)
+    return y, h
 
 
 def rms_norm_fp8(x: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor | None = None, residual: torch.Tensor | None = None,
-                 eps: float = 1e-6, output_type: torch.dtype = torch.float8_e4m3fn) -> tuple[torch.Tensor, torch.Tensor]:
-    _check_norm("rms_norm_fp8", x, weight, residual)
-    scale = _scalar_on(scale, x.device, "scale")
-    y = torch.empty(x.shape, dtype=output_type, device=x.device)
-    cols = x.shape[-1]
-    rows = x.numel() // cols if cols else 0
-    return y, _rms_norm("rms_norm_fp8", x, weight, residual, eps, scale, y, None, rows, cols, 0)
+                 eps: float = 1e-6, output_type: torch.dtype = torch.float8_e4m3fn) -> tuple[torch.Tensor, torch.Tensor | None]:
+    codes, _, h = _rms_norm("rms_norm_fp8", x, weight, residual, eps, _scalar_on(scale, x.device, "scale"), output_type, None)
+    return codes, h
 
 
 def rms_norm_mxfp8(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torch.Tensor | None = None, eps: float = 1e-6,
-                   pad_32x: bool = False) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    _check_norm("rms_norm_mxfp8", x, weight, residual)
-    rows, cols = x.shape
-    out_rows, out_cols = (roundup(rows, 32), roundup(cols, 32)) if pad_32x else (rows, cols)
-    if out_cols % 32:
-        raise ValueError(f"K dimension must be divisible by 32 (got {cols}); pass pad_32x=True")
-    y = torch.empty((out_rows, out_cols), dtype=torch.float8_e4m3fn, device=x.device)
-    scales = torch.empty((roundup(rows, 128), roundup(out_cols // 32, 4)), dtype=torch.float8_e8m0fnu, device=x.device)
-    return y, scales, _rms_norm("rms_norm_mxfp8", x, weight, residual, eps, None, y, scales, out_rows, out_cols, 1)
+                   pad_32x: bool = False) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    return _rms_norm("rms_norm_mxfp8", x, weight, residual, eps, None, torch.float8_e4m3fn, bool(pad_32x))
 
 
 # ---------------------------------------------------------------------------- sampling

@@ -381,9 +381,10 @@ def paged_write_rope(q: torch.Tensor, key: torch.Tensor, value: torch.Tensor, po
                      rates: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
                      interleaved: bool, magnitude: float, k_scale: torch.Tensor | None, v_scale: torch.Tensor | None,
                      keep_key: bool) -> tuple[torch.Tensor, torch.Tensor]:
-    return _dispatch("paged_write_rope", q=q, key=key, value=value, positions=positions, rates=rates, k_cache=k_cache,
-                     v_cache=v_cache, slots=slots, interleaved=interleaved, magnitude=magnitude, k_scale=k_scale,
-                     v_scale=v_scale, keep_key=keep_key)
+    turned, kept = _dispatch("paged_write_rope", q=q, key=key, value=value, positions=positions, rates=rates,
+                             k_cache=k_cache, v_cache=v_cache, slots=slots, interleaved=interleaved, magnitude=magnitude,
+                             k_scale=k_scale, v_scale=v_scale, keep_key=keep_key)
+    return turned, key.new_empty((0, *key.shape[1:])) if kept is None else kept
 
 
 @paged_write_rope.register_fake
@@ -392,10 +393,15 @@ def _(q, key, value, positions, rates, k_cache, v_cache, slots, interleaved, mag
 
 
 # ---------------------------------------------------------------- norms, sampling
+def _whole(x: torch.Tensor, *results):
+    """An op's results: a tensor of no elements in the place of a sum that was not formed."""
+    return tuple(x.new_empty(0) if r is None else r for r in results)
+
+
 @torch.library.custom_op("comfy_kitchen::rms_norm", mutates_args=())
 def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Tensor | None,
              eps: float) -> tuple[torch.Tensor, torch.Tensor]:
-    return _dispatch("rms_norm", x=x, weight=weight, residual=residual, eps=eps)
+    return _whole(x, *_dispatch("rms_norm", x=x, weight=weight, residual=residual, eps=eps))
 
 
 def _fake_sum(x, residual):
@@ -410,8 +416,8 @@ def _(x, weight, residual, eps):
 @torch.library.custom_op("comfy_kitchen::rms_norm_fp8", mutates_args=())
 def rms_norm_fp8(x: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor | None, residual: torch.Tensor | None,
                  eps: float, output_dtype_code: int) -> tuple[torch.Tensor, torch.Tensor]:
-    return _dispatch("rms_norm_fp8", x=x, scale=scale, weight=weight, residual=residual, eps=eps,
-                     output_type=DTYPE_CODE_TO_DTYPE[output_dtype_code])
+    return _whole(x, *_dispatch("rms_norm_fp8", x=x, scale=scale, weight=weight, residual=residual, eps=eps,
+                                output_type=DTYPE_CODE_TO_DTYPE[output_dtype_code]))
 
 
 @rms_norm_fp8.register_fake
@@ -422,7 +428,7 @@ def _(x, scale, weight, residual, eps, output_dtype_code):
 @torch.library.custom_op("comfy_kitchen::rms_norm_mxfp8", mutates_args=())
 def rms_norm_mxfp8(x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Tensor | None, eps: float,
                    pad_32x: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _dispatch("rms_norm_mxfp8", x=x, weight=weight, residual=residual, eps=eps, pad_32x=pad_32x)
+    return _whole(x, *_dispatch("rms_norm_mxfp8", x=x, weight=weight, residual=residual, eps=eps, pad_32x=pad_32x))
 
 
 @rms_norm_mxfp8.register_fake

@@ -5,9 +5,10 @@
 // quantize_mxfp8: bit for bit those of the two calls, without y's way through memory.
 //
 // Bound by the bytes of x, residual, h and the result.  A workgroup holds a row in its registers, so
-// every input is read once: a thread has 8 consecutive elements of every so many, the squares are summed
-// in fp32 within the thread, over the wave's lanes and over the waves in LDS.  A block of 32 that shares
-// a scale lies in four neighbouring lanes, the four blocks of a scale word in sixteen.
+// every input is read once: a thread has 8 consecutive elements of every so many.  The squares are summed
+// in fp32 in one order whatever the launch: those of 8 elements, of 64 such pieces over a wave's lanes, then of
+// these in LDS; so y does not depend on how many rows there are, on alignment, or on what becomes of it.
+// A block of 32 that shares a scale lies in four neighbouring lanes, the four blocks of a scale word in sixteen.
 #include <algorithm>
 
 #include "ckh_common.h"
@@ -92,7 +93,7 @@ __device__ __forceinline__ void write8(uint8_t* p, int left, const float (&v)[8]
 template <int C, int OUT, int N, bool VEC>
 __global__ void norm_kernel(Args a) {
     constexpr int ES = ElemSize<C>::value;
-    __shared__ float part[16];
+    __shared__ float part[128];  // of 64 pieces each
     const int threads = blockDim.x;
     int row = blockIdx.x;
     if constexpr (OUT == kMX) {
@@ -132,14 +133,20 @@ __global__ void norm_kernel(Args a) {
             }
         }
     }
-    float sum = 0.0f;
+    float squares[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+    for (int i = 0; i < N; ++i) {
+        squares[i] = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum = __fmaf_rn(v[i][e], v[i][e], sum);
+        for (int e = 0; e < 8; ++e) squares[i] = __fmaf_rn(v[i][e], v[i][e], squares[i]);
+    }
 #pragma unroll
-    for (int s = 32; s >= 1; s >>= 1) sum += __shfl_xor(sum, s, 64);
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
+    for (int s = 32; s >= 1; s >>= 1)
+#pragma unroll
+        for (int i = 0; i < N; ++i) squares[i] += __shfl_xor(squares[i], s, 64);
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int i = 0; i < N; ++i) part[(threadIdx.x + i * threads) >> 6] = squares[i];
     if (r) {
         uint8_t* h = a.h + static_cast<int64_t>(row) * a.cols * ES;
 #pragma unroll
@@ -149,8 +156,8 @@ __global__ void norm_kernel(Args a) {
         }
     }
     __syncthreads();
-    sum = part[0];
-    for (int w = 1; w < threads >> 6; ++w) sum += part[w];
+    float sum = part[0];
+    for (int w = 1; w < (a.cols + 511) >> 9; ++w) sum += part[w];
     const float f = rsqrtf(__fmaf_rn(sum, a.inv_cols, a.eps));
 
     float sc = 1.0f, inv = 1.0f;
@@ -220,7 +227,11 @@ __global__ void norm_kernel(Args a) {
 template <int C, int OUT>
 void launch(const Args& a, bool vec, hipStream_t st) {
     const int pieces = OUT == kMX ? a.scale_words * 16 : static_cast<int>(cdiv(a.cols, 8));
-    const int n = !vec ? 8 : pieces <= 512 ? 1 : pieces <= 2048 ? 2 : pieces <= 4096 ? 4 : 8;
+    // A thread's pieces.  Few rows: one, for the shortest way through a row (1 row of 5120 in bf16: 2.7 us; two 3.4).  Many: two, and
+    // four where codes are written, which leaves more rows to a CU at once (16384 rows of 5120: to bf16 113 us, one 127, four
+    // 119; to MXFP8 107, two 115).
+    const int least = a.rows < 2 * device_cus() ? 1 : OUT == kMX ? 4 : 2;
+    const int n = !vec ? 8 : std::max(least, pieces <= 1024 ? 1 : pieces <= 2048 ? 2 : pieces <= 4096 ? 4 : 8);
     const int threads = static_cast<int>(std::max<int64_t>(64, rup(cdiv(pieces, n), 64)));
     const unsigned grid = OUT == kMX ? static_cast<unsigned>(rup(cdiv(a.rows, 128), 8) * 128) : static_cast<unsigned>(a.rows);
     if (!vec) norm_kernel<C, OUT, 8, false><<<grid, threads, 0, st>>>(a);

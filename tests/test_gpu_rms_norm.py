@@ -2,8 +2,8 @@
 calls it stands for.
 
 The bound: one rounding of the result, unit |y| (bf16 2^-8, f16 2^-11, f32 2^-24), and fp32 arithmetic: the
-sum of squares is a sum of at most 64 terms in a thread and two trees of 6 and 4 levels, each 2^-24 off, the root
-and three products as many again: under 2^-17 |y| in all.  f16's results under 2^-14 have steps of 2^-24."""
+sum of squares is a sum of 8 terms, a tree of 6 levels and a sum of at most 128, each step 2^-24 off, half of which
+the root passes on, with as much again of root and products: under 2^-17 |y| in all.  f16's results under 2^-14 have steps of 2^-24."""
 import pytest
 import torch
 
@@ -118,6 +118,18 @@ def test_strides_shapes_and_weight_types(hip):
             total = (x.float() * 2).bfloat16().cpu()
             assert torch.equal(h.cpu(), total) and y.is_contiguous() and h.is_contiguous()
             check(y, total, w.cpu(), "bf16")
+
+
+@pytest.mark.parametrize("cols", [64, 1000, 4104, 5120, 9000, 20000])
+def test_a_row_alone_or_among_others(cols, hip):
+    """The same row gives the same result: among many rows, alone, and where it does not lie on 16 bytes."""
+    x, r, w = (t.cuda() for t in make(1100, cols, "bf16", cols))
+    y, h = ck.rms_norm(x, w, r)
+    off = torch.zeros(cols + 3, dtype=torch.bfloat16, device="cuda")
+    for i in (0, 7, 1099):
+        assert torch.equal(ck.rms_norm(x[i:i + 1], w, r[i:i + 1])[0], y[i:i + 1])
+        off[3:] = h[i]
+        assert torch.equal(ck.rms_norm(off[3:], w), y[i])
 
 
 def test_nothing_to_do(hip):
