@@ -1,5 +1,6 @@
 """A key-value cache held in pages: which sequence owns which page, kept on the host; the rows
-themselves are written, read and moved by `ck.paged_write`, `ck.paged_attention`, `ck.paged_copy`.
+themselves are written, read and moved by `ck.paged_write` and `ck.paged_write_rope`, `ck.paged_attention` and
+`ck.shared_attention`, `ck.paged_copy`.
 
 A sequence is a list of page numbers and a length.  Pages are shared by counting: a fork owns its
 parent's pages with it, and whoever first appends to a partly filled page that others own copies
@@ -16,6 +17,14 @@ import torch
 
 class OutOfPages(RuntimeError):
     """The cache has fewer free pages than the call needs; the cache is as it was before."""
+
+
+def _common(a: list[int], b: list[int]) -> int:
+    """With how many of the same pages both begin, up to one that was given back."""
+    most = min(len(a), len(b))
+    if a[:most] == b[:most] and -1 not in a[:most]:
+        return most
+    return next(n for n in range(most) if a[n] != b[n] or a[n] < 0)
 
 
 class _Owner:
@@ -217,10 +226,58 @@ class PagedKVCache:
 
         ck.paged_write(key, value, self.k[layer], self.v[layer], slots, self.k_scale, self.v_scale)
 
-    def attend(self, layer: int, q: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
-               scale: float | None = None, window: int = 0, sinks: int = 0) -> torch.Tensor:
-        """`ck.paged_attention` of q [B, heads, head_dim] on one layer."""
+    def write_rope(self, layer: int, q: torch.Tensor, key: torch.Tensor, value: torch.Tensor, positions: torch.Tensor,
+                   rates: torch.Tensor, slots: torch.Tensor, interleaved: bool = True, magnitude: float = 1.0,
+                   keep_key: bool = False) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+        """`write` of keys turned to their positions, and queries with them: `ck.paged_write_rope` on one layer."""
         import comfy_kitchen as ck
 
+        return ck.paged_write_rope(q, key, value, positions, rates, self.k[layer], self.v[layer], slots, interleaved,
+                                   magnitude, self.k_scale, self.v_scale, keep_key)
+
+    def groups(self, sequences: Sequence[int], least_bytes: int = 80 << 20) -> tuple[torch.Tensor, torch.Tensor] | None:
+        """(groups, shared) of the sequences in this order for `attend`, int32 on the device: neighbours that begin with the
+        same pages (forks of one sequence) are a group.  None where reading common rows once saves less than
+        `least_bytes` of K and V a layer, which is what finding them costs (4 sequences of 40 heads over 8: 24 us both ways
+        at 8192 common tokens of 16 bits, 96 MB; 18 against 15 at 2048, 38 against 83 at 32768)."""
+        owners = [self._sequences[s] for s in sequences]
+        starts, shared = [], []
+        first: list[int] = []  # the pages of the group's first sequence that all of it have
+        for i, owner in enumerate(owners):
+            same = _common(first, owner.pages) if starts else 0
+            if same:
+                members = i - starts[-1]
+                after = _common(owner.pages, owners[i + 1].pages) if i + 1 < len(owners) else 0
+                # it would cost the others more than it gains, or gains far more with those behind it
+                if members * same < (members - 1) * len(first) or (2 * same < after and members * same < after):
+                    same = 0
+            if same:
+                first = first[:same]
+            else:
+                if starts:
+                    shared.append(len(first))
+                starts.append(i)
+                first = owner.pages[:_common(owner.pages, owner.pages)]
+        if starts:
+            shared.append(len(first))
+        starts.append(len(owners))
+        tokens = [min(n * self.page_size, min(o.length for o in owners[a:b])) for n, a, b in zip(shared, starts, starts[1:])]
+        row = 2 * self.k[0, 0, 0].numel() * self.k.element_size()
+        saved = sum((b - a - 1) * n for n, a, b in zip(tokens, starts, starts[1:])) * row
+        if saved < max(least_bytes, 1):
+            return None
+        return self._on_device(starts), self._on_device(tokens)
+
+    def attend(self, layer: int, q: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+               scale: float | None = None, window: int = 0, sinks: int = 0,
+               groups: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+        """`ck.paged_attention` of q [B, heads, head_dim] on one layer, or, with what `groups` gives, `ck.shared_attention`."""
+        import comfy_kitchen as ck
+
+        if groups is not None:
+            if window:
+                raise ValueError("attend takes groups or a window, not both")
+            return ck.shared_attention(q, self.k[layer], self.v[layer], page_table, lengths, *groups, scale, self.k_scale,
+                                       self.v_scale)
         return ck.paged_attention(q, self.k[layer], self.v[layer], page_table, lengths, scale, window, sinks,
                                   self.k_scale, self.v_scale)

@@ -4,9 +4,11 @@ text-generation operators are for, in one place.
     python comfy-kitchen_amd/samples/text_generation.py        # random weights, a few tokens
 
 A prompt goes through `ck.window_attention` and leaves its keys and values in a `ck.PagedKVCache`;
-then every step runs `F.linear` on GroupInt4Layout weights (`ck.linear_int4`), `ck.apply_rope`, one
-`PagedKVCache.write` and one `PagedKVCache.attend` a layer for all sequences together.  Several
-continuations of one prompt fork its sequence instead of copying the cache.
+then every step runs, a layer and for all sequences together, `ck.rms_norm` with the residual's addition,
+`F.linear` on GroupInt4Layout weights (`ck.linear_int4`), one `PagedKVCache.write_rope` and one
+`PagedKVCache.attend`, and at its end `ck.sample_tokens`.  Several continuations of one prompt fork its
+sequence instead of copying the cache, and read what they share of it once (`PagedKVCache.groups`).
+With linears="mxfp8" the weights are TensorCoreMXFP8Layout, and the norms in front of linears write MXFP8.
 """
 from __future__ import annotations
 
@@ -20,7 +22,7 @@ import torch.nn.functional as F
 sys.path.insert(0, str(Path(__file__).resolve().parent.parent))
 
 import comfy_kitchen as ck  # noqa: E402
-from comfy_kitchen.tensor import QuantizedTensor  # noqa: E402
+from comfy_kitchen.tensor import QuantizedTensor, TensorCoreMXFP8Layout  # noqa: E402
 
 
 @dataclass(frozen=True)
@@ -34,6 +36,7 @@ class Config:
     ffn: int = 1024
     window: int = 0  # of attention; 0: none
     sinks: int = 0
+    linears: str = "int4"  # or "mxfp8"
     group_size: int = 128
     eps: float = 1e-6
     rope_base: float = 10000.0
@@ -48,16 +51,18 @@ def rope_matrices(positions: torch.Tensor, dim: int, base: float) -> torch.Tenso
 
 
 class TextDecoder:
-    """weights: a dict of [out, in] matrices and norms by name; the matrices are quantized here."""
+    """weights: a dict of [out, in] matrices and norms by name; the matrices are quantized here.
+    share_from: bytes of K and V a layer from which on what sequences share is read once (PagedKVCache.groups)."""
 
     def __init__(self, config: Config, weights: dict[str, torch.Tensor], pages: int = 256, page_size: int = 16,
-                 cache_dtype: torch.dtype | None = None, cache_scale: float | None = None):
-        self.config = config
+                 cache_dtype: torch.dtype | None = None, cache_scale: float | None = None, share_from: int = 80 << 20):
+        self.config, self.share_from = config, share_from
         self.embedding = weights["embedding"]
         dtype, device = self.embedding.dtype, self.embedding.device
-        self.weights = {name: w if name == "embedding" or w.dim() == 1 else
-                        QuantizedTensor.from_float(w, "GroupInt4Layout", group_size=config.group_size)
+        layout, how = {"int4": ("GroupInt4Layout", {"group_size": config.group_size}), "mxfp8": ("TensorCoreMXFP8Layout", {})}[config.linears]
+        self.weights = {name: w if name == "embedding" or w.dim() == 1 else QuantizedTensor.from_float(w, layout, **how)
                         for name, w in weights.items()}
+        self.rates = ck.rope_rates(config.head_dim, config.rope_base, device=device)
         self.cache = ck.PagedKVCache(config.layers, pages, page_size, config.kv_heads, config.head_dim,
                                      cache_dtype or dtype, device, cache_scale, cache_scale)
 
@@ -80,63 +85,77 @@ class TextDecoder:
             w[f"{i}.down"] = matrix(c.hidden, c.ffn)
         return w
 
-    def _norm(self, x: torch.Tensor, name: str) -> torch.Tensor:
-        y = x.float()
-        y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + self.config.eps)
-        return y.to(x.dtype) * self.weights[name]
+    def _norm(self, x: torch.Tensor, name: str, residual: torch.Tensor | None = None):
+        """What the linears behind the norm take, and the sum x + residual."""
+        w, eps = self.weights[name], self.config.eps
+        if self.config.linears == "mxfp8":
+            codes, scales, *h = ck.rms_norm_mxfp8(x, w, residual, eps, pad_32x=True)
+            params = TensorCoreMXFP8Layout.Params(scale=scales, orig_dtype=x.dtype, orig_shape=tuple(x.shape))
+            return QuantizedTensor(codes, "TensorCoreMXFP8Layout", params), h[0] if h else x
+        y = ck.rms_norm(x, w, residual, eps)
+        return (y, x) if residual is None else y
 
-    def _layers(self, x: torch.Tensor, positions: torch.Tensor, attend) -> torch.Tensor:
-        """x [T, hidden] at `positions` [T] through all layers; attend(layer, q, k, v) of [T, heads,
-        head_dim] tensors stores k and v and gives [T, heads, head_dim]."""
-        c, w = self.config, self.weights
-        freqs = rope_matrices(positions, c.head_dim, c.rope_base)[None, :, None]  # [1, T, 1, dim / 2, 2, 2]
+    def _linear(self, x: torch.Tensor, name: str) -> torch.Tensor:
+        if self.config.linears == "mxfp8" and not isinstance(x, QuantizedTensor):
+            x = QuantizedTensor.from_float(x, "TensorCoreMXFP8Layout")
+        return F.linear(x, self.weights[name])
+
+    def _layers(self, x: torch.Tensor, attend, rows: slice = slice(None)) -> torch.Tensor:
+        """x [T, hidden] through all layers: the logits behind its `rows`.  attend(layer, q, k, v) of [T, heads,
+        head_dim] tensors turns them to their positions, stores k and v and gives [T, heads, head_dim]."""
+        c = self.config
+        more = None  # what is still to be added to x
         for i in range(c.layers):
-            qkv = F.linear(self._norm(x, f"{i}.norm1"), w[f"{i}.qkv"]).unflatten(-1, (-1, c.head_dim))
+            y, x = self._norm(x, f"{i}.norm1") if more is None else self._norm(more, f"{i}.norm1", x)
+            qkv = self._linear(y, f"{i}.qkv").unflatten(-1, (-1, c.head_dim))
             q, k, v = qkv.split((c.heads, c.kv_heads, c.kv_heads), 1)
-            q, k = (t[0] for t in ck.apply_rope(q[None], k[None], freqs))
-            x = x + F.linear(attend(i, q, k, v).flatten(1), w[f"{i}.out"])
-            gate, up = F.linear(self._norm(x, f"{i}.norm2"), w[f"{i}.up"]).chunk(2, -1)
-            x = x + F.linear(F.silu(gate) * up, w[f"{i}.down"])
-        return self._norm(x, "norm")
+            y, x = self._norm(self._linear(attend(i, q, k, v).flatten(1), f"{i}.out"), f"{i}.norm2", x)
+            gate, up = self._linear(y, f"{i}.up").chunk(2, -1)
+            more = self._linear(F.silu(gate) * up, f"{i}.down")
+        y, _ = self._norm(x[rows], "norm") if more is None else self._norm(more[rows], "norm", x[rows])
+        return self._linear(y, "head")
 
     def prompt(self, tokens: torch.Tensor) -> tuple[int, torch.Tensor]:
         """A new sequence that holds `tokens` [T]: (its number, the logits behind its last token)."""
         c, n = self.config, tokens.shape[0]
         sequence = self.cache.add()
         slots = self.cache.append([sequence], n)
+        positions = torch.arange(n, device=tokens.device)
 
         def attend(layer, q, k, v):
-            self.cache.write(layer, k, v, slots)
+            q, k = self.cache.write_rope(layer, q, k, v, positions, self.rates, slots, keep_key=True)
             return ck.window_attention(q[None], k[None], v[None], c.window, c.sinks)[0]
 
-        x = self._layers(self.embedding[tokens], torch.arange(n, device=tokens.device), attend)
-        return sequence, F.linear(x[-1:], self.weights["head"])[0]
+        return sequence, self._layers(self.embedding[tokens], attend, slice(-1, None))[0]
 
     def step(self, sequences: list[int], tokens: torch.Tensor) -> torch.Tensor:
         """Append one token to each sequence: the logits behind them, [B, vocab]."""
         c = self.config
         slots = self.cache.append(sequences)
         table, lengths = self.cache.tables(sequences)
+        positions = lengths - 1
+        groups = None if c.window else self.cache.groups(sequences, self.share_from)
 
         def attend(layer, q, k, v):
-            self.cache.write(layer, k, v, slots)
-            return self.cache.attend(layer, q, table, lengths, window=c.window, sinks=c.sinks)
+            q = self.cache.write_rope(layer, q, k, v, positions, self.rates, slots)
+            return self.cache.attend(layer, q, table, lengths, window=c.window, sinks=c.sinks, groups=groups)
 
-        x = self._layers(self.embedding[tokens], lengths - 1, attend)
+        logits = self._layers(self.embedding[tokens], attend)
         if c.window:
             for s in sequences:  # pages that left the window
                 self.cache.trim(s, c.window, c.sinks)
-        return F.linear(x, self.weights["head"])
+        return logits
 
     def generate(self, tokens: torch.Tensor, steps: int, samples: int = 1, temperature: float = 1.0,
-                 generator: torch.Generator | None = None) -> torch.Tensor:
+                 generator: torch.Generator | None = None, top_k: int = 0, top_p: float = 1.0,
+                 min_p: float = 0.0) -> torch.Tensor:
         """`samples` continuations of a prompt, [samples, steps]."""
         first, logits = self.prompt(tokens)
         sequences = [first] + [self.cache.fork(first) for _ in range(samples - 1)]
         logits, out = logits.expand(samples, -1), []
+        u = torch.rand(steps, samples, device=tokens.device, generator=generator)
         for i in range(steps):
-            p = torch.softmax(logits.float() / temperature, -1)
-            out.append(torch.multinomial(p, 1, generator=generator)[:, 0])
+            out.append(ck.sample_tokens(logits, u[i], temperature, top_k, top_p, min_p))
             if i + 1 < steps:
                 logits = self.step(sequences, out[-1])
         for s in sequences:
@@ -148,7 +167,8 @@ def main() -> None:
     config = Config(window=64, sinks=4)
     model = TextDecoder(config, TextDecoder.random_weights(config))
     prompt = torch.randint(0, config.vocab, (100,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
-    out = model.generate(prompt, steps=20, samples=4, generator=torch.Generator(device="cuda").manual_seed(2))
+    out = model.generate(prompt, steps=20, samples=4, generator=torch.Generator(device="cuda").manual_seed(2), temperature=0.8,
+                         top_p=0.95)
     for row in out.tolist():
         print(*row)
 
