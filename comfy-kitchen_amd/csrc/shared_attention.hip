@@ -95,7 +95,7 @@ __device__ __forceinline__ void plan_scan(int64_t (&v)[2], int64_t (&total)[2], 
 
 template <int T>
 __global__ __launch_bounds__(T) void plan_kernel(SharedArgs a) {
-    constexpr int kSpans = T == 256 ? 256 : kMaxSpans;
+    constexpr int kSpans = T == 1024 ? kMaxSpans : T;
     __shared__ int start[kSpans + 1], common[kSpans];
     __shared__ int64_t sums[T / 64][2];
     __shared__ int top[T / 64];
@@ -623,7 +623,9 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
 
 template <int C, int D>
 void launch_shared(const SharedArgs& a, int64_t slots, bool f8, hipStream_t st) {
-    if (a.batch + a.groups <= 256) plan_kernel<256><<<1, 256, 0, st>>>(a);
+    if (a.batch + a.groups <= 64) plan_kernel<64><<<1, 64, 0, st>>>(a);
+    else if (a.batch + a.groups <= 128) plan_kernel<128><<<1, 128, 0, st>>>(a);
+    else if (a.batch + a.groups <= 256) plan_kernel<256><<<1, 256, 0, st>>>(a);
     else plan_kernel<1024><<<1, 1024, 0, st>>>(a);
     const bool whole = a.page_size % 16 == 0;
     const unsigned grid = static_cast<unsigned>(slots);
