@@ -4,8 +4,9 @@
 // and then y itself, the codes quantize_per_tensor_fp8 gives for it, or the codes and swizzled scales of
 // quantize_mxfp8: bit for bit those of the two calls, without y's way through memory.
 //
-// Bound by the bytes of x, residual, h and the result.  A workgroup holds a row in its registers, so
-// every input is read once: a thread has 8 consecutive elements of every so many.  The squares are summed
+// Bound by the bytes of x, residual, h and the result (16384 rows of 5120 with a residual, bf16: 112 us, 6.0 TB/s; to MXFP8 106;
+// 16384 rows of 5119, on no boundary of 16 bytes, 88 us without a residual for 65).  A workgroup holds a row in its registers (of
+// short rows several), so every input is read once: a thread has 8 consecutive elements of every so many.  The squares are summed
 // in fp32 in one order whatever the launch: those of 8 elements, of 64 such pieces over a wave's lanes, then of
 // these in LDS; so y does not depend on how many rows there are, on alignment, or on what becomes of it.
 // A block of 32 that shares a scale lies in four neighbouring lanes, the four blocks of a scale word in sixteen.
@@ -30,14 +31,41 @@ struct Args {
     float eps, inv_cols;
 };
 
+// 16 bytes on the boundaries of elements.
+template <int ES>
+struct __attribute__((packed, aligned(ES))) Loose {
+    uint32_t w[4];
+};
+
+template <int C>
+__device__ __forceinline__ void unpack_loose(const uint8_t* p, float (&v)[8]) {
+    if constexpr (C == CKH_F32) {
+        const auto a = *reinterpret_cast<const Loose<4>*>(p), b = *reinterpret_cast<const Loose<4>*>(p + 16);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = as_f(e < 4 ? a.w[e & 3] : b.w[e & 3]);
+    } else {
+        const auto a = *reinterpret_cast<const Loose<2>*>(p);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t h = (a.w[e >> 1] >> (16 * (e & 1))) & 0xffffu;
+            v[e] = C == CKH_BF16 ? bf16_to_f(h) : f16_to_f(h);
+        }
+    }
+}
+
 // 8 elements at p, of which those from `left` on are zeros.
 template <int C, bool VEC>
 __device__ __forceinline__ void read8(const uint8_t* p, int left, float (&v)[8]) {
     if constexpr (VEC) {
         load8<C>(p, v);
+    } else if (left >= 8) {
+        unpack_loose<C>(p, v);
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = e < left ? load1<C>(p, e) : 0.0f;
+        for (int e = 0; e < 8; ++e) {
+            const float f = load1<C>(p, min(e, left - 1));
+            v[e] = e < left ? f : 0.0f;
+        }
     }
 }
 
@@ -46,23 +74,11 @@ __device__ __forceinline__ void read_weight(const Args& a, int at, int left, flo
     if (!a.weight) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[e] = 1.0f;
-    } else if (a.weight_code == CKH_F32) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = VEC || e < left ? reinterpret_cast<const float*>(a.weight)[at + e] : 0.0f;
-    } else {
-        uint32_t b[8];
-        if constexpr (VEC) {
-            const uint4 u = *reinterpret_cast<const uint4*>(a.weight + static_cast<int64_t>(at) * 2);
-            const uint32_t d[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) b[e] = (d[e >> 1] >> (16 * (e & 1))) & 0xffffu;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) b[e] = e < left ? reinterpret_cast<const uint16_t*>(a.weight)[at + e] : 0u;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = a.weight_code == CKH_BF16 ? bf16_to_f(b[e]) : f16_to_f(b[e]);
+        return;
     }
+    if (a.weight_code == CKH_F32) read8<CKH_F32, VEC>(a.weight + static_cast<int64_t>(at) * 4, left, w);
+    else if (a.weight_code == CKH_BF16) read8<CKH_BF16, VEC>(a.weight + static_cast<int64_t>(at) * 2, left, w);
+    else read8<CKH_F16, VEC>(a.weight + static_cast<int64_t>(at) * 2, left, w);
 }
 
 template <int C>
@@ -79,13 +95,114 @@ __device__ __forceinline__ void write8(uint8_t* p, int left, const float (&v)[8]
         st_stream16(p + 16, make_uint4(as_u(v[4]), as_u(v[5]), as_u(v[6]), as_u(v[7])));
     } else if constexpr (VEC) {
         st_stream16(p, make_uint4(pack16<C>(v[0], v[1]), pack16<C>(v[2], v[3]), pack16<C>(v[4], v[5]), pack16<C>(v[6], v[7])));
+    } else if (left >= 8) {
+        if constexpr (C == CKH_F32) {
+            *reinterpret_cast<Loose<4>*>(p) = {as_u(v[0]), as_u(v[1]), as_u(v[2]), as_u(v[3])};
+            *reinterpret_cast<Loose<4>*>(p + 16) = {as_u(v[4]), as_u(v[5]), as_u(v[6]), as_u(v[7])};
+        } else {
+            *reinterpret_cast<Loose<2>*>(p) = {pack16<C>(v[0], v[1]), pack16<C>(v[2], v[3]), pack16<C>(v[4], v[5]), pack16<C>(v[6], v[7])};
+        }
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            if (e >= left) break;
+            if (e >= left) continue;
             if constexpr (C == CKH_F32) reinterpret_cast<float*>(p)[e] = v[e];
             else reinterpret_cast<uint16_t*>(p)[e] = static_cast<uint16_t>(pack16<C>(v[e], 0.0f));
         }
+    }
+}
+
+// What becomes of 8 elements v, from `at` on, of a row whose factor is f: y, or its codes.  `live`: the row and the elements are
+// there.  MXFP8: sixteen lanes have the four blocks of a scale word, `lane` is this one's place among them.
+template <int C, int OUT, bool VEC>
+__device__ __forceinline__ void emit(const Args& a, int64_t row, int at, bool live, float (&v)[8], float f, float sc, int lane) {
+    constexpr int ES = ElemSize<C>::value;
+    if (OUT != kMX && !live) return;
+    if (live) {
+        float w[8];
+        read_weight<VEC>(a, at, a.cols - at, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = round_to_hw<C>(v[e] * f * w[e]);
+    }
+    if constexpr (OUT == kSame) {
+        write8<C, VEC>(a.y + row * a.y_row + static_cast<int64_t>(at) * ES, a.cols - at, v);
+    } else if constexpr (OUT != kMX) {
+        constexpr int F = OUT == kE4M3 ? CKH_E4M3 : CKH_E5M2;
+        const float inv = round_to<C>(1.0f / sc);
+        uint8_t* y = a.y + row * a.y_row + at;
+        uint32_t code[2] = {0u, 0u};
+        float t[8];
+        bool odd = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            t[e] = round_to_hw<C>(v[e] * inv);
+            odd |= is_nan(t[e]);
+            constexpr float kMax = F == CKH_E4M3 ? 448.0f : 57344.0f;
+            t[e] = __builtin_amdgcn_fmed3f(t[e], -kMax, kMax);
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+            code[q] = F == CKH_E4M3 ? hw_e4m3x4(t[4 * q], t[4 * q + 1], t[4 * q + 2], t[4 * q + 3])
+                                    : hw_e5m2x4(t[4 * q], t[4 * q + 1], t[4 * q + 2], t[4 * q + 3]);
+        if (odd) {
+            code[0] = code[1] = 0u;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) code[e >> 2] |= quantize_one<C, F>(v[e], inv, sc) << (8 * (e & 3));
+        }
+        if constexpr (VEC) {
+            st_stream8(y, make_uint2(code[0], code[1]));
+        } else if (a.cols - at >= 8) {
+            struct __attribute__((packed, aligned(1))) Codes {
+                uint32_t w[2];
+            };
+            *reinterpret_cast<Codes*>(y) = {code[0], code[1]};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < a.cols - at) y[e] = static_cast<uint8_t>(code[e >> 2] >> (8 * (e & 3)));
+        }
+    } else {
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, as_u(v[e]) & 0x7fffffffu);
+        top = max(top, dpp<0xb1>(top));  // the neighbouring lane's, then the other pair's
+        top = max(top, dpp<0x4e>(top));
+        const bool there = row < a.rows && at < a.out_cols;
+        const uint32_t e8 = there ? mx_exponent(top) : 0u;
+        if (row < a.out_rows && at < a.out_cols)
+            *reinterpret_cast<uint2*>(a.y + row * a.out_cols + at) = there ? mx_encode8(v, top, e8) : make_uint2(0u, 0u);
+        uint32_t word = e8 << (8 * (lane >> 2));
+        word |= __shfl_xor(word, 4, 64);
+        word |= __shfl_xor(word, 8, 64);
+        if (lane == 0) a.scales[swz_offset(row, at >> 5, a.scale_words) >> 2] = word;
+    }
+}
+
+// Short rows of whole pieces: P lanes a row, 256 / P rows at once, `passes` times.  (MXFP8: 128 rows a workgroup, those
+// that share lines of scales.)
+template <int C, int OUT, int P>
+__global__ __launch_bounds__(256) void short_kernel(Args a, int passes) {
+    constexpr int ES = ElemSize<C>::value;
+    const int at = static_cast<int>(threadIdx.x % P) * 8;
+    for (int pass = 0; pass < passes; ++pass) {
+        const int64_t row = (static_cast<int64_t>(blockIdx.x) * passes + pass) * (256 / P) + threadIdx.x / P;
+        const bool live = at < a.cols && row < a.rows;
+        float v[8] = {};
+        if (live) load8<C>(a.x + row * a.x_row + at * ES, v);
+        if (a.residual && live) {
+            float u[8];
+            load8<C>(a.residual + row * a.r_row + at * ES, u);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = round_to_hw<C>(v[e] + u[e]);
+            write8<C, true>(a.h + (row * a.cols + at) * ES, 8, v);
+        }
+        float squares = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) squares = __fmaf_rn(v[e], v[e], squares);
+#pragma unroll
+        for (int s = P / 2; s >= 1; s >>= 1) squares += __shfl_xor(squares, s, 64);  // (a longer row's tree, without its zeros)
+        const float f = rsqrtf(__fmaf_rn(squares, a.inv_cols, a.eps));
+        if (OUT != kMX || at < a.scale_words * 128) emit<C, OUT, true>(a, row, at, live, v, f, OUT == kE4M3 || OUT == kE5M2 ? a.scale[0] : 1.0f, threadIdx.x & 15);
     }
 }
 
@@ -160,85 +277,50 @@ __global__ void norm_kernel(Args a) {
     for (int w = 1; w < (a.cols + 511) >> 9; ++w) sum += part[w];
     const float f = rsqrtf(__fmaf_rn(sum, a.inv_cols, a.eps));
 
-    float sc = 1.0f, inv = 1.0f;
-    if constexpr (OUT == kE4M3 || OUT == kE5M2) {
-        sc = a.scale[0];
-        inv = round_to<C>(1.0f / sc);
-    }
+    const float sc = OUT == kE4M3 || OUT == kE5M2 ? a.scale[0] : 1.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int piece = threadIdx.x + i * threads, at = piece * 8;
         const bool live = at < a.cols;
-        if (OUT != kMX && !live) continue;
-        float w[8];
-        if (live) {
-            read_weight<VEC>(a, at, a.cols - at, w);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[i][e] = round_to_hw<C>(v[i][e] * f * w[e]);
-        }
-        if constexpr (OUT == kSame) {
-            write8<C, VEC>(a.y + row * a.y_row + static_cast<int64_t>(at) * ES, a.cols - at, v[i]);
-        } else if constexpr (OUT != kMX) {
-            constexpr int F = OUT == kE4M3 ? CKH_E4M3 : CKH_E5M2;
-            uint8_t* y = a.y + row * a.y_row + at;
-            uint32_t code[2] = {0u, 0u};
-            float t[8];
-            bool odd = false;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                t[e] = round_to_hw<C>(v[i][e] * inv);
-                odd |= is_nan(t[e]);
-                constexpr float kMax = F == CKH_E4M3 ? 448.0f : 57344.0f;
-                t[e] = __builtin_amdgcn_fmed3f(t[e], -kMax, kMax);
-            }
-#pragma unroll
-            for (int q = 0; q < 2; ++q)
-                code[q] = F == CKH_E4M3 ? hw_e4m3x4(t[4 * q], t[4 * q + 1], t[4 * q + 2], t[4 * q + 3])
-                                        : hw_e5m2x4(t[4 * q], t[4 * q + 1], t[4 * q + 2], t[4 * q + 3]);
-            if (odd) {
-                code[0] = code[1] = 0u;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) code[e >> 2] |= quantize_one<C, F>(v[i][e], inv, sc) << (8 * (e & 3));
-            }
-            if constexpr (VEC) {
-                *reinterpret_cast<uint2*>(y) = make_uint2(code[0], code[1]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (e < a.cols - at) y[e] = static_cast<uint8_t>(code[e >> 2] >> (8 * (e & 3)));
-            }
-        } else {
-            if (piece >= a.scale_words * 16) continue;  // whole groups of sixteen lanes
-            uint32_t top = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) top = max(top, as_u(v[i][e]) & 0x7fffffffu);
-            top = max(top, dpp<0xb1>(top));  // the neighbouring lane's, then the other pair's
-            top = max(top, dpp<0x4e>(top));
-            const uint32_t e8 = at < a.out_cols ? mx_exponent(top) : 0u;
-            if (at < a.out_cols) *reinterpret_cast<uint2*>(a.y + static_cast<int64_t>(row) * a.out_cols + at) = mx_encode8(v[i], top, e8);
-            uint32_t word = e8 << (8 * ((threadIdx.x & 15) >> 2));
-            word |= __shfl_xor(word, 4, 64);
-            word |= __shfl_xor(word, 8, 64);
-            if ((threadIdx.x & 15) == 0) a.scales[swz_offset(row, piece >> 2, a.scale_words) >> 2] = word;
-        }
+        if (OUT == kMX && piece >= a.scale_words * 16) continue;  // whole groups of sixteen lanes
+        emit<C, OUT, VEC>(a, row, at, live, v[i], f, sc, threadIdx.x & 15);
     }
+}
+
+template <int C, int OUT, bool VEC>
+void launch_rows(const Args& a, hipStream_t st) {
+    const int pieces = OUT == kMX ? a.scale_words * 16 : static_cast<int>(cdiv(a.cols, 8));
+    // A thread's pieces.  Few rows: one, for the shortest way through a row (1 row of 5120 in bf16: 2.7 us; two 3.4).  Many: two, and
+    // four where codes are written, which leaves more rows to a CU at once, as long as every lane has some (16384 rows of 5120: to bf16
+    // 113 us, one 127, four 119; to MXFP8 107, two 115; replayed, to E4M3 60 us, two 73; 110000 rows of 1024 to E4M3, two 79 us, four 85).
+    const int least = a.rows < 2 * device_cus() ? 1 : std::min(OUT != kSame ? 4 : 2, std::max(1, pieces / 64));
+    const int n = std::max(least, pieces <= 1024 ? 1 : pieces <= 2048 ? 2 : pieces <= 4096 ? 4 : 8);
+    const int threads = static_cast<int>(std::max<int64_t>(64, rup(cdiv(pieces, n), 64)));
+    const unsigned grid = OUT == kMX ? static_cast<unsigned>(rup(cdiv(a.rows, 128), 8) * 128) : static_cast<unsigned>(a.rows);
+    if (n == 1) norm_kernel<C, OUT, 1, VEC><<<grid, threads, 0, st>>>(a);
+    else if (n == 2) norm_kernel<C, OUT, 2, VEC><<<grid, threads, 0, st>>>(a);
+    else if (n == 4) norm_kernel<C, OUT, 4, VEC><<<grid, threads, 0, st>>>(a);
+    else norm_kernel<C, OUT, 8, VEC><<<grid, threads, 0, st>>>(a);
+}
+
+template <int C, int OUT, int P>
+void launch_short(const Args& a, hipStream_t st) {
+    const int passes = OUT == kMX ? 128 * P / 256 : 1;
+    const unsigned grid = static_cast<unsigned>(cdiv(a.rows, 256 / P * passes));
+    short_kernel<C, OUT, P><<<grid, 256, 0, st>>>(a, passes);
 }
 
 template <int C, int OUT>
 void launch(const Args& a, bool vec, hipStream_t st) {
     const int pieces = OUT == kMX ? a.scale_words * 16 : static_cast<int>(cdiv(a.cols, 8));
-    // A thread's pieces.  Few rows: one, for the shortest way through a row (1 row of 5120 in bf16: 2.7 us; two 3.4).  Many: two, and
-    // four where codes are written, which leaves more rows to a CU at once (16384 rows of 5120: to bf16 113 us, one 127, four
-    // 119; to MXFP8 107, two 115).
-    const int least = a.rows < 2 * device_cus() ? 1 : OUT == kMX ? 4 : 2;
-    const int n = !vec ? 8 : std::max(least, pieces <= 1024 ? 1 : pieces <= 2048 ? 2 : pieces <= 4096 ? 4 : 8);
-    const int threads = static_cast<int>(std::max<int64_t>(64, rup(cdiv(pieces, n), 64)));
-    const unsigned grid = OUT == kMX ? static_cast<unsigned>(rup(cdiv(a.rows, 128), 8) * 128) : static_cast<unsigned>(a.rows);
-    if (!vec) norm_kernel<C, OUT, 8, false><<<grid, threads, 0, st>>>(a);
-    else if (n == 1) norm_kernel<C, OUT, 1, true><<<grid, threads, 0, st>>>(a);
-    else if (n == 2) norm_kernel<C, OUT, 2, true><<<grid, threads, 0, st>>>(a);
-    else if (n == 4) norm_kernel<C, OUT, 4, true><<<grid, threads, 0, st>>>(a);
-    else norm_kernel<C, OUT, 8, true><<<grid, threads, 0, st>>>(a);
+    if (!vec) launch_rows<C, OUT, false>(a, st);
+    // Many short rows: a workgroup each is a matter of launching them (replayed, bf16: 900001 rows of 128 258 us, here 92; 450000 of
+    // 256 142 and 86; 220000 of 512 86 and 83, to MXFP8 95 and 85), and few of them have a place each anyway.
+    else if (pieces > 64 || a.rows < 8 * device_cus()) launch_rows<C, OUT, true>(a, st);
+    else if (OUT != kMX && pieces <= 8) launch_short<C, OUT, 8>(a, st);
+    else if (pieces <= 16) launch_short<C, OUT, 16>(a, st);
+    else if (pieces <= 32) launch_short<C, OUT, 32>(a, st);
+    else launch_short<C, OUT, 64>(a, st);
 }
 
 template <int C>

@@ -16,8 +16,9 @@
 //     the places in them: one wave where there are at most 64, else by counting over ever narrower ranges of
 //     (logit, number).  Bins that do not fit LDS are narrowed over the row in memory.
 // What bounds them: the first, instructions and LDS atomics, 18 of 64 bits for a logit (256 rows of 128000 in f32, 131 MB:
-// 29 us); the second, one CU's loads and instructions for a row, and some 8 us of steps that wait for each other (41 us of
-// that case; 64 rows of 150001 in bf16: 12 + 27; one row of 32000: 4.4 + 12.8).
+// 29 us); the second, one CU's loads and instructions for a row, and some 8 us of steps that wait for each other (40 us of
+// that case; 64 rows of 150001 in bf16: 12 + 26; one row of 32000: 4.4 + 12.6).  A row of the second by several workgroups
+// would need a launch more, or workgroups that wait for each other, for less than the 8 us that stay.
 //
 // A weight is a 32-bit fixed-point number relative to its bin's upper end, taken from the logit in 64 bits;
 // sums of them are whole numbers, so they do not depend on the order in which atomics add them.  The
@@ -34,7 +35,7 @@ constexpr int kChunk = 8192;      // logits of a workgroup of the first launch
 constexpr int kFirst = 512;       // its threads
 constexpr int kThreads = 512;     // of the second launch's workgroup
 constexpr int kList = 4096;       // logits that it holds
-constexpr int kQueue = 3072;      // 16-byte pieces of the row that it looks at twice
+constexpr int kQueue = 3008;      // 16-byte pieces of the row that it looks at twice
 constexpr int kSubBits = 9, kSub = 1 << kSubBits;  // ranges that it counts by
 static_assert(kSub == kThreads && kBins <= kThreads, "a range and a bin a thread");
 constexpr int kMaxChunks = 2048;

@@ -10,12 +10,21 @@
 //   - A small first launch turns lengths and groups, which only the device knows, into a list of pieces of work: a
 //     span's tokens in chunks of one size for the whole call, chosen so that there are about two a CU,
 //     times its blocks of 128 rows and the key-value heads.
-//   - The second works on one piece a workgroup, as prompts are (attn.h): a wave owns 32 rows, the columns of
-//     32x32x16 MFMAs, with running maximum and sum; tiles of 64 tokens go to LDS, the next while this
-//     one is used, each token's row found by its page, which is looked up a tile before.  A 16-bit cache goes there
-//     without passing registers; E4M3 codes are widened on the way, once for all rows.
+//   - The second works on one piece a workgroup.  Spans of up to 16 rows (a sequence's own tokens, mostly) are read
+//     by the wave, each wave its own tiles, as ckh_paged_attention does (paged_tiles.h).  Wider ones go as prompts do:
+//     a wave owns 32 rows, the columns of 32x32x16 MFMAs, with running maximum and sum; tiles of 64 tokens go to
+//     LDS, the next while this one is used, each token's row found by its page, which is looked up a tile before.  A
+//     16-bit cache goes there without passing registers; E4M3 codes are widened on the way, once for all rows.
 //   - The third joins each row's chunks, those of its group and its own, in their order: results do not
 //     depend on timing.
+//
+// Measured: 64 sequences of 40 heads on 8 over a common 16384 tokens and 1 .. 512 of their own, D 128, E4M3 pages: 4.5 +
+// 48 + 8 us, 0.46 PF of the 22 GF; the wide pieces alone run at some 1 PF, and what is lost stands at the thin pieces,
+// which follow them, and in 480 pieces on 256 CUs.  Six groups of 12 sequences of 24 heads on 24 over 9001 and 700, D 64, f16:
+// 4.5 + 86 + 5, 4.2 TB/s (rows of 128 bytes: ckh_paged_attention reads such a cache at the same rate).  Eight sequences
+// and less: 20 us, of which 12 are steps that wait for each other.
+// Against ckh_paged_attention over the same cache: 64 sequences over a common 16384 tokens in bf16, 76 us for 575;
+// 16 over 8192, 27 for 52; 4 over 8192, 24 for 23.  It pays from some 80 MB of keys and values that are not read again.
 #include <algorithm>
 
 #include "paged_tiles.h"
@@ -404,6 +413,13 @@ __device__ __forceinline__ void wide_piece(const SharedArgs& a, const Piece& pie
                 const uint8_t* kr = kt + t * R::kBytes;
                 s[h] = mfma32<C>(*reinterpret_cast<const v4u*>(kr + (((2 * n + g) ^ R::k_swizzle(t)) << 4)), q[n], s[h]);
             }
+        // two steps' keys are read ahead of the products (left to the compiler: 64 spans of 16 rows over a prefix of 4096, 46.3 us instead of 44.8)
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);  // LDS reads
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);  // products
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
         const int t0 = first + i * kTileTokens;
         if (t0 < from || t0 + kTileTokens > to) {
             const int low = from - t0 - 4 * g, high = to - t0 - 4 * g;

@@ -182,3 +182,29 @@ def test_refusals(hip):
         ck.rms_norm_mxfp8(x[0])
     with pytest.raises(ck.NoCapableBackendError):
         ck.rms_norm(x.cpu())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows,cols", [(2048, 8), (2049, 64), (4099, 72), (3001, 96), (9001, 128), (2500, 136), (2177, 200), (4096, 256)])
+def test_many_short_rows(rows, cols, dtype, hip):
+    """A head's norm: the same bits as a few rows at a time, in 8 bits as the two calls."""
+    x, r, w = make(rows, cols, dtype, rows * cols + 3)
+    x[7], r[7], x[11, 3] = 0, 0, float("nan")
+    keep = torch.arange(rows) != 11
+    xc, rc, wc = x.cuda(), r.cuda(), w.cuda()
+    y, h = ck.rms_norm(xc, wc, rc)
+    total = (x.float() + r.float()).to(x.dtype)
+    assert torch.equal(bits(h[keep]), bits(total[keep])) and bool(h[11, 3].isnan()) and bool(y[11].isnan().all())
+    check(y.cpu()[keep], total[keep], w, dtype)
+    plain = ck.rms_norm(xc)
+    check(plain.cpu()[keep], x[keep], None, dtype)
+    for i in range(0, rows, 1000):
+        a, b = ck.rms_norm(xc[i:i + 1000], wc, rc[i:i + 1000])
+        assert torch.equal(bits(y[i:i + 1000]), bits(a)) and torch.equal(bits(h[i:i + 1000]), bits(b))
+    scale = torch.tensor(0.02, device="cuda")
+    for out in (torch.float8_e4m3fn, torch.float8_e5m2):
+        codes, h8 = ck.rms_norm_fp8(xc, scale, wc, rc, output_type=out)
+        assert torch.equal(bits(codes), bits(ck.quantize_per_tensor_fp8(y, scale, out))) and torch.equal(bits(h), bits(h8))
+    codes, scales, h8 = ck.rms_norm_mxfp8(xc, wc, rc, pad_32x=True)
+    q, s = ck.quantize_mxfp8(y, pad_32x=True)
+    assert torch.equal(bits(h), bits(h8)) and torch.equal(bits(codes), bits(q)) and torch.equal(bits(scales), bits(s))
