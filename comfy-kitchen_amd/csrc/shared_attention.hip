@@ -72,7 +72,8 @@ struct SharedArgs {
     FastDiv by_page, by_group;
 };
 
-// Blocks of rows.
+// Blocks of rows.  (16 rows by the wave: 16 groups of two sequences of 8 heads to a key-value head, D 128, bf16, 128 us and 158 by the
+// workgroup's 128; one such group over 32768 tokens 43 and 36.)
 __host__ __device__ __forceinline__ int64_t blocks_of(int64_t rows) {
     return rows <= kThinRows ? (rows > 0) : (rows + kWideRows - 1) / kWideRows;
 }
@@ -639,10 +640,12 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
 
 template <int C, int D>
 void launch_shared(const SharedArgs& a, int64_t slots, bool f8, hipStream_t st) {
+    // A span a thread, and barriers only where there are several waves (5 spans: 3.8 us by one wave, 4.8 by sixteen).
     if (a.batch + a.groups <= 64) plan_kernel<64><<<1, 64, 0, st>>>(a);
     else if (a.batch + a.groups <= 128) plan_kernel<128><<<1, 128, 0, st>>>(a);
     else if (a.batch + a.groups <= 256) plan_kernel<256><<<1, 256, 0, st>>>(a);
     else plan_kernel<1024><<<1, 1024, 0, st>>>(a);
+    // 16 tokens lie on one page (64 sequences over a common 16384 in bf16, pages of 64: 53 us; of 72: 59).
     const bool whole = a.page_size % 16 == 0;
     const unsigned grid = static_cast<unsigned>(slots);
     if (f8 && whole) shared_kernel<C, D, true, true><<<grid, 256, 0, st>>>(a);
