@@ -402,7 +402,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: float | to
                   top_k: int | torch.Tensor = 0, top_p: float | torch.Tensor = 1.0,
                   min_p: float | torch.Tensor = 0.0) -> torch.Tensor:
     """The next token of each row of logits [B, vocab] (f32 / f16 / bf16), int64 [B], drawn with the random
-    numbers u (fp32 [B], 0 <= u < 1): the same inputs give the same tokens.
+    numbers u (fp32 [B], 0 <= u < 1; others count as the nearest of these, NaN as 0): the same inputs give the same
+    tokens.
 
     Tokens stand in the order of their logits, the largest first, equal ones by number, and weigh
     w = exp((logit - max) / temperature).  Kept are those that are among the first top_k (0: all), and of these

@@ -355,6 +355,9 @@ extern "C" int ckh_rms_norm(const void* x, const void* residual, const void* wei
                     static_cast<long long>(out_cols), static_cast<long long>(rows), static_cast<long long>(cols));
     else
         CKH_REQUIRE(out_rows == rows && out_cols == cols, "rms_norm: only MXFP8 codes are padded");
+    // (a launch's threads are counted in 32 bits)
+    CKH_REQUIRE(rup(rows, 1024) * rup(cdiv(out_cols, 8), 64) <= UINT32_MAX, "rms_norm: too many elements (%lld rows of %lld)",
+                static_cast<long long>(rows), static_cast<long long>(cols));
     if (rows == 0 || cols == 0) return CKH_OK;
     const int es = x_code == CKH_F32 ? 4 : 2;
     const norm::Out out = mx ? norm::kMX : out_code == CKH_E4M3 ? norm::kE4M3 : out_code == CKH_E5M2 ? norm::kE5M2 : norm::kSame;

@@ -627,7 +627,7 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(Args a) {
     const int top_k = a.top_k_of(row);
     const double top_p = a.top_p ? a.top_p[row] : a.top_p_all;
     const double min_p = fmin(a.min_p ? a.min_p[row] : a.min_p_all, 1.0);
-    const double u = fmin(fmax(static_cast<double>(a.u[row]), 0.0), 1.0 - 0x1p-25);
+    const double u = fmin(fmax(static_cast<double>(a.u[row]), 0.0), 1.0 - 0x1p-24);  // (fp32 numbers, 0 <= u < 1)
     const bool by_p = top_p < 1.0, by_min = min_p > 0.0;
     if (threadIdx.x < 64) {
         // running sums

@@ -45,6 +45,8 @@ def test_rms_norm(lib, mem):
                          (dict(out=5, mx=1, scales=p, y=p + 4), "misaligned"), (dict(step=-64), "negative stride")):
         refused(lib, call(**kwargs), text)
     assert call(rows=0, out_rows=0, x=None) == 0 and call(cols=0, out_cols=0, x=None) == 0
+    for rows, cols in ((1 << 26, 8), (1 << 26, 7), (1 << 19, 65536)):
+        refused(lib, call(rows=rows, out_rows=rows, cols=cols, out_cols=cols, step=cols), "too many elements")
 
 
 def test_paged_write_rope(lib, mem):
