@@ -41,8 +41,9 @@ typedef __attribute__((address_space(3))) v4s lds_v4s;
 constexpr int kTileTokens = 64;
 constexpr int kWideRows = 128;  // of a piece
 constexpr int kThinRows = 16;
-constexpr int kMinTiles = 4;    // of a chunk, where a span has several
-constexpr int kMinThinTiles = 2;
+constexpr int kMinTiles = 2;    // of a chunk, where a span has several
+constexpr int kMinThinTiles = 1;
+constexpr int kThinChunks = 8;  // of few rows, for one of many
 constexpr int kMaxSpans = 4096; // sequences and groups of a call
 
 struct Span {
@@ -190,7 +191,7 @@ __global__ __launch_bounds__(T) void plan_kernel(SharedArgs a) {
             s = i0 == 0 ? held : span(i0 + t);
             // a workgroup works on one block of many rows, or on the few rows of kWaves chunks or heads
             const bool thin = rows_of(s) <= kThinRows;
-            s.size = static_cast<int>(thin ? max((size + kWaves - 1) / kWaves, static_cast<int64_t>(kMinThinTiles)) : size);
+            s.size = static_cast<int>(thin ? max((size + kThinChunks - 1) / kThinChunks, static_cast<int64_t>(kMinThinTiles)) : size);
             s.chunks = (tiles_of(s) + s.size - 1) / s.size;
             n[0] = s.chunks * blocks_of(rows_of(s)) * a.kv_heads;
             s.pieces = static_cast<int>(n[0]);
@@ -673,9 +674,9 @@ struct SharedSpace {
         const int64_t group = heads / kv_heads, all = batch * group;  // rows of a key-value head
         target = 2 * device_cus();
         // workgroups for a chunk of every span (one more where they share it out), and `target` for those that have several: the
-        // plan's chunks are at least tiles / target long, those of few rows a quarter of that
-        slots = target + kv_heads * (batch * blocks_of(group) + groups + all / kWideRows) + 2 * (batch + groups);
-        rows = target * std::max(std::min<int64_t>(kWideRows, all), kWaves * std::min<int64_t>(kThinRows, all)) + 2 * kv_heads * all;
+        // plan's chunks are at least tiles / target long, those of few rows, one a wave, a part of that
+        slots = std::max(1, kThinChunks / kWaves) * target + kv_heads * (batch * blocks_of(group) + groups + all / kWideRows) + 2 * (batch + groups);
+        rows = target * std::max(std::min<int64_t>(kWideRows, all), kThinChunks * std::min<int64_t>(kThinRows, all)) + 2 * kv_heads * all;
         firsts = rup((batch + groups) * sizeof(Span), 256);
         part = firsts + rup((batch + groups + 1) * 4, 256);
         stat = part + rup(rows * dim * 4, 256);
