@@ -19,12 +19,12 @@
 //     depend on timing.
 //
 // Measured: 64 sequences of 40 heads on 8 over a common 16384 tokens and 1 .. 512 of their own, D 128, E4M3 pages: 4.5 +
-// 48 + 8 us, 0.46 PF of the 22 GF; the wide pieces alone run at some 1 PF, and what is lost stands at the thin pieces,
-// which follow them, and in 480 pieces on 256 CUs.  Six groups of 12 sequences of 24 heads on 24 over 9001 and 700, D 64, f16:
-// 4.5 + 86 + 5, 4.2 TB/s (rows of 128 bytes: ckh_paged_attention reads such a cache at the same rate).  Eight sequences
-// and less: 20 us, of which 12 are steps that wait for each other.
-// Against ckh_paged_attention over the same cache: 64 sequences over a common 16384 tokens in bf16, 76 us for 575;
-// 16 over 8192, 27 for 52; 4 over 8192, 24 for 23.  It pays from some 80 MB of keys and values that are not read again.
+// 48 + 8 us, 0.46 PF of the 22 GF (bf16 pages: 56 us in all); a tile's products, exponentials and LDS reads take a third of
+// its time each, two workgroups a CU overlap them in part, and 480 pieces on 256 CUs leave some idle.  Six groups of 12
+// sequences of 24 heads on 24 over 9001 and 700, D 64, f16: 4.5 + 86 + 5, 4.2 TB/s (rows of 128 bytes: ckh_paged_attention
+// reads such a cache at the same rate).  Eight sequences and less: 16 us, of which 8 are steps that wait for each other.
+// Against ckh_paged_attention over the same cache: 64 sequences over a common 32768 tokens in bf16, 73 us for 575;
+// 16 over 8192, 27 for 52; 4 over 8192, 24 for 25; 4 over 2048, 18 for 15.  It pays from some 80 MB of keys and values that are not read again.
 #include <algorithm>
 
 #include "paged_tiles.h"
@@ -42,8 +42,9 @@ constexpr int kTileTokens = 64;
 constexpr int kWideRows = 128;  // of a piece
 constexpr int kThinRows = 16;
 constexpr int kMinTiles = 2;    // of a chunk, where a span has several
-constexpr int kMinThinTiles = 1;
-constexpr int kThinChunks = 8;  // of few rows, for one of many
+constexpr int kMinThinTiles = 1;  // (4 sequences over 777 and 100: 16.7 us; of 4 and 2 tiles 19.7)
+constexpr int kThinChunks = 8;  // of few rows, for one of many: they follow these and end the launch (64 sequences over a common 16384
+                                // and 512 of their own in bf16: 56 us; 4: 68, 16: 58)
 constexpr int kMaxSpans = 4096; // sequences and groups of a call
 
 struct Span {
@@ -672,7 +673,7 @@ struct SharedSpace {
     int64_t target, slots, rows, firsts, part, stat, bytes;  // slots: pieces of work at most; rows: of partial results
     SharedSpace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t groups) {
         const int64_t group = heads / kv_heads, all = batch * group;  // rows of a key-value head
-        target = 2 * device_cus();
+        target = 2 * device_cus();  // (64 over 16384 and 512, bf16: 56 us; one a CU 64, three 63)
         // workgroups for a chunk of every span (one more where they share it out), and `target` for those that have several: the
         // plan's chunks are at least tiles / target long, those of few rows, one a wave, a part of that
         slots = std::max(1, kThinChunks / kWaves) * target + kv_heads * (batch * blocks_of(group) + groups + all / kWideRows) + 2 * (batch + groups);
