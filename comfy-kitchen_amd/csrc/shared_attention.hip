@@ -671,13 +671,18 @@ void launch_shared(int dim, const SharedArgs& a, int64_t slots, bool f8, hipStre
 // Places in the workspace.
 struct SharedSpace {
     int64_t target, slots, rows, firsts, part, stat, bytes;  // slots: pieces of work at most; rows: of partial results
-    SharedSpace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t groups) {
+    SharedSpace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t groups, int64_t capacity) {
         const int64_t group = heads / kv_heads, all = batch * group;  // rows of a key-value head
+        const int64_t tiles = cdiv(capacity, kTileTokens);            // of a span
         target = 2 * device_cus();  // (64 over 16384 and 512, bf16: 56 us; one a CU 64, three 63)
         // workgroups for a chunk of every span (one more where they share it out), and `target` for those that have several: the
         // plan's chunks are at least tiles / target long, those of few rows, one a wave, a part of that
         slots = std::max(1, kThinChunks / kWaves) * target + kv_heads * (batch * blocks_of(group) + groups + all / kWideRows) + 2 * (batch + groups);
         rows = target * std::max(std::min<int64_t>(kWideRows, all), kThinChunks * std::min<int64_t>(kThinRows, all)) + 2 * kv_heads * all;
+        // nor are there more chunks than tiles
+        const int64_t own = group <= kThinRows ? cdiv(tiles * kv_heads, kWaves) : tiles * kv_heads * blocks_of(group);
+        slots = std::max<int64_t>(std::min(slots, batch * own + tiles * kv_heads * (groups + all / kWideRows)), 1);
+        rows = std::min(rows, 2 * kv_heads * all * tiles);
         firsts = rup((batch + groups) * sizeof(Span), 256);
         part = firsts + rup((batch + groups + 1) * 4, 256);
         stat = part + rup(rows * dim * 4, 256);
@@ -693,7 +698,7 @@ using namespace ckh;
 extern "C" int64_t ckh_shared_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t groups,
                                                         int64_t page_size, int64_t max_pages) {
     if (batch <= 0 || kv_heads <= 0 || heads < kv_heads || dim <= 0 || groups < 0 || page_size <= 0 || max_pages < 0) return 0;
-    return attn::SharedSpace(batch, heads, kv_heads, dim, groups).bytes;
+    return attn::SharedSpace(batch, heads, kv_heads, dim, groups, max_pages * page_size).bytes;
 }
 
 extern "C" int ckh_shared_attention(const void* q, const void* k_cache, const void* v_cache, const void* page_table,
@@ -730,7 +735,7 @@ extern "C" int ckh_shared_attention(const void* q, const void* k_cache, const vo
                     aligned(lengths, 4) && aligned(group_starts, 4) && aligned(shared, 4) && aligned(k_scale, 4) && aligned(v_scale, 4) &&
                     aligned(workspace, 16),
                 "shared_attention: misaligned pointer");
-    const attn::SharedSpace space(batch, heads, kv_heads, dim, groups);
+    const attn::SharedSpace space(batch, heads, kv_heads, dim, groups, max_pages * page_size);
     CKH_REQUIRE(space.slots <= (1 << 24), "shared_attention: too many heads and sequences");
     CKH_REQUIRE(workspace_bytes >= space.bytes, "shared_attention: a workspace of %lld bytes, needs %lld",
                 static_cast<long long>(workspace_bytes), static_cast<long long>(space.bytes));

@@ -106,6 +106,16 @@ def test_shared_attention(lib, mem):
     assert f(0, 8, 8, 128, 1, 16, 8) == 0 < f(1, 8, 8, 128, 0, 16, 8) and f(4, 8, 0, 128, 1, 16, 8) == 0
 
 
+def test_shared_attention_workspace(lib):
+    """No more than the tables' tokens need, nor than a long context's chunks do."""
+    small = lib.ckh_shared_attention_workspace_bytes(4, 40, 8, 128, 1, 16, 55)
+    assert small < 4 << 20
+    sizes = [lib.ckh_shared_attention_workspace_bytes(4, 40, 8, 128, 1, 16, n) for n in (1, 55, 1000, 10 ** 5, 10 ** 7)]
+    assert sizes == sorted(sizes) and sizes[-1] == sizes[-2] < 64 << 20
+    for tokens in (0, 1, 63, 64, 65):
+        assert lib.ckh_shared_attention_workspace_bytes(1, 1, 1, 64, 0, 1, tokens) > 0
+
+
 def test_rope_rates():
     plain = ck.rope_rates(64, 10000.0, device="cpu")
     assert plain.dtype == torch.float32 and plain.shape == (32,)
