@@ -326,7 +326,7 @@ def shared_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     its shortest sequence holds, that many).  PagedKVCache.groups gives both.  All else, and the result, as for
     paged_attention.
     It pays where some 80 MB of keys and values are not read again: 64 sequences of 40 heads over 8 on a common 32768
-    tokens of 16 bits take 73 us for 575, four on 8192 24 for 25, on 2048 18 for 15.
+    tokens of 16 bits take 73 us for 575, four on 8192 22 for 23, on 2048 16 for 15.
     At most 4096 sequences and groups together."""
     if (direct(q, k_cache, v_cache, page_table, lengths, groups, shared, k_scale, v_scale)
             and untouched("shared_attention")):

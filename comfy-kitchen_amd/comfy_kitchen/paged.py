@@ -238,8 +238,8 @@ class PagedKVCache:
     def groups(self, sequences: Sequence[int], least_bytes: int = 80 << 20) -> tuple[torch.Tensor, torch.Tensor] | None:
         """(groups, shared) of the sequences in this order for `attend`, int32 on the device: neighbours that begin with the
         same pages (forks of one sequence) are a group.  None where reading common rows once saves less than
-        `least_bytes` of K and V a layer, which is what finding them costs (4 sequences of 40 heads over 8: 24 us for 25
-        at 8192 common tokens of 16 bits, 96 MB; 18 for 15 at 2048, 36 for 83 at 32768)."""
+        `least_bytes` of K and V a layer, which is what finding them costs (4 sequences of 40 heads over 8: 22 us for 23
+        at 8192 common tokens of 16 bits, 96 MB; 16 for 15 at 2048, 36 for 83 at 32768)."""
         owners = [self._sequences[s] for s in sequences]
         starts, shared = [], []
         first: list[int] = []  # the pages of the group's first sequence that all of it have

@@ -7,9 +7,9 @@
 // lies behind it, seen by one.  Its rows are these sequences' query heads of a key-value head; so the common
 // tokens are a matrix product of many rows, read once for each 128 of them, and bound by the matrix units
 // from some 300 rows on, by HBM below.
-//   - A small first launch turns lengths and groups, which only the device knows, into a list of pieces of work: a
-//     span's tokens in chunks of one size for the whole call, chosen so that there are about two a CU,
-//     times its blocks of 128 rows and the key-value heads.
+//   - A small first launch (of a small call, every workgroup for itself) turns lengths and groups, which only the device
+//     knows, into a list of pieces of work: a span's tokens in chunks of one size for the whole call, chosen so that there
+//     are about two a CU, times its blocks of 128 rows and the key-value heads.
 //   - The second works on one piece a workgroup.  Spans of up to 16 rows (a sequence's own tokens, mostly) are read
 //     by the wave, each wave its own tiles, as ckh_paged_attention does (paged_tiles.h).  Wider ones go as prompts do:
 //     a wave owns 32 rows, the columns of 32x32x16 MFMAs, with running maximum and sum; tiles of 64 tokens go to
@@ -22,9 +22,10 @@
 // 48 + 8 us, 0.46 PF of the 22 GF (bf16 pages: 56 us in all); a tile's products, exponentials and LDS reads take a third of
 // its time each, two workgroups a CU overlap them in part, and 480 pieces on 256 CUs leave some idle.  Six groups of 12
 // sequences of 24 heads on 24 over 9001 and 700, D 64, f16: 4.5 + 86 + 5, 4.2 TB/s (rows of 128 bytes: ckh_paged_attention
-// reads such a cache at the same rate).  Eight sequences and less: 16 us, of which 8 are steps that wait for each other.
+// reads such a cache at the same rate).  Four sequences over 777 and 100: 11 + 4 us, nearly all of it steps that wait for
+// each other.
 // Against ckh_paged_attention over the same cache: 64 sequences over a common 32768 tokens in bf16, 73 us for 575;
-// 16 over 8192, 27 for 52; 4 over 8192, 24 for 25; 4 over 2048, 18 for 15.  It pays from some 80 MB of keys and values that are not read again.
+// 16 over 8192, 27 for 52; 4 over 8192, 22 for 23; 4 over 2048, 16 for 15.  It pays from some 80 MB of keys and values that are not read again.
 #include <algorithm>
 
 #include "paged_tiles.h"
@@ -42,7 +43,7 @@ constexpr int kTileTokens = 64;
 constexpr int kWideRows = 128;  // of a piece
 constexpr int kThinRows = 16;
 constexpr int kMinTiles = 2;    // of a chunk, where a span has several
-constexpr int kMinThinTiles = 1;  // (4 sequences over 777 and 100: 16.7 us; of 4 and 2 tiles 19.7)
+constexpr int kMinThinTiles = 1;  // (4 sequences over 777 and 100, replayed: 16.7 us; of 4 and 2 tiles 19.7)
 constexpr int kThinChunks = 8;  // of few rows, for one of many: they follow these and end the launch (64 sequences over a common 16384
                                 // and 512 of their own in bf16: 56 us; 4: 68, 16: 58)
 constexpr int kMaxSpans = 4096; // sequences and groups of a call
@@ -70,6 +71,7 @@ struct SharedArgs {
     int64_t table_stride;
     int batch, heads, kv_heads, group, groups;  // group: query heads of a key-value head
     int pages, page_size, capacity, target;
+    bool plans;  // shared_kernel makes the plan
     float scale;
     FastDiv by_page, by_group;
 };
@@ -80,7 +82,13 @@ __host__ __device__ __forceinline__ int64_t blocks_of(int64_t rows) {
     return rows <= kThinRows ? (rows > 0) : (rows + kWideRows - 1) / kWideRows;
 }
 
-// Inclusive sums over the T threads of the workgroup; `total`: of all.
+template <int T>
+__device__ __forceinline__ void plan_sync() {
+    if constexpr (T > 64) __syncthreads();
+    else __asm__ volatile("" ::: "memory");  // (one wave: LDS keeps its order)
+}
+
+// Inclusive sums over T threads; `total`: of all.
 template <int T>
 __device__ __forceinline__ void plan_scan(int64_t (&v)[2], int64_t (&total)[2], int64_t (*sums)[2]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -91,9 +99,9 @@ __device__ __forceinline__ void plan_scan(int64_t (&v)[2], int64_t (&total)[2], 
             const int64_t u = __shfl_up(static_cast<long long>(v[n]), d, 64);
             if (lane >= d) v[n] += u;
         }
-    __syncthreads();
+    plan_sync<T>();
     if (lane == 63) sums[wave][0] = v[0], sums[wave][1] = v[1];
-    __syncthreads();
+    plan_sync<T>();
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
         total[n] = 0;
@@ -106,11 +114,17 @@ __device__ __forceinline__ void plan_scan(int64_t (&v)[2], int64_t (&total)[2], 
 }
 
 template <int T>
-__global__ __launch_bounds__(T) void plan_kernel(SharedArgs a) {
-    constexpr int kSpans = T == 1024 ? kMaxSpans : T;
-    __shared__ int start[kSpans + 1], common[kSpans];
-    __shared__ int64_t sums[T / 64][2];
-    __shared__ int top[T / 64];
+struct PlanSpace {
+    static constexpr int kSpans = T == 1024 ? kMaxSpans : T;
+    int64_t sums[T / 64][2];
+    int start[kSpans + 1], common[kSpans], top[T / 64];
+};
+
+// T threads (64: one wave, which needs no barriers) call put(i, span i), each for its own.  Returns the workgroups of all.
+template <int T, typename Put>
+__device__ __forceinline__ int64_t plan(const SharedArgs& a, PlanSpace<T>& space, Put put) {
+    int *const start = space.start, *const common = space.common, *const top = space.top;
+    auto& sums = space.sums;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int spans = a.groups + a.batch;
     const auto length = [&](int b) { return max(0, min(a.lengths[b], a.capacity)); };
@@ -126,9 +140,9 @@ __global__ __launch_bounds__(T) void plan_kernel(SharedArgs a) {
             const int u = __shfl_up(v, d, 64);
             if (lane >= d) v = max(v, u);
         }
-        __syncthreads();
+        plan_sync<T>();
         if (lane == 63) top[wave] = v;
-        __syncthreads();
+        plan_sync<T>();
         v = max(v, before);
         for (int w = 0; w < T / 64; ++w) {
             if (w < wave) v = max(v, top[w]);
@@ -136,7 +150,7 @@ __global__ __launch_bounds__(T) void plan_kernel(SharedArgs a) {
         }
         if (i0 + t <= a.groups) start[i0 + t] = v;
     }
-    __syncthreads();
+    plan_sync<T>();
     const auto group_of = [&](int b) {  // the last group that begins at or before b, if b is in it
         int lo = 0, hi = a.groups;      // groups lo .. hi - 1
         while (lo < hi) {
@@ -150,7 +164,7 @@ __global__ __launch_bounds__(T) void plan_kernel(SharedArgs a) {
         const int g = group_of(b);
         if (g >= 0) atomicMin(&common[g], start[g + 1] - start[g] > 1 ? (b == t ? own_length : length(b)) : 0);
     }
-    __syncthreads();
+    plan_sync<T>();
 
     const auto span = [&](int i) {
         Span s{};
@@ -205,13 +219,21 @@ __global__ __launch_bounds__(T) void plan_kernel(SharedArgs a) {
         s.part = row + end[1] - n[1];
         slot += total[0];
         row += total[1];
-        if (i0 + t < spans) {
-            a.firsts[i0 + t] = s.first;
-            a.spans[i0 + t] = s;
-        }
+        if (i0 + t < spans) put(i0 + t, s);
     }
-    if (t == 0) a.firsts[spans] = static_cast<int>(slot);
+    return slot;
 }
+
+template <int T>
+__global__ __launch_bounds__(T) void plan_kernel(SharedArgs a) {
+    __shared__ PlanSpace<T> space;
+    const int64_t slots = plan<T>(a, space, [&](int i, const Span& s) {
+        a.firsts[i] = s.first;
+        a.spans[i] = s;
+    });
+    if (threadIdx.x == 0) a.firsts[a.groups + a.batch] = static_cast<int>(slots);
+}
+
 
 // LDS rows are D (96: 128) values of 16 bits; 16-byte piece c of token t's row is at piece c ^ swizzle(t), so that the
 // 16 lanes that read K at once (16 tokens' pieces), and the 32 that read V (4 tokens', 4 pieces of each), touch all 64 banks.
@@ -542,15 +564,41 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void shared_kernel(SharedArg
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
     // the span of this workgroup: the last that begins at or before it
     const int spans = a.groups + a.batch, id = blockIdx.x;
-    if (id >= a.firsts[spans]) return;
-    int before = 0;
-    for (int i0 = 0; i0 < spans; i0 += 64) {
-        const int i = i0 + static_cast<int>(threadIdx.x & 63);
-        const uint64_t here = __ballot(i < spans && a.firsts[i] <= id);
-        before += __popcll(here);
-        if (here != ~0ull) break;
+    Span s;
+    if (a.plans) {  // no launch before this one: each workgroup makes the plan for itself, the first also for the join
+        auto& space = *reinterpret_cast<PlanSpace<64>*>(lds);
+        Span& found = *reinterpret_cast<Span*>(lds + 2048);
+        int& all = *reinterpret_cast<int*>(lds + 2048 + sizeof(Span));
+        static_assert(sizeof(PlanSpace<64>) <= 2048 && 2048 + sizeof(Span) + 4 <= kLds, "both fit");
+        if (threadIdx.x < 64) {
+            Span mine{};
+            const int64_t slots = plan<64>(a, space, [&](int i, const Span& x) {
+                mine = x;
+                if (id == 0) a.spans[i] = x;
+            });
+            const int lane = threadIdx.x;
+            const uint64_t here = __ballot(lane < spans && mine.first <= id);
+            if (lane == __popcll(here) - 1) found = mine;
+            if (lane == 0) all = static_cast<int>(slots);
+        }
+        __syncthreads();
+        if (id >= all) return;
+        s = found;
+        int* const w = reinterpret_cast<int*>(&s);
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(Span) / 4); ++i) w[i] = __builtin_amdgcn_readfirstlane(w[i]);
+        __syncthreads();
+    } else {
+        if (id >= a.firsts[spans]) return;
+        int before = 0;
+        for (int i0 = 0; i0 < spans; i0 += 64) {
+            const int i = i0 + static_cast<int>(threadIdx.x & 63);
+            const uint64_t here = __ballot(i < spans && a.firsts[i] <= id);
+            before += __popcll(here);
+            if (here != ~0ull) break;
+        }
+        s = a.spans[__builtin_amdgcn_readfirstlane(before) - 1];
     }
-    const Span s = a.spans[__builtin_amdgcn_readfirstlane(before) - 1];
     if (s.sequences * a.group <= kThinRows) {
         const int at = (id - s.first) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         if (at < s.pieces) thin_piece<C, D, F8, WHOLE>(a, Piece(a, s, at), lds);
@@ -643,7 +691,8 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
 template <int C, int D>
 void launch_shared(const SharedArgs& a, int64_t slots, bool f8, hipStream_t st) {
     // A span a thread, and barriers only where there are several waves (5 spans: 3.8 us by one wave, 4.8 by sixteen).
-    if (a.batch + a.groups <= 64) plan_kernel<64><<<1, 64, 0, st>>>(a);
+    if (a.plans) {
+    } else if (a.batch + a.groups <= 64) plan_kernel<64><<<1, 64, 0, st>>>(a);
     else if (a.batch + a.groups <= 128) plan_kernel<128><<<1, 128, 0, st>>>(a);
     else if (a.batch + a.groups <= 256) plan_kernel<256><<<1, 256, 0, st>>>(a);
     else plan_kernel<1024><<<1, 1024, 0, st>>>(a);
@@ -762,6 +811,9 @@ extern "C" int ckh_shared_attention(const void* q, const void* k_cache, const vo
     a.target = static_cast<int>(space.target);
     a.scale = scale;
     a.by_page = fast_div(static_cast<uint32_t>(page_size)), a.by_group = fast_div(static_cast<uint32_t>(a.group));
+    // Where all workgroups are on the GPU at once, each makes the plan for itself, and a launch is spared (4 sequences over 777 and 100:
+    // 15.2 us, 16.8 with it); where they follow each other it would cost more (8 over 8192 and 2048: 30.9, 28.0 with it).
+    a.plans = batch + groups <= 64 && space.slots <= 4 * device_cus();
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (q_code == CKH_BF16) attn::launch_shared<CKH_BF16>(static_cast<int>(dim), a, space.slots, es == 1, st);
     else attn::launch_shared<CKH_F16>(static_cast<int>(dim), a, space.slots, es == 1, st);
