@@ -19,6 +19,9 @@ class OutOfPages(RuntimeError):
     """The cache has fewer free pages than the call needs; the cache is as it was before."""
 
 
+MOST_SPANS = 4096  # sequences and groups together that `ck.shared_attention` takes
+
+
 def _common(a: list[int], b: list[int]) -> int:
     """With how many of the same pages both begin, up to one that was given back."""
     most = min(len(a), len(b))
@@ -239,7 +242,8 @@ class PagedKVCache:
         """(groups, shared) of the sequences in this order for `attend`, int32 on the device: neighbours that begin with the
         same pages (forks of one sequence) are a group.  None where reading common rows once saves less than
         `least_bytes` of K and V a layer, which is what finding them costs (4 sequences of 40 heads over 8: 22 us for 23
-        at 8192 common tokens of 16 bits, 96 MB; 16 for 15 at 2048, 36 for 83 at 32768)."""
+        at 8192 common tokens of 16 bits, 96 MB; 16 for 15 at 2048, 36 for 83 at 32768), and where there are more sequences
+        and groups than `ck.shared_attention` takes (MOST_SPANS)."""
         owners = [self._sequences[s] for s in sequences]
         starts, shared = [], []
         first: list[int] = []  # the pages of the group's first sequence that all of it have
@@ -266,6 +270,13 @@ class PagedKVCache:
         saved = sum((b - a - 1) * n for n, a, b in zip(tokens, starts, starts[1:])) * row
         if saved < max(least_bytes, 1):
             return None
+        if len(owners) + len(tokens) > MOST_SPANS:  # neighbours that share nothing are then one group, of no common tokens
+            alone = [b - a == 1 for a, b in zip(starts, starts[1:])]
+            kept = [i for i in range(len(alone)) if not (i and alone[i] and alone[i - 1])]
+            tokens = [0 if alone[i] else tokens[i] for i in kept]
+            starts = [starts[i] for i in kept] + starts[-1:]
+            if len(owners) + len(tokens) > MOST_SPANS:
+                return None
         return self._on_device(starts), self._on_device(tokens)
 
     def attend(self, layer: int, q: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
