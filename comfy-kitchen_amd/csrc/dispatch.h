@@ -1,4 +1,4 @@
-// Which kernel serves a GEMM call (and one quantizer's): the rules, apart from the kernels and the
+// Which kernel serves a GEMM call (and one quantizer's, and the norm's): the rules, apart from the kernels and the
 // launches, so that they can be asked on any machine.  A call's sizes, whether it brings a split-K
 // workspace and the device's CUs decide; every rule gives both sides' measurements.
 #pragma once
@@ -363,6 +363,25 @@ constexpr int64_t kNvPadFastElems = 3 << 20;
 
 inline bool nv_quantize_fast_rows(int64_t rows, int64_t orig_rows, int64_t cols) {
     return rows == orig_rows || orig_rows * cols >= kNvPadFastElems;
+}
+
+// ------------------------------------------------------------------- the norm's rows
+// norm_kernel of rows of `pieces` times 8 elements: a thread's pieces, of which there is a kernel each for 1, 2, 4 and 8, and the
+// threads of a row's workgroup.
+struct NormLaunch {
+    int held, threads;
+};
+
+// A thread's pieces, as long as every lane has some.  Few rows: one, for the shortest way through a row (1 row of 5120 in bf16: 2.7
+// us; two 3.4).  More: two (777 rows to E4M3 8.9 us; one 9.5, four 10.5; 6000: 43.5, 53, 47).  Many: four where codes are
+// written, which leaves more rows to a CU at once (16384 rows: to MXFP8 107 us, two 115; to E4M3 60 and 70 without a
+// residual; but to bf16 119 and 113).  Where lanes have three, two (16384 rows of 1920 with a residual to E4M3 42 us, four 47; of 1536 36 and
+// 37; without a residual 26 and 25, 23 and 20).
+inline NormLaunch norm_launch(int pieces, int64_t rows, bool codes, int cus) {
+    const int most = rows < cus ? 1 : !codes || rows < 32 * cus ? 2 : 4;
+    const int full = std::min(most, std::max(1, pieces / 64)), least = full == 3 ? 2 : full;
+    const int held = std::max(least, pieces <= 1024 ? 1 : pieces <= 2048 ? 2 : pieces <= 4096 ? 4 : 8);
+    return {held, static_cast<int>(std::max<int64_t>(64, rup(cdiv(pieces, held), 64)))};
 }
 
 }  // namespace ckh

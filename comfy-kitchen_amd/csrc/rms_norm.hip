@@ -13,6 +13,7 @@
 #include <algorithm>
 
 #include "ckh_common.h"
+#include "dispatch.h"
 #include "quant_math.h"
 
 namespace ckh {
@@ -290,14 +291,7 @@ __global__ void norm_kernel(Args a) {
 template <int C, int OUT, bool VEC>
 void launch_rows(const Args& a, hipStream_t st) {
     const int pieces = OUT == kMX ? a.scale_words * 16 : static_cast<int>(cdiv(a.cols, 8));
-    // A thread's pieces, as long as every lane has some.  Few rows: one, for the shortest way through a row (1 row of 5120 in bf16: 2.7
-    // us; two 3.4).  More: two (777 rows to E4M3 8.9 us; one 9.5, four 10.5; 6000: 43.5, 53, 47).  Many: four where codes are
-    // written, which leaves more rows to a CU at once (16384 rows: to MXFP8 107 us, two 115; to E4M3 60 and 70 without a
-    // residual; but to bf16 119 and 113).
-    const int most = a.rows < device_cus() ? 1 : OUT == kSame || a.rows < 32 * device_cus() ? 2 : 4;
-    const int least = std::min(most, std::max(1, pieces / 64));
-    const int n = std::max(least, pieces <= 1024 ? 1 : pieces <= 2048 ? 2 : pieces <= 4096 ? 4 : 8);
-    const int threads = static_cast<int>(std::max<int64_t>(64, rup(cdiv(pieces, n), 64)));
+    const auto [n, threads] = norm_launch(pieces, a.rows, OUT != kSame, device_cus());
     const unsigned grid = OUT == kMX ? static_cast<unsigned>(rup(cdiv(a.rows, 128), 8) * 128) : static_cast<unsigned>(a.rows);
     if (n == 1) norm_kernel<C, OUT, 1, VEC><<<grid, threads, 0, st>>>(a);
     else if (n == 2) norm_kernel<C, OUT, 2, VEC><<<grid, threads, 0, st>>>(a);
