@@ -124,6 +124,10 @@ __device__ __forceinline__ void emit(const Args& a, int64_t row, int at, bool li
         read_weight<VEC>(a, at, a.cols - at, w);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = round_to_hw<C>(v[e] * f * w[e]);
+        if constexpr (OUT == kMX && !VEC) {  // padding is zeros, whatever f is
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = e < a.cols - at ? v[e] : 0.0f;
+        }
     }
     if constexpr (OUT == kSame) {
         write8<C, VEC>(a.y + row * a.y_row + static_cast<int64_t>(at) * ES, a.cols - at, v);
