@@ -22,19 +22,32 @@ class OutOfPages(RuntimeError):
 MOST_SPANS = 4096  # sequences and groups together that `ck.shared_attention` takes
 
 
-def _common(a: list[int], b: list[int]) -> int:
-    """With how many of the same pages both begin, up to one that was given back."""
-    most = min(len(a), len(b))
-    if a[:most] == b[:most] and -1 not in a[:most]:
-        return most
-    return next(n for n in range(most) if a[n] != b[n] or a[n] < 0)
-
-
 class _Owner:
-    __slots__ = ("length", "pages")
+    __slots__ = ("length", "pages", "whole")
 
-    def __init__(self, pages: list[int], length: int):
+    def __init__(self, pages: list[int], length: int, whole: int | None = None):
         self.pages, self.length = pages, length
+        self.whole = whole  # the pages before the first that was given back, or None: none was
+
+    def held(self) -> int:
+        """The pages that it begins with, up to the first that was given back."""
+        return len(self.pages) if self.whole is None else self.whole
+
+
+def _common(a: _Owner, b: _Owner) -> int:
+    """With how many of the same pages both begin.  Two come to have a page at the same place by a fork, which gave them all
+    that lie before it too, and these stay: so the first that differ are found by halving."""
+    p, q = a.pages, b.pages
+    same, most = 0, min(a.held(), b.held())
+    if most and p[most - 1] == q[most - 1]:
+        return most
+    while same < most:
+        middle = (same + most) // 2
+        if p[middle] == q[middle]:
+            same = middle + 1
+        else:
+            most = middle
+    return same
 
 
 class PagedKVCache:
@@ -100,9 +113,9 @@ class PagedKVCache:
                 if self._owners[page] == 0:
                     self._free.append(page)
 
-    def _new(self, pages: list[int], length: int) -> int:
+    def _new(self, pages: list[int], length: int, whole: int | None = None) -> int:
         sequence, self._next = self._next, self._next + 1
-        self._sequences[sequence] = _Owner(pages, length)
+        self._sequences[sequence] = _Owner(pages, length, whole)
         return sequence
 
     def _on_device(self, values, dtype=torch.int32) -> torch.Tensor:
@@ -122,7 +135,7 @@ class PagedKVCache:
         for page in owner.pages:
             if page >= 0:
                 self._owners[page] += 1
-        return self._new(list(owner.pages), owner.length)
+        return self._new(list(owner.pages), owner.length, owner.whole)
 
     def free(self, sequence: int) -> None:
         """Forget a sequence; pages that no other owns can be handed out again."""
@@ -188,6 +201,8 @@ class PagedKVCache:
         self._drop(owner.pages[i] for i in gone)
         for i in gone:
             owner.pages[i] = -1
+        if gone:
+            owner.whole = min(gone[0], owner.held())
         return len(gone)
 
     def compact(self, sequence: int, keep: Sequence[int]) -> None:
@@ -207,7 +222,7 @@ class PagedKVCache:
                        [new[i // size] * size + i % size for i in range(len(keep))])
         self._take(need)
         self._drop(owner.pages)
-        owner.pages, owner.length = new, len(keep)
+        owner.pages, owner.length, owner.whole = new, len(keep), None
 
     # ------------------------------------------------------------ device calls
     def _copy(self, src: list[int], dst: list[int]) -> None:
@@ -241,34 +256,39 @@ class PagedKVCache:
     def groups(self, sequences: Sequence[int], least_bytes: int = 80 << 20) -> tuple[torch.Tensor, torch.Tensor] | None:
         """(groups, shared) of the sequences in this order for `attend`, int32 on the device: neighbours that begin with the
         same pages (forks of one sequence) are a group.  None where reading common rows once saves less than
-        `least_bytes` of K and V a layer, which is what finding them costs (4 sequences of 40 heads over 8: 22 us for 23
-        at 8192 common tokens of 16 bits, 96 MB; 16 for 15 at 2048, 36 for 83 at 32768), and where there are more sequences
-        and groups than `ck.shared_attention` takes (MOST_SPANS)."""
+        `least_bytes` of K and V a layer, from where on `ck.shared_attention` is the faster (4 sequences of 40 heads over 8: 22 us
+        for 23 at 8192 common tokens of 16 bits, 96 MB; 16 for 15 at 2048, 36 for 83 at 32768), and where there are more
+        sequences and groups than it takes (MOST_SPANS).  The host's time for it grows with the sequences, hardly with their
+        tokens."""
         owners = [self._sequences[s] for s in sequences]
+        near = [_common(a, b) for a, b in zip(owners, owners[1:])]  # of each and the next
+        row = 2 * self.k.shape[3] * self.k.shape[4] * self.k.element_size()
+        least = max(least_bytes, 1)
+        if sum(near) * self.page_size * row < least:  # (more than any groups save)
+            return None
         starts, shared = [], []
-        first: list[int] = []  # the pages of the group's first sequence that all of it have
+        first = 0  # pages that the group so far begins with
         for i, owner in enumerate(owners):
-            same = _common(first, owner.pages) if starts else 0
+            same = min(first, near[i - 1]) if i else 0
             if same:
                 members = i - starts[-1]
-                after = _common(owner.pages, owners[i + 1].pages) if i + 1 < len(owners) else 0
+                after = near[i] if i + 1 < len(owners) else 0
                 # it would cost the others more than it gains, or gains far more with those behind it
-                if members * same < (members - 1) * len(first) or (2 * same < after and members * same < after):
+                if members * same < (members - 1) * first or (2 * same < after and members * same < after):
                     same = 0
             if same:
-                first = first[:same]
+                first = same
             else:
                 if starts:
-                    shared.append(len(first))
+                    shared.append(first)
                 starts.append(i)
-                first = owner.pages[:_common(owner.pages, owner.pages)]
+                first = owner.held()
         if starts:
-            shared.append(len(first))
+            shared.append(first)
         starts.append(len(owners))
         tokens = [min(n * self.page_size, min(o.length for o in owners[a:b])) for n, a, b in zip(shared, starts, starts[1:])]
-        row = 2 * self.k[0, 0, 0].numel() * self.k.element_size()
         saved = sum((b - a - 1) * n for n, a, b in zip(tokens, starts, starts[1:])) * row
-        if saved < max(least_bytes, 1):
+        if saved < least:
             return None
         if len(owners) + len(tokens) > MOST_SPANS:  # neighbours that share nothing are then one group, of no common tokens
             alone = [b - a == 1 for a, b in zip(starts, starts[1:])]
