@@ -1,4 +1,4 @@
-// Which kernel serves a GEMM call (and one quantizer's, and the norm's): the rules, apart from the kernels and the
+// Which kernel serves a GEMM call (and one quantizer's, the norm's and shared attention's): the rules, apart from the kernels and the
 // launches, so that they can be asked on any machine.  A call's sizes, whether it brings a split-K
 // workspace and the device's CUs decide; every rule gives both sides' measurements.
 #pragma once
@@ -382,6 +382,20 @@ inline NormLaunch norm_launch(int pieces, int64_t rows, bool codes, int cus) {
     const int full = std::min(most, std::max(1, pieces / 64)), least = full == 3 ? 2 : full;
     const int held = std::max(least, pieces <= 1024 ? 1 : pieces <= 2048 ? 2 : pieces <= 4096 ? 4 : 8);
     return {held, static_cast<int>(std::max<int64_t>(64, rup(cdiv(pieces, held), 64)))};
+}
+
+// ------------------------------------------------------------- attention of shared tokens
+// The plan of at most this many spans is one wave's.
+constexpr int kOneWaveSpans = 64;
+
+// Whether a call's workgroups (`slots` of them at most) make the plan each for itself, which spares a launch, instead of reading
+// that of a launch before them.  It pays while few of them follow others on their CU: of heads of 256 one has a CU to itself, of
+// 96 and 128 two share one (LDS), of 64 more.  Replayed, bf16, with the plan in the workgroups and with its launch: 4 sequences of 40
+// heads over 8 on a common 3800, 976 slots, D 64 14.4 and 15.8 us, D 128 18.2 and 17.9, D 256 31.0 and 27.7; on 2900, 752
+// slots, D 128 16.4 and 17.8, D 256 26.7 and 25.3; on 2200, 576 slots, D 256 22.6 and 23.6.  12 of 24 heads on 500, 960 slots, D
+// 128 17.4 and 18.4, D 256 29.8 and 25.8.  (8 sequences over 8192 and 2048, 16 slots a CU, D 128: 30.9 and 28.0.)
+inline bool shared_plans_itself(int64_t spans, int64_t slots, int dim, int cus) {
+    return spans <= kOneWaveSpans && 2 * slots <= (dim == 256 ? 5 : 8) * static_cast<int64_t>(cus);
 }
 
 }  // namespace ckh

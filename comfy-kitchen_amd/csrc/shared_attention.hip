@@ -28,6 +28,7 @@
 // 16 over 8192, 27 for 52; 4 over 8192, 22 for 23; 4 over 2048, 16 for 15.  It pays from some 80 MB of keys and values that are not read again.
 #include <algorithm>
 
+#include "dispatch.h"
 #include "paged_tiles.h"
 
 namespace ckh {
@@ -692,7 +693,7 @@ template <int C, int D>
 void launch_shared(const SharedArgs& a, int64_t slots, bool f8, hipStream_t st) {
     // A span a thread, and barriers only where there are several waves (5 spans: 3.8 us by one wave, 4.8 by sixteen).
     if (a.plans) {
-    } else if (a.batch + a.groups <= 64) plan_kernel<64><<<1, 64, 0, st>>>(a);
+    } else if (a.batch + a.groups <= kOneWaveSpans) plan_kernel<64><<<1, 64, 0, st>>>(a);
     else if (a.batch + a.groups <= 128) plan_kernel<128><<<1, 128, 0, st>>>(a);
     else if (a.batch + a.groups <= 256) plan_kernel<256><<<1, 256, 0, st>>>(a);
     else plan_kernel<1024><<<1, 1024, 0, st>>>(a);
@@ -811,9 +812,7 @@ extern "C" int ckh_shared_attention(const void* q, const void* k_cache, const vo
     a.target = static_cast<int>(space.target);
     a.scale = scale;
     a.by_page = fast_div(static_cast<uint32_t>(page_size)), a.by_group = fast_div(static_cast<uint32_t>(a.group));
-    // Where all workgroups are on the GPU at once, each makes the plan for itself, and a launch is spared (4 sequences over 777 and 100:
-    // 15.2 us, 16.8 with it); where they follow each other it would cost more (8 over 8192 and 2048: 30.9, 28.0 with it).
-    a.plans = batch + groups <= 64 && space.slots <= 4 * device_cus();
+    a.plans = shared_plans_itself(batch + groups, space.slots, static_cast<int>(dim), device_cus());
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (q_code == CKH_BF16) attn::launch_shared<CKH_BF16>(static_cast<int>(dim), a, space.slots, es == 1, st);
     else attn::launch_shared<CKH_F16>(static_cast<int>(dim), a, space.slots, es == 1, st);
