@@ -413,8 +413,9 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: float | to
     always is.  The result is the first token whose running weight in that order exceeds u times the weight of
     all that are kept.  temperature 0 takes the first of the largest logits.
     Each of the four is a number or a tensor on the device of one a row (fp32; top_k int32).
-    -inf (a masked token) and NaN are never drawn, nor is a token over 32 temperatures under the largest; a
-    row that holds nothing else gives -1."""
+    -inf (a masked token) and NaN are never drawn, nor is a token 32 temperatures or more (some from 31.94 on) under
+    the largest; a row that holds nothing else gives -1.  Weights are held to some 2^-33 of themselves, and a running weight
+    within 2^-36 of a border has reached it."""
     given = [v if isinstance(v, torch.Tensor) else None for v in (temperature, top_k, top_p, min_p)]
     if direct(logits, u, *given) and untouched("sample_tokens"):
         return _dispatch("sample_tokens", logits=logits, u=u, temperature=temperature, top_k=top_k, top_p=top_p,

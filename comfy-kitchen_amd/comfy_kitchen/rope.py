@@ -14,6 +14,8 @@ def rope_rates(dim: int, base: float = 10000.0, factor: float = 1.0, context: in
     every rate is divided by it.  With the trained context, only the slow pairs' are: those that turn less
     than `slow` times over it wholly, those that turn over `fast` times not at all, those between by the share
     that lies between, (turns - slow) / (fast - slow) of a pair's own rate and the rest of the divided one.
+    Checkpoints that were trained with another ramp, such as one that is linear in a pair's number between two
+    pairs, need rates of their own: `ck.paged_write_rope` takes any.
     """
     if dim < 0 or dim % 2:
         raise ValueError(f"rope_rates: {dim} elements do not make pairs")

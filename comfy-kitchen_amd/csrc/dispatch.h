@@ -372,11 +372,12 @@ struct NormLaunch {
     int held, threads;
 };
 
-// A thread's pieces, as long as every lane has some.  Few rows: one, for the shortest way through a row (1 row of 5120 in bf16: 2.7
-// us; two 3.4).  More: two (777 rows to E4M3 8.9 us; one 9.5, four 10.5; 6000: 43.5, 53, 47).  Many: four where codes are
-// written, which leaves more rows to a CU at once (16384 rows: to MXFP8 107 us, two 115; to E4M3 60 and 70 without a
-// residual; but to bf16 119 and 113).  Where lanes have three, two (16384 rows of 1920 with a residual to E4M3 42 us, four 47; of 1536 36 and
-// 37; without a residual 26 and 25, 23 and 20).
+// A thread's pieces, as long as every lane has some.  Few rows: one, for the shortest way through a row (1 row of 5120: the kernel takes
+// 2.7 us; with two 3.4).  More: two (replayed, one, two and four: 777 rows of 4608 with a residual to E4M3 8.5, 8.4 and 9.6 us; 16384 of
+// 5120 with a residual to bf16 125, 113 and 119).  Many: four where codes are written, which leaves more rows to a CU at once
+// (16384 of 5120 to E4M3 87, 69 and 58, with a residual 135, 108 and 107; to MXFP8 93, 66 and 60, with a residual 128, 108 and 108).
+// Where lanes have three, two (16384 rows of 1920 with a residual to E4M3 42 us, four 47; of 1536 36 and 37; without a residual
+// 26 and 25, 23 and 20).  All in bf16.
 inline NormLaunch norm_launch(int pieces, int64_t rows, bool codes, int cus) {
     const int most = rows < cus ? 1 : !codes || rows < 32 * cus ? 2 : 4;
     const int full = std::min(most, std::max(1, pieces / 64)), least = full == 3 ? 2 : full;

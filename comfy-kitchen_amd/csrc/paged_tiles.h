@@ -230,6 +230,7 @@ __device__ __forceinline__ void paged_tiles(const PagedRows& a, const PagedTiles
             sum += p[e];
         }
         l += sum;
+        // (rounded to the values' 16-bit type, as the product takes them: half a step of each weight, of unlike signs)
         const v4u pb = v4u{pack2<QC>(p[0], p[1]), pack2<QC>(p[2], p[3]), pack2<QC>(p[4], p[5]), pack2<QC>(p[6], p[7])};
         int n = 0;
 #pragma unroll

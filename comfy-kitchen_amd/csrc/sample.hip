@@ -6,7 +6,8 @@
 //   are needed to reach top_p of the weight of those,
 //   have w >= min_p,
 // and the first is; the result is the first token whose running weight exceeds u times the weight of
-// all that are kept.  What lies more than 32 temperatures (kBins bins) under the largest logit is not kept.
+// all that are kept.  What lies 32 temperatures or more (kBins bins: 31.94 to 32, by where in its bin the largest lies) under the
+// largest logit is not kept: e^-31.94 each, 2^-22 of the row where 2^24 logits lie there.
 //
 // Nothing is sorted.  Logits fall into bins of 1/16 temperature, and
 //   - a first launch (a workgroup for 8192 logits, which it holds in registers) counts and sums the

@@ -472,7 +472,8 @@ __device__ __forceinline__ void wide_piece(const SharedArgs& a, const Piece& pie
 #pragma unroll
             for (int n = 0; n < D / 32; ++n) acc[n] *= f;
         }
-        // The weights of 16 tokens are made while the matrix units multiply those of the 16 before with their values.
+        // The weights of 16 tokens are made while the matrix units multiply those of the 16 before with their values.  They are
+        // rounded to the values' 16-bit type, as the product takes them and as ckh_paged_attention does; their sum is taken before that.
         float sum = 0.0f;  // the tile's own: single small weights would be lost in a large l
         const auto weigh = [&](int w) __attribute__((always_inline)) {
             float x[8];

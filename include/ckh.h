@@ -416,7 +416,8 @@ int ckh_paged_write_rope(const void* q, const void* key, const void* value, cons
  * the first top_k (0: all), and needed to reach top_p of the weight of those (1 and over: all), and have
  * w >= min_p; the first always is.  out [rows] (int64) is the first token whose running weight exceeds u times
  * the weight of all kept.  Temperature 0: the first of the largest logits.  -inf and NaN are never drawn, nor
- * what lies over 32 temperatures under the largest; a row of nothing else gives -1.
+ * what lies 32 temperatures or more (some of it from 31.94 on) under the largest; a row of nothing else gives -1.
+ * Weights are held to some 2^-33 of themselves, and a running weight within 2^-36 of a border has reached it.
  * temperature, top_p, min_p (f32) and top_k (int32): device arrays of one a row, or NULL, then the *_all
  * values hold.  In an array, a temperature that is not over 0 counts as 0, a top_k under 1 as all, a min_p over
  * 1 as 1.  vocab up to 2^24.  The workspace is needed.
