@@ -253,17 +253,18 @@ class PagedKVCache:
         return ck.paged_write_rope(q, key, value, positions, rates, self.k[layer], self.v[layer], slots, interleaved,
                                    magnitude, self.k_scale, self.v_scale, keep_key)
 
-    def groups(self, sequences: Sequence[int], least_bytes: int = 80 << 20) -> tuple[torch.Tensor, torch.Tensor] | None:
+    def groups(self, sequences: Sequence[int], least_bytes: int | None = None) -> tuple[torch.Tensor, torch.Tensor] | None:
         """(groups, shared) of the sequences in this order for `attend`, int32 on the device: neighbours that begin with the
         same pages (forks of one sequence) are a group.  None where reading common rows once saves less than
-        `least_bytes` of K and V a layer, from where on `ck.shared_attention` is the faster (4 sequences of 40 heads over 8: 22 us
-        for 23 at 8192 common tokens of 16 bits, 96 MB; 16 for 15 at 2048, 36 for 83 at 32768), and where there are more
-        sequences and groups than it takes (MOST_SPANS).  The host's time for it grows with the sequences, hardly with their
-        tokens."""
+        `least_bytes` of K and V a layer, and where there are more sequences and groups than `ck.shared_attention` takes
+        (MOST_SPANS).
+        By default that is 80 MB, from where on `ck.shared_attention` is the faster (4 sequences of 40 heads over 8: 22 us
+        for 23 at 8192 common tokens of 16 bits, 96 MB; 16 for 15 at 2048, 36 for 83 at 32768), and 400 MB by the layers, for the
+        host's time of this call, some 0.05 to 0.08 ms for 4 to 64 sequences, hardly more for many tokens."""
         owners = [self._sequences[s] for s in sequences]
         near = [_common(a, b) for a, b in zip(owners, owners[1:])]  # of each and the next
         row = 2 * self.k.shape[3] * self.k.shape[4] * self.k.element_size()
-        least = max(least_bytes, 1)
+        least = max((80 << 20) + (400 << 20) / self.k.shape[0] if least_bytes is None else least_bytes, 1)
         if sum(near) * self.page_size * row < least:  # (more than any groups save)
             return None
         starts, shared = [], []

@@ -52,10 +52,10 @@ def rope_matrices(positions: torch.Tensor, dim: int, base: float) -> torch.Tenso
 
 class TextDecoder:
     """weights: a dict of [out, in] matrices and norms by name; the matrices are quantized here.
-    share_from: bytes of K and V a layer from which on what sequences share is read once (PagedKVCache.groups)."""
+    share_from: bytes of K and V a layer from which on what sequences share is read once (PagedKVCache.groups; None: its default)."""
 
     def __init__(self, config: Config, weights: dict[str, torch.Tensor], pages: int = 256, page_size: int = 16,
-                 cache_dtype: torch.dtype | None = None, cache_scale: float | None = None, share_from: int = 80 << 20):
+                 cache_dtype: torch.dtype | None = None, cache_scale: float | None = None, share_from: int | None = None):
         self.config, self.share_from = config, share_from
         self.embedding = weights["embedding"]
         dtype, device = self.embedding.dtype, self.embedding.device
